@@ -339,6 +339,87 @@ int64_t jasperx_prerotate_seed(int64_t handle);
  * 255 values, dim 112 or 128; JASPER_SEARCH_BYTES=0 turns them off)}. No
  * reference counterpart (an inspection call for tests and tooling). */
 int64_t jasperx_row_format(int64_t handle, int64_t* out4);
+/* ---- A paged cache of keys and values, and the attention that reads it.
+ * No reference counterpart: the index's rows are then the keys of a model's
+ * earlier tokens, its queries a new token's query heads.
+ *
+ * K and V are [layers][pages][heads][page_size][dim] with the strides given
+ * (in values; a row's dim values are contiguous, rows start on 16 bytes), the
+ * same for both. page_size: a power of two, 8 to 256; dim: up to 256, a
+ * multiple of 8 (of 16 for e4m3). Types: 0 fp16, 1 bf16, 2 OCP e4m3 (then a
+ * stored value times its head's scale is the value; NULL scales are 1).
+ * Token t of a sequence is row t % page_size of page table[t / page_size].
+ * All pointers are device memory; calls enqueue on the stream, allocate
+ * nothing and may be captured in a graph. */
+typedef struct jasperx_kv_pages {
+  void* k;
+  void* v;
+  const float* k_scale; /* [heads] or NULL */
+  const float* v_scale;
+  int64_t layer_stride, page_stride, head_stride, row_stride;
+  int32_t layers, pages, heads, page_size, dim, type;
+} jasperx_kv_pages;
+
+/* Rows [n][heads][dim] of a tensor, strides in values. */
+typedef struct jasperx_head_rows {
+  const void* data;
+  int64_t stride, head_stride, heads;
+} jasperx_head_rows;
+
+#define JASPERX_ROTARY_INTERLEAVED 1u /* pairs are neighbours (2i, 2i + 1), not (i, i + rot_dim / 2) */
+#define JASPERX_ROTARY_INVERSE 2u     /* by the opposite angles: the gradient */
+/* Rotary positions: of every head of q and k (heads 0: absent; fp16 or bf16)
+ * the first rot_dim values are turned in pairs, x' = x cos - y sin,
+ * y' = y cos + x sin, by row positions[i] of the fp32 tables cos, sin
+ * [table_rows][rot_dim / 2]; the rest is copied. positions: index_bytes 4 or
+ * 8 each; a row whose position is outside the table becomes NaN. Outputs are
+ * contiguous [n][heads][dim]. */
+int64_t jasperx_rotary(const jasperx_head_rows* q, const jasperx_head_rows* k, int32_t type, int64_t n, int64_t dim,
+                       const void* positions, int32_t index_bytes, const float* cos, const float* sin,
+                       int64_t table_rows, int64_t rot_dim, uint32_t flags, void* q_out, void* k_out, void* stream);
+/* The tokens of a step into the cache: q rotated to q_out, k rotated (as
+ * above; rot_dim 0: not at all) and v to row slots[i] % page_size of page
+ * slots[i] / page_size. The cache has q's type or e4m3 (values divided by
+ * their head's scale, rounded to nearest, saturating at 448). A slot outside
+ * the cache stores nothing (padding: -1). layers must be 1. */
+int64_t jasperx_append_tokens(const jasperx_head_rows* q, const jasperx_head_rows* k, const jasperx_head_rows* v,
+                              int32_t type, int64_t n, const void* positions, const void* slots,
+                              int32_t index_bytes, const float* cos, const float* sin, int64_t table_rows,
+                              int64_t rot_dim, uint32_t flags, const jasperx_kv_pages* pages, void* q_out,
+                              void* stream);
+/* Pages src[i] to dst[i], K and V of every layer. With tables (NULL: none),
+ * each of table_entries entries that equals src[i] becomes dst[i]. A page may
+ * be the source of several copies (not with tables) and the destination of
+ * one, not both. Pairs with an id outside the cache are skipped. */
+int64_t jasperx_copy_pages(const jasperx_kv_pages* pages, const int32_t* src, const int32_t* dst, int64_t n,
+                           int32_t* tables, int64_t table_entries, void* stream);
+/* Attention of one new token per sequence: with t over the last `window` (0:
+ * all) of the lens[b] tokens of sequence b, s_t = scale * <q, k_t>, out =
+ * sum softmax(s)_t v_t and lse = log sum exp s_t (NULL: not written); no
+ * tokens give 0 and -inf. q [batch][heads][dim] fp16 or bf16 (heads: a
+ * multiple of the cache's, consecutive ones share a key head), out
+ * contiguous; lengths count at most min(max_len, table_width * page_size)
+ * tokens; tokens whose table entry is outside the cache are left out.
+ * workspace: jasperx_attention_workspace bytes, 16-byte aligned. */
+int64_t jasperx_decode_attention(const jasperx_head_rows* q, int32_t type, int64_t batch,
+                                 const jasperx_kv_pages* pages, const int32_t* tables, int64_t table_stride,
+                                 int64_t table_width, const int32_t* lens, int64_t max_len, double scale,
+                                 int64_t window, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
+/* The same over a choice of tokens: the first `first`, the last `last` and,
+ * between them, the ids [batch][lists][count] (what a search over the keys
+ * returned; lists = query heads or the cache's heads). Ids outside that range
+ * (-1 among them) are left out; one listed twice counts twice. */
+int64_t jasperx_retrieved_attention(const jasperx_head_rows* q, int32_t type, int64_t batch,
+                                    const jasperx_kv_pages* pages, const int32_t* tables, int64_t table_stride,
+                                    int64_t table_width, const int32_t* lens, const int32_t* ids, int64_t lists,
+                                    int64_t count, int64_t first, int64_t last, double scale, void* out, float* lse,
+                                    void* workspace, int64_t workspace_bytes, void* stream);
+/* Scratch bytes of the two calls above for their sizes (pages: sizes and type
+ * only). max_tokens: the tokens one head reads at most, min(max_len, window)
+ * or first + last + count; lists 0: decode_attention. */
+int64_t jasperx_attention_workspace(int64_t batch, int64_t q_heads, const jasperx_kv_pages* pages,
+                                    int64_t max_tokens, int64_t lists);
 /* Library build identifier (git-independent), for load checks. */
 const char* jasperx_version(void);
 

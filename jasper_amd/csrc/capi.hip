@@ -23,6 +23,7 @@
 #include "directional.hpp"
 #include "directional_api.hpp"
 #include "graph.hpp"
+#include "kvcache.hpp"
 #include "rabitq.hpp"
 #include "search.hpp"
 
@@ -871,6 +872,178 @@ extern "C" int64_t jasperx_search_stats(int64_t h, const void* q, int64_t nq, in
     (void)hipFree(bits);
     (void)hipFree(st);
     return 0;
+  });
+}
+
+// ---- the paged cache of keys and values ----
+
+namespace {
+
+void check_type(int32_t type) {
+  if (type != kF16 && type != kBF16) throw std::invalid_argument("type must be 0 (fp16) or 1 (bf16)");
+}
+
+KvPages kv_pages(const jasperx_kv_pages* p) {
+  if (!p) throw std::invalid_argument("null pages");
+  if (p->type < kF16 || p->type > kE4M3) throw std::invalid_argument("page type must be 0 (fp16), 1 (bf16) or 2 (e4m3)");
+  if (p->layers < 1 || p->pages < 0 || p->heads < 1) throw std::invalid_argument("bad cache sizes");
+  if (p->page_size < 8 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
+    throw std::invalid_argument("page_size must be a power of two from 8 to 256");
+  const int64_t bytes = kv_bytes(p->type), unit = 16 / bytes;
+  if (p->dim < unit || p->dim > 256 || p->dim % unit)
+    throw std::invalid_argument("dim must be up to 256 and a multiple of 16 bytes of values");
+  if (p->layer_stride % unit || p->page_stride % unit || p->head_stride % unit || p->row_stride % unit ||
+      ((uintptr_t)p->k & 15u) || ((uintptr_t)p->v & 15u))
+    throw std::invalid_argument("pages and their strides must be 16-byte aligned");
+  if (p->row_stride < p->dim) throw std::invalid_argument("row_stride must be at least dim");
+  if (p->pages && (!p->k || !p->v)) throw std::invalid_argument("null pages");
+  KvPages r;
+  r.k = (char*)p->k, r.v = (char*)p->v, r.k_scale = p->k_scale, r.v_scale = p->v_scale;
+  r.layer_stride = p->layer_stride, r.page_stride = p->page_stride;
+  r.head_stride = p->head_stride, r.row_stride = p->row_stride;
+  r.layers = p->layers, r.pages = p->pages, r.heads = p->heads, r.page = p->page_size, r.page_shift = __builtin_ctz((unsigned)p->page_size), r.dim = p->dim, r.type = p->type;
+  if (r.type != kE4M3 && (r.k_scale || r.v_scale)) throw std::invalid_argument("scales must be null unless pages are e4m3");
+  return r;
+}
+
+HeadRows head_rows(const jasperx_head_rows* r) {
+  HeadRows h;
+  if (!r || !r->heads) return h;
+  if (r->heads < 0 || r->heads > 65535) throw std::invalid_argument("heads must be in 0..65535");
+  h.p = r->data, h.stride = r->stride, h.head_stride = r->head_stride, h.heads = (int32_t)r->heads;
+  return h;
+}
+
+RotaryArgs rotary_args(const jasperx_head_rows* q, const jasperx_head_rows* k, int32_t type, int64_t n, int64_t dim,
+                       const void* positions, int32_t index_bytes, const float* cos, const float* sin,
+                       int64_t table_rows, int64_t rot_dim, uint32_t flags) {
+  check_type(type);
+  if (n < 0 || dim < 2 || dim > 2048 || dim % 2) throw std::invalid_argument("dim must be even, 2 to 2048");
+  if (rot_dim < 0 || rot_dim > dim || rot_dim % 2) throw std::invalid_argument("rot_dim must be even, up to dim");
+  if (index_bytes != 4 && index_bytes != 8) throw std::invalid_argument("index_bytes must be 4 or 8");
+  if (flags & ~(JASPERX_ROTARY_INTERLEAVED | JASPERX_ROTARY_INVERSE)) throw std::invalid_argument("unknown rotary flags");
+  if (n && rot_dim && (!positions || !cos || !sin || table_rows < 0)) throw std::invalid_argument("null positions or tables");
+  RotaryArgs a;
+  a.q = head_rows(q), a.k = head_rows(k);
+  a.positions = positions, a.pos64 = index_bytes == 8;
+  a.interleaved = flags & JASPERX_ROTARY_INTERLEAVED, a.back = flags & JASPERX_ROTARY_INVERSE;
+  a.cos = cos, a.sin = sin, a.n = n, a.table_rows = table_rows;
+  a.dim = (int32_t)dim, a.half = (int32_t)rot_dim / 2, a.type = type;
+  return a;
+}
+
+AttendArgs attend_args(const jasperx_head_rows* q, int32_t type, int64_t batch, const KvPages& pages,
+                       const int32_t* tables, int64_t table_stride, int64_t table_width, const int32_t* lens,
+                       double scale, void* out, float* lse, void* workspace, int64_t workspace_bytes) {
+  check_type(type);
+  AttendArgs a;
+  a.q = head_rows(q);
+  if (batch < 0 || batch > 65535) throw std::invalid_argument("batch must be in 0..65535");
+  if (a.q.heads < 1 || a.q.heads % pages.heads) throw std::invalid_argument("query heads must be a multiple of the cache's heads");
+  if (pages.type != kE4M3 && pages.type != type) throw std::invalid_argument("pages must be of the queries' type or e4m3");
+  if (pages.layers != 1) throw std::invalid_argument("pages must be of one layer");
+  if (((uintptr_t)a.q.p & 15u) || a.q.stride % 8 || a.q.head_stride % 8 || ((uintptr_t)out & 15u))
+    throw std::invalid_argument("queries and output must be 16-byte aligned");
+  if (table_width < 0 || table_width > 0x7FFFFFFF) throw std::invalid_argument("bad table width");
+  if (batch && (!a.q.p || !out || !lens || (table_width && !tables))) throw std::invalid_argument("null argument");
+  a.type = type, a.batch = batch, a.tables = tables, a.table_stride = table_stride;
+  a.table_width = (int32_t)table_width, a.lens = lens, a.scale = (float)scale, a.out = out, a.lse = lse;
+  a.workspace = workspace, a.workspace_bytes = workspace_bytes;
+  return a;
+}
+
+}  // namespace
+
+extern "C" int64_t jasperx_rotary(const jasperx_head_rows* q, const jasperx_head_rows* k, int32_t type, int64_t n,
+                                  int64_t dim, const void* positions, int32_t index_bytes, const float* cos,
+                                  const float* sin, int64_t table_rows, int64_t rot_dim, uint32_t flags, void* q_out,
+                                  void* k_out, void* stream) {
+  return guarded([&]() -> int64_t {
+    const RotaryArgs a = rotary_args(q, k, type, n, dim, positions, index_bytes, cos, sin, table_rows, rot_dim, flags);
+    if (n && ((a.q.heads && (!a.q.p || !q_out)) || (a.k.heads && (!a.k.p || !k_out))))
+      throw std::invalid_argument("null rows");
+    if (((uintptr_t)q_out & 15u) || ((uintptr_t)k_out & 15u)) throw std::invalid_argument("outputs must be 16-byte aligned");
+    rotary(a, q_out, k_out, (hipStream_t)stream);
+    return 0;
+  });
+}
+
+extern "C" int64_t jasperx_append_tokens(const jasperx_head_rows* q, const jasperx_head_rows* k,
+                                         const jasperx_head_rows* v, int32_t type, int64_t n, const void* positions,
+                                         const void* slots, int32_t index_bytes, const float* cos, const float* sin,
+                                         int64_t table_rows, int64_t rot_dim, uint32_t flags,
+                                         const jasperx_kv_pages* pages, void* q_out, void* stream) {
+  return guarded([&]() -> int64_t {
+    const KvPages p = kv_pages(pages);
+    const RotaryArgs a = rotary_args(q, k, type, n, p.dim, positions, index_bytes, cos, sin, table_rows, rot_dim, flags);
+    const HeadRows vr = head_rows(v);
+    if (a.k.heads != p.heads || vr.heads != p.heads) throw std::invalid_argument("keys and values must be of the cache's heads");
+    if (p.type != kE4M3 && p.type != type) throw std::invalid_argument("pages must be of the keys' type or e4m3");
+    if (p.layers != 1) throw std::invalid_argument("pages must be of one layer");
+    if (n && (!a.k.p || !vr.p || !slots || (a.q.heads && (!a.q.p || !q_out)))) throw std::invalid_argument("null argument");
+    if ((uintptr_t)q_out & 15u) throw std::invalid_argument("outputs must be 16-byte aligned");
+    append_tokens(a, vr, slots, index_bytes == 8, p, q_out, (hipStream_t)stream);
+    return 0;
+  });
+}
+
+extern "C" int64_t jasperx_copy_pages(const jasperx_kv_pages* pages, const int32_t* src, const int32_t* dst, int64_t n,
+                                      int32_t* tables, int64_t table_entries, void* stream) {
+  return guarded([&]() -> int64_t {
+    const KvPages p = kv_pages(pages);
+    if (n < 0 || table_entries < 0 || (n && (!src || !dst))) throw std::invalid_argument("bad page lists");
+    copy_pages(p, src, dst, n, tables, table_entries, (hipStream_t)stream);
+    return 0;
+  });
+}
+
+extern "C" int64_t jasperx_decode_attention(const jasperx_head_rows* q, int32_t type, int64_t batch,
+                                            const jasperx_kv_pages* pages, const int32_t* tables,
+                                            int64_t table_stride, int64_t table_width, const int32_t* lens,
+                                            int64_t max_len, double scale, int64_t window, void* out, float* lse,
+                                            void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int64_t {
+    const KvPages p = kv_pages(pages);
+    AttendArgs a = attend_args(q, type, batch, p, tables, table_stride, table_width, lens, scale, out, lse, workspace,
+                               workspace_bytes);
+    if (max_len < 0 || window < 0) throw std::invalid_argument("max_len and window must be at least 0");
+    a.max_len = max_len;
+    a.last = window ? window : -1;
+    attend(a, p, (hipStream_t)stream);
+    return 0;
+  });
+}
+
+extern "C" int64_t jasperx_retrieved_attention(const jasperx_head_rows* q, int32_t type, int64_t batch,
+                                               const jasperx_kv_pages* pages, const int32_t* tables,
+                                               int64_t table_stride, int64_t table_width, const int32_t* lens,
+                                               const int32_t* ids, int64_t lists, int64_t count, int64_t first,
+                                               int64_t last, double scale, void* out, float* lse, void* workspace,
+                                               int64_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int64_t {
+    const KvPages p = kv_pages(pages);
+    AttendArgs a = attend_args(q, type, batch, p, tables, table_stride, table_width, lens, scale, out, lse, workspace,
+                               workspace_bytes);
+    if (lists != a.q.heads && lists != p.heads) throw std::invalid_argument("lists must be the query heads or the cache's heads");
+    if (count < 0 || first < 0 || last < 0 || first + last + count > 0x3FFFFFFF)
+      throw std::invalid_argument("first, last and count must be at least 0, at most 2^30 in sum");
+    if (batch && count && !ids) throw std::invalid_argument("null ids");
+    a.max_len = (int64_t)1 << 31;
+    a.ids = ids, a.lists = (int32_t)lists, a.count = (int32_t)count, a.first = first, a.last = last;
+    attend(a, p, (hipStream_t)stream);
+    return 0;
+  });
+}
+
+extern "C" int64_t jasperx_attention_workspace(int64_t batch, int64_t q_heads, const jasperx_kv_pages* pages,
+                                               int64_t max_tokens, int64_t lists) {
+  return guarded([&]() -> int64_t {
+    jasperx_kv_pages sizes = pages ? *pages : jasperx_kv_pages{};
+    sizes.k = sizes.v = nullptr, sizes.pages = 0;
+    const KvPages p = kv_pages(&sizes);
+    if (batch < 0 || batch > 65535 || q_heads < 1 || q_heads % p.heads || max_tokens < 0 || lists < 0)
+      throw std::invalid_argument("bad sizes");
+    return attend_workspace(batch, q_heads, p, max_tokens, lists);
   });
 }
 

@@ -1,0 +1,292 @@
+// kvcache.hip -- rotary positions, appending to the paged cache, and copying
+// its pages.
+#include "kvcache.hpp"
+
+#include "graph.hpp"
+#include "kvtypes.hpp"
+
+#include <algorithm>
+#include <stdexcept>
+
+namespace jasper_amd {
+
+namespace {
+
+// One launch turns the heads of q and k and, when APPEND, writes k and v to
+// the cache. The heads of a token are one list: q's, then k's, then v's.
+struct TokenParams {
+  const char *q, *k, *v;
+  int64_t q_stride, q_head, k_stride, k_head, v_stride, v_head;
+  int q_heads, k_heads, v_heads;
+  const void* positions;
+  const void* slots;
+  const float *cos, *sin;
+  int64_t n, table_rows;
+  int dim, half;
+  bool pos64, slots64, interleaved, back;
+  char *q_out, *k_out;
+  KvPages pages;
+  int64_t rows;  // of the cache: pages * page size
+};
+
+__device__ __forceinline__ int64_t index_at(const void* p, bool wide, int64_t i) {
+  return wide ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+}
+
+// A thread has one chunk of 2 * P values of a head (threadIdx.x) and walks
+// the heads of its token (threadIdx.y on) with the chunk's P cosines and
+// sines in registers. In the half layout the chunk is P values of each half,
+// otherwise 2 * P neighbours; the unrotated tail is chunks of neighbours.
+// The products and sums are rounded one by one (no fused multiply-add): the
+// same bits as the formula in fp32 operations.
+template <typename T, typename CT, int P, bool APPEND>
+__global__ void token_kernel(TokenParams a) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
+  if (i >= a.n) return;
+  const int c = threadIdx.x, turned = a.half / P;
+  const bool turn = c < turned;
+  const bool split = turn && !a.interleaved;
+  const int at = split ? c * P : c * 2 * P;
+  const int to = split ? a.half + at : at + P;
+  float co[P], si[P];
+  if (turn) {
+    const int64_t pos = index_at(a.positions, a.pos64, i);
+    const bool known = pos >= 0 && pos < a.table_rows;
+    const int64_t row = known ? pos * a.half + c * P : 0;
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      co[e] = known ? a.cos[row + e] : __builtin_nanf("");
+      si[e] = known ? (a.back ? -a.sin[row + e] : a.sin[row + e]) : __builtin_nanf("");
+    }
+  }
+  int64_t slot = -1;
+  if (APPEND) slot = index_at(a.slots, a.slots64, i);
+  const bool kept = APPEND && slot >= 0 && slot < a.rows;
+  const int64_t page = kept ? slot >> a.pages.page_shift : 0;
+  const int64_t in_page = kept ? slot & (a.pages.page - 1) : 0;
+  const int all = a.q_heads + a.k_heads + a.v_heads;
+  for (int h = blockIdx.y * blockDim.y + threadIdx.y; h < all; h += blockDim.y * gridDim.y) {
+    const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.k_heads;
+    const int hh = is_q ? h : is_v ? h - a.q_heads - a.k_heads : h - a.q_heads;
+    if (APPEND && !is_q && !kept) continue;
+    const T* src = (const T*)(is_q ? a.q : is_v ? a.v : a.k) +
+                   (is_q ? i * a.q_stride + hh * a.q_head : is_v ? i * a.v_stride + hh * a.v_head
+                                                                 : i * a.k_stride + hh * a.k_head);
+    // v is not rotated: its chunks are neighbours
+    const int from = is_v ? c * 2 * P : at, other = is_v ? c * 2 * P + P : to;
+    float x[2 * P];
+    widen(*(const Pack<T, P>*)(src + from), x);
+    widen(*(const Pack<T, P>*)(src + other), x + P);
+    if (turn && !is_v) {
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        float& u = a.interleaved ? x[2 * e] : x[e];
+        float& w = a.interleaved ? x[2 * e + 1] : x[P + e];
+        const float u0 = u, w0 = w;
+        u = u0 * co[e] - w0 * si[e];
+        w = w0 * co[e] + u0 * si[e];
+      }
+    }
+    if (!APPEND || is_q) {
+      T* dst = (T*)(is_q ? a.q_out : a.k_out) + (i * (is_q ? a.q_heads : a.k_heads) + hh) * a.dim;
+      *(Pack<T, P>*)(dst + from) = narrow<T, P>(x);
+      *(Pack<T, P>*)(dst + other) = narrow<T, P>(x + P);
+    } else {
+      const float* scales = is_v ? a.pages.v_scale : a.pages.k_scale;
+      if (sizeof(CT) == 1 && scales) {
+        const float scale = scales[hh];
+#pragma unroll
+        for (int e = 0; e < 2 * P; ++e) x[e] = x[e] / scale;
+      }
+      CT* dst = (CT*)(is_v ? a.pages.v : a.pages.k) + page * a.pages.page_stride + hh * a.pages.head_stride +
+                in_page * a.pages.row_stride;
+      *(Pack<CT, P>*)(dst + from) = narrow<CT, P>(x);
+      *(Pack<CT, P>*)(dst + other) = narrow<CT, P>(x + P);
+    }
+  }
+}
+
+template <typename T, typename CT, bool APPEND>
+void launch_token(const TokenParams& p, int P, hipStream_t s) {
+  const int all = p.q_heads + p.k_heads + p.v_heads;
+  if (p.n == 0 || all == 0) return;
+  const int chunks = p.dim / (2 * P);
+  if (chunks > 1024) throw std::invalid_argument("a head is too large");
+  // Few tokens: a thread per chunk of a head, so that a token is as many
+  // waves as it has work. Many: a wave per token, whose threads keep their
+  // cosines for several heads.
+  const int wide = std::max(1, 256 / chunks);
+  dim3 block, grid;
+  if (p.n < 1024) {
+    block = dim3(chunks, std::min(all, wide), 1);
+    grid = dim3((unsigned)p.n, (all + (int)block.y - 1) / (int)block.y);
+  } else {
+    block = dim3(chunks, std::max(1, 64 / chunks), 1);
+    block.z = std::max(1u, 256u / (block.x * block.y));
+    const int64_t blocks = (p.n + block.z - 1) / block.z;
+    if (blocks > 0x7FFFFFFF) throw std::invalid_argument("too many tokens (too large)");
+    grid = dim3((unsigned)blocks, 1);
+  }
+  auto kernel = P == 8 ? token_kernel<T, CT, 8, APPEND> : P == 4 ? token_kernel<T, CT, 4, APPEND>
+                                                                 : token_kernel<T, CT, 1, APPEND>;
+  kernel<<<grid, block, 0, s>>>(p);
+  hip_check(hipGetLastError(), "rotary");
+}
+
+bool rows_fit(const void* p, int64_t stride, int64_t head_stride, int heads, int width, int bytes) {
+  const int64_t unit = (int64_t)width * bytes;
+  return heads == 0 || ((uintptr_t)p % (uintptr_t)unit == 0 && stride * bytes % unit == 0 && head_stride * bytes % unit == 0);
+}
+
+TokenParams token_params(const RotaryArgs& a) {
+  TokenParams p{};
+  p.q = (const char*)a.q.p, p.q_stride = a.q.stride, p.q_head = a.q.head_stride, p.q_heads = a.q.heads;
+  p.k = (const char*)a.k.p, p.k_stride = a.k.stride, p.k_head = a.k.head_stride, p.k_heads = a.k.heads;
+  p.positions = a.positions, p.pos64 = a.pos64, p.cos = a.cos, p.sin = a.sin, p.n = a.n, p.table_rows = a.table_rows;
+  p.dim = a.dim, p.half = a.half, p.interleaved = a.interleaved, p.back = a.back;
+  return p;
+}
+
+// The widest chunks that the sizes, strides and addresses allow.
+int chunk_of(const TokenParams& p, int type) {
+  const int rest = p.dim - 2 * p.half;
+  for (int P : {8, 4}) {
+    if (p.half % P || rest % (2 * P)) continue;
+    const int b = kv_bytes(type);
+    if (rows_fit(p.q, p.q_stride, p.q_head, p.q_heads, P, b) && rows_fit(p.k, p.k_stride, p.k_head, p.k_heads, P, b) &&
+        rows_fit(p.v, p.v_stride, p.v_head, p.v_heads, P, b))
+      return P;
+  }
+  return 1;
+}
+
+}  // namespace
+
+void rotary(const RotaryArgs& a, void* q_out, void* k_out, hipStream_t s) {
+  TokenParams p = token_params(a);
+  p.q_out = (char*)q_out, p.k_out = (char*)k_out;
+  const int P = chunk_of(p, a.type);
+  if (a.type == kF16) launch_token<f16, f16, false>(p, P, s);
+  else launch_token<bf16, bf16, false>(p, P, s);
+}
+
+void append_tokens(const RotaryArgs& a, const HeadRows& v, const void* slots, bool slots64, const KvPages& pages,
+                   void* q_out, hipStream_t s) {
+  TokenParams p = token_params(a);
+  p.v = (const char*)v.p, p.v_stride = v.stride, p.v_head = v.head_stride, p.v_heads = v.heads;
+  p.slots = slots, p.slots64 = slots64, p.pages = pages, p.q_out = (char*)q_out;
+  p.rows = (int64_t)pages.pages * pages.page;
+  const int P = chunk_of(p, a.type);
+  if (pages.type == kE4M3) {
+    if (a.type == kF16) launch_token<f16, e4m3, true>(p, P, s);
+    else launch_token<bf16, e4m3, true>(p, P, s);
+  } else if (a.type == kF16) {
+    launch_token<f16, f16, true>(p, P, s);
+  } else {
+    launch_token<bf16, bf16, true>(p, P, s);
+  }
+}
+
+// ---- copying pages ----
+
+namespace {
+
+constexpr int kCopyThreads = 256, kCopyUnits = 4;  // 16-byte units a thread moves
+
+struct CopyParams {
+  char *k, *v;
+  int64_t layer_bytes, page_bytes, head_bytes, row_bytes;
+  int layers, pages, page;
+  uint32_t units, row_units;  // of a page, of a row
+  const int32_t *src, *dst;
+  int64_t n;
+  uint32_t parts;        // work-groups a page is cut into
+  int64_t copy_groups;   // of the grid; the rest rewrite table entries
+  int32_t* tables;
+  int64_t entries;
+};
+
+// A work-group moves 16 KB of one page of one layer's K or V: a thread's
+// four 16-byte loads go out before its stores. Further work-groups rewrite
+// the table entries, each comparing 256 of them with all sources.
+template <bool FLAT>
+__global__ __launch_bounds__(kCopyThreads) void copy_kernel(CopyParams a) {
+  if ((int64_t)blockIdx.x >= a.copy_groups) {
+    __shared__ int32_t from[1024], to[1024];
+    const int64_t e = ((int64_t)blockIdx.x - a.copy_groups) * kCopyThreads + threadIdx.x;
+    const int32_t old = e < a.entries ? a.tables[e] : -1;
+    int32_t now = old;
+    for (int64_t b = 0; b < a.n; b += 1024) {
+      const int m = (int)(a.n - b < 1024 ? a.n - b : 1024);
+      __syncthreads();
+      for (int j = threadIdx.x; j < m; j += kCopyThreads) {
+        const int32_t f = a.src[b + j], t = a.dst[b + j];
+        const bool fine = f >= 0 && f < a.pages && t >= 0 && t < a.pages;
+        from[j] = fine ? f : -1, to[j] = t;
+      }
+      __syncthreads();
+      if (old >= 0)
+        for (int j = 0; j < m; ++j) now = from[j] == old ? to[j] : now;
+    }
+    if (now != old) a.tables[e] = now;
+    return;
+  }
+  const uint32_t part = blockIdx.x % a.parts;
+  const int64_t rest = blockIdx.x / a.parts;
+  const int64_t i = rest % a.n, plane = rest / a.n;
+  const int32_t f = a.src[i], t = a.dst[i];
+  if (f < 0 || f >= a.pages || t < 0 || t >= a.pages) return;
+  char* base = (plane & 1 ? a.v : a.k) + (plane >> 1) * a.layer_bytes;
+  const char* from = base + f * a.page_bytes;
+  char* to = base + t * a.page_bytes;
+  uintx4 x[kCopyUnits];
+  int64_t off[kCopyUnits];
+#pragma unroll
+  for (int j = 0; j < kCopyUnits; ++j) {
+    const uint32_t u = (part * kCopyUnits + j) * kCopyThreads + threadIdx.x;
+    if (u >= a.units) {
+      off[j] = -1;
+      continue;
+    }
+    if (FLAT) {
+      off[j] = (int64_t)u * 16;
+    } else {
+      const uint32_t row = u / a.row_units;
+      off[j] = (int64_t)(row / a.page) * a.head_bytes + (int64_t)(row % a.page) * a.row_bytes +
+               (int64_t)(u % a.row_units) * 16;
+    }
+    x[j] = *(const uintx4*)(from + off[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kCopyUnits; ++j)
+    if (off[j] >= 0) *(uintx4*)(to + off[j]) = x[j];
+}
+
+}  // namespace
+
+void copy_pages(const KvPages& pages, const int32_t* src, const int32_t* dst, int64_t n, int32_t* tables,
+                int64_t table_entries, hipStream_t s) {
+  if (n == 0) return;
+  const int b = kv_bytes(pages.type);
+  CopyParams p{};
+  p.k = pages.k, p.v = pages.v;
+  p.layer_bytes = pages.layer_stride * b, p.page_bytes = pages.page_stride * b;
+  p.head_bytes = pages.head_stride * b, p.row_bytes = pages.row_stride * b;
+  p.layers = pages.layers, p.pages = pages.pages, p.page = pages.page;
+  p.row_units = (uint32_t)(pages.dim * b / 16);
+  const int64_t units = (int64_t)pages.heads * pages.page * p.row_units;
+  if (units > 0x7FFFFFFF - kCopyThreads * kCopyUnits) throw std::invalid_argument("a page is too large");
+  p.units = (uint32_t)units;
+  p.src = src, p.dst = dst, p.n = n;
+  p.parts = (uint32_t)((units + kCopyThreads * kCopyUnits - 1) / (kCopyThreads * kCopyUnits));
+  p.copy_groups = 2 * (int64_t)pages.layers * n * p.parts;
+  p.tables = tables, p.entries = tables ? table_entries : 0;
+  const int64_t groups = p.copy_groups + (p.entries + kCopyThreads - 1) / kCopyThreads;
+  if (groups > 0x7FFFFFFF) throw std::invalid_argument("too many pages in one call (too large)");
+  const bool flat = pages.row_stride == pages.dim && pages.head_stride == (int64_t)pages.page * pages.dim;
+  auto kernel = flat ? copy_kernel<true> : copy_kernel<false>;
+  kernel<<<(unsigned)groups, kCopyThreads, 0, s>>>(p);
+  hip_check(hipGetLastError(), "copy pages");
+}
+
+}  // namespace jasper_amd

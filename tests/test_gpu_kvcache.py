@@ -1,0 +1,675 @@
+"""GPU tests of the paged cache's operators against plain 64-bit ones.
+
+Tolerances come from the arithmetic, per output value:
+
+- rotary: two products and a sum in 32 bits (3 half-ulps of 2^-24 of the
+  products' sizes), then one rounding to the type: half the distance of
+  neighbours, u = 2^-(stored bits + 1) of the value (fp16 2^-11, bf16 2^-8,
+  e4m3 2^-4), or half the type's smallest step.
+- attention: a score is dim products summed in 32 bits in any order, error at
+  most (dim + 4) 2^-24 scale sum|q||k| plus 2^-22 of its distance from the
+  maximum (exponential); a weight is held in two terms of the type (error
+  below 2^-16), sums over T tokens add (T + 64) 2^-24. The weights' relative
+  error e counts twice (numerator, denominator):
+  |out error| <= u |out| + 2 e sum p|v|, |lse error| <= e + 2^-22 |lse|.
+"""
+
+import itertools
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F8 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
+UNIT = {F16: 2.0 ** -11, BF16: 2.0 ** -8, F8: 2.0 ** -4}
+STEP = {F16: 2.0 ** -25, BF16: 2.0 ** -134, F8: 2.0 ** -10}  # half the smallest step
+
+
+def randn(shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(shape, device="cuda", generator=g) * scale
+    return x.to(dtype)
+
+
+def raw(x):
+    return x.view(torch.uint8) if x.dtype == F8 else x
+
+
+def near(got, want, tol, what=""):
+    got, want, tol = got.double().cpu(), want.cpu(), tol.cpu()
+    assert got.shape == want.shape, what
+    assert torch.equal(torch.isfinite(got), torch.isfinite(want)), what
+    fine = torch.isfinite(want)
+    assert torch.equal(got[~fine & ~want.isnan()], want[~fine & ~want.isnan()]), what
+    off = (got - want)[fine].abs() - tol[fine]
+    assert off.numel() == 0 or off.max() <= 0, f"{what}: over the bound by {off.max().item():.3g}"
+
+
+# ---- rotary ----
+
+def ref_rotary(x, positions, cos, sin, interleaved, back=False):
+    """(value, size of the sums) in 64 bits on the CPU."""
+    x, positions = x.double().cpu(), positions.cpu().long()
+    c, s = cos.double().cpu()[positions][..., None, :], sin.double().cpu()[positions][..., None, :]
+    if back:
+        s = -s
+    rot = 2 * cos.size(1)
+    y, size = x.clone(), torch.zeros_like(x)
+    half = rot // 2
+    for i in range(half):
+        a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
+        ci, si = c[..., i], s[..., i]
+        y[..., a] = x[..., a] * ci - x[..., b] * si
+        y[..., b] = x[..., b] * ci + x[..., a] * si
+        size[..., a] = (x[..., a] * ci).abs() + (x[..., b] * si).abs()
+        size[..., b] = (x[..., b] * ci).abs() + (x[..., a] * si).abs()
+    return y, size
+
+
+def rotary_tol(want, size, dtype):
+    return UNIT[dtype] * 1.001 * want.abs() + 3 * 2.0 ** -24 * size + STEP[dtype]
+
+
+@pytest.mark.parametrize("n,hq,hk,dim,rot,interleaved,dtype", [
+    (1, 1, 1, 2, 2, False, F16), (1, 8, 2, 64, 64, True, BF16), (7, 3, 3, 80, 40, False, F16),
+    (5, 2, 1, 80, 80, True, BF16), (33, 12, 4, 96, 48, True, F16), (130, 32, 8, 128, 128, False, BF16),
+    (1500, 5, 5, 128, 64, False, F16), (2049, 4, 1, 256, 256, True, BF16), (1100, 2, 1, 10, 6, False, F16),
+    (3, 1, 0, 34, 34, False, BF16), (6, 64, 8, 256, 96, False, F16)])
+@pytest.mark.parametrize("idx", [torch.int32, torch.int64])
+def test_rotary_values(jasper, n, hq, hk, dim, rot, interleaved, dtype, idx):
+    cos, sin = jasper.rotary_table(5000, rot)
+    q = randn((n, hq, dim), dtype, 1)
+    k = randn((n, hk, dim), dtype, 2) if hk else None
+    pos = torch.randint(0, 5000, (n,), device="cuda", dtype=idx)
+    out = jasper.rotary(q, k, pos, cos, sin, interleaved=interleaved)
+    for x, y in ((q, out[0]), (k, out[1])):
+        if x is None:
+            assert y is None
+            continue
+        want, size = ref_rotary(x, pos, cos, sin, interleaved)
+        near(y, want, rotary_tol(want, size, dtype))
+        assert torch.equal(y[..., rot:], x[..., rot:])
+
+
+def test_rotary_shapes_strides_and_alignment(jasper):
+    cos, sin = jasper.rotary_table(64, 64)
+    pos = torch.arange(24, device="cuda").view(2, 12) * 2
+    fused = randn((2, 12, 6, 65), F16, 3)
+    q, k = fused[:, :, :4, 1:], fused[:, :, 4:, 1:]  # odd addresses and strides
+    a, b = jasper.rotary(q, k, pos, cos, sin)
+    c, d = jasper.rotary(q.contiguous(), k.contiguous(), pos, cos, sin)
+    assert torch.equal(a, c) and torch.equal(b, d) and a.shape == q.shape
+    t, _ = jasper.rotary(q.transpose(0, 1), None, pos.t(), cos, sin)
+    assert torch.equal(t, a.transpose(0, 1))
+    flipped = torch.stack([q[..., i] for i in range(64)], dim=0).permute(1, 2, 3, 0)  # values apart
+    assert torch.equal(jasper.rotary(flipped, None, pos, cos, sin)[0], a)
+    one, _ = jasper.rotary(q[0, 5], None, pos[0, 5], cos, sin)  # no leading size at all
+    assert torch.equal(one, a[0, 5])
+    none, _ = jasper.rotary(q[:0], None, pos[:0], cos, sin)
+    assert none.shape == (0, 12, 4, 64)
+
+
+def test_rotary_position_outside_the_tables(jasper):
+    cos, sin = jasper.rotary_table(10, 32)
+    q = randn((4, 2, 48), BF16, 4)
+    y, _ = jasper.rotary(q, None, torch.tensor([0, 10, -1, 9], device="cuda"), cos, sin)
+    assert y[1:3, :, :32].isnan().all() and y[[0, 3]].isfinite().all() and torch.equal(y[..., 32:], q[..., 32:])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rot,scaling", [(64, 64, None), (96, 48, "yarn"), (128, 128, "ntk"), (20, 12, "linear")])
+def test_rotary_gradient(jasper, dim, rot, scaling, interleaved):
+    cos, sin = jasper.rotary_table(300, rot, scaling=scaling, factor=4.0 if scaling else 1.0, original=64)
+    n = 37
+    pos = torch.randint(0, 300, (n,), device="cuda")
+    q = randn((n, 6, dim), F16, 5).requires_grad_()
+    k = randn((n, 2, dim), F16, 6).requires_grad_()
+    gq, gk = randn((n, 6, dim), F16, 7), randn((n, 2, dim), F16, 8)
+    out = jasper.rotary(q, k, pos, cos, sin, interleaved=interleaved)
+    dq, dk = torch.autograd.grad(out, (q, k), (gq, gk), retain_graph=True)
+    for g, d in ((gq, dq), (gk, dk)):
+        want, size = ref_rotary(g, pos, cos, sin, interleaved, back=True)
+        near(d, want, rotary_tol(want, size, F16))
+    # differences: the map is linear, so a step of any size is exact but for rounding
+    for at in range(0, dim, 5):
+        step = torch.zeros_like(q)
+        step[..., at] = 1.0
+        up, _ = jasper.rotary((q + step).detach(), None, pos, cos, sin, interleaved=interleaved)
+        dn, _ = jasper.rotary((q - step).detach(), None, pos, cos, sin, interleaved=interleaved)
+        slope = ((up.double() - dn.double()) / 2 * gq.double()).sum(-1)
+        # q +- 1 and the outputs are each rounded to fp16 (values below 8): 2^-8 each, over up to dim terms of |g|
+        tol = 4 * 2.0 ** -8 * gq.double().abs().sum(-1)
+        near(dq[..., at], slope.cpu(), tol)
+    only, = torch.autograd.grad(out, (k,), (gq, gk))
+    assert torch.equal(only, dk)
+    again, _ = jasper.rotary(q, None, pos, cos, sin, interleaved=interleaved)
+    assert torch.equal(torch.autograd.grad(again, q, gq)[0], dq)
+
+
+# ---- appending ----
+
+def make_pages(pages, heads, page, dim, cache, seed=None, layout="heads"):
+    """A pair of page tensors; layout rows: [n, page, heads, dim] seen with the heads first; pair: K beside V."""
+    if layout == "rows":
+        shape = (pages, page, heads, dim)
+    elif layout == "pair":
+        shape = (pages, 2, heads, page, dim)
+    else:
+        shape = (pages, heads, page, dim)
+    scale = 32.0 if cache == F8 else 1.0
+    out = []
+    for i in range(1 if layout == "pair" else 2):
+        out.append(torch.zeros(shape, dtype=cache, device="cuda") if seed is None
+                   else randn(shape, cache, seed + i, scale))
+    if layout == "rows":
+        return [x.transpose(1, 2) for x in out]
+    return [out[0][:, 0], out[0][:, 1]] if layout == "pair" else out
+
+
+@pytest.mark.parametrize("n,hq,heads,dim,rot,interleaved,dtype,cache,page,layout", [
+    (1, 8, 2, 64, 64, False, F16, F16, 8, "heads"), (1, 32, 8, 128, 128, False, BF16, BF16, 16, "rows"),
+    (45, 5, 5, 80, 40, True, F16, F16, 16, "pair"), (300, 16, 2, 128, 64, False, BF16, F8, 32, "heads"),
+    (2000, 4, 4, 96, 96, True, F16, F8, 64, "rows"), (70, 2, 1, 256, 256, False, F16, F16, 256, "heads"),
+    (33, 0, 3, 128, 0, False, BF16, BF16, 16, "heads"), (19, 1, 1, 8, 6, False, F16, F16, 8, "heads"),
+    (1030, 10, 10, 64, 62, False, BF16, F8, 16, "heads")])
+def test_append_tokens(jasper, n, hq, heads, dim, rot, interleaved, dtype, cache, page, layout):
+    pages = -(-n // page) + 3
+    kp, vp = make_pages(pages, heads, page, dim, cache, layout=layout)
+    qkv = randn((n, hq + 2 * heads, dim), dtype, 11)
+    q, k, v = qkv.split([hq, heads, heads], dim=1)
+    cos, sin = jasper.rotary_table(4096, rot) if rot else (None, None)
+    pos = torch.randint(0, 4096, (n,), device="cuda") if rot else None
+    slots = torch.randperm(pages * page, device="cuda")[:n]
+    skipped = torch.zeros(n, dtype=torch.bool)
+    if n > 10:
+        slots[3], slots[7], slots[9] = -1, pages * page, -2 ** 40
+        skipped[[3, 7, 9]] = True
+    ks = vs = None
+    if cache == F8:
+        ks, vs = torch.rand(heads, device="cuda") * 0.01 + 0.004, torch.rand(heads, device="cuda") * 0.02 + 0.02
+        ks[0] = 0.001  # values over 448 scales saturate
+    out = jasper.append_tokens(q if hq else None, k, v, pos, slots, cos, sin, kp, vp, interleaved=interleaved,
+                               k_scale=ks, v_scale=vs)
+    if hq:
+        want, size = ref_rotary(q, pos, cos, sin, interleaved) if rot else (q.double().cpu(), torch.zeros(1))
+        near(out, want, rotary_tol(want, size, dtype))
+    else:
+        assert out is None
+    kept = (~skipped).nonzero()[:, 0]
+    at = slots.cpu()[kept]
+    for store, x, scale, turned in ((kp, k, ks, bool(rot)), (vp, v, vs, False)):
+        want, size = ref_rotary(x, pos, cos, sin, interleaved) if turned else (x.double().cpu(), torch.zeros(x.shape))
+        if scale is not None:
+            f = scale.double().cpu()[None, :, None]
+            want, size = (want / f).clamp(-448, 448), size / f
+            size = size + want.abs()  # the division rounds too
+        tol = rotary_tol(want, size, cache)
+        full = torch.zeros((pages, page, heads, dim), dtype=torch.float64)
+        bound = torch.zeros_like(full)
+        full[at // page, at % page] = want.expand(x.shape)[kept]
+        bound[at // page, at % page] = tol.expand(x.shape)[kept]
+        near(store.float().transpose(1, 2), full, bound)  # every other row is still zero
+
+
+def test_append_e4m3_rounds_like_torch(jasper):
+    """Every fp16 value, through an e4m3 cache without a scale."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).cuda().view(F16)
+    k = bits.view(256, 1, 256)
+    kp, vp = make_pages(32, 1, 8, 256, F8)
+    jasper.append_tokens(None, k, k, None, torch.arange(256, device="cuda"), None, None, kp, vp)
+    want = k.float().clamp(-448, 448).to(F8).float().view(-1)
+    for store in (kp, vp):
+        got = store.float().view(-1)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got[~got.isnan()], want[~got.isnan()])
+
+
+# ---- pages ----
+
+@pytest.mark.parametrize("cache", [F16, F8])
+@pytest.mark.parametrize("layers,heads,page,dim,layout", [
+    (1, 1, 8, 16, "heads"), (3, 2, 16, 80, "heads"), (2, 8, 16, 128, "rows"), (1, 5, 32, 96, "pair"), (32, 4, 64, 64, "heads")])
+def test_copy_pages(jasper, cache, layers, heads, page, dim, layout):
+    pages = 40
+    pair = [make_pages(pages, heads, page, dim, cache, seed=20 + 2 * i, layout=layout) for i in range(layers)]
+    if layout == "pair" or layers == 1:
+        kp, vp = pair[0]
+    else:
+        kp, vp = (torch.stack([x[j] for x in pair]) for j in range(2))
+        if layout == "rows":
+            kp, vp = (x.transpose(2, 3).contiguous().transpose(2, 3) for x in (kp, vp))
+    src = torch.tensor([3, 7, 3, 39, 50, 0, -1], dtype=torch.int32, device="cuda")
+    dst = torch.tensor([4, 0, 9, 38, 1, -1, 2], dtype=torch.int32, device="cuda")
+    want = []
+    for x in (kp, vp):
+        w = raw(x).clone()
+        dim_of = x.ndim - 4
+        for s, d in ((3, 4), (7, 0), (3, 9), (39, 38)):
+            w.select(dim_of, d).copy_(raw(x).select(dim_of, s))
+        want.append(w)
+    jasper.copy_pages(kp, vp, src, dst)
+    assert torch.equal(raw(kp), want[0]) and torch.equal(raw(vp), want[1])
+    jasper.copy_pages(kp, vp, src[:0], dst[:0])
+    assert torch.equal(raw(kp), want[0])
+
+
+@pytest.mark.parametrize("moves,sequences,width", [(1, 1, 1), (513, 5, 77), (1025, 64, 130), (2500, 300, 33)])
+def test_copy_pages_moves_tables(jasper, moves, sequences, width):
+    pages = 2 * moves + 100
+    kp, vp = make_pages(pages, 1, 8, 16, F16, seed=30)
+    before = kp.clone()
+    order = torch.randperm(pages)
+    src, dst = order[:moves].int(), order[moves:2 * moves].int()
+    owned = torch.cat([order[:moves], order[2 * moves:]])
+    tables = owned[torch.randint(0, owned.numel(), (sequences, width))].int()
+    tables[torch.rand(tables.shape) < 0.2] = -1
+    to = torch.arange(pages).int()
+    to[src.long()] = dst
+    want = torch.where(tables < 0, tables, to[tables.clamp(min=0).long()])
+    got = tables.cuda()
+    jasper.copy_pages(kp, vp, src.cuda(), dst.cuda(), tables=got)
+    assert torch.equal(got.cpu(), want)
+    assert torch.equal(kp[dst.long().cuda()], before[src.long().cuda()])
+
+
+# ---- attention ----
+
+def build_cache(lens, heads, page, dim, cache, seed, layout="heads", spare=3, hostile=True):
+    """(k_pages, v_pages, tables, keys, values): pages in random order, and whatever no sequence owns is NaN or
+    infinite; table entries past a sequence's pages are wild."""
+    count = [-(-max(0, n) // page) for n in lens]
+    pages = sum(count) + spare
+    kp, vp = make_pages(pages, heads, page, dim, cache, seed=seed, layout=layout)
+    g = torch.Generator().manual_seed(seed)
+    order = torch.randperm(pages, generator=g)
+    tables = torch.randint(-5, 10 ** 6, (len(lens), max(count) + 2), dtype=torch.int32, generator=g)
+    if hostile:
+        tables[:, -1] = -2 ** 31
+    owned = torch.zeros((pages, page), dtype=torch.bool)
+    at, keys, values = 0, [], []
+    for i, (n, c) in enumerate(zip(lens, count)):
+        mine = order[at:at + c]
+        at += c
+        tables[i, :c] = mine.int()
+        rows = torch.arange(max(0, n))
+        owned[mine[rows // page], rows % page] = True
+        keys.append(kp.float()[mine.cuda()].transpose(0, 1).reshape(heads, c * page, dim)[:, :max(0, n)].double().cpu())
+        values.append(vp.float()[mine.cuda()].transpose(0, 1).reshape(heads, c * page, dim)[:, :max(0, n)].double().cpu())
+    if hostile:
+        free = (~owned).cuda()
+        for x in (kp, vp):
+            view = raw(x).transpose(1, 2)  # [pages, page, heads, dim]
+            junk = 0x7F if cache == F8 else float("nan")
+            view[free] = junk
+            if cache != F8:
+                view[free & (torch.arange(page, device="cuda") % 2 == 0)] = float("inf")
+    return kp, vp, tables.cuda(), keys, values
+
+
+def ref_attention(q, keys, values, scale, choose, dtype, k_scale=None, v_scale=None, lists=None):
+    """Per sequence and list of query heads, in 64 bits: (out, its bound, lse, its bound)."""
+    b, hq, dim = q.shape
+    heads = keys[0].size(0)
+    lists = lists or heads
+    out, tol = torch.zeros((b, hq, dim), dtype=torch.float64), torch.zeros((b, hq, dim), dtype=torch.float64)
+    lse, ltol = torch.full((b, hq), -math.inf, dtype=torch.float64), torch.zeros((b, hq), dtype=torch.float64)
+    qd = q.double().cpu()
+    for i, j in itertools.product(range(b), range(lists)):
+        h, g = j * heads // lists, hq // lists
+        at = choose(i, j)
+        mine = slice(j * g, j * g + g)
+        tol[i, mine] = STEP[dtype]
+        if len(at) == 0:
+            continue
+        k, v = keys[i][h][at], values[i][h][at]
+        if k_scale is not None:
+            k, v = k * k_scale[h].double().cpu(), v * v_scale[h].double().cpu()
+        s = qd[i, mine] @ k.T * scale
+        size = (qd[i, mine].abs() @ k.abs().T * abs(scale)).amax(1, keepdim=True)
+        p = torch.softmax(s, dim=1)
+        out[i, mine] = p @ v
+        lse[i, mine] = torch.logsumexp(s, dim=1)
+        away = (s.amax(1, keepdim=True) - s).amax(1, keepdim=True).clamp(max=100)
+        e = (dim + 4) * 2.0 ** -24 * size + 2.0 ** -22 * away + 2.0 ** -16 + (len(at) + 64) * 2.0 ** -24
+        tol[i, mine] += UNIT[dtype] * 1.001 * out[i, mine].abs() + 2 * e * (p @ v.abs())
+        ltol[i, mine] = (e + 2.0 ** -22 * lse[i, mine][:, None].abs())[:, 0]
+    return out, tol, lse, ltol
+
+
+EDGES = [0, 1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 511, 513, 1000, 2047, 2500]
+
+
+def check(got, ref):
+    near(got[0], ref[0], ref[1], "out")
+    near(got[1], ref[2], ref[3], "lse")
+
+
+def f8_scales(heads, cache, seed):
+    if cache != F8:
+        return None, None
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.rand(heads, device="cuda", generator=g) * 0.02 + 0.02,
+            torch.rand(heads, device="cuda", generator=g) * 0.02 + 0.02)
+
+
+@pytest.mark.parametrize("hq,heads,dim,page,dtype,cache,layout", [
+    (8, 2, 128, 16, F16, F16, "heads"), (32, 8, 128, 16, BF16, BF16, "rows"), (5, 5, 64, 32, F16, F16, "pair"),
+    (16, 1, 96, 8, BF16, BF16, "heads"), (17, 1, 128, 16, F16, F16, "heads"), (64, 2, 128, 64, BF16, F8, "heads"),
+    (3, 3, 80, 16, F16, F8, "rows"), (12, 4, 256, 16, F16, F16, "heads"), (40, 1, 256, 8, BF16, BF16, "heads"),
+    (2, 1, 8, 128, F16, F16, "heads"), (6, 2, 200, 256, BF16, BF16, "heads"), (4, 2, 256, 32, F16, F8, "heads"),
+    (2, 2, 16, 8, BF16, F8, "heads"), (7, 7, 72, 16, F16, F16, "heads")])
+def test_decode_lengths(jasper, hq, heads, dim, page, dtype, cache, layout):
+    kp, vp, tables, keys, values = build_cache(EDGES, heads, page, dim, cache, 40, layout)
+    ks, vs = f8_scales(heads, cache, 41)
+    q = randn((len(EDGES), hq, dim), dtype, 42, 2.0)
+    lens = torch.tensor(EDGES, dtype=torch.int32, device="cuda")
+    ref = ref_attention(q, keys, values, dim ** -0.5, lambda i, j: torch.arange(EDGES[i]), dtype, ks, vs)
+    check(jasper.decode_attention(q, kp, vp, tables, lens, k_scale=ks, v_scale=vs, return_lse=True), ref)
+    out = jasper.decode_attention(q, kp, vp, tables, lens, k_scale=ks, v_scale=vs, max_len=2500)
+    near(out, ref[0], ref[1])
+
+
+@pytest.mark.parametrize("window", [1, 5, 16, 33, 100, 1000, 10 ** 9])
+@pytest.mark.parametrize("cache,page", [(F16, 16), (F8, 8)])
+def test_decode_window(jasper, window, cache, page):
+    kp, vp, tables, keys, values = build_cache(EDGES, 2, page, 64, cache, 50)
+    ks, vs = f8_scales(2, cache, 51)
+    q = randn((len(EDGES), 6, 64), F16, 52, 2.0)
+    lens = torch.tensor(EDGES, dtype=torch.int32, device="cuda")
+    ref = ref_attention(q, keys, values, 0.3, lambda i, j: torch.arange(max(0, EDGES[i] - window), EDGES[i]), F16, ks, vs)
+    check(jasper.decode_attention(q, kp, vp, tables, lens, scale=0.3, window=window, k_scale=ks, v_scale=vs,
+                                  return_lse=True), ref)
+
+
+@pytest.mark.parametrize("batch,length,hq,heads,cache", [(1, 70_001, 8, 1, F16), (1, 33_333, 4, 2, F8), (2, 20_000, 2, 2, F16)])
+def test_decode_long(jasper, batch, length, hq, heads, cache):
+    lens = [length - 5 * i for i in range(batch)]
+    kp, vp, tables, keys, values = build_cache(lens, heads, 16, 128, cache, 60)
+    ks, vs = f8_scales(heads, cache, 61)
+    q = randn((batch, hq, 128), F16, 62, 3.0)
+    ref = ref_attention(q, keys, values, 128 ** -0.5, lambda i, j: torch.arange(lens[i]), F16, ks, vs)
+    check(jasper.decode_attention(q, kp, vp, tables, torch.tensor(lens, dtype=torch.int32, device="cuda"), k_scale=ks,
+                                  v_scale=vs, return_lse=True), ref)
+
+
+def test_decode_large_scores_and_infinities(jasper):
+    """Scores in the hundreds, of one sign; keys of minus infinity weigh nothing, NaN in a read row is seen."""
+    lens = [300, 300, 40, 5]
+    kp, vp, tables, keys, values = build_cache(lens, 1, 16, 64, BF16, 70, hostile=False)
+    q = randn((4, 2, 64), BF16, 71, 40.0)
+    tens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ref = ref_attention(q, keys, values, 1.0, lambda i, j: torch.arange(lens[i]), BF16)
+    check(jasper.decode_attention(q, kp, vp, tables, tens, scale=1.0, return_lse=True), ref)
+    q = q.abs().contiguous()
+    for x, t in ((3, 10), (2, 7), (2, 39)):
+        page = tables[x, t // 16].item() if t < lens[x] else None
+        if page is not None:
+            kp[page, 0, t % 16] = -math.inf
+            keys[x][0][t] = -math.inf
+    for t in range(5):
+        kp[tables[3, 0].item(), 0, t] = -math.inf
+    bad = tables[1, 2].item()
+    vp[bad, 0, 3, 9] = math.nan
+    kp[tables[0, 1].item(), 0, 3, 9] = math.nan
+    out, lse = jasper.decode_attention(q, kp, vp, tables, tens, scale=1.0, return_lse=True)
+    ref = ref_attention(q, keys, values, 1.0, lambda i, j: torch.arange(lens[i]) if i != 2 else
+                        torch.tensor([t for t in range(40) if t not in (7, 39)]), BF16)
+    near(out[2:3], ref[0][2:3], ref[1][2:3])
+    assert (out[3] == 0).all() and (lse[3] == -math.inf).all()
+    assert out[1, :, 9].isnan().all() and out[1, :, :9].isfinite().all()
+    assert out[0].isnan().all() and lse[0].isnan().all()
+
+
+def test_decode_pages_outside_and_query_strides(jasper):
+    lens = [100, 64]
+    kp, vp, tables, keys, values = build_cache(lens, 2, 16, 64, F16, 80)
+    tables[0, 2], tables[1, 0] = -7, kp.size(0)  # lost pages: their tokens are left out
+    fused = randn((2, 9, 64), F16, 81, 2.0)
+    q = fused[:, 2:6]
+    tens = torch.tensor([100, 0, 64, 0], dtype=torch.int32, device="cuda")[::2]
+    ref = ref_attention(q, keys, values, 0.125, lambda i, j: torch.cat([torch.arange(32), torch.arange(48, 100)]) if i == 0
+                        else torch.arange(16, 64), F16)
+    check(jasper.decode_attention(q, kp, vp, tables, tens, return_lse=True), ref)
+    odd = torch.empty(2 * 4 * 64 + 1, dtype=F16, device="cuda")[1:].view(2, 4, 64).copy_(q)
+    check(jasper.decode_attention(odd, kp, vp, tables, tens, return_lse=True), ref)
+    wide = torch.empty((2, 64, 4), dtype=F16, device="cuda").transpose(1, 2).copy_(q)
+    check(jasper.decode_attention(wide, kp, vp, tables, tens, return_lse=True), ref)
+    # lengths over what the table holds, and below zero
+    out, lse = jasper.decode_attention(q, kp, vp, tables[:, :4].contiguous(),
+                                       torch.tensor([1000, -3], dtype=torch.int32, device="cuda"), return_lse=True)
+    cut = ref_attention(q, keys, values, 0.125, lambda i, j: torch.cat([torch.arange(32), torch.arange(48, 64)]), F16)
+    near(out[:1], cut[0][:1], cut[1][:1])
+    assert (out[1] == 0).all() and (lse[1] == -math.inf).all()
+
+
+def test_offsets_past_32_bits(jasper):
+    """More than 2^32 bytes of keys: rows at the far end are the ones read, written and copied."""
+    heads, page, dim = 8, 64, 128
+    pages = 2 ** 32 // (heads * page * dim * 2) + 70
+    kp = torch.zeros((pages, heads, page, dim), dtype=F16, device="cuda")
+    vp = torch.zeros_like(kp)
+    n = 150
+    k, v = randn((n, heads, dim), F16, 90), randn((n, heads, dim), F16, 91)
+    table = torch.tensor([[pages - 1, 0, pages - 40]], dtype=torch.int32, device="cuda")
+    at = torch.arange(n, device="cuda")
+    slots = table[0, at // page].long() * page + at % page
+    jasper.append_tokens(None, k, v, None, slots, None, None, kp, vp)
+    q = randn((1, 16, dim), F16, 92, 2.0)
+    keys, values = [k.double().cpu().transpose(0, 1)], [v.double().cpu().transpose(0, 1)]
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    ref = ref_attention(q, keys, values, dim ** -0.5, lambda i, j: torch.arange(n), F16)
+    check(jasper.decode_attention(q, kp, vp, table, lens, return_lse=True), ref)
+    ids = torch.randperm(n)[:77].int()
+    some = ref_attention(q, keys, values, dim ** -0.5, lambda i, j: ids.long(), F16)
+    listed = ids.cuda().expand(1, heads, 77).contiguous()
+    check(jasper.retrieved_attention(q, kp, vp, table, lens, listed, return_lse=True), some)
+    moved = torch.tensor([pages - 1, pages - 40], dtype=torch.int32, device="cuda")
+    to = torch.tensor([pages - 2, pages - 3], dtype=torch.int32, device="cuda")
+    jasper.copy_pages(kp, vp, moved, to, tables=table)
+    assert table.tolist() == [[pages - 2, 0, pages - 3]]
+    kp[pages - 1], kp[pages - 40] = 0, 0
+    check(jasper.decode_attention(q, kp, vp, table, lens, return_lse=True), ref)
+
+
+@pytest.mark.parametrize("hq,heads,lists,dim,page,dtype,cache,count,first,last,layout", [
+    (8, 2, 2, 128, 16, F16, F16, 100, 4, 20, "heads"), (8, 2, 8, 128, 16, BF16, BF16, 33, 0, 0, "rows"),
+    (32, 8, 32, 128, 16, F16, F16, 128, 4, 64, "heads"), (4, 4, 4, 64, 32, BF16, F8, 300, 16, 256, "heads"),
+    (24, 1, 1, 96, 8, F16, F16, 1, 1, 1, "pair"), (24, 1, 24, 80, 16, F16, F8, 7, 3, 0, "heads"),
+    (6, 3, 3, 256, 16, BF16, BF16, 500, 0, 33, "heads"), (2, 1, 2, 8, 8, F16, F16, 50, 2, 2, "heads"),
+    (16, 2, 2, 128, 16, F16, F16, 0, 5, 40, "heads"), (4, 2, 4, 256, 64, F16, F8, 64, 0, 7, "heads"),
+    (4, 1, 1, 128, 16, F16, F16, 3000, 300, 700, "heads")])
+def test_retrieved(jasper, hq, heads, lists, dim, page, dtype, cache, count, first, last, layout):
+    lens = [0, 1, 5, 33, 64, 129, 700, 2500]
+    kp, vp, tables, keys, values = build_cache(lens, heads, page, dim, cache, 100, layout)
+    ks, vs = f8_scales(heads, cache, 101)
+    q = randn((len(lens), hq, dim), dtype, 102, 2.0)
+    g = torch.Generator().manual_seed(103)
+    ids = torch.empty((len(lens), lists, count), dtype=torch.int32)
+    for i, n in enumerate(lens):  # in order of no kind, some twice, some missing, some past the end
+        ids[i] = torch.randint(0, max(1, n), (lists, count), generator=g, dtype=torch.int32)
+    ids[torch.rand(ids.shape, generator=g) < 0.1] = -1
+    ids[torch.rand(ids.shape, generator=g) < 0.05] = 2 ** 31 - 1
+    ids[torch.rand(ids.shape, generator=g) < 0.05] = -2 ** 31
+    ids[6] = -1  # a search that found nothing
+
+    def choose(i, j):
+        n = lens[i]
+        a, z = min(first, n), max(n - last, min(first, n))
+        mine = ids[i, j].long()
+        return torch.cat([torch.arange(a), torch.arange(z, n), mine[(mine >= a) & (mine < z)]])
+
+    ref = ref_attention(q, keys, values, dim ** -0.5, choose, dtype, ks, vs, lists)
+    tens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    check(jasper.retrieved_attention(q, kp, vp, tables, tens, ids.cuda(), first=first, last=last, k_scale=ks,
+                                     v_scale=vs, return_lse=True), ref)
+    strided = ids.cuda().transpose(1, 2).contiguous().transpose(1, 2)
+    out = jasper.retrieved_attention(q, kp, vp, tables, tens, strided, first=first, last=last, k_scale=ks, v_scale=vs)
+    near(out, ref[0], ref[1])
+
+
+def test_retrieved_everything_is_decode(jasper):
+    lens = [777, 50]
+    kp, vp, tables, keys, values = build_cache(lens, 2, 16, 128, F16, 110)
+    q = randn((2, 8, 128), F16, 111, 2.0)
+    tens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ids = torch.randperm(777).int().cuda().expand(2, 2, 777).contiguous()
+    ref = ref_attention(q, keys, values, 128 ** -0.5, lambda i, j: torch.arange(lens[i]), F16)
+    check(jasper.retrieved_attention(q, kp, vp, tables, tens, ids, first=3, last=9, return_lse=True), ref)
+    check(jasper.decode_attention(q, kp, vp, tables, tens, return_lse=True), ref)
+
+
+def test_many_sequences(jasper):
+    g = torch.Generator().manual_seed(120)
+    lens = torch.randint(0, 60, (700,), generator=g).tolist()
+    kp, vp, tables, keys, values = build_cache(lens, 1, 8, 64, F16, 121)
+    q = randn((700, 2, 64), F16, 122, 2.0)
+    ref = ref_attention(q, keys, values, 0.125, lambda i, j: torch.arange(lens[i]), F16)
+    check(jasper.decode_attention(q, kp, vp, tables, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                                  return_lse=True), ref)
+
+
+def test_repeats_and_streams_give_the_same_bits(jasper):
+    lens = [5000, 3, 900]
+    kp, vp, tables, _, _ = build_cache(lens, 2, 16, 128, BF16, 130)
+    q = randn((3, 8, 128), BF16, 131, 2.0)
+    tens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ids = torch.randint(0, 3, (3, 2, 100), dtype=torch.int32, device="cuda")
+
+    def both():
+        return (*jasper.decode_attention(q, kp, vp, tables, tens, return_lse=True),
+                *jasper.retrieved_attention(q, kp, vp, tables, tens, ids, first=4, last=200, return_lse=True))
+
+    want = both()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            got = both()
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_graph_capture(jasper):
+    """A serving step's calls in a graph, replayed on changed inputs with eager work in between."""
+    heads, hq, dim, page, b = 2, 8, 128, 16, 3
+    kp, vp = make_pages(3 * 40, heads, page, dim, F16)
+    tables = torch.randperm(120).int().view(3, 40).cuda()
+    cos, sin = jasper.rotary_table(700, dim)
+    qkv = randn((b, hq + 2 * heads, dim), F16, 140)
+    lens = torch.tensor([600, 17, 0], dtype=torch.int32, device="cuda")
+    pos, slots = torch.zeros(b, dtype=torch.int64, device="cuda"), torch.zeros(b, dtype=torch.int64, device="cuda")
+    ids = torch.zeros((b, heads, 50), dtype=torch.int32, device="cuda")
+    src, dst = torch.tensor([5], dtype=torch.int32, device="cuda"), torch.tensor([-1], dtype=torch.int32, device="cuda")
+
+    def step():
+        q, k, v = qkv.split([hq, heads, heads], dim=1)
+        q = jasper.append_tokens(q, k, v, pos, slots, cos, sin, kp, vp)
+        jasper.copy_pages(kp, vp, src, dst)
+        return (q, *jasper.decode_attention(q, kp, vp, tables, lens, return_lse=True),
+                *jasper.retrieved_attention(q, kp, vp, tables, lens, ids, first=2, last=9, return_lse=True))
+
+    kp.copy_(randn(kp.shape, F16, 141))
+    vp.copy_(randn(vp.shape, F16, 142))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        lens += 1
+        pos.copy_(lens.long() - 1)
+        slots.copy_(tables.gather(1, (pos // page)[:, None])[:, 0].long() * page + pos % page)
+        qkv.copy_(randn(qkv.shape, F16, 150 + i))
+        ids.copy_(torch.randint(0, 600, ids.shape, dtype=torch.int32, device="cuda"))
+        before = kp.clone(), vp.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in out] + [kp.clone(), vp.clone()]
+        kp.copy_(before[0])
+        vp.copy_(before[1])
+        want = [*step(), kp, vp]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+# ---- refusals ----
+
+def test_refusals(jasper):
+    kp, vp = make_pages(8, 2, 16, 64, F16, seed=160)
+    q = randn((2, 4, 64), F16, 161)
+    tables = torch.zeros((2, 4), dtype=torch.int32, device="cuda")
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    ids = torch.zeros((2, 2, 5), dtype=torch.int32, device="cuda")
+    scale = torch.ones(2, device="cuda")
+    dec, ret = jasper.decode_attention, jasper.retrieved_attention
+    bad = [
+        lambda: dec(q.float(), kp, vp, tables, lens), lambda: dec(q.bfloat16(), kp, vp, tables, lens),
+        lambda: dec(q[:, :3], kp, vp, tables, lens), lambda: dec(q[..., :32], kp, vp, tables, lens),
+        lambda: dec(q.cpu(), kp, vp, tables, lens), lambda: dec(q, kp.cpu(), vp.cpu(), tables, lens),
+        lambda: dec(q, kp, vp[:4], tables, lens), lambda: dec(q, kp, vp.bfloat16(), tables, lens),
+        lambda: dec(q, kp, vp, tables.long(), lens), lambda: dec(q, kp, vp, tables[:1], lens),
+        lambda: dec(q, kp, vp, tables, lens.long()), lambda: dec(q, kp, vp, tables, lens[:1]),
+        lambda: dec(q, kp, vp, tables, lens, window=-1), lambda: dec(q, kp, vp, tables, lens, max_len=-1),
+        lambda: dec(q, kp, vp, tables, lens, k_scale=scale), lambda: dec(q, kp[:, :, :12], vp[:, :, :12], tables, lens),
+        lambda: dec(q, kp[0], vp[0], tables, lens), lambda: dec(q, kp.float(), vp.float(), tables, lens),
+        lambda: dec(q.detach().requires_grad_(), kp, vp, tables, lens),
+        lambda: dec(q, kp, vp, tables.t(), lens[:1].expand(4)),
+        lambda: dec(q, kp, vp.transpose(1, 2).contiguous().transpose(1, 2), tables, lens),
+        lambda: dec(q[..., :60], kp[..., :60], vp[..., :60], tables, lens),
+        lambda: dec(q[..., :56], kp[..., 4:60], vp[..., 4:60], tables, lens),
+        lambda: ret(q, kp, vp, tables, lens, ids.long()), lambda: ret(q, kp, vp, tables, lens, ids[:, :1]),
+        lambda: ret(q, kp, vp, tables, lens, ids[:1]), lambda: ret(q, kp, vp, tables, lens, ids, first=-1),
+        lambda: ret(q, kp, vp, tables, lens, ids, last=2 ** 30),
+        lambda: jasper.copy_pages(kp, vp, lens, lens[:1]), lambda: jasper.copy_pages(kp, vp, lens.long(), lens.long()),
+        lambda: jasper.copy_pages(kp, vp, lens, lens, tables=tables.long()),
+        lambda: jasper.copy_pages(kp, vp, lens, lens, tables=tables.t()),
+        lambda: jasper.copy_pages(kp.cpu(), vp.cpu(), lens.cpu(), lens.cpu()),
+    ]
+    cos, sin = jasper.rotary_table(16, 64)
+    pos = torch.zeros(2, dtype=torch.int64, device="cuda")
+    k = q[:, :2]
+    bad += [
+        lambda: jasper.rotary(q.float(), None, pos, cos, sin), lambda: jasper.rotary(q, k.bfloat16(), pos, cos, sin),
+        lambda: jasper.rotary(q, None, pos[:1], cos, sin), lambda: jasper.rotary(q, None, pos.float(), cos, sin),
+        lambda: jasper.rotary(q[..., :62], None, pos, cos, sin), lambda: jasper.rotary(q, None, pos, cos, None),
+        lambda: jasper.rotary(q, None, pos, cos.half(), sin.half()), lambda: jasper.rotary(q, None, pos, cos, sin[:5]),
+        lambda: jasper.rotary(q, None, pos.cpu(), cos, sin), lambda: jasper.rotary(q[..., :63], None, pos, cos, sin),
+        lambda: jasper.append_tokens(q, k, k, pos, pos, cos, sin, kp.bfloat16(), vp.bfloat16()),
+        lambda: jasper.append_tokens(q, q, q, pos, pos, cos, sin, kp, vp),
+        lambda: jasper.append_tokens(q, k, k[:1], pos, pos, cos, sin, kp, vp),
+        lambda: jasper.append_tokens(q, k, k, None, pos, cos, sin, kp, vp),
+        lambda: jasper.append_tokens(q, k, k, pos, pos[:1], cos, sin, kp, vp),
+        lambda: jasper.append_tokens(q, k, k, pos, pos.float(), cos, sin, kp, vp),
+        lambda: jasper.append_tokens(q, k, k, pos, pos, cos, sin, kp, vp, k_scale=scale),
+        lambda: jasper.append_tokens(q.detach().requires_grad_(), k, k, pos, pos, cos, sin, kp, vp),
+        lambda: jasper.rotary_table(4, 3), lambda: jasper.rotary_table(4, 4, scaling="other"),
+        lambda: jasper.rotary_table(4, 4, scaling="yarn", factor=2.0),
+        lambda: jasper.rotary_table(4, 4, scaling="linear", factor=0.5),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"call {i} was accepted")
+    torch.cuda.synchronize()
+
+
+def test_empty_calls(jasper):
+    kp, vp = make_pages(8, 2, 16, 64, F16, seed=170)
+    tables = torch.zeros((0, 4), dtype=torch.int32, device="cuda")
+    lens = torch.zeros(0, dtype=torch.int32, device="cuda")
+    out, lse = jasper.decode_attention(randn((0, 4, 64), F16, 1), kp, vp, tables, lens, return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    ids = torch.zeros((0, 2, 5), dtype=torch.int32, device="cuda")
+    assert jasper.retrieved_attention(randn((0, 4, 64), F16, 1), kp, vp, tables, lens, ids).shape == (0, 4, 64)
+    none = torch.zeros((2, 0), dtype=torch.int32, device="cuda")
+    out, lse = jasper.decode_attention(randn((2, 4, 64), F16, 1), kp, vp, none,
+                                       torch.tensor([3, 0], dtype=torch.int32, device="cuda"), return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    empty, _ = make_pages(0, 2, 16, 64, F16)
+    out = jasper.decode_attention(randn((1, 4, 64), F16, 1), empty, empty, torch.zeros((1, 4), dtype=torch.int32, device="cuda"),
+                                  torch.tensor([9], dtype=torch.int32, device="cuda"))
+    assert (out == 0).all()
