@@ -8,87 +8,580 @@
 
 #include <algorithm>
 #include <stdexcept>
+#include <type_traits>
 
 namespace jasper_amd {
 
 namespace {
 
-constexpr int kMaxDim = 256;
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kTile = 32;                // tokens a wave takes at once
+constexpr int kUnit = kTile * kWaves;    // tokens a work-group takes at once
+constexpr int kStage = 2048;             // row offsets held in LDS
+constexpr int kHeads = 16;               // query heads of a matrix instruction
 
-// A work-group of four waves per sequence and query head; a wave takes every
-// fourth token, a lane four of the dims, with the softmax's running maximum
-// and sum per wave, joined at the end.
-template <typename T, typename CT>
-__global__ __launch_bounds__(256) void attend_kernel(AttendArgs a, KvPages pages) {
-  const int64_t b = blockIdx.x;
-  const int hq = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int group = a.q.heads / pages.heads, h = hq / group;
-  const int64_t width = (int64_t)a.table_width << pages.page_shift;
-  const int64_t limit = a.max_len < width ? a.max_len : width;
-  int64_t len = a.lens[b];
-  len = len < 0 ? 0 : len > limit ? limit : len;
-  const int64_t first = a.lists ? (a.first < len ? a.first : len) : 0;
-  int64_t last = a.last < 0 ? 0 : len - a.last;
-  if (last < first) last = first;
-  const int64_t always = first + (len - last);
-  const int64_t total = always + a.count;
-  const int32_t* ids = a.lists ? a.ids + ((int64_t)b * a.lists + hq / (a.q.heads / a.lists)) * a.count : nullptr;
-  const bool mine = lane * 4 < pages.dim;
-  float q[4] = {0, 0, 0, 0}, acc[4] = {0, 0, 0, 0};
-  if (mine) widen(*(const Pack<T, 4>*)((const T*)a.q.p + b * a.q.stride + hq * a.q.head_stride + lane * 4), q);
-  const float ks = pages.k_scale ? pages.k_scale[h] : 1.f, vs = pages.v_scale ? pages.v_scale[h] : 1.f;
-  float top = -__builtin_inff(), sum = 0;
-  for (int64_t i = wave; i < total; i += 4) {
-    int64_t t = i < first ? i : i < always ? last + (i - first) : ids[i - always];
-    if (i >= always && (t < first || t >= last)) continue;
-    const int32_t page = a.tables[b * a.table_stride + (t >> pages.page_shift)];
-    if (page < 0 || page >= pages.pages) continue;
-    const int64_t off = page * pages.page_stride + h * pages.head_stride +
-                        (t & (pages.page - 1)) * pages.row_stride + lane * 4;
-    float k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
-    if (mine) {
-      widen(*(const Pack<CT, 4>*)((const CT*)pages.k + off), k);
-      widen(*(const Pack<CT, 4>*)((const CT*)pages.v + off), v);
-    }
-    float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-    for (int m = 32; m; m >>= 1) s += __shfl_xor(s, m, 64);
-    s *= a.scale * ks;
-    const float now = fmaxf(top, s);
-    const float ref = now == -__builtin_inff() ? 0.f : now;  // scores of -inf weigh nothing
-    const float keep = expf(top - ref), p = expf(s - ref);
-    sum = sum * keep + p;
-    for (int e = 0; e < 4; ++e) acc[e] = acc[e] * keep + p * v[e];
-    top = now;
+struct Params {
+  const char* q;
+  int64_t q_stride, q_head;
+  const char *k, *v;
+  int64_t page_stride, head_stride, row_stride;
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* lens;
+  const int32_t* ids;
+  const float *k_scale, *v_scale;
+  char* out;
+  float* lse;
+  float* parts;
+  int2* ends;
+  float scale;  // times log2(e)
+  int batch, heads, q_heads, lists, group, tiles, count;
+  int page_shift, pages, dim, groups;
+  int64_t limit, first, last;
+};
+
+typedef uintx4 Frag;  // 8 values of 16 bits
+
+template <typename T>
+__device__ __forceinline__ floatx4 mfma(Frag a, Frag b, floatx4 c) {
+  typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
+  if constexpr (std::is_same_v<T, f16>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef T pair __attribute__((ext_vector_type(2)));
+  const pair p = {(T)a, (T)b};
+  return __builtin_bit_cast(uint32_t, p);
+}
+
+template <typename T>
+__device__ __forceinline__ floatx2 unpack2(uint32_t w) {
+  if constexpr (std::is_same_v<T, f16>) {
+    typedef T pair __attribute__((ext_vector_type(2)));
+    const pair p = __builtin_bit_cast(pair, w);
+    return floatx2{(float)p.x, (float)p.y};
+  } else {
+    return floatx2{__builtin_bit_cast(float, w << 16), __builtin_bit_cast(float, w & 0xFFFF0000u)};
   }
-  __shared__ float tops[4], sums[4], accs[4][kMaxDim];
-  if (lane == 0) tops[wave] = top, sums[wave] = sum;
-  for (int e = 0; e < 4; ++e) accs[wave][lane * 4 + e] = acc[e];
+}
+
+// Four e4m3 bytes as two words of T (exact in both types).
+template <typename T>
+__device__ __forceinline__ uint32_t from_e4m3(uint32_t w, bool high) {
+  const floatx2 a = high ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  return pack2<T>(a.x, a.y);
+}
+
+// What a sequence's units are: the tokens [begin, end) it reads, the count of
+// units, and for lists how many of the first and last come before the ids.
+struct Span {
+  int64_t base, begin, end, units;  // base: begin rounded down to whole groups of 8 rows
+  int64_t first, last;
+};
+
+template <bool LISTED>
+__device__ __forceinline__ Span span_of(const Params& p, int b) {
+  Span s;
+  int64_t len = p.lens[b];
+  len = len < 0 ? 0 : len > p.limit ? p.limit : len;
+  if (LISTED) {
+    s.first = p.first < len ? p.first : len;
+    s.last = len - p.last > s.first ? len - p.last : s.first;
+    s.base = s.begin = 0;
+    s.end = s.first + (len - s.last) + p.count;
+  } else {
+    s.begin = p.last >= 0 && len > p.last ? len - p.last : 0;
+    s.base = s.begin & ~(int64_t)7;
+    s.end = len;
+  }
+  s.units = (s.end - s.base + kUnit - 1) / kUnit;
+  if (s.units < 1) s.units = 1;  // a sequence of no tokens has its zeros written
+  return s;
+}
+
+// The units before sequence b of all, and their sum: every work-group adds
+// up the lengths. Returns the sequence that unit u (of one stream) lies in.
+template <bool LISTED>
+__device__ int find_sequence(const Params& p, int64_t share_num, int64_t share_den, int64_t streams, int64_t* total,
+                             int64_t* u0, int64_t* u1, int64_t* before, int64_t* groups, int64_t* red) {
+  // thread i adds a run of sequences
+  const int run = (p.batch + kThreads - 1) / kThreads;
+  const int b0 = min((int)threadIdx.x * run, p.batch), b1 = min(b0 + run, p.batch);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += span_of<LISTED>(p, b).units;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t incl = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 63) red[wave] = incl;
   __syncthreads();
-  if (wave) return;
-  const float all = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  float total_sum = 0, out[4] = {0, 0, 0, 0};
-  for (int w = 0; w < 4; ++w) {
-    const float f = tops[w] == -__builtin_inff() ? 1.f : expf(tops[w] - all);  // then its sum is 0 (or NaN)
-    total_sum += f * sums[w];
-    for (int e = 0; e < 4; ++e) out[e] += f * accs[w][lane * 4 + e];
+  int64_t sum = 0, off = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) off += red[w];
+    sum += red[w];
   }
-  const bool empty = total_sum == 0.f;
-  for (int e = 0; e < 4; ++e) out[e] = empty ? 0.f : out[e] / total_sum * vs;
-  if (mine) *(Pack<T, 4>*)((T*)a.out + (b * a.q.heads + hq) * pages.dim + lane * 4) = narrow<T, 4>(out);
-  if (a.lse && lane == 0) a.lse[b * a.q.heads + hq] = empty ? -__builtin_inff() : all + logf(total_sum);
+  const int64_t excl = off + incl - mine;
+  *total = sum * streams;
+  *groups = *total < share_den ? *total : share_den;
+  if (share_num >= *groups) return -1;
+  *u0 = *total * share_num / *groups;
+  *u1 = *total * (share_num + 1) / *groups;
+  const int64_t at = *u0;
+  if (at >= excl * streams && at < (excl + mine) * streams) {
+    int64_t pre = excl;
+    int b = b0;
+    for (;; ++b) {
+      const int64_t n = span_of<LISTED>(p, b).units;
+      if (at < (pre + n) * streams) break;
+      pre += n;
+    }
+    red[4] = b, red[5] = pre;
+  }
+  __syncthreads();
+  *before = red[5];
+  return (int)red[4];
+}
+
+// S = K Q^T and O^T = V^T P^T on 16x16x32 instructions, all in registers. With
+// g = lane / 16, i = lane % 16 and 8 tokens to a group, a tile of 32 tokens is
+//  K  two operands' rows i: token 8 (i / 4) + i % 4 (+ 4 in the second); so
+//  S  comes out with lane (g, i) holding head i's scores of group g's eight
+//     tokens, which is where P has to be as the operand of the second product:
+//     nothing crosses lanes.
+//  V  lane (g, i) loads the VD dims from VD i on of group g's eight tokens (a
+//     row is one contiguous read of 16 lanes); the 8 x VD values are turned
+//     with byte permutes into VD operands, product j giving dims VD m + j.
+//  O  lane (g, i): head i, dims VD (4 g + r) + j.
+// Heads past the group's are zero queries: the loads bound the kernel, not
+// the products (32 instructions of 16 cycles per 16 KB of a wave).
+template <typename T, bool F8, int DT, bool LISTED>
+__global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Params p) {
+  constexpr int VD = DT / 16, KS = DT / 32, ES = F8 ? 1 : 2;
+  typedef std::conditional_t<F8, f16, T> PT;  // e4m3 values are exact in fp16, where weights keep more bits
+  constexpr float kTop = std::is_same_v<PT, f16> ? 12.f : 0.f, kLag = 3.f;
+  __shared__ union {
+    int64_t rows[kStage];
+    float sums[kWaves][kHeads][DT];
+  } lds;
+  __shared__ float refs[kWaves][kHeads], tots[kWaves][kHeads];
+  __shared__ int64_t red[8];
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  const int streams = p.lists * p.tiles;
+  int64_t total, u, u1, before, groups;
+  int b = find_sequence<LISTED>(p, blockIdx.x, gridDim.x, streams, &total, &u, &u1, &before, &groups, red);
+  if (b < 0) return;
+  Span sp = span_of<LISTED>(p, b);
+  int64_t in_seq = u - before * streams;
+  int x = (int)(in_seq / sp.units);
+  int64_t c = in_seq % sp.units;
+
+  while (u < u1) {
+    const int list = x / p.tiles, head0 = (x % p.tiles) * kHeads;
+    const int h = list * p.heads / p.lists;
+    const int n_heads = min(kHeads, p.group - head0);
+    const int64_t c1 = min(sp.units, c + (u1 - u));
+    const int64_t v0 = c * kUnit, v1 = min(c1 * kUnit, sp.end - sp.base);
+    const char* kb = p.k + h * p.head_stride * ES;
+    const char* vb = p.v + h * p.head_stride * ES;
+    const float cs = p.scale * (p.k_scale ? p.k_scale[h] : 1.f);
+    const int qh = list * p.group + head0;
+
+    Frag q[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = F8 ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+      q[s] = Frag{0, 0, 0, 0};
+      if (i < n_heads && d < p.dim) q[s] = *(const Frag*)(p.q + (b * p.q_stride + (qh + i) * p.q_head + d) * 2);
+    }
+    floatx4 o[VD];
+#pragma unroll
+    for (int j = 0; j < VD; ++j) o[j] = floatx4{0, 0, 0, 0};
+    float ref = -__builtin_inff(), use = 0.f, sum = 0.f;
+
+    for (int64_t s0 = v0; s0 < v1; s0 += LISTED ? kStage : 8 * kStage) {
+      const int64_t left = v1 - s0;
+      const int n_tok = (int)(left < (LISTED ? kStage : 8 * kStage) ? left : (LISTED ? kStage : 8 * kStage));
+      const int n_tiles = (n_tok + kTile - 1) / kTile;
+      // offsets of the rows: one per token of a list, one per 8 tokens else
+      for (int e = threadIdx.x; e < n_tiles * (LISTED ? kTile : kTile / 8); e += kThreads) {
+        int64_t t, off = -1;
+        bool known;
+        if (LISTED) {
+          const int64_t at = s0 + e;
+          const int64_t always = sp.end - p.count;
+          known = at < sp.end;
+          t = at < sp.first ? at : sp.last + (at - sp.first);
+          if (known && at >= always) {
+            t = p.ids[((int64_t)b * p.lists + list) * p.count + (at - always)];
+            known = t >= sp.first && t < sp.last;
+          }
+        } else {
+          t = sp.base + s0 + 8 * e;
+          known = t < sp.end;
+        }
+        if (known) {
+          const int32_t page = p.tables[b * p.table_stride + (t >> p.page_shift)];
+          if (page >= 0 && page < p.pages)
+            off = (page * p.page_stride + (t & ((1 << p.page_shift) - 1)) * p.row_stride) * ES;
+        }
+        lds.rows[e] = off;
+      }
+      __syncthreads();
+
+      Frag kf[2][KS];
+      auto load_k = [&](int tile) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int tok = 8 * (i >> 2) + (i & 3) + 4 * r;
+          int64_t off = LISTED ? lds.rows[tile * kTile + tok] : lds.rows[tile * (kTile / 8) + (i >> 2)];
+          off = off < 0 ? 0 : off;
+          if (!LISTED) off += ((i & 3) + 4 * r) * p.row_stride * ES;
+          const char* row = kb + off;
+          if constexpr (F8) {
+#pragma unroll
+            for (int s = 0; s < KS; s += 2) {
+              const int d = 32 * s + 16 * g;
+              const bool in = d < p.dim;
+              uintx4 w = *(const uintx4*)(row + (in ? d : 0));
+              if (!in) w = uintx4{0, 0, 0, 0};
+              kf[r][s] = Frag{w.x, w.y, 0, 0};
+              kf[r][s + 1] = Frag{w.z, w.w, 0, 0};
+            }
+          } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              const int d = 32 * s + 8 * g;
+              const bool in = d < p.dim;
+              uintx4 w = *(const uintx4*)(row + (in ? d : 0) * 2);
+              if (!in) w = uintx4{0, 0, 0, 0};
+              kf[r][s] = w;
+            }
+          }
+        }
+      };
+      constexpr int VW = VD * ES / 4;  // words of V per token and lane
+      uint32_t vw[8][VW];
+      // a chunk of V past the end of a row is the row's first instead: those dims are never stored
+      const auto v_at = [&](int w) { return i * VD + w * (4 / ES) < p.dim ? i * VD * ES + 4 * w : 0; };
+
+      if (wave < n_tiles) load_k(wave);
+      for (int tile = wave; tile < n_tiles; tile += kWaves) {
+        // V of this tile; what is masked is known with its rows
+        uint32_t valid = 0;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          int64_t off = LISTED ? lds.rows[tile * kTile + 8 * g + t] : lds.rows[tile * (kTile / 8) + g];
+          bool in = off >= 0;
+          if (!LISTED) {
+            const int64_t tok = sp.base + s0 + tile * kTile + 8 * g + t;
+            in = in && tok >= sp.begin && tok < sp.end;
+          }
+          valid |= in ? 1u << t : 0u;
+          off = off < 0 ? 0 : off;
+          if (!LISTED) off += t * p.row_stride * ES;
+          const char* row = vb + off;
+          if constexpr (VW >= 4) {
+#pragma unroll
+            for (int w = 0; w < VW; w += 4) {
+              const uintx4 y = *(const uintx4*)(row + v_at(w));
+              vw[t][w] = y.x, vw[t][w + 1] = y.y, vw[t][w + 2] = y.z, vw[t][w + 3] = y.w;
+            }
+          } else if constexpr (VW == 2) {
+            const uintx2 y = *(const uintx2*)(row + v_at(0));
+            vw[t][0] = y.x, vw[t][1] = y.y;
+          } else {
+            vw[t][0] = *(const uint32_t*)(row + v_at(0));
+          }
+        }
+        floatx4 s[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          s[r] = floatx4{0, 0, 0, 0};
+#pragma unroll
+          for (int e = 0; e < KS; ++e) {
+            Frag a = kf[r][e];
+            if constexpr (F8)
+              a = Frag{from_e4m3<T>(a.x, false), from_e4m3<T>(a.x, true), from_e4m3<T>(a.y, false), from_e4m3<T>(a.y, true)};
+            s[r] = mfma<T>(a, q[e], s[r]);
+          }
+        }
+        if (tile + kWaves < n_tiles) load_k(tile + kWaves);
+        float z[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) z[t] = s[t >> 2][t & 3] * cs;
+        if (!__all(valid == 0xFFu)) {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            const bool in = valid >> t & 1;
+            z[t] = in ? z[t] : -__builtin_inff();
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vw[t][w] = in ? vw[t][w] : 0u;
+          }
+        }
+        float top = z[0];
+#pragma unroll
+        for (int t = 1; t < 8; ++t) top = fmaxf(top, z[t]);
+        if (__any(top > ref + (kTop + kLag))) {
+          top = fmaxf(top, __shfl_xor(top, 16, 64));
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const float now = fmaxf(ref, top - kTop);
+          const float to = now == -__builtin_inff() ? 0.f : now;
+          const float keep = __builtin_amdgcn_exp2f(ref - to);
+          sum *= keep;
+#pragma unroll
+          for (int j = 0; j < VD; ++j) o[j] *= keep;
+          ref = now, use = to;
+        }
+        Frag hi, lo;
+#pragma unroll
+        for (int t = 0; t < 8; t += 2) {
+          const float a = __builtin_amdgcn_exp2f(z[t] - use), bb = __builtin_amdgcn_exp2f(z[t + 1] - use);
+          sum += a + bb;
+          hi[t / 2] = pack2<PT>(a, bb);
+          const floatx2 back = unpack2<PT>(hi[t / 2]);
+          lo[t / 2] = pack2<PT>(a - back.x, bb - back.y);
+        }
+        // turn V: word w of tokens t, t + 1 holds dims 2w, 2w + 1 (bytes: 4)
+        if constexpr (F8) {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            Frag f[4];
+#pragma unroll
+            for (int t = 0; t < 8; t += 2) {
+              const uint32_t a = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x05010400u);
+              const uint32_t c2 = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x07030602u);
+              f[0][t / 2] = from_e4m3<PT>(a, false), f[1][t / 2] = from_e4m3<PT>(a, true);
+              f[2][t / 2] = from_e4m3<PT>(c2, false), f[3][t / 2] = from_e4m3<PT>(c2, true);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o[4 * w + j] = mfma<PT>(f[j], hi, o[4 * w + j]);
+              o[4 * w + j] = mfma<PT>(f[j], lo, o[4 * w + j]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            Frag f[2];
+#pragma unroll
+            for (int t = 0; t < 8; t += 2) {
+              f[0][t / 2] = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x05040100u);
+              f[1][t / 2] = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x07060302u);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              o[2 * w + j] = mfma<PT>(f[j], hi, o[2 * w + j]);
+              o[2 * w + j] = mfma<PT>(f[j], lo, o[2 * w + j]);
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+
+    // join the waves: all to the largest reference
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (g == 0) refs[wave][i] = ref, tots[wave][i] = sum;
+    __syncthreads();
+    float most = refs[0][i];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) most = fmaxf(most, refs[w][i]);
+    const float f = ref == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ref - most);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < VD; ++j) lds.sums[wave][i][VD * (4 * g + r) + j] = o[j][r] * f;
+    __syncthreads();
+    const bool whole = c == 0 && c1 == sp.units;
+    float* part = p.parts + ((int64_t)blockIdx.x * 2 + (c == 0 ? 1 : 0)) * kHeads * (DT + 2);
+    const float vs = p.v_scale ? p.v_scale[h] : 1.f;
+    for (int e = threadIdx.x; e < n_heads * (DT / 2); e += kThreads) {
+      const int n = e / (DT / 2), d = e % (DT / 2) * 2;
+      float a = 0, bb = 0, l = 0, m = refs[0][n];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) m = fmaxf(m, refs[w][n]);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        a += lds.sums[w][n][d], bb += lds.sums[w][n][d + 1];
+        l += tots[w][n] * (refs[w][n] == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(refs[w][n] - m));
+      }
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : vs / l;
+        const int64_t row = (int64_t)b * p.q_heads + qh + n;
+        if (d < p.dim) *(uint32_t*)(p.out + (row * p.dim + d) * 2) = pack2<T>(l == 0.f ? 0.f : a * inv, l == 0.f ? 0.f : bb * inv);
+        if (d == 0 && p.lse) p.lse[row] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+      } else {
+        *(floatx2*)(part + n * DT + d) = floatx2{a, bb};
+        if (d == 0) part[kHeads * DT + 2 * n] = m, part[kHeads * DT + 2 * n + 1] = l;
+      }
+    }
+    if (c == 0 && threadIdx.x == 0) {
+      // the work-group that has the last of this stream's units
+      const int64_t end = u + sp.units;
+      p.ends[(int64_t)b * streams + x] = int2{(int)blockIdx.x, (int)((end * groups - 1) / total)};
+    }
+    __syncthreads();
+    u += c1 - c;
+    c = 0;
+    if (++x == streams) {
+      x = 0;
+      if (++b < p.batch) sp = span_of<LISTED>(p, b);
+    }
+  }
+}
+
+// Joins the parts of a stream that several work-groups had: a work-group per
+// sequence, stream and head; the parts' weights first, then their sums.
+template <typename T, int DT>
+__global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
+  const int streams = p.lists * p.tiles;
+  const int64_t seq = blockIdx.x;
+  const int n = blockIdx.y;
+  const int b = (int)(seq / streams), x = (int)(seq % streams);
+  const int list = x / p.tiles, head0 = (x % p.tiles) * kHeads;
+  if (n >= p.group - head0) return;
+  const int2 range = p.ends[seq];
+  const int parts = range.y - range.x + 1;
+  if (parts == 1) return;
+  constexpr int kSize = kHeads * (DT + 2), kLanes = DT / 4, kRows = kThreads / kLanes;
+  __shared__ float tops[kWaves], tots[kWaves];
+  __shared__ floatx4 sums[kRows][kLanes];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto part = [&](int i) { return p.parts + ((int64_t)(range.x + i) * 2 + (i == 0 ? 1 : 0)) * kSize; };
+  float top = -__builtin_inff();
+  for (int i = threadIdx.x; i < parts; i += kThreads) top = fmaxf(top, part(i)[kHeads * DT + 2 * n]);
+  for (int m = 32; m; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const int d = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
+  floatx4 acc = {0, 0, 0, 0};
+  float tot = 0;
+  for (int i = row; i < parts; i += kRows) {
+    const float* a = part(i);
+    const float m = a[kHeads * DT + 2 * n];
+    const float f = m == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    tot += f * a[kHeads * DT + 2 * n + 1];
+    acc += *(const floatx4*)(a + n * DT + 4 * d) * f;
+  }
+  __shared__ float rows[kRows];
+  sums[row][d] = acc;
+  if (d == 0) rows[row] = tot;
+  __syncthreads();
+  if (row) return;
+  tot = rows[0];
+  for (int r = 1; r < kRows; ++r) tot += rows[r], acc += sums[r][d];
+  const float vs = p.v_scale ? p.v_scale[list * p.heads / p.lists] : 1.f;
+  const int64_t at = (int64_t)b * p.q_heads + list * p.group + head0 + n;
+  const float inv = vs / tot;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] = tot == 0.f ? 0.f : acc[e] * inv;
+  if (4 * d < p.dim) {
+    *(uintx2*)(p.out + (at * p.dim + 4 * d) * 2) = uintx2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
+  }
+  if (d == 0 && p.lse) p.lse[at] = tot == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(tot)) * 0.6931471805599453f;
+}
+
+int compute_units() {
+  static const int n = [] {
+    int device = 0, v = 0;
+    hip_check(hipGetDevice(&device), "get device");
+    hip_check(hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, device), "device attribute");
+    return v > 0 ? v : 256;
+  }();
+  return n;
+}
+
+// How a call's work is laid out, from its sizes alone.
+struct Plan {
+  int dt, lists, group, tiles;
+  int64_t streams, work_groups;
+  bool joins;
+  int64_t ends_bytes, bytes;
+};
+
+Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_tokens, int64_t lists) {
+  Plan a;
+  a.dt = pages.dim <= 64 ? 64 : pages.dim <= 128 ? 128 : 256;
+  a.lists = (int)(lists ? lists : pages.heads);
+  a.group = (int)(q_heads / a.lists);
+  a.tiles = (a.group + kHeads - 1) / kHeads;
+  a.streams = (int64_t)a.lists * a.tiles;
+  // a window's first group of 8 rows may start 7 tokens early
+  const int64_t units = std::max<int64_t>(1, (max_tokens + (lists ? 0 : 7) + kUnit - 1) / kUnit);
+  const int64_t resident = (int64_t)compute_units() * (a.dt == 256 ? 1 : 2);
+  a.work_groups = std::min(batch * a.streams * units, resident);
+  a.joins = units > 1;
+  a.ends_bytes = (batch * a.streams * 8 + 15) / 16 * 16;
+  a.bytes = a.ends_bytes + a.work_groups * 2 * kHeads * (a.dt + 2) * 4;
+  return a;
+}
+
+template <typename T, bool F8, int DT>
+void launch(const Params& p, const Plan& plan, bool listed, hipStream_t s) {
+  auto kernel = listed ? attend_kernel<T, F8, DT, true> : attend_kernel<T, F8, DT, false>;
+  kernel<<<(unsigned)plan.work_groups, kThreads, 0, s>>>(p);
+  hip_check(hipGetLastError(), "attention");
+  if (plan.joins) {
+    join_kernel<T, DT><<<dim3((unsigned)(p.batch * plan.streams), (unsigned)std::min(kHeads, plan.group)), kThreads, 0, s>>>(p);
+    hip_check(hipGetLastError(), "attention join");
+  }
+}
+
+template <typename T, bool F8>
+void launch_dim(const Params& p, const Plan& plan, bool listed, hipStream_t s) {
+  if (plan.dt == 64) launch<T, F8, 64>(p, plan, listed, s);
+  else if (plan.dt == 128) launch<T, F8, 128>(p, plan, listed, s);
+  else launch<T, F8, 256>(p, plan, listed, s);
 }
 
 }  // namespace
 
-int64_t attend_workspace(int64_t, int64_t, const KvPages&, int64_t, int64_t) { return 0; }
+int64_t attend_workspace(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_tokens, int64_t lists) {
+  return batch ? plan_of(batch, q_heads, pages, max_tokens, lists).bytes : 0;
+}
 
 void attend(const AttendArgs& a, const KvPages& pages, hipStream_t s) {
-  if (a.batch == 0 || a.q.heads == 0) return;
-  const dim3 grid((unsigned)a.batch, (unsigned)a.q.heads);
-  auto kernel = pages.type == kE4M3 ? (a.type == kF16 ? attend_kernel<f16, e4m3> : attend_kernel<bf16, e4m3>)
-                                    : (a.type == kF16 ? attend_kernel<f16, f16> : attend_kernel<bf16, bf16>);
-  kernel<<<grid, 256, 0, s>>>(a, pages);
-  hip_check(hipGetLastError(), "attention");
+  if (a.batch == 0) return;
+  const int64_t width = (int64_t)a.table_width << pages.page_shift;
+  const bool listed = a.lists != 0;
+  Params p{};
+  p.limit = pages.pages ? std::min(a.max_len, width) : 0;
+  const int64_t most = listed ? a.first + a.last + a.count : a.last < 0 ? a.max_len : std::min(a.max_len, a.last);
+  const Plan plan = plan_of(a.batch, a.q.heads, pages, most, a.lists);
+  if (a.workspace_bytes < plan.bytes || !a.workspace || ((uintptr_t)a.workspace & 15u))
+    throw std::invalid_argument("workspace must be 16-byte aligned and hold " + std::to_string(plan.bytes) + " bytes");
+  p.q = (const char*)a.q.p, p.q_stride = a.q.stride, p.q_head = a.q.head_stride;
+  p.k = pages.k, p.v = pages.v;
+  p.page_stride = pages.page_stride, p.head_stride = pages.head_stride, p.row_stride = pages.row_stride;
+  p.tables = a.tables, p.table_stride = a.table_stride, p.lens = a.lens, p.ids = a.ids;
+  p.k_scale = pages.k_scale, p.v_scale = pages.v_scale;
+  p.out = (char*)a.out, p.lse = a.lse;
+  p.ends = (int2*)a.workspace, p.parts = (float*)((char*)a.workspace + plan.ends_bytes);
+  p.scale = a.scale * 1.4426950408889634f;
+  p.batch = (int)a.batch, p.heads = pages.heads, p.q_heads = a.q.heads;
+  p.lists = plan.lists, p.group = plan.group, p.tiles = plan.tiles, p.count = pages.pages ? a.count : 0;
+  p.page_shift = pages.page_shift, p.pages = pages.pages, p.dim = pages.dim;
+  p.first = a.first, p.last = a.last;
+  if (pages.type == kE4M3) {
+    if (a.type == kF16) launch_dim<f16, true>(p, plan, listed, s);
+    else launch_dim<bf16, true>(p, plan, listed, s);
+  } else if (a.type == kF16) {
+    launch_dim<f16, false>(p, plan, listed, s);
+  } else {
+    launch_dim<bf16, false>(p, plan, listed, s);
+  }
 }
 
 }  // namespace jasper_amd
