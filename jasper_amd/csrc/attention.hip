@@ -14,11 +14,11 @@ namespace jasper_amd {
 
 namespace {
 
-constexpr int kThreads = 256, kWaves = 4;
-constexpr int kTile = 32;                // tokens a wave takes at once
-constexpr int kUnit = kTile * kWaves;    // tokens a work-group takes at once
-constexpr int kStage = 2048;             // row offsets held in LDS
-constexpr int kHeads = 16;               // query heads of a matrix instruction
+constexpr int kTile = 32;    // tokens a wave takes at once
+constexpr int kStage = 512;  // row offsets held in LDS
+constexpr int kHeads = 16;   // query heads of a matrix instruction
+constexpr int kJoin = 256;   // threads of a joining work-group
+constexpr float kLn2 = 0.6931471805599453f;
 
 struct Params {
   const char* q;
@@ -35,9 +35,10 @@ struct Params {
   float* parts;
   int2* ends;
   float scale;  // times log2(e)
-  int batch, heads, q_heads, lists, group, tiles, count;
-  int page_shift, pages, dim, groups;
-  int64_t limit, first, last;
+  int batch, heads, q_heads, lists, group, tiles, count;  // tiles: of 16 heads per list
+  int part_heads;
+  int page_shift, pages, dim;
+  int limit, first, last;  // tokens; last: -1 for all
 };
 
 typedef uintx4 Frag;  // 8 values of 16 bits
@@ -77,78 +78,76 @@ __device__ __forceinline__ uint32_t from_e4m3(uint32_t w, bool high) {
   return pack2<T>(a.x, a.y);
 }
 
-// What a sequence's units are: the tokens [begin, end) it reads, the count of
-// units, and for lists how many of the first and last come before the ids.
+// What a sequence has its queries read: the tokens [begin, end), counted from
+// base in tiles; of a list's places [0, end) the first `first` are tokens,
+// then come the tokens from `last` on, then the ids.
 struct Span {
-  int64_t base, begin, end, units;  // base: begin rounded down to whole groups of 8 rows
-  int64_t first, last;
+  int base, begin, end, tiles;  // base: begin rounded down to whole groups of 8 rows
+  int first, last;
 };
 
 template <bool LISTED>
 __device__ __forceinline__ Span span_of(const Params& p, int b) {
   Span s;
-  int64_t len = p.lens[b];
-  len = len < 0 ? 0 : len > p.limit ? p.limit : len;
+  const int len = min(max(p.lens[b], 0), p.limit);
   if (LISTED) {
-    s.first = p.first < len ? p.first : len;
-    s.last = len - p.last > s.first ? len - p.last : s.first;
+    s.first = min(p.first, len);
+    s.last = max(len - p.last, s.first);
     s.base = s.begin = 0;
     s.end = s.first + (len - s.last) + p.count;
   } else {
     s.begin = p.last >= 0 && len > p.last ? len - p.last : 0;
-    s.base = s.begin & ~(int64_t)7;
+    s.base = s.begin & ~7;
     s.end = len;
   }
-  s.units = (s.end - s.base + kUnit - 1) / kUnit;
-  if (s.units < 1) s.units = 1;  // a sequence of no tokens has its zeros written
+  s.tiles = max(1, (s.end - s.base + kTile - 1) / kTile);  // a sequence of no tokens has its zeros written
   return s;
 }
 
-// The units before sequence b of all, and their sum: every work-group adds
-// up the lengths. Returns the sequence that unit u (of one stream) lies in.
+// How the tiles of all sequences and streams are shared out: the first
+// `more` of `waves` waves have each tiles + 1, the others each tiles.
+struct Share {
+  int each, more, waves;
+  __device__ int begin(int w) const { return each * w + min(w, more); }
+  __device__ int owner(int tile) const {
+    const int longer = (each + 1) * more;
+    return tile < longer ? tile / (each + 1) : more + (tile - longer) / each;
+  }
+};
+
+// Every wave adds up the lengths for itself (lane i a run of sequences) and
+// finds the sequence its first tile lies in, and the tiles of one stream
+// before that sequence. -1: there is no work for it.
 template <bool LISTED>
-__device__ int find_sequence(const Params& p, int64_t share_num, int64_t share_den, int64_t streams, int64_t* total,
-                             int64_t* u0, int64_t* u1, int64_t* before, int64_t* groups, int64_t* red) {
-  // thread i adds a run of sequences
-  const int run = (p.batch + kThreads - 1) / kThreads;
-  const int b0 = min((int)threadIdx.x * run, p.batch), b1 = min(b0 + run, p.batch);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += span_of<LISTED>(p, b).units;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t incl = mine;
+__device__ int find_sequence(const Params& p, int streams, Share& share, int& before) {
+  const int lane = threadIdx.x;
+  const int run = (p.batch + 63) / 64;
+  const int b0 = min(lane * run, p.batch), b1 = min(b0 + run, p.batch);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += span_of<LISTED>(p, b).tiles;
+  int incl = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(incl, d, 64);
+    const int o = __shfl_up(incl, d, 64);
     if (lane >= d) incl += o;
   }
-  if (lane == 63) red[wave] = incl;
-  __syncthreads();
-  int64_t sum = 0, off = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) off += red[w];
-    sum += red[w];
-  }
-  const int64_t excl = off + incl - mine;
-  *total = sum * streams;
-  *groups = *total < share_den ? *total : share_den;
-  if (share_num >= *groups) return -1;
-  *u0 = *total * share_num / *groups;
-  *u1 = *total * (share_num + 1) / *groups;
-  const int64_t at = *u0;
-  if (at >= excl * streams && at < (excl + mine) * streams) {
-    int64_t pre = excl;
-    int b = b0;
+  const int total = __shfl(incl, 63, 64) * streams;
+  share.waves = min(total, (int)gridDim.x);
+  share.each = total / share.waves;
+  share.more = total % share.waves;
+  if ((int)blockIdx.x >= share.waves) return -1;
+  const int at = share.begin(blockIdx.x) / streams;  // tile of a stream, were the streams side by side
+  const int src = __ffsll((unsigned long long)__ballot(at < incl)) - 1;
+  int pre = incl - mine, b = b0;
+  if (lane == src) {
     for (;; ++b) {
-      const int64_t n = span_of<LISTED>(p, b).units;
-      if (at < (pre + n) * streams) break;
+      const int n = span_of<LISTED>(p, b).tiles;
+      if (at < pre + n) break;
       pre += n;
     }
-    red[4] = b, red[5] = pre;
   }
-  __syncthreads();
-  *before = red[5];
-  return (int)red[4];
+  before = __builtin_amdgcn_readlane(pre, src);
+  return __builtin_amdgcn_readlane(b, src);
 }
 
 // S = K Q^T and O^T = V^T P^T on 16x16x32 instructions, all in registers. With
@@ -163,34 +162,39 @@ __device__ int find_sequence(const Params& p, int64_t share_num, int64_t share_d
 //  O  lane (g, i): head i, dims VD (4 g + r) + j.
 // Heads past the group's are zero queries: the loads bound the kernel, not
 // the products (32 instructions of 16 cycles per 16 KB of a wave).
+//
+// A work-group is one wave with an equal run of the tiles of all sequences
+// and streams: waves in different phases (finding their rows, streaming,
+// writing) share a compute unit without waiting for each other. A stream that
+// one wave has whole is finished here, the others' parts go to the workspace:
+// a wave has at most one that an earlier wave began (slot 0) and one that it
+// begins itself (slot 1).
 template <typename T, bool F8, int DT, bool LISTED>
-__global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Params p) {
+__global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p) {
   constexpr int VD = DT / 16, KS = DT / 32, ES = F8 ? 1 : 2;
   typedef std::conditional_t<F8, f16, T> PT;  // e4m3 values are exact in fp16, where weights keep more bits
+  // fp16 weights are 2^12 larger, so that those far below the largest are not
+  // lost; the reference is moved once a score is 2^3 above it
   constexpr float kTop = std::is_same_v<PT, f16> ? 12.f : 0.f, kLag = 3.f;
-  __shared__ union {
-    int64_t rows[kStage];
-    float sums[kWaves][kHeads][DT];
-  } lds;
-  __shared__ float refs[kWaves][kHeads], tots[kWaves][kHeads];
-  __shared__ int64_t red[8];
+  __shared__ int64_t rows[kStage];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  const int lane = threadIdx.x, g = lane >> 4, i = lane & 15;
   const int streams = p.lists * p.tiles;
-  int64_t total, u, u1, before, groups;
-  int b = find_sequence<LISTED>(p, blockIdx.x, gridDim.x, streams, &total, &u, &u1, &before, &groups, red);
+  Share share;
+  int before;
+  int b = find_sequence<LISTED>(p, streams, share, before);
   if (b < 0) return;
+  int u = share.begin(blockIdx.x);
+  const int u1 = share.begin(blockIdx.x + 1);
   Span sp = span_of<LISTED>(p, b);
-  int64_t in_seq = u - before * streams;
-  int x = (int)(in_seq / sp.units);
-  int64_t c = in_seq % sp.units;
+  int x = (u - before * streams) / sp.tiles;
+  int c = (u - before * streams) % sp.tiles;
 
   while (u < u1) {
     const int list = x / p.tiles, head0 = (x % p.tiles) * kHeads;
     const int h = list * p.heads / p.lists;
     const int n_heads = min(kHeads, p.group - head0);
-    const int64_t c1 = min(sp.units, c + (u1 - u));
-    const int64_t v0 = c * kUnit, v1 = min(c1 * kUnit, sp.end - sp.base);
+    const int c1 = min(sp.tiles, c + (u1 - u));
     const char* kb = p.k + h * p.head_stride * ES;
     const char* vb = p.v + h * p.head_stride * ES;
     const float cs = p.scale * (p.k_scale ? p.k_scale[h] : 1.f);
@@ -208,17 +212,18 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Par
     for (int j = 0; j < VD; ++j) o[j] = floatx4{0, 0, 0, 0};
     float ref = -__builtin_inff(), use = 0.f, sum = 0.f;
 
-    for (int64_t s0 = v0; s0 < v1; s0 += LISTED ? kStage : 8 * kStage) {
-      const int64_t left = v1 - s0;
-      const int n_tok = (int)(left < (LISTED ? kStage : 8 * kStage) ? left : (LISTED ? kStage : 8 * kStage));
-      const int n_tiles = (n_tok + kTile - 1) / kTile;
+    constexpr int kStageTiles = LISTED ? kStage / kTile : kStage / (kTile / 8);
+    const int n_all = sp.end > sp.base ? c1 : c;  // no tokens, no tiles
+    for (int c0 = c; c0 < n_all; c0 += kStageTiles) {
+      const int n_tiles = min(n_all - c0, kStageTiles);
       // offsets of the rows: one per token of a list, one per 8 tokens else
-      for (int e = threadIdx.x; e < n_tiles * (LISTED ? kTile : kTile / 8); e += kThreads) {
-        int64_t t, off = -1;
+      __syncthreads();
+      for (int e = lane; e < n_tiles * (LISTED ? kTile : kTile / 8); e += 64) {
+        int t;
+        int64_t off = -1;
         bool known;
         if (LISTED) {
-          const int64_t at = s0 + e;
-          const int64_t always = sp.end - p.count;
+          const int at = c0 * kTile + e, always = sp.end - p.count;
           known = at < sp.end;
           t = at < sp.first ? at : sp.last + (at - sp.first);
           if (known && at >= always) {
@@ -226,7 +231,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Par
             known = t >= sp.first && t < sp.last;
           }
         } else {
-          t = sp.base + s0 + 8 * e;
+          t = sp.base + c0 * kTile + 8 * e;
           known = t < sp.end;
         }
         if (known) {
@@ -234,7 +239,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Par
           if (page >= 0 && page < p.pages)
             off = (page * p.page_stride + (t & ((1 << p.page_shift) - 1)) * p.row_stride) * ES;
         }
-        lds.rows[e] = off;
+        rows[e] = off;
       }
       __syncthreads();
 
@@ -243,7 +248,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Par
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const int tok = 8 * (i >> 2) + (i & 3) + 4 * r;
-          int64_t off = LISTED ? lds.rows[tile * kTile + tok] : lds.rows[tile * (kTile / 8) + (i >> 2)];
+          int64_t off = LISTED ? rows[tile * kTile + tok] : rows[tile * (kTile / 8) + (i >> 2)];
           off = off < 0 ? 0 : off;
           if (!LISTED) off += ((i & 3) + 4 * r) * p.row_stride * ES;
           const char* row = kb + off;
@@ -270,20 +275,19 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Par
         }
       };
       constexpr int VW = VD * ES / 4;  // words of V per token and lane
-      uint32_t vw[8][VW];
       // a chunk of V past the end of a row is the row's first instead: those dims are never stored
       const auto v_at = [&](int w) { return i * VD + w * (4 / ES) < p.dim ? i * VD * ES + 4 * w : 0; };
 
-      if (wave < n_tiles) load_k(wave);
-      for (int tile = wave; tile < n_tiles; tile += kWaves) {
-        // V of this tile; what is masked is known with its rows
+      // one tile, with the next one's keys on their way while its values are
+      auto step = [&](int tile, auto more) {
+        uint32_t vw[8][VW];
         uint32_t valid = 0;
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-          int64_t off = LISTED ? lds.rows[tile * kTile + 8 * g + t] : lds.rows[tile * (kTile / 8) + g];
+          int64_t off = LISTED ? rows[tile * kTile + 8 * g + t] : rows[tile * (kTile / 8) + g];
           bool in = off >= 0;
           if (!LISTED) {
-            const int64_t tok = sp.base + s0 + tile * kTile + 8 * g + t;
+            const int tok = sp.base + (c0 + tile) * kTile + 8 * g + t;
             in = in && tok >= sp.begin && tok < sp.end;
           }
           valid |= in ? 1u << t : 0u;
@@ -315,11 +319,12 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Par
             s[r] = mfma<T>(a, q[e], s[r]);
           }
         }
-        if (tile + kWaves < n_tiles) load_k(tile + kWaves);
+        if constexpr (more.value) load_k(tile + 1);
         float z[8];
 #pragma unroll
         for (int t = 0; t < 8; ++t) z[t] = s[t >> 2][t & 3] * cs;
         if (!__all(valid == 0xFFu)) {
+          // what stands in masked rows may be anything: neither its scores nor its values are used
 #pragma unroll
           for (int t = 0; t < 8; ++t) {
             const bool in = valid >> t & 1;
@@ -342,6 +347,8 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Par
           for (int j = 0; j < VD; ++j) o[j] *= keep;
           ref = now, use = to;
         }
+        // the weights in two terms of their type, so that their rounding adds
+        // nothing to the output's own
         Frag hi, lo;
 #pragma unroll
         for (int t = 0; t < 8; t += 2) {
@@ -352,86 +359,64 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Par
           lo[t / 2] = pack2<PT>(a - back.x, bb - back.y);
         }
         // turn V: word w of tokens t, t + 1 holds dims 2w, 2w + 1 (bytes: 4)
-        if constexpr (F8) {
+        constexpr int kPer = 4 / ES;
 #pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            Frag f[4];
+        for (int w = 0; w < VW; ++w) {
+          Frag f[kPer];
 #pragma unroll
-            for (int t = 0; t < 8; t += 2) {
-              const uint32_t a = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x05010400u);
-              const uint32_t c2 = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x07030602u);
-              f[0][t / 2] = from_e4m3<PT>(a, false), f[1][t / 2] = from_e4m3<PT>(a, true);
-              f[2][t / 2] = from_e4m3<PT>(c2, false), f[3][t / 2] = from_e4m3<PT>(c2, true);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              o[4 * w + j] = mfma<PT>(f[j], hi, o[4 * w + j]);
-              o[4 * w + j] = mfma<PT>(f[j], lo, o[4 * w + j]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            Frag f[2];
-#pragma unroll
-            for (int t = 0; t < 8; t += 2) {
+          for (int t = 0; t < 8; t += 2) {
+            if constexpr (F8) {
+              const uint32_t even = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x05010400u);
+              const uint32_t odd = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x07030602u);
+              f[0][t / 2] = from_e4m3<PT>(even, false), f[1][t / 2] = from_e4m3<PT>(even, true);
+              f[2][t / 2] = from_e4m3<PT>(odd, false), f[3][t / 2] = from_e4m3<PT>(odd, true);
+            } else {
               f[0][t / 2] = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x05040100u);
               f[1][t / 2] = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x07060302u);
             }
+          }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              o[2 * w + j] = mfma<PT>(f[j], hi, o[2 * w + j]);
-              o[2 * w + j] = mfma<PT>(f[j], lo, o[2 * w + j]);
-            }
+          for (int j = 0; j < kPer; ++j) {
+            o[kPer * w + j] = mfma<PT>(f[j], hi, o[kPer * w + j]);
+            o[kPer * w + j] = mfma<PT>(f[j], lo, o[kPer * w + j]);
           }
         }
-      }
-      __syncthreads();
+      };
+      load_k(0);
+      for (int tile = 0; tile + 1 < n_tiles; ++tile) step(tile, std::true_type{});
+      step(n_tiles - 1, std::false_type{});
     }
 
-    // join the waves: all to the largest reference
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
-    if (g == 0) refs[wave][i] = ref, tots[wave][i] = sum;
-    __syncthreads();
-    float most = refs[0][i];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) most = fmaxf(most, refs[w][i]);
-    const float f = ref == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ref - most);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int j = 0; j < VD; ++j) lds.sums[wave][i][VD * (4 * g + r) + j] = o[j][r] * f;
-    __syncthreads();
-    const bool whole = c == 0 && c1 == sp.units;
-    float* part = p.parts + ((int64_t)blockIdx.x * 2 + (c == 0 ? 1 : 0)) * kHeads * (DT + 2);
-    const float vs = p.v_scale ? p.v_scale[h] : 1.f;
-    for (int e = threadIdx.x; e < n_heads * (DT / 2); e += kThreads) {
-      const int n = e / (DT / 2), d = e % (DT / 2) * 2;
-      float a = 0, bb = 0, l = 0, m = refs[0][n];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) m = fmaxf(m, refs[w][n]);
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        a += lds.sums[w][n][d], bb += lds.sums[w][n][d + 1];
-        l += tots[w][n] * (refs[w][n] == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(refs[w][n] - m));
-      }
+    const bool whole = c == 0 && c1 == sp.tiles;
+    if (i < n_heads) {
       if (whole) {
-        const float inv = l == 0.f ? 0.f : vs / l;
-        const int64_t row = (int64_t)b * p.q_heads + qh + n;
-        if (d < p.dim) *(uint32_t*)(p.out + (row * p.dim + d) * 2) = pack2<T>(l == 0.f ? 0.f : a * inv, l == 0.f ? 0.f : bb * inv);
-        if (d == 0 && p.lse) p.lse[row] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+        const int64_t row = (int64_t)b * p.q_heads + qh + i;
+        const float inv = (p.v_scale ? p.v_scale[h] : 1.f) / sum;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int d = VD * (4 * g + r);
+#pragma unroll
+          for (int j = 0; j < VD; j += 4) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = sum == 0.f ? 0.f : o[j + e][r] * inv;
+            if (d + j < p.dim) *(uintx2*)(p.out + (row * p.dim + d + j) * 2) = uintx2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+          }
+        }
+        if (g == 0 && p.lse) p.lse[row] = sum == 0.f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
       } else {
-        *(floatx2*)(part + n * DT + d) = floatx2{a, bb};
-        if (d == 0) part[kHeads * DT + 2 * n] = m, part[kHeads * DT + 2 * n + 1] = l;
+        float* part = p.parts + ((int64_t)blockIdx.x * 2 + (c == 0 ? 1 : 0)) * p.part_heads * (DT + 2);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < VD; j += 4)
+            *(floatx4*)(part + i * DT + VD * (4 * g + r) + j) = floatx4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
+        if (g == 0) *(floatx2*)(part + p.part_heads * DT + 2 * i) = floatx2{ref, sum};
       }
     }
-    if (c == 0 && threadIdx.x == 0) {
-      // the work-group that has the last of this stream's units
-      const int64_t end = u + sp.units;
-      p.ends[(int64_t)b * streams + x] = int2{(int)blockIdx.x, (int)((end * groups - 1) / total)};
-    }
-    __syncthreads();
+    if (c == 0 && lane == 0) p.ends[(int64_t)b * streams + x] = int2{(int)blockIdx.x, share.owner(u + sp.tiles - 1)};
     u += c1 - c;
     c = 0;
     if (++x == streams) {
@@ -444,7 +429,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void attend_kernel(Par
 // Joins the parts of a stream that several work-groups had: a work-group per
 // sequence, stream and head; the parts' weights first, then their sums.
 template <typename T, int DT>
-__global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
+__global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
   const int streams = p.lists * p.tiles;
   const int64_t seq = blockIdx.x;
   const int n = blockIdx.y;
@@ -454,13 +439,14 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
   const int2 range = p.ends[seq];
   const int parts = range.y - range.x + 1;
   if (parts == 1) return;
-  constexpr int kSize = kHeads * (DT + 2), kLanes = DT / 4, kRows = kThreads / kLanes;
-  __shared__ float tops[kWaves], tots[kWaves];
+  constexpr int kLanes = DT / 4, kRows = kJoin / kLanes;
+  const int size = p.part_heads * (DT + 2), stats = p.part_heads * DT + 2 * n;
+  __shared__ float tops[kJoin / 64];
   __shared__ floatx4 sums[kRows][kLanes];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  auto part = [&](int i) { return p.parts + ((int64_t)(range.x + i) * 2 + (i == 0 ? 1 : 0)) * kSize; };
+  auto part = [&](int i) { return p.parts + ((int64_t)(range.x + i) * 2 + (i == 0 ? 1 : 0)) * size; };
   float top = -__builtin_inff();
-  for (int i = threadIdx.x; i < parts; i += kThreads) top = fmaxf(top, part(i)[kHeads * DT + 2 * n]);
+  for (int i = threadIdx.x; i < parts; i += kJoin) top = fmaxf(top, part(i)[stats]);
   for (int m = 32; m; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
   if (lane == 0) tops[wave] = top;
   __syncthreads();
@@ -470,9 +456,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
   float tot = 0;
   for (int i = row; i < parts; i += kRows) {
     const float* a = part(i);
-    const float m = a[kHeads * DT + 2 * n];
-    const float f = m == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - top);
-    tot += f * a[kHeads * DT + 2 * n + 1];
+    const floatx2 m = *(const floatx2*)(a + stats);
+    const float f = m.x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m.x - top);
+    tot += f * m.y;
     acc += *(const floatx4*)(a + n * DT + 4 * d) * f;
   }
   __shared__ float rows[kRows];
@@ -490,7 +476,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
   if (4 * d < p.dim) {
     *(uintx2*)(p.out + (at * p.dim + 4 * d) * 2) = uintx2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
   }
-  if (d == 0 && p.lse) p.lse[at] = tot == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(tot)) * 0.6931471805599453f;
+  if (d == 0 && p.lse) p.lse[at] = tot == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(tot)) * kLn2;
 }
 
 int compute_units() {
@@ -505,8 +491,8 @@ int compute_units() {
 
 // How a call's work is laid out, from its sizes alone.
 struct Plan {
-  int dt, lists, group, tiles;
-  int64_t streams, work_groups;
+  int dt, lists, group, tiles, part_heads;
+  int64_t streams, waves;
   bool joins;
   int64_t ends_bytes, bytes;
 };
@@ -517,24 +503,26 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
   a.lists = (int)(lists ? lists : pages.heads);
   a.group = (int)(q_heads / a.lists);
   a.tiles = (a.group + kHeads - 1) / kHeads;
+  a.part_heads = std::min(a.group, kHeads);
   a.streams = (int64_t)a.lists * a.tiles;
   // a window's first group of 8 rows may start 7 tokens early
-  const int64_t units = std::max<int64_t>(1, (max_tokens + (lists ? 0 : 7) + kUnit - 1) / kUnit);
-  const int64_t resident = (int64_t)compute_units() * (a.dt == 256 ? 1 : 2);
-  a.work_groups = std::min(batch * a.streams * units, resident);
-  a.joins = units > 1;
+  const int64_t tiles = std::max<int64_t>(1, (max_tokens + (lists ? 0 : 7) + kTile - 1) / kTile);
+  if (tiles > 0x7FFFFFFF / std::max<int64_t>(1, batch * a.streams)) throw std::invalid_argument("batch x heads x tokens is too large");
+  const int64_t resident = (int64_t)compute_units() * (a.dt == 256 ? 4 : 8);
+  a.waves = std::min(batch * a.streams * tiles, resident);
+  a.joins = tiles > 1;
   a.ends_bytes = (batch * a.streams * 8 + 15) / 16 * 16;
-  a.bytes = a.ends_bytes + a.work_groups * 2 * kHeads * (a.dt + 2) * 4;
+  a.bytes = a.ends_bytes + a.waves * 2 * a.part_heads * (a.dt + 2) * 4;
   return a;
 }
 
 template <typename T, bool F8, int DT>
 void launch(const Params& p, const Plan& plan, bool listed, hipStream_t s) {
   auto kernel = listed ? attend_kernel<T, F8, DT, true> : attend_kernel<T, F8, DT, false>;
-  kernel<<<(unsigned)plan.work_groups, kThreads, 0, s>>>(p);
+  kernel<<<(unsigned)plan.waves, 64, 0, s>>>(p);
   hip_check(hipGetLastError(), "attention");
   if (plan.joins) {
-    join_kernel<T, DT><<<dim3((unsigned)(p.batch * plan.streams), (unsigned)std::min(kHeads, plan.group)), kThreads, 0, s>>>(p);
+    join_kernel<T, DT><<<dim3((unsigned)(p.batch * plan.streams), (unsigned)plan.part_heads), kJoin, 0, s>>>(p);
     hip_check(hipGetLastError(), "attention join");
   }
 }
@@ -557,7 +545,7 @@ void attend(const AttendArgs& a, const KvPages& pages, hipStream_t s) {
   const int64_t width = (int64_t)a.table_width << pages.page_shift;
   const bool listed = a.lists != 0;
   Params p{};
-  p.limit = pages.pages ? std::min(a.max_len, width) : 0;
+  p.limit = pages.pages ? (int)std::min<int64_t>({a.max_len, width, 0x7FFFFF00}) : 0;
   const int64_t most = listed ? a.first + a.last + a.count : a.last < 0 ? a.max_len : std::min(a.max_len, a.last);
   const Plan plan = plan_of(a.batch, a.q.heads, pages, most, a.lists);
   if (a.workspace_bytes < plan.bytes || !a.workspace || ((uintptr_t)a.workspace & 15u))
@@ -573,7 +561,7 @@ void attend(const AttendArgs& a, const KvPages& pages, hipStream_t s) {
   p.batch = (int)a.batch, p.heads = pages.heads, p.q_heads = a.q.heads;
   p.lists = plan.lists, p.group = plan.group, p.tiles = plan.tiles, p.count = pages.pages ? a.count : 0;
   p.page_shift = pages.page_shift, p.pages = pages.pages, p.dim = pages.dim;
-  p.first = a.first, p.last = a.last;
+  p.first = (int)a.first, p.last = (int)std::min<int64_t>(a.last, 0x7FFFFF00), p.part_heads = plan.part_heads;
   if (pages.type == kE4M3) {
     if (a.type == kF16) launch_dim<f16, true>(p, plan, listed, s);
     else launch_dim<bf16, true>(p, plan, listed, s);
