@@ -17,6 +17,8 @@ namespace {
 constexpr int kTile = 32;    // tokens a wave takes at once
 constexpr int kStage = 512;  // row offsets held in LDS
 constexpr int kHeads = 16;   // query heads of a matrix instruction
+constexpr int kStart = 2;    // what beginning a stream costs a wave, in tiles
+constexpr int kWaves = 2048;  // at most; of a call
 constexpr int kJoin = 256;   // threads of a joining work-group
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -82,7 +84,7 @@ __device__ __forceinline__ uint32_t from_e4m3(uint32_t w, bool high) {
 // base in tiles; of a list's places [0, end) the first `first` are tokens,
 // then come the tokens from `last` on, then the ids.
 struct Span {
-  int base, begin, end, tiles;  // base: begin rounded down to whole groups of 8 rows
+  int base, begin, end, tiles, cost;  // base: begin rounded down to whole groups of 8 rows
   int first, last;
 };
 
@@ -101,22 +103,26 @@ __device__ __forceinline__ Span span_of(const Params& p, int b) {
     s.end = len;
   }
   s.tiles = max(1, (s.end - s.base + kTile - 1) / kTile);  // a sequence of no tokens has its zeros written
+  s.cost = kStart + s.tiles;
   return s;
 }
 
-// How the tiles of all sequences and streams are shared out: the first
-// `more` of `waves` waves have each tiles + 1, the others each tiles.
+// How the work of all sequences and streams is shared out. A stream of n
+// tiles counts kStart + n units, as a wave that begins it first waits for its
+// queries and rows: of sequences with 17 to 8192 tokens, waves with equal
+// tiles took 71 us, the slowest ones eight short streams each. The first
+// `more` of `waves` waves have each + 1 units, the others each.
 struct Share {
   int each, more, waves;
   __device__ int begin(int w) const { return each * w + min(w, more); }
-  __device__ int owner(int tile) const {
+  __device__ int owner(int unit) const {
     const int longer = (each + 1) * more;
-    return tile < longer ? tile / (each + 1) : more + (tile - longer) / each;
+    return unit < longer ? unit / (each + 1) : more + (unit - longer) / each;
   }
 };
 
 // Every wave adds up the lengths for itself (lane i a run of sequences) and
-// finds the sequence its first tile lies in, and the tiles of one stream
+// finds the sequence its first unit lies in, and the units of one stream
 // before that sequence. -1: there is no work for it.
 template <bool LISTED>
 __device__ int find_sequence(const Params& p, int streams, Share& share, int& before) {
@@ -124,7 +130,7 @@ __device__ int find_sequence(const Params& p, int streams, Share& share, int& be
   const int run = (p.batch + 63) / 64;
   const int b0 = min(lane * run, p.batch), b1 = min(b0 + run, p.batch);
   int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += span_of<LISTED>(p, b).tiles;
+  for (int b = b0; b < b1; ++b) mine += span_of<LISTED>(p, b).cost;
   int incl = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -136,12 +142,12 @@ __device__ int find_sequence(const Params& p, int streams, Share& share, int& be
   share.each = total / share.waves;
   share.more = total % share.waves;
   if ((int)blockIdx.x >= share.waves) return -1;
-  const int at = share.begin(blockIdx.x) / streams;  // tile of a stream, were the streams side by side
+  const int at = share.begin(blockIdx.x) / streams;  // unit of a stream, were the streams side by side
   const int src = __ffsll((unsigned long long)__ballot(at < incl)) - 1;
   int pre = incl - mine, b = b0;
   if (lane == src) {
     for (;; ++b) {
-      const int n = span_of<LISTED>(p, b).tiles;
+      const int n = span_of<LISTED>(p, b).cost;
       if (at < pre + n) break;
       pre += n;
     }
@@ -187,14 +193,19 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
   int u = share.begin(blockIdx.x);
   const int u1 = share.begin(blockIdx.x + 1);
   Span sp = span_of<LISTED>(p, b);
-  int x = (u - before * streams) / sp.tiles;
-  int c = (u - before * streams) % sp.tiles;
+  int x = (u - before * streams) / sp.cost;
+  int pos = (u - before * streams) % sp.cost;
 
-  while (u < u1) {
+  for (; u < u1; u += sp.cost - pos, pos = 0, ++x) {
+    if (x == streams) {
+      x = 0;
+      sp = span_of<LISTED>(p, ++b);
+    }
+    const int c = max(0, pos - kStart), c1 = max(0, min(sp.cost, pos + (u1 - u)) - kStart);
+    if (c1 == c) continue;
     const int list = x / p.tiles, head0 = (x % p.tiles) * kHeads;
     const int h = list * p.heads / p.lists;
     const int n_heads = min(kHeads, p.group - head0);
-    const int c1 = min(sp.tiles, c + (u1 - u));
     const char* kb = p.k + h * p.head_stride * ES;
     const char* vb = p.v + h * p.head_stride * ES;
     const float cs = p.scale * (p.k_scale ? p.k_scale[h] : 1.f);
@@ -416,66 +427,76 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
         if (g == 0) *(floatx2*)(part + p.part_heads * DT + 2 * i) = floatx2{ref, sum};
       }
     }
-    if (c == 0 && lane == 0) p.ends[(int64_t)b * streams + x] = int2{(int)blockIdx.x, share.owner(u + sp.tiles - 1)};
-    u += c1 - c;
-    c = 0;
-    if (++x == streams) {
-      x = 0;
-      if (++b < p.batch) sp = span_of<LISTED>(p, b);
-    }
+    if (c == 0 && lane == 0) p.ends[(int64_t)b * streams + x] = int2{(int)blockIdx.x, share.owner(u - pos + sp.cost - 1)};
   }
 }
 
-// Joins the parts of a stream that several work-groups had: a work-group per
-// sequence, stream and head; the parts' weights first, then their sums.
+// Joins the parts of a stream that several waves had: a work-group per
+// sequence, stream and head. The parts' weights go to LDS, then a thread has
+// four dims of every kRows-th part, eight loads in flight.
 template <typename T, int DT>
 __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
   const int streams = p.lists * p.tiles;
-  const int64_t seq = blockIdx.x;
-  const int n = blockIdx.y;
-  const int b = (int)(seq / streams), x = (int)(seq % streams);
+  const int b = blockIdx.x / streams, x = blockIdx.x % streams, n = blockIdx.y;
   const int list = x / p.tiles, head0 = (x % p.tiles) * kHeads;
   if (n >= p.group - head0) return;
-  const int2 range = p.ends[seq];
+  const int2 range = p.ends[blockIdx.x];
   const int parts = range.y - range.x + 1;
   if (parts == 1) return;
-  constexpr int kLanes = DT / 4, kRows = kJoin / kLanes;
-  const int size = p.part_heads * (DT + 2), stats = p.part_heads * DT + 2 * n;
-  __shared__ float tops[kJoin / 64];
+  constexpr int kLanes = DT / 4, kRows = kJoin / kLanes, kBatch = 8;
+  __shared__ float weight[kWaves];
+  __shared__ float tops[kJoin / 64], tots[kJoin / 64];
   __shared__ floatx4 sums[kRows][kLanes];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  auto part = [&](int i) { return p.parts + ((int64_t)(range.x + i) * 2 + (i == 0 ? 1 : 0)) * size; };
+  const int size = p.part_heads * (DT + 2), stats = p.part_heads * DT + 2 * n;
+  const float* const own = p.parts + ((int64_t)range.x * 2 + 1) * size;  // the part that begins the stream
+  const float* const rest = own - size;                                   // part i > 0: 2 * size * i from here
+  const auto part = [&](int i) { return i ? rest + (int64_t)i * 2 * size : own; };
   float top = -__builtin_inff();
-  for (int i = threadIdx.x; i < parts; i += kJoin) top = fmaxf(top, part(i)[stats]);
+  for (int i = threadIdx.x; i < parts; i += kJoin) {
+    const float m = part(i)[stats];
+    weight[i] = m;
+    top = fmaxf(top, m);
+  }
   for (int m = 32; m; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
   if (lane == 0) tops[wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  float tot = 0;
+  for (int i = threadIdx.x; i < parts; i += kJoin) {
+    const float m = weight[i];
+    const float f = m == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - top);  // then its sums are zero (or NaN)
+    weight[i] = f;
+    tot += f * part(i)[stats + 1];
+  }
+  for (int m = 32; m; m >>= 1) tot += __shfl_xor(tot, m, 64);
+  if (lane == 0) tots[wave] = tot;
+  __syncthreads();
+  tot = (tots[0] + tots[1]) + (tots[2] + tots[3]);
   const int d = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
   floatx4 acc = {0, 0, 0, 0};
-  float tot = 0;
-  for (int i = row; i < parts; i += kRows) {
-    const float* a = part(i);
-    const floatx2 m = *(const floatx2*)(a + stats);
-    const float f = m.x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m.x - top);
-    tot += f * m.y;
-    acc += *(const floatx4*)(a + n * DT + 4 * d) * f;
+  for (int i0 = row; i0 < parts; i0 += kRows * kBatch) {
+    floatx4 y[kBatch];
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) {
+      const int i = i0 + e * kRows;
+      y[e] = *(const floatx4*)(part(i < parts ? i : i0) + n * DT + 4 * d);
+    }
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) {
+      const int i = i0 + e * kRows;
+      if (i < parts) acc += y[e] * weight[i];
+    }
   }
-  __shared__ float rows[kRows];
   sums[row][d] = acc;
-  if (d == 0) rows[row] = tot;
   __syncthreads();
   if (row) return;
-  tot = rows[0];
-  for (int r = 1; r < kRows; ++r) tot += rows[r], acc += sums[r][d];
-  const float vs = p.v_scale ? p.v_scale[list * p.heads / p.lists] : 1.f;
+  for (int r = 1; r < kRows; ++r) acc += sums[r][d];
   const int64_t at = (int64_t)b * p.q_heads + list * p.group + head0 + n;
-  const float inv = vs / tot;
+  const float inv = (p.v_scale ? p.v_scale[list * p.heads / p.lists] : 1.f) / tot;
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc[e] = tot == 0.f ? 0.f : acc[e] * inv;
-  if (4 * d < p.dim) {
-    *(uintx2*)(p.out + (at * p.dim + 4 * d) * 2) = uintx2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
-  }
+  if (4 * d < p.dim) *(uintx2*)(p.out + (at * p.dim + 4 * d) * 2) = uintx2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
   if (d == 0 && p.lse) p.lse[at] = tot == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(tot)) * kLn2;
 }
 
@@ -507,9 +528,9 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
   a.streams = (int64_t)a.lists * a.tiles;
   // a window's first group of 8 rows may start 7 tokens early
   const int64_t tiles = std::max<int64_t>(1, (max_tokens + (lists ? 0 : 7) + kTile - 1) / kTile);
-  if (tiles > 0x7FFFFFFF / std::max<int64_t>(1, batch * a.streams)) throw std::invalid_argument("batch x heads x tokens is too large");
-  const int64_t resident = (int64_t)compute_units() * (a.dt == 256 ? 4 : 8);
-  a.waves = std::min(batch * a.streams * tiles, resident);
+  if (tiles + kStart > 0x7FFFFFFF / std::max<int64_t>(1, batch * a.streams)) throw std::invalid_argument("batch x heads x tokens is too large");
+  const int64_t resident = std::min(kWaves, compute_units() * (a.dt == 256 ? 4 : 8));
+  a.waves = std::min(batch * a.streams * (tiles + kStart), resident);
   a.joins = tiles > 1;
   a.ends_bytes = (batch * a.streams * 8 + 15) / 16 * 16;
   a.bytes = a.ends_bytes + a.waves * 2 * a.part_heads * (a.dt + 2) * 4;
