@@ -33,6 +33,17 @@ __device__ __forceinline__ int64_t index_at(const void* p, bool wide, int64_t i)
   return wide ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
 }
 
+// x / d, with r = 1 / d rounded to nearest: one correction of x * r by its
+// exact remainder gives the quotient rounded to nearest (Markstein 1990),
+// short of under- and overflow; where x * r is too large for the cache, or not
+// finite, it is taken as it is. Three operations instead of the ten of a
+// division: 6007 tokens of 8 heads into an e4m3 cache 38.7 -> 31.8 us.
+__device__ __forceinline__ float quotient(float x, float d, float r) {
+  const float q = x * r;
+  const float fixed = __builtin_fmaf(__builtin_fmaf(-q, d, x), r, q);
+  return __builtin_fabsf(q) < 1e6f ? fixed : q;
+}
+
 // A thread has one chunk of 2 * P values of a head (threadIdx.x) and walks
 // the heads of its token (threadIdx.y on) with the chunk's P cosines and
 // sines in registers. In the half layout the chunk is P values of each half,
@@ -94,9 +105,9 @@ __global__ void token_kernel(TokenParams a) {
     } else {
       const float* scales = is_v ? a.pages.v_scale : a.pages.k_scale;
       if (sizeof(CT) == 1 && scales) {
-        const float scale = scales[hh];
+        const float scale = scales[hh], inverse = 1.f / scale;
 #pragma unroll
-        for (int e = 0; e < 2 * P; ++e) x[e] = x[e] / scale;
+        for (int e = 0; e < 2 * P; ++e) x[e] = quotient(x[e], scale, inverse);
       }
       CT* dst = (CT*)(is_v ? a.pages.v : a.pages.k) + page * a.pages.page_stride + hh * a.pages.head_stride +
                 in_page * a.pages.row_stride;
@@ -113,15 +124,16 @@ void launch_token(const TokenParams& p, int P, hipStream_t s) {
   const int chunks = p.dim / (2 * P);
   if (chunks > 1024) throw std::invalid_argument("a head is too large");
   // Few tokens: a thread per chunk of a head, so that a token is as many
-  // waves as it has work. Many: a wave per token, whose threads keep their
-  // cosines for several heads.
+  // waves as it has work. Many: half a wave per token, whose threads keep
+  // their cosines for several heads (8192 tokens of 32 + 8 heads of 128: 37.5
+  // us, 42.0 with a wave, 43.5 with two waves to a token).
   const int wide = std::max(1, 256 / chunks);
   dim3 block, grid;
   if (p.n < 1024) {
     block = dim3(chunks, std::min(all, wide), 1);
     grid = dim3((unsigned)p.n, (all + (int)block.y - 1) / (int)block.y);
   } else {
-    block = dim3(chunks, std::max(1, 64 / chunks), 1);
+    block = dim3(chunks, std::max(1, 32 / chunks), 1);
     block.z = std::max(1u, 256u / (block.x * block.y));
     const int64_t blocks = (p.n + block.z - 1) / block.z;
     if (blocks > 0x7FFFFFFF) throw std::invalid_argument("too many tokens (too large)");
