@@ -895,14 +895,15 @@ def save_groundtruth(path: str, indices: torch.Tensor, distances: torch.Tensor):
 
 
 from .groundtruth import bruteforce_knn, generate_groundtruth  # noqa: E402
-from .kvcache import (append_tokens, copy_pages, decode_attention, retrieved_attention, rotary,  # noqa: E402
-                      rotary_table)
+from .kvcache import (PagedCache, append_tokens, copy_pages, decode_attention, retrieved_attention,  # noqa: E402
+                      rotary, rotary_table)
 
 __all__ = [
     "Graph", "DistanceFunc", "DataType", "JasperError", "read_bin", "read_groundtruth",
     "get_recall", "generate_groundtruth", "bruteforce_knn", "save_groundtruth", "parse_storage_size",
     "last_build_stats", "last_scale_stats", "last_diskann_stats", "diskann_assign", "library_path",
     "rotary_table", "rotary", "append_tokens", "copy_pages", "decode_attention", "retrieved_attention",
+    "PagedCache",
 ]
 
 

@@ -25,37 +25,34 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 
 import numpy as np
 import torch
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1}
 _PAGE_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
+_F8 = torch.float8_e4m3fn
 
-_i32, _i64, _ptr, _f64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_double
+_i32, _i64, _ptr, _f64, _u32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_double, ctypes.c_uint32
+_struct = ctypes.c_char_p  # a struct's bytes, or None
 
-
-class _Pages(ctypes.Structure):
-    _fields_ = [("k", _ptr), ("v", _ptr), ("k_scale", _ptr), ("v_scale", _ptr),
-                ("layer_stride", _i64), ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64),
-                ("layers", _i32), ("pages", _i32), ("heads", _i32), ("page_size", _i32), ("dim", _i32), ("type", _i32)]
-
-
-class _Rows(ctypes.Structure):
-    _fields_ = [("data", _ptr), ("stride", _i64), ("head_stride", _i64), ("heads", _i64)]
-
+# jasperx_kv_pages and jasperx_head_rows. The calls here take about 10 us on
+# the host, as long as a small call's kernels: structs are packed, not
+# built as ctypes objects, and checks format their texts only when they fail.
+_pack_pages = struct.Struct("@PPPPqqqqiiiiii").pack
+_pack_rows = struct.Struct("@Pqqq").pack
 
 _SIGNATURES = {
-    "jasperx_rotary": [_ptr, _ptr, _i32, _i64, _i64, _ptr, _i32, _ptr, _ptr, _i64, _i64, ctypes.c_uint32, _ptr, _ptr,
-                       _ptr],
-    "jasperx_append_tokens": [_ptr, _ptr, _ptr, _i32, _i64, _ptr, _ptr, _i32, _ptr, _ptr, _i64, _i64,
-                              ctypes.c_uint32, _ptr, _ptr, _ptr],
-    "jasperx_copy_pages": [_ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr],
-    "jasperx_decode_attention": [_ptr, _i32, _i64, _ptr, _ptr, _i64, _i64, _ptr, _i64, _f64, _i64, _ptr, _ptr, _ptr,
-                                 _i64, _ptr],
-    "jasperx_retrieved_attention": [_ptr, _i32, _i64, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64, _i64,
-                                    _f64, _ptr, _ptr, _ptr, _i64, _ptr],
-    "jasperx_attention_workspace": [_i64, _i64, _ptr, _i64, _i64],
+    "jasperx_rotary": [_struct, _struct, _i32, _i64, _i64, _ptr, _i32, _ptr, _ptr, _i64, _i64, _u32, _ptr, _ptr, _ptr],
+    "jasperx_append_tokens": [_struct, _struct, _struct, _i32, _i64, _ptr, _ptr, _i32, _ptr, _ptr, _i64, _i64, _u32,
+                              _struct, _ptr, _ptr],
+    "jasperx_copy_pages": [_struct, _ptr, _ptr, _i64, _ptr, _i64, _ptr],
+    "jasperx_decode_attention": [_struct, _i32, _i64, _struct, _ptr, _i64, _i64, _ptr, _i64, _f64, _i64, _ptr, _ptr,
+                                 _ptr, _i64, _ptr],
+    "jasperx_retrieved_attention": [_struct, _i32, _i64, _struct, _ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64,
+                                    _i64, _f64, _ptr, _ptr, _ptr, _i64, _ptr],
+    "jasperx_attention_workspace": [_i64, _i64, _struct, _i64, _i64],
 }
 
 
@@ -65,72 +62,66 @@ def _fn(name):
     return _bind(name, _SIGNATURES[name])
 
 
+# the current stream's handle without a Stream object around it
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def _call(name, device, *args):
-    """The C call `name` on the device's current stream (its last argument)."""
-    if device.index != torch.cuda.current_device():
+    """The C call `name` on the current stream of GPU `device` (an index)."""
+    if device != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _fn(name)(*args, torch.cuda.current_stream(device).cuda_stream)
-    return _fn(name)(*args, torch.cuda.current_stream(device).cuda_stream)
+            _fn(name)(*args, _stream(device))
+    else:
+        _fn(name)(*args, _stream(device))
 
 
-def _need(ok, text):
-    if not ok:
-        raise ValueError(text)
+def _place(device):
+    return "a CPU tensor" if device < 0 else f"on GPU {device}"
 
 
-def _on_gpu(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must be on {device}, got {t.device}")
-
-
-def _index(name, t, device):
+def _indexes(name, t, device):
     """An int32 or int64 tensor as a contiguous one."""
     if t.dtype != torch.int64 and t.dtype != torch.int32:
         raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on GPU {device}, is {_place(t.get_device())}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _int32(name, t, ndim, device):
-    if t.dtype != torch.int32 or t.ndim != ndim:
-        raise ValueError(f"{name} must be a {ndim}D int32 tensor, got {t.ndim}D {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    return t
-
-
-def _scales(name, t, heads, pages):
+def _scale_ptr(name, t, heads, pages):
     if t is None:
-        return None
-    _need(pages.dtype == torch.float8_e4m3fn, f"{name} needs float8_e4m3fn pages")
-    _need(t.dtype == torch.float32 and t.shape == (heads,) and t.is_contiguous() and t.device == pages.device,
-          f"{name} must be a contiguous float32 [{heads}] tensor on the pages' device")
+        return 0
+    if pages.dtype != _F8:
+        raise ValueError(f"{name} needs float8_e4m3fn pages")
+    if t.dtype != torch.float32 or t.shape != (heads,) or not t.is_contiguous() or t.device != pages.device:
+        raise ValueError(f"{name} must be a contiguous float32 [{heads}] tensor on the pages' device")
     return t.data_ptr()
 
 
 def _pages(k_pages, v_pages, k_scale=None, v_scale=None, layers=False):
-    """The C description of a pair of page tensors, checked."""
-    if k_pages.dtype not in _PAGE_TYPES:
+    """(C struct, sizes (heads, page_size, dim), type, GPU) of a pair of page tensors, checked."""
+    shape, stride, device = k_pages.shape, k_pages.stride(), k_pages.get_device()
+    type_ = _PAGE_TYPES.get(k_pages.dtype)
+    if type_ is None:
         raise ValueError(f"pages must be float16, bfloat16 or float8_e4m3fn, got {k_pages.dtype}")
-    if (v_pages.dtype != k_pages.dtype or v_pages.shape != k_pages.shape or v_pages.device != k_pages.device
-            or v_pages.stride() != k_pages.stride()):
+    if (v_pages.dtype != k_pages.dtype or v_pages.shape != shape or v_pages.get_device() != device
+            or v_pages.stride() != stride):
         raise ValueError("k_pages and v_pages must have the same type, shape, strides and device")
-    if not k_pages.is_cuda:
+    if device < 0:
         raise ValueError("k_pages must be a CUDA tensor")
-    shape, stride = k_pages.shape, k_pages.stride()
-    if layers and len(shape) == 4:
-        shape, stride = (1, *shape), (0, *stride)
-    if len(shape) != (5 if layers else 4):
-        raise ValueError(f"pages must be [{'layers, ' if layers else ''}n_pages, kv_heads, page_size, dim], got {k_pages.ndim}D")
-    if not layers:
-        shape, stride = (1, *shape), (0, *stride)
-    if stride[4] != 1:
+    count, layer_stride = 1, 0
+    if layers and len(shape) == 5:
+        count, layer_stride, shape, stride = shape[0], stride[0], shape[1:], stride[1:]
+    if len(shape) != 4:
+        raise ValueError(f"pages must be [{'layers, ' if layers else ''}n_pages, kv_heads, page_size, dim], "
+                         f"got {k_pages.ndim}D")
+    if stride[3] != 1:
         raise ValueError("the last dimension of the pages must be contiguous")
-    return _Pages(k_pages.data_ptr(), v_pages.data_ptr(), _scales("k_scale", k_scale, shape[2], k_pages),
-                  _scales("v_scale", v_scale, shape[2], k_pages), stride[0], stride[1], stride[2], stride[3],
-                  shape[0], shape[1], shape[2], shape[3], shape[4], _PAGE_TYPES[k_pages.dtype])
+    n, heads, page, dim = shape
+    c = _pack_pages(k_pages.data_ptr(), v_pages.data_ptr(), _scale_ptr("k_scale", k_scale, heads, k_pages),
+                    _scale_ptr("v_scale", v_scale, heads, k_pages), layer_stride, stride[0], stride[1], stride[2],
+                    count, n, heads, page, dim, type_)
+    return c, (heads, page, dim), type_, device
 
 
 # ---- rotary positions ----
@@ -149,10 +140,12 @@ def rotary_table(n_positions: int, rot_dim: int, base: float = 10000.0, scaling:
     blends between, and scales the tables by 0.1 ln(factor) + 1. Angles are
     made in 64 bits: at position 100,000 a 32-bit angle is off by 0.004.
     """
-    _need(n_positions >= 0, "n_positions must be at least 0")
-    _need(rot_dim > 0 and rot_dim % 2 == 0, "rot_dim must be even and positive")
-    _need(scaling in (None, "linear", "ntk", "yarn"), f"Unknown scaling: {scaling!r}")
-    _need(scaling is None or factor >= 1.0, "factor must be at least 1")
+    if n_positions < 0 or rot_dim <= 0 or rot_dim % 2:
+        raise ValueError("n_positions must be at least 0 and rot_dim even and positive")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"Unknown scaling: {scaling!r}")
+    if scaling is not None and factor < 1.0:
+        raise ValueError("factor must be at least 1")
     pair = torch.arange(0, rot_dim, 2, dtype=torch.float64)
     size = 1.0
     if scaling == "ntk" and rot_dim > 2:
@@ -161,7 +154,8 @@ def rotary_table(n_positions: int, rot_dim: int, base: float = 10000.0, scaling:
     if scaling == "linear":
         freq = freq / factor
     elif scaling == "yarn":
-        _need(original is not None and original > 0, "yarn scaling needs the original context length")
+        if original is None or original <= 0:
+            raise ValueError("yarn scaling needs the original context length")
 
         def at(turns):  # the pair that turns so many times within the original context
             return rot_dim * math.log(original / (2 * math.pi * turns)) / (2 * math.log(base))
@@ -176,52 +170,48 @@ def rotary_table(n_positions: int, rot_dim: int, base: float = 10000.0, scaling:
 
 
 def _table(cos, sin, device):
+    """(cos, sin pointers, positions, rotated values) of a pair of tables."""
     if cos is None and sin is None:
         return None, None, 0, 0
-    _need(cos is not None and sin is not None, "cos and sin come together")
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.ndim != 2 or cos.shape != sin.shape
-            or not cos.is_contiguous() or not sin.is_contiguous()):
-        raise ValueError("cos and sin must be contiguous float32 [n_positions, rot_dim / 2] tensors")
-    _on_gpu(device, cos=cos, sin=sin)
+    if (cos is None or sin is None or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.ndim != 2
+            or cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous()
+            or cos.get_device() != device or sin.get_device() != device):
+        raise ValueError(f"cos and sin must be contiguous float32 [n_positions, rot_dim / 2] tensors on GPU {device}")
     return cos.data_ptr(), sin.data_ptr(), cos.size(0), 2 * cos.size(1)
 
 
-def _heads(name, t, like):
-    """[..., heads, dim] as rows [n, heads, dim] whose values are contiguous."""
-    if t.ndim < 2:
-        raise ValueError(f"{name} must be [..., heads, dim]")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape[:-2] != like.shape[:-2]
-                             or t.size(-1) != like.size(-1)):
-        raise ValueError(f"{name} must match the other rows in type, device, leading sizes and dim")
+def _head_rows(t):
+    """(C struct, the tensor it describes) of [..., heads, dim] as rows [n, heads, dim] with contiguous values."""
     if t.ndim != 3:
         t = t.flatten(0, -3) if t.ndim > 3 else t[None]
-    return t if t.stride(2) == 1 else t.contiguous()
+    stride = t.stride()
+    if stride[2] != 1:
+        t = t.contiguous()
+        stride = t.stride()
+    return _pack_rows(t.data_ptr(), stride[0], stride[1], t.size(1)), t
 
 
-def _rows(t):
-    return _Rows(t.data_ptr(), t.stride(0), t.stride(1), t.size(1))
+def _alike(name, t, like):
+    if (t.dtype != like.dtype or t.get_device() != like.get_device() or t.ndim != like.ndim
+            or t.shape[:-2] != like.shape[:-2] or t.size(-1) != like.size(-1)):
+        raise ValueError(f"{name} must match the other rows in type, device, leading sizes and dim")
 
 
 def _rotate(q, k, positions, cos, sin, interleaved, back):
+    """The rotation of checked arguments."""
     first = q if q is not None else k
-    device = first.device
-    n = math.prod(first.shape[:-2])
-    dim = first.size(-1)
+    device = first.get_device()
     c, s, table_rows, rot = _table(cos, sin, device)
-    outs, rows = [], []
-    for name, t in (("q", q), ("k", k)):
-        if t is None:
-            outs.append(None)
-            rows.append(None)
-            continue
-        flat = _heads(name, t, first)
-        rows.append((flat, _rows(flat)))
-        outs.append(torch.empty(t.shape, dtype=t.dtype, device=device))
+    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    n = positions.numel()
     if n:
-        _call("jasperx_rotary", device, *(None if r is None else ctypes.byref(r[1]) for r in rows),
-              _TYPES[first.dtype], n, dim, positions.data_ptr(), positions.element_size(), c, s, table_rows, rot,
-              (1 if interleaved else 0) | (2 if back else 0), *(None if o is None else o.data_ptr() for o in outs))
-    return outs
+        q_rows, q = (None, None) if q is None else _head_rows(q)
+        k_rows, k = (None, None) if k is None else _head_rows(k)
+        _call("jasperx_rotary", device, q_rows, k_rows, _TYPES[first.dtype], n, first.size(-1), positions.data_ptr(),
+              positions.element_size(), c, s, table_rows, rot, (1 if interleaved else 0) | (2 if back else 0),
+              None if q_out is None else q_out.data_ptr(), None if k_out is None else k_out.data_ptr())
+    return q_out, k_out
 
 
 class _Rotary(torch.autograd.Function):
@@ -233,17 +223,20 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(positions, cos, sin)
         ctx.flags = interleaved, back
         ctx.set_materialize_grads(False)
-        return tuple(_rotate(q, k, positions, cos, sin, interleaved, back))
+        return _rotate(q, k, positions, cos, sin, interleaved, back)
 
     @staticmethod
     def backward(ctx, gq, gk):
-        gq = gq if ctx.needs_input_grad[0] else None
-        gk = gk if ctx.needs_input_grad[1] else None
+        if not ctx.needs_input_grad[0]:
+            gq = None
+        if not ctx.needs_input_grad[1]:
+            gk = None
         if gq is None and gk is None:
             return (None,) * 7
         interleaved, back = ctx.flags
-        out = _Rotary.apply(gq, gk, *ctx.saved_tensors, interleaved, not back)
-        return (*out, None, None, None, None, None)
+        turn = _Rotary.apply if torch.is_grad_enabled() else _rotate
+        dq, dk = turn(gq, gk, *ctx.saved_tensors, interleaved, not back)
+        return dq, dk, None, None, None, None, None
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -257,20 +250,21 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos
     """
     if q.dtype not in _TYPES:
         raise ValueError(f"q must be float16 or bfloat16, got {q.dtype}")
-    if not q.is_cuda:
+    device = q.get_device()
+    if device < 0:
         raise ValueError("q must be a CUDA tensor")
     if q.ndim < 2 or q.size(-1) % 2:
         raise ValueError("q must be [..., heads, dim] with an even dim")
     if k is not None:
-        _heads("k", k, q)
-    positions = _index("positions", positions, q.device)
-    _need(positions.shape == q.shape[:-2], f"positions must be {list(q.shape[:-2])}, got {list(positions.shape)}")
-    _need(cos is not None and sin is not None, "cos and sin are needed")
-    _table(cos, sin, q.device)
-    _need(2 * cos.size(1) <= q.size(-1), "the tables rotate more values than a head has")
+        _alike("k", k, q)
+    positions = _indexes("positions", positions, device)
+    if positions.shape != q.shape[:-2]:
+        raise ValueError(f"positions must be {list(q.shape[:-2])}, got {list(positions.shape)}")
+    if cos is None or sin is None or cos.ndim != 2 or 2 * cos.size(1) > q.size(-1):
+        raise ValueError("cos and sin must be [n_positions, rot_dim / 2] with rot_dim at most dim")
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(q, k, positions, cos, sin, bool(interleaved), False)
-    return tuple(_rotate(q, k, positions, cos, sin, bool(interleaved), False))
+        return _Rotary.apply(q, k, positions, cos, sin, interleaved, False)
+    return _rotate(q, k, positions, cos, sin, interleaved, False)
 
 
 # ---- the cache ----
@@ -287,40 +281,44 @@ def append_tokens(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, posi
     rounded to nearest and saturated at +-448. No two tokens may have one
     slot. q, k and v may be slices of one projection's output.
     """
-    p = _pages(k_pages, v_pages, k_scale, v_scale)
-    device = k_pages.device
-    if k.dtype not in _TYPES:
-        raise ValueError(f"k must be float16 or bfloat16, got {k.dtype}")
-    if k_pages.dtype != torch.float8_e4m3fn and k_pages.dtype != k.dtype:
-        raise ValueError(f"pages must be {k.dtype} or float8_e4m3fn, got {k_pages.dtype}")
-    _need(k.ndim == 3 and k.size(1) == p.heads and k.size(2) == p.dim, f"k must be [n, {p.heads}, {p.dim}]")
-    _need(v.shape == k.shape, "v must have k's shape")
-    _on_gpu(device, k=k)
-    k, v = _heads("k", k, None), _heads("v", v, k)
-    n = k.size(0)
-    out = None
+    pages, (heads, _, dim), type_, device = _pages(k_pages, v_pages, k_scale, v_scale)
+    if k.dtype not in _TYPES or (type_ != 2 and k_pages.dtype != k.dtype):
+        raise ValueError(f"k must be float16 or bfloat16 and the pages of its type or float8_e4m3fn, got {k.dtype} "
+                         f"and {k_pages.dtype}")
+    if k.ndim != 3 or k.size(1) != heads or k.size(2) != dim or k.get_device() != device:
+        raise ValueError(f"k must be [n, {heads}, {dim}] on GPU {device}")
+    _alike("v", v, k)
+    if v.size(1) != heads:
+        raise ValueError(f"v must be [n, {heads}, {dim}]")
     if q is not None:
-        _need(q.ndim == 3, "q must be [n, heads, dim]")
-        q = _heads("q", q, k)
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        _alike("q", q, k)
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
         raise ValueError("append_tokens has no gradient: use rotary, or torch.no_grad()")
-    slots = _index("slots", slots, device)
-    _need(slots.shape == (n,), f"slots must be [{n}]")
+    n = k.size(0)
+    slots = _indexes("slots", slots, device)
+    if slots.shape != (n,):
+        raise ValueError(f"slots must be [{n}]")
     c, s, table_rows, rot = _table(cos, sin, device)
-    _need(rot <= p.dim, "the tables rotate more values than a head has")
     at = None
     if rot:
-        _need(positions is not None, "positions are needed with cos and sin")
-        positions = _index("positions", positions, device)
-        _need(positions.shape == (n,), f"positions must be [{n}]")
+        if rot > dim:
+            raise ValueError("the tables rotate more values than a head has")
+        if positions is None:
+            raise ValueError("positions are needed with cos and sin")
+        positions = _indexes("positions", positions, device)
+        if positions.shape != (n,):
+            raise ValueError(f"positions must be [{n}]")
         if positions.dtype != slots.dtype:
             positions, slots = positions.long(), slots.long()
         at = positions.data_ptr()
+    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if n:
-        _call("jasperx_append_tokens", device, None if q is None else ctypes.byref(_rows(q)), ctypes.byref(_rows(k)),
-              ctypes.byref(_rows(v)), _TYPES[k.dtype], n, at, slots.data_ptr(), slots.element_size(), c, s,
-              table_rows, rot, 1 if interleaved else 0, ctypes.byref(p), None if out is None else out.data_ptr())
+        q_rows, q = (None, None) if q is None else _head_rows(q)
+        k_rows, k = _head_rows(k)
+        v_rows, v = _head_rows(v)
+        _call("jasperx_append_tokens", device, q_rows, k_rows, v_rows, _TYPES[k.dtype], n, at, slots.data_ptr(),
+              slots.element_size(), c, s, table_rows, rot, 1 if interleaved else 0, pages,
+              None if out is None else out.data_ptr())
     return out
 
 
@@ -332,50 +330,55 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     entries equal to src[i] become dst[i]. No page may be a source and a
     destination, or the destination of two. Pairs with an id outside the
     cache are skipped."""
-    p = _pages(k_pages, v_pages, layers=True)
-    device = k_pages.device
-    src, dst = _int32("src", src, 1, device), _int32("dst", dst, 1, device)
-    _need(src.shape == dst.shape, "src and dst must have the same length")
-    entries = 0
+    pages, _, _, device = _pages(k_pages, v_pages, layers=True)
+    for name, t in (("src", src), ("dst", dst)):
+        if t.dtype != torch.int32 or t.ndim != 1 or t.get_device() != device or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous 1D int32 tensor on GPU {device}")
+    n, entries = src.numel(), 0
+    if dst.numel() != n:
+        raise ValueError("src and dst must have the same length")
     if tables is not None:
-        _need(tables.dtype == torch.int32 and tables.is_contiguous() and tables.device == device,
-              "tables must be a contiguous int32 tensor on the pages' device")
+        if tables.dtype != torch.int32 or not tables.is_contiguous() or tables.get_device() != device:
+            raise ValueError(f"tables must be a contiguous int32 tensor on GPU {device}")
         entries = tables.numel()
-    src, dst = src.contiguous(), dst.contiguous()
-    if src.numel():
-        _call("jasperx_copy_pages", device, ctypes.byref(p), src.data_ptr(), dst.data_ptr(), src.numel(),
+    if n:
+        _call("jasperx_copy_pages", device, pages, src.data_ptr(), dst.data_ptr(), n,
               tables.data_ptr() if entries else None, entries)
 
 
 # ---- attention of one new token ----
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(device, batch, q_heads, heads, page_size, dim, type_, max_tokens, lists):
-    p = _Pages(None, None, None, None, 0, 0, 0, dim, 1, 0, heads, page_size, dim, type_)
+def _workspace_bytes(device, batch, q_heads, sizes, type_, max_tokens, lists):
+    heads, page, dim = sizes
+    pages = _pack_pages(0, 0, 0, 0, 0, 0, 0, dim, 1, 0, heads, page, dim, type_)
     with torch.cuda.device(device):
-        return _fn("jasperx_attention_workspace")(batch, q_heads, ctypes.byref(p), max_tokens, lists)
+        return _fn("jasperx_attention_workspace")(batch, q_heads, pages, max_tokens, lists)
 
 
-def _attention_args(q, p, k_pages, tables, lens):
-    device = k_pages.device
-    if q.dtype not in _TYPES or (k_pages.dtype != torch.float8_e4m3fn and k_pages.dtype != q.dtype):
+def _query(q, sizes, type_, k_pages, tables, lens, device):
+    """(C struct, q, lens) of checked queries, tables and lengths."""
+    heads, _, dim = sizes
+    if q.dtype not in _TYPES or (type_ != 2 and k_pages.dtype != q.dtype):
         raise ValueError(f"q must be float16 or bfloat16 and the pages of its type or float8_e4m3fn, got {q.dtype} "
                          f"and {k_pages.dtype}")
-    _need(q.ndim == 3 and q.size(2) == p.dim, f"q must be [batch, heads, {p.dim}]")
-    if q.device != device:
-        raise ValueError(f"q must be on {device}, got {q.device}")
-    _need(q.size(1) > 0 and q.size(1) % p.heads == 0, f"q's heads must be a multiple of the cache's {p.heads}")
-    if torch.is_grad_enabled() and q.requires_grad:
+    if q.ndim != 3 or q.size(2) != dim or q.size(1) == 0 or q.size(1) % heads or q.get_device() != device:
+        raise ValueError(f"q must be [batch, a multiple of {heads} heads, {dim}] on GPU {device}")
+    if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("attention over the cache has no gradient: use torch.no_grad()")
     b = q.size(0)
-    _int32("tables", tables, 2, device)
-    _need(tables.size(0) == b and (tables.size(1) <= 1 or tables.stride(1) == 1),
-          f"tables must be [{b}, pages] with contiguous rows")
-    _int32("lens", lens, 1, device)
-    _need(lens.size(0) == b, f"lens must be [{b}]")
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    if (tables.dtype != torch.int32 or tables.ndim != 2 or tables.size(0) != b or tables.get_device() != device
+            or (tables.size(1) > 1 and tables.stride(1) != 1)):
+        raise ValueError(f"tables must be int32 [{b}, pages] with contiguous rows, on GPU {device}")
+    if lens.dtype != torch.int32 or lens.shape != (b,) or lens.get_device() != device:
+        raise ValueError(f"lens must be int32 [{b}] on GPU {device}")
+    if not lens.is_contiguous():
+        lens = lens.contiguous()
+    stride, at = q.stride(), q.data_ptr()
+    if stride[2] != 1 or stride[0] % 8 or stride[1] % 8 or at % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    return q, tables, lens if lens.is_contiguous() else lens.contiguous(), device
+        stride, at = q.stride(), q.data_ptr()
+    return _pack_rows(at, stride[0], stride[1], q.size(1)), q, lens
 
 
 def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
@@ -391,26 +394,26 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     Returns out [batch, heads, dim] in q's type, and with return_lse the
     logarithm of the sum of exp(scores) in float32 [batch, heads]; a sequence
     without tokens gives 0 and -inf. Whatever the rows past a sequence's end
-    hold is not seen. max_len: no sequence is longer (default: what tables can
-    hold); the work is laid out for it, and tokens past it are not read.
+    hold is not seen, nor are tokens whose table entry is no page. max_len: no
+    sequence is longer (default: what tables can hold); the work is laid out
+    for it, and tokens past it are not read.
     """
-    p = _pages(k_pages, v_pages, k_scale, v_scale)
-    q, tables, lens, device = _attention_args(q, p, k_pages, tables, lens)
-    _need(window >= 0, "window must be at least 0")
+    pages, sizes, type_, device = _pages(k_pages, v_pages, k_scale, v_scale)
+    rows, q, lens = _query(q, sizes, type_, k_pages, tables, lens, device)
+    if window < 0 or (max_len is not None and max_len < 0):
+        raise ValueError("window and max_len must be at least 0")
     b, heads, dim = q.shape
-    capacity = tables.size(1) * p.page_size
-    max_len = capacity if max_len is None else min(int(max_len), capacity)
-    _need(max_len >= 0, "max_len must be at least 0")
-    out = torch.empty((b, heads, dim), dtype=q.dtype, device=device)
-    lse = torch.empty((b, heads), dtype=torch.float32, device=device) if return_lse else None
+    most = tables.size(1) * sizes[1]
+    if max_len is not None and max_len < most:
+        most = max_len
+    out = torch.empty((b, heads, dim), dtype=q.dtype, device=q.device)
+    lse = torch.empty((b, heads), dtype=torch.float32, device=q.device) if return_lse else None
     if b:
-        size = _workspace_bytes(device, b, heads, p.heads, p.page_size, dim, p.type,
-                                min(max_len, window) if window else max_len, 0)
-        scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        _call("jasperx_decode_attention", device, ctypes.byref(_rows(q)), _TYPES[q.dtype], b, ctypes.byref(p),
-              tables.data_ptr(), tables.stride(0), tables.size(1), lens.data_ptr(), max_len,
-              dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
-              lse.data_ptr() if return_lse else None, scratch.data_ptr() if size else None, size)
+        size = _workspace_bytes(device, b, heads, sizes, type_, window if 0 < window < most else most, 0)
+        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
+        _call("jasperx_decode_attention", device, rows, _TYPES[q.dtype], b, pages, tables.data_ptr(),
+              tables.stride(0), tables.size(1), lens.data_ptr(), most, dim ** -0.5 if scale is None else scale, window,
+              out.data_ptr(), lse.data_ptr() if return_lse else None, scratch.data_ptr(), size)
     return (out, lse) if return_lse else out
 
 
@@ -424,22 +427,279 @@ def retrieved_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     query heads (each has its own) or of key heads (shared). Ids outside
     [first, len - last), such as a search's -1, are left out: the first and
     last tokens are there already. An id listed twice counts twice."""
-    p = _pages(k_pages, v_pages, k_scale, v_scale)
-    q, tables, lens, device = _attention_args(q, p, k_pages, tables, lens)
+    pages, sizes, type_, device = _pages(k_pages, v_pages, k_scale, v_scale)
+    rows, q, lens = _query(q, sizes, type_, k_pages, tables, lens, device)
     b, heads, dim = q.shape
-    _int32("ids", ids, 3, device)
+    if (ids.dtype != torch.int32 or ids.ndim != 3 or ids.size(0) != b or ids.size(1) not in (heads, sizes[0])
+            or ids.get_device() != device):
+        raise ValueError(f"ids must be int32 [{b}, {heads} or {sizes[0]}, count] on GPU {device}")
+    if first < 0 or last < 0:
+        raise ValueError("first and last must be at least 0")
     lists, count = ids.size(1), ids.size(2)
-    _need(ids.size(0) == b and lists in (heads, p.heads), f"ids must be [{b}, {heads} or {p.heads}, count]")
-    _need(first >= 0 and last >= 0, "first and last must be at least 0")
     if not ids.is_contiguous():
         ids = ids.contiguous()
-    out = torch.empty((b, heads, dim), dtype=q.dtype, device=device)
-    lse = torch.empty((b, heads), dtype=torch.float32, device=device) if return_lse else None
+    out = torch.empty((b, heads, dim), dtype=q.dtype, device=q.device)
+    lse = torch.empty((b, heads), dtype=torch.float32, device=q.device) if return_lse else None
     if b:
-        size = _workspace_bytes(device, b, heads, p.heads, p.page_size, dim, p.type, first + last + count, lists)
-        scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        _call("jasperx_retrieved_attention", device, ctypes.byref(_rows(q)), _TYPES[q.dtype], b, ctypes.byref(p),
-              tables.data_ptr(), tables.stride(0), tables.size(1), lens.data_ptr(), ids.data_ptr(), lists, count,
-              first, last, dim ** -0.5 if scale is None else scale, out.data_ptr(),
-              lse.data_ptr() if return_lse else None, scratch.data_ptr() if size else None, size)
+        size = _workspace_bytes(device, b, heads, sizes, type_, first + last + count, lists)
+        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
+        _call("jasperx_retrieved_attention", device, rows, _TYPES[q.dtype], b, pages, tables.data_ptr(),
+              tables.stride(0), tables.size(1), lens.data_ptr(), ids.data_ptr(), lists, count, first, last,
+              dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr() if return_lse else None,
+              scratch.data_ptr(), size)
     return (out, lse) if return_lse else out
+
+
+# ---- pages and sequences ----
+
+class PageTable:
+    """Which pages the sequences of a cache have: host bookkeeping, with the
+    copies and table entries that follow from it for the GPU. Pages are
+    counted by their owners; a sequence that is forked shares all of them, and
+    has its last one copied when it grows while that page is shared."""
+
+    def __init__(self, n_pages: int, page_size: int, max_sequences: int, max_pages: int):
+        if min(n_pages, max_sequences, max_pages) < 1 or page_size < 1:
+            raise ValueError("n_pages, page_size, max_sequences and max_pages must be at least 1")
+        self.page_size = page_size
+        self.pages = np.full((max_sequences, max_pages), -1, dtype=np.int32)
+        self.lens = np.full(max_sequences, -1, dtype=np.int64)  # -1: no such sequence
+        self.refs = np.zeros(n_pages, dtype=np.int32)
+        self._free = list(range(n_pages - 1, -1, -1))
+
+    @property
+    def n_free(self) -> int:
+        return len(self._free)
+
+    def check(self, seqs) -> np.ndarray:
+        seqs = np.atleast_1d(np.asarray(seqs, dtype=np.int64))
+        if seqs.ndim != 1 or len(np.unique(seqs)) != len(seqs):
+            raise ValueError("sequences must be a list without repeats")
+        if ((seqs < 0) | (seqs >= len(self.lens))).any() or (self.lens[seqs] < 0).any():
+            raise ValueError(f"no such sequence among {seqs.tolist()}")
+        return seqs
+
+    def _count(self, seq) -> int:
+        return -(-int(self.lens[seq]) // self.page_size)
+
+    def new(self) -> int:
+        free = np.flatnonzero(self.lens < 0)
+        if not len(free):
+            raise RuntimeError(f"all {len(self.lens)} sequences are in use")
+        self.lens[free[0]] = 0
+        return int(free[0])
+
+    def fork(self, seq: int) -> int:
+        seq = int(self.check([seq])[0])
+        other, n = self.new(), self._count(seq)
+        self.lens[other] = self.lens[seq]
+        self.pages[other, :n] = self.pages[seq, :n]
+        np.add.at(self.refs, self.pages[seq, :n], 1)
+        return other
+
+    def free(self, seqs) -> None:
+        for seq in self.check(seqs):
+            mine = self.pages[seq, :self._count(seq)]
+            self.refs[mine] -= 1
+            self._free.extend(sorted((int(p) for p in mine if self.refs[p] == 0), reverse=True))
+            self.lens[seq] = -1
+
+    def extend(self, seqs, counts):
+        """Room for counts[i] more tokens of seqs[i]. Returns (positions,
+        slots) of the new tokens, sequence by sequence, the pages to copy
+        first [(src, dst)] and the changed entries [(sequence, index, page)].
+        Without enough pages nothing is changed."""
+        seqs = self.check(seqs)
+        counts = np.broadcast_to(np.asarray(counts, dtype=np.int64), seqs.shape)
+        if (counts < 0).any():
+            raise ValueError("counts must be at least 0")
+        ps, old = self.page_size, self.lens[seqs]
+        new = old + counts
+        have, need = -(-old // ps), -(-new // ps)
+        if len(seqs) and need.max() > self.pages.shape[1]:
+            raise ValueError(f"a sequence of {int(new.max())} tokens is too large for a table of {self.pages.shape[1]} pages")
+        tail = (counts > 0) & (old % ps != 0)
+        last = self.pages[seqs, np.maximum(have - 1, 0)]
+        shared, growing = np.unique(last[tail], return_counts=True)
+        copies_needed = np.minimum(growing, self.refs[shared] - 1).sum()  # the last owner keeps the page
+        if (need - have).sum() + copies_needed > len(self._free):
+            raise RuntimeError(f"out of pages: {int((need - have).sum() + copies_needed)} needed, {len(self._free)} free")
+        copies, changed = [], []
+        for i in np.flatnonzero((need > have) | tail):
+            seq = int(seqs[i])
+            if tail[i] and self.refs[last[i]] > 1:
+                page = self._free.pop()
+                self.refs[last[i]] -= 1
+                self.refs[page] = 1
+                copies.append((int(last[i]), page))
+                self.pages[seq, have[i] - 1] = page
+                changed.append((seq, int(have[i]) - 1, page))
+            for at in range(int(have[i]), int(need[i])):
+                page = self._free.pop()
+                self.refs[page] = 1
+                self.pages[seq, at] = page
+                changed.append((seq, at, page))
+        self.lens[seqs] = new
+        of = np.repeat(np.arange(len(seqs)), counts)
+        starts = np.cumsum(counts) - counts
+        positions = np.arange(int(counts.sum())) - np.repeat(starts - old, counts)
+        slots = self.pages[seqs[of], positions // ps].astype(np.int64) * ps + positions % ps
+        return positions, slots, copies, changed
+
+    def compact(self):
+        """(src, dst): the moves after which the pages in use come first."""
+        used = np.flatnonzero(self.refs > 0)
+        n = len(used)
+        src = used[used >= n].astype(np.int32)
+        dst = np.flatnonzero(self.refs[:n] == 0).astype(np.int32)
+        to = np.arange(len(self.refs), dtype=np.int32)
+        to[src] = dst
+        self.pages = np.where(self.pages >= 0, to[self.pages], -1).astype(np.int32)
+        self.refs[dst] = self.refs[src]
+        self.refs[src] = 0
+        self._free = list(range(len(self.refs) - 1, n - 1, -1))
+        return src, dst
+
+
+class Step:
+    """The new tokens of some sequences (PagedCache.extend): where they go,
+    and the sequences' tables and lengths with them. All layers use one."""
+
+    def __init__(self, seqs, positions, slots, tables, lens, max_len):
+        self.seqs, self.positions, self.slots = seqs, positions, slots
+        self.tables, self.lens, self.max_len = tables, lens, max_len
+
+
+class PagedCache:
+    """The keys and values of all layers of a model in pages, for sequences
+    that grow, are forked and freed.
+
+    k_pages, v_pages [n_layers, n_pages, kv_heads, page_size, dim] and tables
+    [max_sequences, max_pages] (int32) are device tensors that the functions
+    above take layer by layer; who owns which page is kept on the host
+    (PageTable), so that an exhausted cache raises where it is asked for more,
+    before anything is changed. dtype float8_e4m3fn takes k_scale, v_scale
+    [n_layers, kv_heads] (float32; None: 1).
+
+        step = cache.extend(seqs, 1)
+        for layer in range(n_layers):
+            q = cache.append(layer, step, q, k, v, cos, sin)
+            out = cache.decode(layer, step, q)
+    """
+
+    def __init__(self, n_pages: int, n_layers: int, kv_heads: int, dim: int, page_size: int = 16,
+                 dtype: torch.dtype = torch.float16, max_sequences: int = 64, max_pages: int | None = None,
+                 device: str = "cuda", k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
+        if dtype not in _PAGE_TYPES:
+            raise ValueError(f"dtype must be float16, bfloat16 or float8_e4m3fn, got {dtype}")
+        if page_size < 8 or page_size > 256 or page_size & (page_size - 1):
+            raise ValueError("page_size must be a power of two from 8 to 256")
+        if n_layers < 1 or kv_heads < 1 or dim < 1 or dim > 256 or dim % (16 if dtype == _F8 else 8):
+            raise ValueError("n_layers and kv_heads must be at least 1, dim up to 256 and a multiple of 16 bytes")
+        self.table = PageTable(n_pages, page_size, max_sequences, max_pages or n_pages)
+        shape = (n_layers, n_pages, kv_heads, page_size, dim)
+        self.k_pages = torch.empty(shape, dtype=dtype, device=device)
+        self.v_pages = torch.empty(shape, dtype=dtype, device=device)
+        self.tables = torch.full((max_sequences, max_pages or n_pages), -1, dtype=torch.int32, device=device)
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is not None and (dtype != _F8 or t.shape != (n_layers, kv_heads)):
+                raise ValueError(f"{name} must be [{n_layers}, {kv_heads}] with float8_e4m3fn pages")
+        place = self.k_pages.device
+        self.k_scale, self.v_scale = (None if t is None else t.to(place, torch.float32).contiguous()
+                                      for t in (k_scale, v_scale))
+
+    def new(self) -> int:
+        """An empty sequence."""
+        return self.table.new()
+
+    def length(self, seq: int) -> int:
+        return int(self.table.lens[self.table.check([seq])[0]])
+
+    @property
+    def n_free(self) -> int:
+        """Pages that no sequence has."""
+        return self.table.n_free
+
+    def free(self, seqs) -> None:
+        """Gives back the sequences and the pages that only they have."""
+        self.table.free(seqs)
+
+    def fork(self, seq: int) -> int:
+        """A sequence with the tokens of `seq`, sharing its pages."""
+        other = self.table.fork(seq)
+        self.tables[other].copy_(self.tables[int(seq)])
+        return other
+
+    def _upload(self, *arrays):
+        """Host arrays as int64 device tensors, through pinned memory in one copy that is not waited for."""
+        flat = [np.asarray(a, dtype=np.int64).reshape(-1) for a in arrays]
+        host = torch.empty(sum(len(a) for a in flat), dtype=torch.int64, pin_memory=True)
+        np.concatenate(flat, out=host.numpy())
+        return host.to(self.k_pages.device, non_blocking=True).split([len(a) for a in flat])
+
+    def _copy(self, src, dst, tables=None):
+        copy_pages(self.k_pages, self.v_pages, src.int(), dst.int(), tables=tables)
+
+    def extend(self, seqs, counts=1) -> Step:
+        """Room for `counts` (one number, or one per sequence) new tokens of
+        each of the sequences; pages that other sequences share are copied
+        first. Raises RuntimeError, with nothing changed, when pages run out."""
+        positions, slots, copies, changed = self.table.extend(seqs, counts)
+        seqs = self.table.check(seqs)
+        lens = self.table.lens[seqs]
+        copies, changed = np.reshape(copies, (-1, 2)), np.reshape(changed, (-1, 3))
+        parts = self._upload(seqs, lens, positions, slots, copies[:, 0], copies[:, 1], *changed.T)
+        at, lens_gpu, positions, slots, src, dst, rows, cols, pages = parts
+        if len(copies):
+            self._copy(src, dst)
+        if len(changed):
+            self.tables[rows, cols] = pages.int()
+        longest = int(lens.max()) if len(lens) else 0
+        width = max(1, -(-longest // self.table.page_size))
+        return Step(seqs, positions, slots, self.tables[:, :width].index_select(0, at), lens_gpu.int(), longest)
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front, in all layers, and returns how
+        many moved. Steps taken before are void."""
+        src, dst = self.table.compact()
+        if len(src):
+            self._copy(*self._upload(src, dst), tables=self.tables)
+        return len(src)
+
+    def _layer(self, layer):
+        scales = {"k_scale": None if self.k_scale is None else self.k_scale[layer],
+                  "v_scale": None if self.v_scale is None else self.v_scale[layer]}
+        return self.k_pages[layer], self.v_pages[layer], scales
+
+    def append(self, layer: int, step: Step, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+               cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, interleaved: bool = False):
+        """append_tokens for the step's tokens."""
+        k_pages, v_pages, scales = self._layer(layer)
+        return append_tokens(q, k, v, step.positions, step.slots, cos, sin, k_pages, v_pages, interleaved=interleaved,
+                             **scales)
+
+    def decode(self, layer: int, step: Step, q: torch.Tensor, **options):
+        """decode_attention for the step's sequences, q [sequences, heads, dim]."""
+        k_pages, v_pages, scales = self._layer(layer)
+        return decode_attention(q, k_pages, v_pages, step.tables, step.lens, max_len=step.max_len, **scales, **options)
+
+    def retrieved(self, layer: int, step: Step, q: torch.Tensor, ids: torch.Tensor, first: int = 0, last: int = 0,
+                  **options):
+        """retrieved_attention for the step's sequences."""
+        k_pages, v_pages, scales = self._layer(layer)
+        return retrieved_attention(q, k_pages, v_pages, step.tables, step.lens, ids, first=first, last=last, **scales,
+                                   **options)
+
+    def keys(self, layer: int, seq: int) -> torch.Tensor:
+        """The keys of a sequence as they are held, [kv_heads, length, dim], contiguous: rows for an index."""
+        n = self.length(seq)
+        own, = self._upload(self.table.pages[seq, :-(-n // self.table.page_size)])
+        store = self.k_pages[layer]
+        rows = store.view(torch.uint8)[own].view(store.dtype) if store.dtype == _F8 else store[own]
+        heads, dim = store.size(1), store.size(3)
+        rows = rows.transpose(0, 1).reshape(heads, -1, dim)[:, :n]
+        if store.dtype == _F8:
+            rows = rows.to(torch.float16)
+            if self.k_scale is not None:
+                rows = (rows.float() * self.k_scale[layer][:, None, None]).to(torch.float16)
+        return rows.contiguous()
