@@ -22,106 +22,31 @@ graph (PagedCache's bookkeeping is on the host and is not captured).
 
 from __future__ import annotations
 
-import ctypes
 import functools
+import importlib.machinery
+import importlib.util
 import math
-import struct
 
 import numpy as np
 import torch
 
-_TYPES = {torch.float16: 0, torch.bfloat16: 1}
-_PAGE_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
+_TYPES = (torch.float16, torch.bfloat16, torch.float8_e4m3fn)
 _F8 = torch.float8_e4m3fn
-
-_i32, _i64, _ptr, _f64, _u32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_double, ctypes.c_uint32
-_struct = ctypes.c_char_p  # a struct's bytes, or None
-
-# jasperx_kv_pages and jasperx_head_rows. The calls here take about 10 us on
-# the host, as long as a small call's kernels: structs are packed, not
-# built as ctypes objects, and checks format their texts only when they fail.
-_pack_pages = struct.Struct("@PPPPqqqqiiiiii").pack
-_pack_rows = struct.Struct("@Pqqq").pack
-
-_SIGNATURES = {
-    "jasperx_rotary": [_struct, _struct, _i32, _i64, _i64, _ptr, _i32, _ptr, _ptr, _i64, _i64, _u32, _ptr, _ptr, _ptr],
-    "jasperx_append_tokens": [_struct, _struct, _struct, _i32, _i64, _ptr, _ptr, _i32, _ptr, _ptr, _i64, _i64, _u32,
-                              _struct, _ptr, _ptr],
-    "jasperx_copy_pages": [_struct, _ptr, _ptr, _i64, _ptr, _i64, _ptr],
-    "jasperx_decode_attention": [_struct, _i32, _i64, _struct, _ptr, _i64, _i64, _ptr, _i64, _f64, _i64, _ptr, _ptr,
-                                 _ptr, _i64, _ptr],
-    "jasperx_retrieved_attention": [_struct, _i32, _i64, _struct, _ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64,
-                                    _i64, _f64, _ptr, _ptr, _ptr, _i64, _ptr],
-    "jasperx_attention_workspace": [_i64, _i64, _struct, _i64, _i64],
-}
 
 
 @functools.lru_cache(maxsize=None)
-def _fn(name):
-    from . import _bind
-    return _bind(name, _SIGNATURES[name])
-
-
-# the current stream's handle without a Stream object around it
-_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-
-
-def _call(name, device, *args):
-    """The C call `name` on the current stream of GPU `device` (an index)."""
-    if device != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            _fn(name)(*args, _stream(device))
-    else:
-        _fn(name)(*args, _stream(device))
-
-
-def _place(device):
-    return "a CPU tensor" if device < 0 else f"on GPU {device}"
-
-
-def _indexes(name, t, device):
-    """An int32 or int64 tensor as a contiguous one."""
-    if t.dtype != torch.int64 and t.dtype != torch.int32:
-        raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
-    if t.get_device() != device:
-        raise ValueError(f"{name} must be on GPU {device}, is {_place(t.get_device())}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _scale_ptr(name, t, heads, pages):
-    if t is None:
-        return 0
-    if pages.dtype != _F8:
-        raise ValueError(f"{name} needs float8_e4m3fn pages")
-    if t.dtype != torch.float32 or t.shape != (heads,) or not t.is_contiguous() or t.device != pages.device:
-        raise ValueError(f"{name} must be a contiguous float32 [{heads}] tensor on the pages' device")
-    return t.data_ptr()
-
-
-def _pages(k_pages, v_pages, k_scale=None, v_scale=None, layers=False):
-    """(C struct, sizes (heads, page_size, dim), type, GPU) of a pair of page tensors, checked."""
-    shape, stride, device = k_pages.shape, k_pages.stride(), k_pages.get_device()
-    type_ = _PAGE_TYPES.get(k_pages.dtype)
-    if type_ is None:
-        raise ValueError(f"pages must be float16, bfloat16 or float8_e4m3fn, got {k_pages.dtype}")
-    if (v_pages.dtype != k_pages.dtype or v_pages.shape != shape or v_pages.get_device() != device
-            or v_pages.stride() != stride):
-        raise ValueError("k_pages and v_pages must have the same type, shape, strides and device")
-    if device < 0:
-        raise ValueError("k_pages must be a CUDA tensor")
-    count, layer_stride = 1, 0
-    if layers and len(shape) == 5:
-        count, layer_stride, shape, stride = shape[0], stride[0], shape[1:], stride[1:]
-    if len(shape) != 4:
-        raise ValueError(f"pages must be [{'layers, ' if layers else ''}n_pages, kv_heads, page_size, dim], "
-                         f"got {k_pages.ndim}D")
-    if stride[3] != 1:
-        raise ValueError("the last dimension of the pages must be contiguous")
-    n, heads, page, dim = shape
-    c = _pack_pages(k_pages.data_ptr(), v_pages.data_ptr(), _scale_ptr("k_scale", k_scale, heads, k_pages),
-                    _scale_ptr("v_scale", v_scale, heads, k_pages), layer_stride, stride[0], stride[1], stride[2],
-                    count, n, heads, page, dim, type_)
-    return c, (heads, page, dim), type_, device
+def _kv():
+    """The module that takes tensors to the HIP library's calls (csrc/torch_kv.cpp)."""
+    from . import _load_lib, library_path
+    _load_lib()
+    path = library_path().parent / "_kv.so"
+    if not path.exists():
+        raise RuntimeError(f"{path} not found; build it with `python -m jasper_amd.build_lib` (there is no other way "
+                           "to these operators)")
+    loader = importlib.machinery.ExtensionFileLoader("jasper_amd._kv", str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("jasper_amd._kv", loader))
+    loader.exec_module(module)
+    return module
 
 
 # ---- rotary positions ----
@@ -169,76 +94,6 @@ def rotary_table(n_positions: int, rot_dim: int, base: float = 10000.0, scaling:
     return (angle.cos() * size).float(), (angle.sin() * size).float()
 
 
-def _table(cos, sin, device):
-    """(cos, sin pointers, positions, rotated values) of a pair of tables."""
-    if cos is None and sin is None:
-        return None, None, 0, 0
-    if (cos is None or sin is None or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.ndim != 2
-            or cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous()
-            or cos.get_device() != device or sin.get_device() != device):
-        raise ValueError(f"cos and sin must be contiguous float32 [n_positions, rot_dim / 2] tensors on GPU {device}")
-    return cos.data_ptr(), sin.data_ptr(), cos.size(0), 2 * cos.size(1)
-
-
-def _head_rows(t):
-    """(C struct, the tensor it describes) of [..., heads, dim] as rows [n, heads, dim] with contiguous values."""
-    if t.ndim != 3:
-        t = t.flatten(0, -3) if t.ndim > 3 else t[None]
-    stride = t.stride()
-    if stride[2] != 1:
-        t = t.contiguous()
-        stride = t.stride()
-    return _pack_rows(t.data_ptr(), stride[0], stride[1], t.size(1)), t
-
-
-def _alike(name, t, like):
-    if (t.dtype != like.dtype or t.get_device() != like.get_device() or t.ndim != like.ndim
-            or t.shape[:-2] != like.shape[:-2] or t.size(-1) != like.size(-1)):
-        raise ValueError(f"{name} must match the other rows in type, device, leading sizes and dim")
-
-
-def _rotate(q, k, positions, cos, sin, interleaved, back):
-    """The rotation of checked arguments."""
-    first = q if q is not None else k
-    device = first.get_device()
-    c, s, table_rows, rot = _table(cos, sin, device)
-    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    n = positions.numel()
-    if n:
-        q_rows, q = (None, None) if q is None else _head_rows(q)
-        k_rows, k = (None, None) if k is None else _head_rows(k)
-        _call("jasperx_rotary", device, q_rows, k_rows, _TYPES[first.dtype], n, first.size(-1), positions.data_ptr(),
-              positions.element_size(), c, s, table_rows, rot, (1 if interleaved else 0) | (2 if back else 0),
-              None if q_out is None else q_out.data_ptr(), None if k_out is None else k_out.data_ptr())
-    return q_out, k_out
-
-
-class _Rotary(torch.autograd.Function):
-    """Linear in q and k: the gradient is the rotation by the opposite
-    angles, which is differentiated the same way."""
-
-    @staticmethod
-    def forward(ctx, q, k, positions, cos, sin, interleaved, back):
-        ctx.save_for_backward(positions, cos, sin)
-        ctx.flags = interleaved, back
-        ctx.set_materialize_grads(False)
-        return _rotate(q, k, positions, cos, sin, interleaved, back)
-
-    @staticmethod
-    def backward(ctx, gq, gk):
-        if not ctx.needs_input_grad[0]:
-            gq = None
-        if not ctx.needs_input_grad[1]:
-            gk = None
-        if gq is None and gk is None:
-            return (None,) * 7
-        interleaved, back = ctx.flags
-        turn = _Rotary.apply if torch.is_grad_enabled() else _rotate
-        dq, dk = turn(gq, gk, *ctx.saved_tensors, interleaved, not back)
-        return dq, dk, None, None, None, None, None
-
-
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
            interleaved: bool = False):
     """(q, k) [..., heads, dim] (fp16 or bf16) with rotary positions: the
@@ -248,23 +103,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos
     Differentiable in q and k. k may be None. A position outside the tables
     gives NaN. Sums are in 32 bits, rounded once.
     """
-    if q.dtype not in _TYPES:
-        raise ValueError(f"q must be float16 or bfloat16, got {q.dtype}")
-    device = q.get_device()
-    if device < 0:
-        raise ValueError("q must be a CUDA tensor")
-    if q.ndim < 2 or q.size(-1) % 2:
-        raise ValueError("q must be [..., heads, dim] with an even dim")
-    if k is not None:
-        _alike("k", k, q)
-    positions = _indexes("positions", positions, device)
-    if positions.shape != q.shape[:-2]:
-        raise ValueError(f"positions must be {list(q.shape[:-2])}, got {list(positions.shape)}")
-    if cos is None or sin is None or cos.ndim != 2 or 2 * cos.size(1) > q.size(-1):
-        raise ValueError("cos and sin must be [n_positions, rot_dim / 2] with rot_dim at most dim")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(q, k, positions, cos, sin, interleaved, False)
-    return _rotate(q, k, positions, cos, sin, interleaved, False)
+    return _kv().rotary(q, k, positions, cos, sin, interleaved)
 
 
 # ---- the cache ----
@@ -281,45 +120,7 @@ def append_tokens(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, posi
     rounded to nearest and saturated at +-448. No two tokens may have one
     slot. q, k and v may be slices of one projection's output.
     """
-    pages, (heads, _, dim), type_, device = _pages(k_pages, v_pages, k_scale, v_scale)
-    if k.dtype not in _TYPES or (type_ != 2 and k_pages.dtype != k.dtype):
-        raise ValueError(f"k must be float16 or bfloat16 and the pages of its type or float8_e4m3fn, got {k.dtype} "
-                         f"and {k_pages.dtype}")
-    if k.ndim != 3 or k.size(1) != heads or k.size(2) != dim or k.get_device() != device:
-        raise ValueError(f"k must be [n, {heads}, {dim}] on GPU {device}")
-    _alike("v", v, k)
-    if v.size(1) != heads:
-        raise ValueError(f"v must be [n, {heads}, {dim}]")
-    if q is not None:
-        _alike("q", q, k)
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
-        raise ValueError("append_tokens has no gradient: use rotary, or torch.no_grad()")
-    n = k.size(0)
-    slots = _indexes("slots", slots, device)
-    if slots.shape != (n,):
-        raise ValueError(f"slots must be [{n}]")
-    c, s, table_rows, rot = _table(cos, sin, device)
-    at = None
-    if rot:
-        if rot > dim:
-            raise ValueError("the tables rotate more values than a head has")
-        if positions is None:
-            raise ValueError("positions are needed with cos and sin")
-        positions = _indexes("positions", positions, device)
-        if positions.shape != (n,):
-            raise ValueError(f"positions must be [{n}]")
-        if positions.dtype != slots.dtype:
-            positions, slots = positions.long(), slots.long()
-        at = positions.data_ptr()
-    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if n:
-        q_rows, q = (None, None) if q is None else _head_rows(q)
-        k_rows, k = _head_rows(k)
-        v_rows, v = _head_rows(v)
-        _call("jasperx_append_tokens", device, q_rows, k_rows, v_rows, _TYPES[k.dtype], n, at, slots.data_ptr(),
-              slots.element_size(), c, s, table_rows, rot, 1 if interleaved else 0, pages,
-              None if out is None else out.data_ptr())
-    return out
+    return _kv().append_tokens(q, k, v, positions, slots, cos, sin, k_pages, v_pages, interleaved, k_scale, v_scale)
 
 
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
@@ -330,56 +131,10 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     entries equal to src[i] become dst[i]. No page may be a source and a
     destination, or the destination of two. Pairs with an id outside the
     cache are skipped."""
-    pages, _, _, device = _pages(k_pages, v_pages, layers=True)
-    for name, t in (("src", src), ("dst", dst)):
-        if t.dtype != torch.int32 or t.ndim != 1 or t.get_device() != device or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous 1D int32 tensor on GPU {device}")
-    n, entries = src.numel(), 0
-    if dst.numel() != n:
-        raise ValueError("src and dst must have the same length")
-    if tables is not None:
-        if tables.dtype != torch.int32 or not tables.is_contiguous() or tables.get_device() != device:
-            raise ValueError(f"tables must be a contiguous int32 tensor on GPU {device}")
-        entries = tables.numel()
-    if n:
-        _call("jasperx_copy_pages", device, pages, src.data_ptr(), dst.data_ptr(), n,
-              tables.data_ptr() if entries else None, entries)
+    _kv().copy_pages(k_pages, v_pages, src, dst, tables)
 
 
 # ---- attention of one new token ----
-
-@functools.lru_cache(maxsize=4096)
-def _workspace_bytes(device, batch, q_heads, sizes, type_, max_tokens, lists):
-    heads, page, dim = sizes
-    pages = _pack_pages(0, 0, 0, 0, 0, 0, 0, dim, 1, 0, heads, page, dim, type_)
-    with torch.cuda.device(device):
-        return _fn("jasperx_attention_workspace")(batch, q_heads, pages, max_tokens, lists)
-
-
-def _query(q, sizes, type_, k_pages, tables, lens, device):
-    """(C struct, q, lens) of checked queries, tables and lengths."""
-    heads, _, dim = sizes
-    if q.dtype not in _TYPES or (type_ != 2 and k_pages.dtype != q.dtype):
-        raise ValueError(f"q must be float16 or bfloat16 and the pages of its type or float8_e4m3fn, got {q.dtype} "
-                         f"and {k_pages.dtype}")
-    if q.ndim != 3 or q.size(2) != dim or q.size(1) == 0 or q.size(1) % heads or q.get_device() != device:
-        raise ValueError(f"q must be [batch, a multiple of {heads} heads, {dim}] on GPU {device}")
-    if q.requires_grad and torch.is_grad_enabled():
-        raise ValueError("attention over the cache has no gradient: use torch.no_grad()")
-    b = q.size(0)
-    if (tables.dtype != torch.int32 or tables.ndim != 2 or tables.size(0) != b or tables.get_device() != device
-            or (tables.size(1) > 1 and tables.stride(1) != 1)):
-        raise ValueError(f"tables must be int32 [{b}, pages] with contiguous rows, on GPU {device}")
-    if lens.dtype != torch.int32 or lens.shape != (b,) or lens.get_device() != device:
-        raise ValueError(f"lens must be int32 [{b}] on GPU {device}")
-    if not lens.is_contiguous():
-        lens = lens.contiguous()
-    stride, at = q.stride(), q.data_ptr()
-    if stride[2] != 1 or stride[0] % 8 or stride[1] % 8 or at % 16:
-        q = q.clone(memory_format=torch.contiguous_format)
-        stride, at = q.stride(), q.data_ptr()
-    return _pack_rows(at, stride[0], stride[1], q.size(1)), q, lens
-
 
 def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
                      lens: torch.Tensor, scale: float | None = None, window: int = 0,
@@ -398,23 +153,7 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     sequence is longer (default: what tables can hold); the work is laid out
     for it, and tokens past it are not read.
     """
-    pages, sizes, type_, device = _pages(k_pages, v_pages, k_scale, v_scale)
-    rows, q, lens = _query(q, sizes, type_, k_pages, tables, lens, device)
-    if window < 0 or (max_len is not None and max_len < 0):
-        raise ValueError("window and max_len must be at least 0")
-    b, heads, dim = q.shape
-    most = tables.size(1) * sizes[1]
-    if max_len is not None and max_len < most:
-        most = max_len
-    out = torch.empty((b, heads, dim), dtype=q.dtype, device=q.device)
-    lse = torch.empty((b, heads), dtype=torch.float32, device=q.device) if return_lse else None
-    if b:
-        size = _workspace_bytes(device, b, heads, sizes, type_, window if 0 < window < most else most, 0)
-        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _call("jasperx_decode_attention", device, rows, _TYPES[q.dtype], b, pages, tables.data_ptr(),
-              tables.stride(0), tables.size(1), lens.data_ptr(), most, dim ** -0.5 if scale is None else scale, window,
-              out.data_ptr(), lse.data_ptr() if return_lse else None, scratch.data_ptr(), size)
-    return (out, lse) if return_lse else out
+    return _kv().decode_attention(q, k_pages, v_pages, tables, lens, scale, window, k_scale, v_scale, max_len, return_lse)
 
 
 def retrieved_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
@@ -427,27 +166,8 @@ def retrieved_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     query heads (each has its own) or of key heads (shared). Ids outside
     [first, len - last), such as a search's -1, are left out: the first and
     last tokens are there already. An id listed twice counts twice."""
-    pages, sizes, type_, device = _pages(k_pages, v_pages, k_scale, v_scale)
-    rows, q, lens = _query(q, sizes, type_, k_pages, tables, lens, device)
-    b, heads, dim = q.shape
-    if (ids.dtype != torch.int32 or ids.ndim != 3 or ids.size(0) != b or ids.size(1) not in (heads, sizes[0])
-            or ids.get_device() != device):
-        raise ValueError(f"ids must be int32 [{b}, {heads} or {sizes[0]}, count] on GPU {device}")
-    if first < 0 or last < 0:
-        raise ValueError("first and last must be at least 0")
-    lists, count = ids.size(1), ids.size(2)
-    if not ids.is_contiguous():
-        ids = ids.contiguous()
-    out = torch.empty((b, heads, dim), dtype=q.dtype, device=q.device)
-    lse = torch.empty((b, heads), dtype=torch.float32, device=q.device) if return_lse else None
-    if b:
-        size = _workspace_bytes(device, b, heads, sizes, type_, first + last + count, lists)
-        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _call("jasperx_retrieved_attention", device, rows, _TYPES[q.dtype], b, pages, tables.data_ptr(),
-              tables.stride(0), tables.size(1), lens.data_ptr(), ids.data_ptr(), lists, count, first, last,
-              dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr() if return_lse else None,
-              scratch.data_ptr(), size)
-    return (out, lse) if return_lse else out
+    return _kv().retrieved_attention(q, k_pages, v_pages, tables, lens, ids, first, last, scale, k_scale, v_scale,
+                                     return_lse)
 
 
 # ---- pages and sequences ----
@@ -590,7 +310,7 @@ class PagedCache:
     def __init__(self, n_pages: int, n_layers: int, kv_heads: int, dim: int, page_size: int = 16,
                  dtype: torch.dtype = torch.float16, max_sequences: int = 64, max_pages: int | None = None,
                  device: str = "cuda", k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
-        if dtype not in _PAGE_TYPES:
+        if dtype not in _TYPES:
             raise ValueError(f"dtype must be float16, bfloat16 or float8_e4m3fn, got {dtype}")
         if page_size < 8 or page_size > 256 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two from 8 to 256")

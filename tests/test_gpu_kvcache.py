@@ -118,6 +118,11 @@ def test_rotary_position_outside_the_tables(jasper):
     assert y[1:3, :, :32].isnan().all() and y[[0, 3]].isfinite().all() and torch.equal(y[..., 32:], q[..., 32:])
 
 
+def rotary_needs_no_graph(jasper, q, k, pos, cos, sin):
+    with torch.no_grad():
+        return any(x.requires_grad for x in jasper.rotary(q, k, pos, cos, sin))
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("dim,rot,scaling", [(64, 64, None), (96, 48, "yarn"), (128, 128, "ntk"), (20, 12, "linear")])
 def test_rotary_gradient(jasper, dim, rot, scaling, interleaved):
@@ -129,6 +134,7 @@ def test_rotary_gradient(jasper, dim, rot, scaling, interleaved):
     gq, gk = randn((n, 6, dim), F16, 7), randn((n, 2, dim), F16, 8)
     out = jasper.rotary(q, k, pos, cos, sin, interleaved=interleaved)
     dq, dk = torch.autograd.grad(out, (q, k), (gq, gk), retain_graph=True)
+    assert not rotary_needs_no_graph(jasper, q, k, pos, cos, sin)
     for g, d in ((gq, dq), (gk, dk)):
         want, size = ref_rotary(g, pos, cos, sin, interleaved, back=True)
         near(d, want, rotary_tol(want, size, F16))
@@ -142,10 +148,17 @@ def test_rotary_gradient(jasper, dim, rot, scaling, interleaved):
         # q +- 1 and the outputs are each rounded to fp16 (values below 8): 2^-8 each, over up to dim terms of |g|
         tol = 4 * 2.0 ** -8 * gq.double().abs().sum(-1)
         near(dq[..., at], slope.cpu(), tol)
-    only, = torch.autograd.grad(out, (k,), (gq, gk))
+    only, = torch.autograd.grad(out, (k,), (gq, gk), retain_graph=True)
     assert torch.equal(only, dk)
     again, _ = jasper.rotary(q, None, pos, cos, sin, interleaved=interleaved)
     assert torch.equal(torch.autograd.grad(again, q, gq)[0], dq)
+    # the gradient is linear in gq: differentiated once more it is the rotation itself
+    seed = gq.clone().requires_grad_()
+    first, = torch.autograd.grad(out[0], q, seed, create_graph=True)
+    other = randn((n, 6, dim), F16, 9)
+    second, = torch.autograd.grad(first, seed, other)
+    want, size = ref_rotary(other, pos, cos, sin, interleaved)
+    near(second, want, rotary_tol(want, size, F16))
 
 
 # ---- appending ----
