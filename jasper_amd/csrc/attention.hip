@@ -80,6 +80,15 @@ __device__ __forceinline__ uint32_t from_e4m3(uint32_t w, bool high) {
   return pack2<T>(a.x, a.y);
 }
 
+// Rows are read once, past the caches (four sequences of 131k tokens: 175 us,
+// 191 with ordinary loads). Not where a row is no whole number of 128-byte
+// lines: neighbours share lines, and 96 dims took 79 us instead of 76.
+template <bool STREAM, typename W>
+__device__ __forceinline__ W load(const W* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 // What a sequence has its queries read: the tokens [begin, end), counted from
 // base in tiles; of a list's places [0, end) the first `first` are tokens,
 // then come the tokens from `last` on, then the ids.
@@ -137,7 +146,7 @@ __device__ int find_sequence(const Params& p, int streams, Share& share, int& be
     const int o = __shfl_up(incl, d, 64);
     if (lane >= d) incl += o;
   }
-  const int total = __shfl(incl, 63, 64) * streams;
+  const int total = __builtin_amdgcn_readlane(incl, 63) * streams;  // known to be the same in all lanes
   share.waves = min(total, (int)gridDim.x);
   share.each = total / share.waves;
   share.more = total % share.waves;
@@ -162,10 +171,11 @@ __device__ int find_sequence(const Params& p, int streams, Share& share, int& be
 //  S  comes out with lane (g, i) holding head i's scores of group g's eight
 //     tokens, which is where P has to be as the operand of the second product:
 //     nothing crosses lanes.
-//  V  lane (g, i) loads the VD dims from VD i on of group g's eight tokens (a
-//     row is one contiguous read of 16 lanes); the 8 x VD values are turned
-//     with byte permutes into VD operands, product j giving dims VD m + j.
-//  O  lane (g, i): head i, dims VD (4 g + r) + j.
+//  V  lane (g, i) loads VD dims of group g's eight tokens, in blocks of up to
+//     16 bytes of which 16 lanes read a contiguous run: dims BD i on, and 16
+//     BD further in each next block. The 8 x VD values are turned with byte
+//     permutes into VD operands, product j giving the j-th dims of all lanes.
+//  O  lane (g, i): head i, of dims that lane 4 g + r loads the j-th in o[j][r].
 // Heads past the group's are zero queries: the loads bound the kernel, not
 // the products (32 instructions of 16 cycles per 16 KB of a wave).
 //
@@ -175,9 +185,10 @@ __device__ int find_sequence(const Params& p, int streams, Share& share, int& be
 // one wave has whole is finished here, the others' parts go to the workspace:
 // a wave has at most one that an earlier wave began (slot 0) and one that it
 // begins itself (slot 1).
-template <typename T, bool F8, int DT, bool LISTED>
+template <typename T, bool F8, int DT, bool LISTED, bool FULL>
 __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p) {
   constexpr int VD = DT / 16, KS = DT / 32, ES = F8 ? 1 : 2;
+  constexpr int BD = VD * ES > 16 ? 16 / ES : VD;  // dims of a lane that lie together
   typedef std::conditional_t<F8, f16, T> PT;  // e4m3 values are exact in fp16, where weights keep more bits
   // fp16 weights are 2^12 larger, so that those far below the largest are not
   // lost; the reference is moved once a score is 2^3 above it
@@ -216,7 +227,7 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
     for (int s = 0; s < KS; ++s) {
       const int d = F8 ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
       q[s] = Frag{0, 0, 0, 0};
-      if (i < n_heads && d < p.dim) q[s] = *(const Frag*)(p.q + (b * p.q_stride + (qh + i) * p.q_head + d) * 2);
+      if (i < n_heads && (FULL || d < p.dim)) q[s] = *(const Frag*)(p.q + (b * p.q_stride + (qh + i) * p.q_head + d) * 2);
     }
     floatx4 o[VD];
 #pragma unroll
@@ -267,8 +278,8 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
 #pragma unroll
             for (int s = 0; s < KS; s += 2) {
               const int d = 32 * s + 16 * g;
-              const bool in = d < p.dim;
-              uintx4 w = *(const uintx4*)(row + (in ? d : 0));
+              const bool in = FULL || d < p.dim;
+              uintx4 w = load<FULL>((const uintx4*)(row + (in ? d : 0)));
               if (!in) w = uintx4{0, 0, 0, 0};
               kf[r][s] = Frag{w.x, w.y, 0, 0};
               kf[r][s + 1] = Frag{w.z, w.w, 0, 0};
@@ -277,8 +288,8 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
               const int d = 32 * s + 8 * g;
-              const bool in = d < p.dim;
-              uintx4 w = *(const uintx4*)(row + (in ? d : 0) * 2);
+              const bool in = FULL || d < p.dim;
+              uintx4 w = load<FULL>((const uintx4*)(row + (in ? d : 0) * 2));
               if (!in) w = uintx4{0, 0, 0, 0};
               kf[r][s] = w;
             }
@@ -287,7 +298,10 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
       };
       constexpr int VW = VD * ES / 4;  // words of V per token and lane
       // a chunk of V past the end of a row is the row's first instead: those dims are never stored
-      const auto v_at = [&](int w) { return i * VD + w * (4 / ES) < p.dim ? i * VD * ES + 4 * w : 0; };
+      const auto v_at = [&](int w) {
+        const int d = w / 4 * 16 * BD + i * BD;
+        return FULL || d < p.dim ? d * ES : 0;
+      };
 
       // one tile, with the next one's keys on their way while its values are
       auto step = [&](int tile, auto more) {
@@ -308,14 +322,14 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
           if constexpr (VW >= 4) {
 #pragma unroll
             for (int w = 0; w < VW; w += 4) {
-              const uintx4 y = *(const uintx4*)(row + v_at(w));
+              const uintx4 y = load<FULL>((const uintx4*)(row + v_at(w)));
               vw[t][w] = y.x, vw[t][w + 1] = y.y, vw[t][w + 2] = y.z, vw[t][w + 3] = y.w;
             }
           } else if constexpr (VW == 2) {
-            const uintx2 y = *(const uintx2*)(row + v_at(0));
+            const uintx2 y = load<FULL>((const uintx2*)(row + v_at(0)));
             vw[t][0] = y.x, vw[t][1] = y.y;
           } else {
-            vw[t][0] = *(const uint32_t*)(row + v_at(0));
+            vw[t][0] = load<FULL>((const uint32_t*)(row + v_at(0)));
           }
         }
         floatx4 s[2];
@@ -401,19 +415,20 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
     const bool whole = c == 0 && c1 == sp.tiles;
+    const auto dim_of = [&](int j, int r) { return j / BD * 16 * BD + (4 * g + r) * BD + j % BD; };
     if (i < n_heads) {
       if (whole) {
         const int64_t row = (int64_t)b * p.q_heads + qh + i;
         const float inv = (p.v_scale ? p.v_scale[h] : 1.f) / sum;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int d = VD * (4 * g + r);
 #pragma unroll
           for (int j = 0; j < VD; j += 4) {
+            const int d = dim_of(j, r);
             float y[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = sum == 0.f ? 0.f : o[j + e][r] * inv;
-            if (d + j < p.dim) *(uintx2*)(p.out + (row * p.dim + d + j) * 2) = uintx2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+            if (FULL || d < p.dim) *(uintx2*)(p.out + (row * p.dim + d) * 2) = uintx2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
           }
         }
         if (g == 0 && p.lse) p.lse[row] = sum == 0.f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
@@ -423,7 +438,7 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
         for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int j = 0; j < VD; j += 4)
-            *(floatx4*)(part + i * DT + VD * (4 * g + r) + j) = floatx4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
+            *(floatx4*)(part + i * DT + dim_of(j, r)) = floatx4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
         if (g == 0) *(floatx2*)(part + p.part_heads * DT + 2 * i) = floatx2{ref, sum};
       }
     }
@@ -539,7 +554,9 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
 
 template <typename T, bool F8, int DT>
 void launch(const Params& p, const Plan& plan, bool listed, hipStream_t s) {
-  auto kernel = listed ? attend_kernel<T, F8, DT, true> : attend_kernel<T, F8, DT, false>;
+  const bool full = p.dim == DT;
+  auto kernel = listed ? (full ? attend_kernel<T, F8, DT, true, true> : attend_kernel<T, F8, DT, true, false>)
+                       : (full ? attend_kernel<T, F8, DT, false, true> : attend_kernel<T, F8, DT, false, false>);
   kernel<<<(unsigned)plan.waves, 64, 0, s>>>(p);
   hip_check(hipGetLastError(), "attention");
   if (plan.joins) {
