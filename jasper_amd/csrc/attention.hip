@@ -15,11 +15,14 @@ namespace jasper_amd {
 namespace {
 
 constexpr int kTile = 32;    // tokens a wave takes at once
-constexpr int kStage = 512;  // row offsets held in LDS
 constexpr int kHeads = 16;   // query heads of a matrix instruction
 constexpr int kStart = 2;    // what beginning a stream costs a wave, in tiles
 constexpr int kWaves = 2048;  // at most; of a call
 constexpr int kJoin = 256;   // threads of a joining work-group
+constexpr int kGroupStage = 256;        // row offsets of a wave of a group, in LDS
+constexpr int kGroupLds = 64 << 10;     // bytes at most
+// waves of a group at most: what a compute unit has registers for
+constexpr int group_waves(int dt) { return dt == 64 ? 16 : dt == 128 ? 8 : 4; }
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -178,23 +181,261 @@ __device__ int find_sequence(const Params& p, int streams, Share& share, int& be
 //  O  lane (g, i): head i, of dims that lane 4 g + r loads the j-th in o[j][r].
 // Heads past the group's are zero queries: the loads bound the kernel, not
 // the products (32 instructions of 16 cycles per 16 KB of a wave).
-//
-// A work-group is one wave with an equal run of the tiles of all sequences
-// and streams: waves in different phases (finding their rows, streaming,
-// writing) share a compute unit without waiting for each other. A stream that
-// one wave has whole is finished here, the others' parts go to the workspace:
-// a wave has at most one that an earlier wave began (slot 0) and one that it
-// begins itself (slot 1).
-template <typename T, bool F8, int DT, bool LISTED, bool FULL>
-__global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p) {
+// A stream: the tokens of one sequence under up to 16 query heads of a list.
+struct Stream {
+  int b, list, heads, q_head, kv_head;
+};
+
+__device__ __forceinline__ Stream stream_of(const Params& p, int b, int x) {
+  const int list = x / p.tiles, head0 = (x % p.tiles) * kHeads;
+  return {b, list, min(kHeads, p.group - head0), list * p.group + head0, list * p.heads / p.lists};
+}
+
+// A wave's sums over some tiles: o (of V, by lane as above) and `sum` (of the
+// weights) are 2^-ref times what they stand for.
+template <int DT>
+struct Sums {
+  floatx4 o[DT / 16];
+  float ref, sum;
+};
+
+// The dims of o[j][r].
+template <bool F8, int DT>
+__device__ __forceinline__ int dim_of(int g, int j, int r) {
+  constexpr int BD = DT / 16 * (F8 ? 1 : 2) > 16 ? 8 : DT / 16;
+  return j / BD * 16 * BD + (4 * g + r) * BD + j % BD;
+}
+
+// LDS that only this wave reads and writes: kept in order, not waited for.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// One wave over tiles [c, c1) of a stream; rows: STAGE offsets in LDS.
+template <typename T, bool F8, int DT, bool LISTED, bool FULL, int STAGE>
+__device__ __forceinline__ Sums<DT> attend_tiles(const Params& p, const Span& sp, const Stream& at, int c, int c1,
+                                                 int64_t* rows) {
   constexpr int VD = DT / 16, KS = DT / 32, ES = F8 ? 1 : 2;
   constexpr int BD = VD * ES > 16 ? 16 / ES : VD;  // dims of a lane that lie together
   typedef std::conditional_t<F8, f16, T> PT;  // e4m3 values are exact in fp16, where weights keep more bits
   // fp16 weights are 2^12 larger, so that those far below the largest are not
   // lost; the reference is moved once a score is 2^3 above it
   constexpr float kTop = std::is_same_v<PT, f16> ? 12.f : 0.f, kLag = 3.f;
-  __shared__ int64_t rows[kStage];
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  const char* kb = p.k + at.kv_head * p.head_stride * ES;
+  const char* vb = p.v + at.kv_head * p.head_stride * ES;
+  const float cs = p.scale * (p.k_scale ? p.k_scale[at.kv_head] : 1.f);
 
+  Frag q[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d = F8 ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+    q[s] = Frag{0, 0, 0, 0};
+    if (i < at.heads && (FULL || d < p.dim)) q[s] = *(const Frag*)(p.q + (at.b * p.q_stride + (at.q_head + i) * p.q_head + d) * 2);
+  }
+  Sums<DT> out;
+  floatx4 (&o)[VD] = out.o;
+#pragma unroll
+  for (int j = 0; j < VD; ++j) o[j] = floatx4{0, 0, 0, 0};
+  float ref = -__builtin_inff(), use = 0.f, sum = 0.f;
+
+  constexpr int kStageTiles = STAGE / (LISTED ? kTile : kTile / 8);
+  const int n_all = sp.end > sp.base ? c1 : c;  // no tokens, no tiles
+  for (int c0 = c; c0 < n_all; c0 += kStageTiles) {
+    const int n_tiles = min(n_all - c0, kStageTiles);
+    // offsets of the rows: one per token of a list, one per 8 tokens else
+    wave_sync();
+    for (int e = lane; e < n_tiles * (LISTED ? kTile : kTile / 8); e += 64) {
+      int t;
+      int64_t off = -1;
+      bool known;
+      if (LISTED) {
+        const int place = c0 * kTile + e, always = sp.end - p.count;
+        known = place < sp.end;
+        t = place < sp.first ? place : sp.last + (place - sp.first);
+        if (known && place >= always) {
+          t = p.ids[((int64_t)at.b * p.lists + at.list) * p.count + (place - always)];
+          known = t >= sp.first && t < sp.last;
+        }
+      } else {
+        t = sp.base + c0 * kTile + 8 * e;
+        known = t < sp.end;
+      }
+      if (known) {
+        const int32_t page = p.tables[at.b * p.table_stride + (t >> p.page_shift)];
+        if (page >= 0 && page < p.pages)
+          off = (page * p.page_stride + (t & ((1 << p.page_shift) - 1)) * p.row_stride) * ES;
+      }
+      rows[e] = off;
+    }
+    wave_sync();
+
+    Frag kf[2][KS];
+    auto load_k = [&](int tile) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int tok = 8 * (i >> 2) + (i & 3) + 4 * r;
+        int64_t off = LISTED ? rows[tile * kTile + tok] : rows[tile * (kTile / 8) + (i >> 2)];
+        off = off < 0 ? 0 : off;
+        if (!LISTED) off += ((i & 3) + 4 * r) * p.row_stride * ES;
+        const char* row = kb + off;
+        if constexpr (F8) {
+#pragma unroll
+          for (int s = 0; s < KS; s += 2) {
+            const int d = 32 * s + 16 * g;
+            const bool in = FULL || d < p.dim;
+            uintx4 w = load<FULL>((const uintx4*)(row + (in ? d : 0)));
+            if (!in) w = uintx4{0, 0, 0, 0};
+            kf[r][s] = Frag{w.x, w.y, 0, 0};
+            kf[r][s + 1] = Frag{w.z, w.w, 0, 0};
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const int d = 32 * s + 8 * g;
+            const bool in = FULL || d < p.dim;
+            uintx4 w = load<FULL>((const uintx4*)(row + (in ? d : 0) * 2));
+            if (!in) w = uintx4{0, 0, 0, 0};
+            kf[r][s] = w;
+          }
+        }
+      }
+    };
+    constexpr int VW = VD * ES / 4;  // words of V per token and lane
+    // a chunk of V past the end of a row is the row's first instead: those dims are never stored
+    const auto v_at = [&](int w) {
+      const int d = w / 4 * 16 * BD + i * BD;
+      return FULL || d < p.dim ? d * ES : 0;
+    };
+
+    // one tile, with the next one's keys on their way while its values are
+    auto step = [&](int tile, auto more) {
+      uint32_t vw[8][VW];
+      uint32_t valid = 0;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        int64_t off = LISTED ? rows[tile * kTile + 8 * g + t] : rows[tile * (kTile / 8) + g];
+        bool in = off >= 0;
+        if (!LISTED) {
+          const int tok = sp.base + (c0 + tile) * kTile + 8 * g + t;
+          in = in && tok >= sp.begin && tok < sp.end;
+        }
+        valid |= in ? 1u << t : 0u;
+        off = off < 0 ? 0 : off;
+        if (!LISTED) off += t * p.row_stride * ES;
+        const char* row = vb + off;
+        if constexpr (VW >= 4) {
+#pragma unroll
+          for (int w = 0; w < VW; w += 4) {
+            const uintx4 y = load<FULL>((const uintx4*)(row + v_at(w)));
+            vw[t][w] = y.x, vw[t][w + 1] = y.y, vw[t][w + 2] = y.z, vw[t][w + 3] = y.w;
+          }
+        } else if constexpr (VW == 2) {
+          const uintx2 y = load<FULL>((const uintx2*)(row + v_at(0)));
+          vw[t][0] = y.x, vw[t][1] = y.y;
+        } else {
+          vw[t][0] = load<FULL>((const uint32_t*)(row + v_at(0)));
+        }
+      }
+      floatx4 s[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        s[r] = floatx4{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < KS; ++e) {
+          Frag a = kf[r][e];
+          if constexpr (F8)
+            a = Frag{from_e4m3<T>(a.x, false), from_e4m3<T>(a.x, true), from_e4m3<T>(a.y, false), from_e4m3<T>(a.y, true)};
+          s[r] = mfma<T>(a, q[e], s[r]);
+        }
+      }
+      if constexpr (more.value) load_k(tile + 1);
+      float z[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) z[t] = s[t >> 2][t & 3] * cs;
+      if (!__all(valid == 0xFFu)) {
+        // what stands in masked rows may be anything: neither its scores nor its values are used
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const bool in = valid >> t & 1;
+          z[t] = in ? z[t] : -__builtin_inff();
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vw[t][w] = in ? vw[t][w] : 0u;
+        }
+      }
+      float top = z[0];
+#pragma unroll
+      for (int t = 1; t < 8; ++t) top = fmaxf(top, z[t]);
+      if (__any(top > ref + (kTop + kLag))) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float now = fmaxf(ref, top - kTop);
+        const float to = now == -__builtin_inff() ? 0.f : now;
+        const float keep = __builtin_amdgcn_exp2f(ref - to);
+        sum *= keep;
+#pragma unroll
+        for (int j = 0; j < VD; ++j) o[j] *= keep;
+        ref = now, use = to;
+      }
+      // the weights in two terms of their type, so that their rounding adds
+      // nothing to the output's own
+      Frag hi, lo;
+#pragma unroll
+      for (int t = 0; t < 8; t += 2) {
+        const float a = __builtin_amdgcn_exp2f(z[t] - use), bb = __builtin_amdgcn_exp2f(z[t + 1] - use);
+        sum += a + bb;
+        hi[t / 2] = pack2<PT>(a, bb);
+        const floatx2 back = unpack2<PT>(hi[t / 2]);
+        lo[t / 2] = pack2<PT>(a - back.x, bb - back.y);
+      }
+      // turn V: word w of tokens t, t + 1 holds dims 2w, 2w + 1 (bytes: 4)
+      constexpr int kPer = 4 / ES;
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        Frag f[kPer];
+#pragma unroll
+        for (int t = 0; t < 8; t += 2) {
+          if constexpr (F8) {
+            const uint32_t even = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x05010400u);
+            const uint32_t odd = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x07030602u);
+            f[0][t / 2] = from_e4m3<PT>(even, false), f[1][t / 2] = from_e4m3<PT>(even, true);
+            f[2][t / 2] = from_e4m3<PT>(odd, false), f[3][t / 2] = from_e4m3<PT>(odd, true);
+          } else {
+            f[0][t / 2] = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x05040100u);
+            f[1][t / 2] = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x07060302u);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          o[kPer * w + j] = mfma<PT>(f[j], hi, o[kPer * w + j]);
+          o[kPer * w + j] = mfma<PT>(f[j], lo, o[kPer * w + j]);
+        }
+      }
+    };
+    load_k(0);
+    for (int tile = 0; tile + 1 < n_tiles; ++tile) step(tile, std::true_type{});
+    step(n_tiles - 1, std::false_type{});
+  }
+
+  sum += __shfl_xor(sum, 16, 64);
+  sum += __shfl_xor(sum, 32, 64);
+  out.ref = ref, out.sum = sum;
+  return out;
+}
+
+// The work is shared out evenly over the waves that a GPU holds at once:
+// every work-group is one wave with an equal run of the units of all
+// sequences and streams, so that waves in different phases (finding their
+// rows, streaming, writing) share a compute unit without waiting for each
+// other. A stream that one wave has whole is finished here, the others' parts
+// go to the workspace: a wave has at most one that an earlier wave began (slot
+// 0) and one that it begins itself (slot 1).
+template <typename T, bool F8, int DT, bool LISTED, bool FULL>
+__global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p) {
+  constexpr int VD = DT / 16, kStage = 512;
+  __shared__ int64_t rows[kStage];
   const int lane = threadIdx.x, g = lane >> 4, i = lane & 15;
   const int streams = p.lists * p.tiles;
   Share share;
@@ -214,235 +455,81 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
     }
     const int c = max(0, pos - kStart), c1 = max(0, min(sp.cost, pos + (u1 - u)) - kStart);
     if (c1 == c) continue;
-    const int list = x / p.tiles, head0 = (x % p.tiles) * kHeads;
-    const int h = list * p.heads / p.lists;
-    const int n_heads = min(kHeads, p.group - head0);
-    const char* kb = p.k + h * p.head_stride * ES;
-    const char* vb = p.v + h * p.head_stride * ES;
-    const float cs = p.scale * (p.k_scale ? p.k_scale[h] : 1.f);
-    const int qh = list * p.group + head0;
-
-    Frag q[KS];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d = F8 ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
-      q[s] = Frag{0, 0, 0, 0};
-      if (i < n_heads && (FULL || d < p.dim)) q[s] = *(const Frag*)(p.q + (b * p.q_stride + (qh + i) * p.q_head + d) * 2);
-    }
-    floatx4 o[VD];
-#pragma unroll
-    for (int j = 0; j < VD; ++j) o[j] = floatx4{0, 0, 0, 0};
-    float ref = -__builtin_inff(), use = 0.f, sum = 0.f;
-
-    constexpr int kStageTiles = LISTED ? kStage / kTile : kStage / (kTile / 8);
-    const int n_all = sp.end > sp.base ? c1 : c;  // no tokens, no tiles
-    for (int c0 = c; c0 < n_all; c0 += kStageTiles) {
-      const int n_tiles = min(n_all - c0, kStageTiles);
-      // offsets of the rows: one per token of a list, one per 8 tokens else
-      __syncthreads();
-      for (int e = lane; e < n_tiles * (LISTED ? kTile : kTile / 8); e += 64) {
-        int t;
-        int64_t off = -1;
-        bool known;
-        if (LISTED) {
-          const int at = c0 * kTile + e, always = sp.end - p.count;
-          known = at < sp.end;
-          t = at < sp.first ? at : sp.last + (at - sp.first);
-          if (known && at >= always) {
-            t = p.ids[((int64_t)b * p.lists + list) * p.count + (at - always)];
-            known = t >= sp.first && t < sp.last;
-          }
-        } else {
-          t = sp.base + c0 * kTile + 8 * e;
-          known = t < sp.end;
-        }
-        if (known) {
-          const int32_t page = p.tables[b * p.table_stride + (t >> p.page_shift)];
-          if (page >= 0 && page < p.pages)
-            off = (page * p.page_stride + (t & ((1 << p.page_shift) - 1)) * p.row_stride) * ES;
-        }
-        rows[e] = off;
-      }
-      __syncthreads();
-
-      Frag kf[2][KS];
-      auto load_k = [&](int tile) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int tok = 8 * (i >> 2) + (i & 3) + 4 * r;
-          int64_t off = LISTED ? rows[tile * kTile + tok] : rows[tile * (kTile / 8) + (i >> 2)];
-          off = off < 0 ? 0 : off;
-          if (!LISTED) off += ((i & 3) + 4 * r) * p.row_stride * ES;
-          const char* row = kb + off;
-          if constexpr (F8) {
-#pragma unroll
-            for (int s = 0; s < KS; s += 2) {
-              const int d = 32 * s + 16 * g;
-              const bool in = FULL || d < p.dim;
-              uintx4 w = load<FULL>((const uintx4*)(row + (in ? d : 0)));
-              if (!in) w = uintx4{0, 0, 0, 0};
-              kf[r][s] = Frag{w.x, w.y, 0, 0};
-              kf[r][s + 1] = Frag{w.z, w.w, 0, 0};
-            }
-          } else {
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              const int d = 32 * s + 8 * g;
-              const bool in = FULL || d < p.dim;
-              uintx4 w = load<FULL>((const uintx4*)(row + (in ? d : 0) * 2));
-              if (!in) w = uintx4{0, 0, 0, 0};
-              kf[r][s] = w;
-            }
-          }
-        }
-      };
-      constexpr int VW = VD * ES / 4;  // words of V per token and lane
-      // a chunk of V past the end of a row is the row's first instead: those dims are never stored
-      const auto v_at = [&](int w) {
-        const int d = w / 4 * 16 * BD + i * BD;
-        return FULL || d < p.dim ? d * ES : 0;
-      };
-
-      // one tile, with the next one's keys on their way while its values are
-      auto step = [&](int tile, auto more) {
-        uint32_t vw[8][VW];
-        uint32_t valid = 0;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          int64_t off = LISTED ? rows[tile * kTile + 8 * g + t] : rows[tile * (kTile / 8) + g];
-          bool in = off >= 0;
-          if (!LISTED) {
-            const int tok = sp.base + (c0 + tile) * kTile + 8 * g + t;
-            in = in && tok >= sp.begin && tok < sp.end;
-          }
-          valid |= in ? 1u << t : 0u;
-          off = off < 0 ? 0 : off;
-          if (!LISTED) off += t * p.row_stride * ES;
-          const char* row = vb + off;
-          if constexpr (VW >= 4) {
-#pragma unroll
-            for (int w = 0; w < VW; w += 4) {
-              const uintx4 y = load<FULL>((const uintx4*)(row + v_at(w)));
-              vw[t][w] = y.x, vw[t][w + 1] = y.y, vw[t][w + 2] = y.z, vw[t][w + 3] = y.w;
-            }
-          } else if constexpr (VW == 2) {
-            const uintx2 y = load<FULL>((const uintx2*)(row + v_at(0)));
-            vw[t][0] = y.x, vw[t][1] = y.y;
-          } else {
-            vw[t][0] = load<FULL>((const uint32_t*)(row + v_at(0)));
-          }
-        }
-        floatx4 s[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          s[r] = floatx4{0, 0, 0, 0};
-#pragma unroll
-          for (int e = 0; e < KS; ++e) {
-            Frag a = kf[r][e];
-            if constexpr (F8)
-              a = Frag{from_e4m3<T>(a.x, false), from_e4m3<T>(a.x, true), from_e4m3<T>(a.y, false), from_e4m3<T>(a.y, true)};
-            s[r] = mfma<T>(a, q[e], s[r]);
-          }
-        }
-        if constexpr (more.value) load_k(tile + 1);
-        float z[8];
-#pragma unroll
-        for (int t = 0; t < 8; ++t) z[t] = s[t >> 2][t & 3] * cs;
-        if (!__all(valid == 0xFFu)) {
-          // what stands in masked rows may be anything: neither its scores nor its values are used
-#pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            const bool in = valid >> t & 1;
-            z[t] = in ? z[t] : -__builtin_inff();
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vw[t][w] = in ? vw[t][w] : 0u;
-          }
-        }
-        float top = z[0];
-#pragma unroll
-        for (int t = 1; t < 8; ++t) top = fmaxf(top, z[t]);
-        if (__any(top > ref + (kTop + kLag))) {
-          top = fmaxf(top, __shfl_xor(top, 16, 64));
-          top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float now = fmaxf(ref, top - kTop);
-          const float to = now == -__builtin_inff() ? 0.f : now;
-          const float keep = __builtin_amdgcn_exp2f(ref - to);
-          sum *= keep;
-#pragma unroll
-          for (int j = 0; j < VD; ++j) o[j] *= keep;
-          ref = now, use = to;
-        }
-        // the weights in two terms of their type, so that their rounding adds
-        // nothing to the output's own
-        Frag hi, lo;
-#pragma unroll
-        for (int t = 0; t < 8; t += 2) {
-          const float a = __builtin_amdgcn_exp2f(z[t] - use), bb = __builtin_amdgcn_exp2f(z[t + 1] - use);
-          sum += a + bb;
-          hi[t / 2] = pack2<PT>(a, bb);
-          const floatx2 back = unpack2<PT>(hi[t / 2]);
-          lo[t / 2] = pack2<PT>(a - back.x, bb - back.y);
-        }
-        // turn V: word w of tokens t, t + 1 holds dims 2w, 2w + 1 (bytes: 4)
-        constexpr int kPer = 4 / ES;
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          Frag f[kPer];
-#pragma unroll
-          for (int t = 0; t < 8; t += 2) {
-            if constexpr (F8) {
-              const uint32_t even = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x05010400u);
-              const uint32_t odd = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x07030602u);
-              f[0][t / 2] = from_e4m3<PT>(even, false), f[1][t / 2] = from_e4m3<PT>(even, true);
-              f[2][t / 2] = from_e4m3<PT>(odd, false), f[3][t / 2] = from_e4m3<PT>(odd, true);
-            } else {
-              f[0][t / 2] = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x05040100u);
-              f[1][t / 2] = __builtin_amdgcn_perm(vw[t + 1][w], vw[t][w], 0x07060302u);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            o[kPer * w + j] = mfma<PT>(f[j], hi, o[kPer * w + j]);
-            o[kPer * w + j] = mfma<PT>(f[j], lo, o[kPer * w + j]);
-          }
-        }
-      };
-      load_k(0);
-      for (int tile = 0; tile + 1 < n_tiles; ++tile) step(tile, std::true_type{});
-      step(n_tiles - 1, std::false_type{});
-    }
-
-    sum += __shfl_xor(sum, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
-    const bool whole = c == 0 && c1 == sp.tiles;
-    const auto dim_of = [&](int j, int r) { return j / BD * 16 * BD + (4 * g + r) * BD + j % BD; };
-    if (i < n_heads) {
-      if (whole) {
-        const int64_t row = (int64_t)b * p.q_heads + qh + i;
-        const float inv = (p.v_scale ? p.v_scale[h] : 1.f) / sum;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-#pragma unroll
-          for (int j = 0; j < VD; j += 4) {
-            const int d = dim_of(j, r);
-            float y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = sum == 0.f ? 0.f : o[j + e][r] * inv;
-            if (FULL || d < p.dim) *(uintx2*)(p.out + (row * p.dim + d) * 2) = uintx2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
-          }
-        }
-        if (g == 0 && p.lse) p.lse[row] = sum == 0.f ? -__builtin_inff() : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
-      } else {
-        float* part = p.parts + ((int64_t)blockIdx.x * 2 + (c == 0 ? 1 : 0)) * p.part_heads * (DT + 2);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int j = 0; j < VD; j += 4)
-            *(floatx4*)(part + i * DT + dim_of(j, r)) = floatx4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
-        if (g == 0) *(floatx2*)(part + p.part_heads * DT + 2 * i) = floatx2{ref, sum};
-      }
-    }
+    const Stream at = stream_of(p, b, x);
+    const Sums<DT> s = attend_tiles<T, F8, DT, LISTED, FULL, kStage>(p, sp, at, c, c1, rows);
     if (c == 0 && lane == 0) p.ends[(int64_t)b * streams + x] = int2{(int)blockIdx.x, share.owner(u - pos + sp.cost - 1)};
+    if (i >= at.heads) continue;
+    if (c == 0 && c1 == sp.tiles) {
+      const int64_t row = (int64_t)b * p.q_heads + at.q_head + i;
+      const float inv = (p.v_scale ? p.v_scale[at.kv_head] : 1.f) / s.sum;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int j = 0; j < VD; j += 4) {
+          const int d = dim_of<F8, DT>(g, j, r);
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = s.sum == 0.f ? 0.f : s.o[j + e][r] * inv;
+          if (FULL || d < p.dim) *(uintx2*)(p.out + (row * p.dim + d) * 2) = uintx2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+        }
+      }
+      if (g == 0 && p.lse) p.lse[row] = s.sum == 0.f ? -__builtin_inff() : (s.ref + __builtin_amdgcn_logf(s.sum)) * kLn2;
+    } else {
+      float* part = p.parts + ((int64_t)blockIdx.x * 2 + (c == 0 ? 1 : 0)) * p.part_heads * (DT + 2);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VD; j += 4)
+          *(floatx4*)(part + i * DT + dim_of<F8, DT>(g, j, r)) = floatx4{s.o[j][r], s.o[j + 1][r], s.o[j + 2][r], s.o[j + 3][r]};
+      if (g == 0) *(floatx2*)(part + p.part_heads * DT + 2 * i) = floatx2{s.ref, s.sum};
+    }
+  }
+}
+
+// Short streams: a work-group has a stream, its waves equal runs of the tiles,
+// and joins them itself. No lengths to add up and no second kernel.
+template <typename T, bool F8, int DT, bool LISTED, bool FULL>
+__global__ __launch_bounds__(64 * group_waves(DT)) void attend_group_kernel(Params p) {
+  constexpr int VD = DT / 16;
+  extern __shared__ int64_t lds[];
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int streams = p.lists * p.tiles;
+  const int b = blockIdx.x / streams;
+  const Span sp = span_of<LISTED>(p, b);
+  const Stream at = stream_of(p, b, blockIdx.x % streams);
+  const Sums<DT> s = attend_tiles<T, F8, DT, LISTED, FULL, kGroupStage>(
+      p, sp, at, sp.tiles * wave / waves, sp.tiles * (wave + 1) / waves, lds + wave * kGroupStage);
+  __syncthreads();  // the rows' offsets make room for the waves' sums
+  float* const sums = (float*)lds;                        // [waves][heads][DT]
+  floatx2* const stats = (floatx2*)(sums + waves * at.heads * DT);  // [waves][heads]
+  if (i < at.heads) {
+    float* mine = sums + (wave * at.heads + i) * DT;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < VD; j += 4)
+        *(floatx4*)(mine + dim_of<F8, DT>(g, j, r)) = floatx4{s.o[j][r], s.o[j + 1][r], s.o[j + 2][r], s.o[j + 3][r]};
+    if (g == 0) stats[wave * at.heads + i] = floatx2{s.ref, s.sum};
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < at.heads * (DT / 4); e += blockDim.x) {
+    const int n = e / (DT / 4), d = e % (DT / 4) * 4;
+    float top = stats[n].x, tot = 0;
+    for (int w = 1; w < waves; ++w) top = fmaxf(top, stats[w * at.heads + n].x);
+    floatx4 acc = {0, 0, 0, 0};
+    for (int w = 0; w < waves; ++w) {
+      const floatx2 m = stats[w * at.heads + n];
+      const float f = m.x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m.x - top);  // then its sums are zero (or NaN)
+      tot += f * m.y;
+      acc += *(const floatx4*)(sums + (w * at.heads + n) * DT + d) * f;
+    }
+    const int64_t row = (int64_t)b * p.q_heads + at.q_head + n;
+    const float inv = (p.v_scale ? p.v_scale[at.kv_head] : 1.f) / tot;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = tot == 0.f ? 0.f : acc[k] * inv;
+    if (FULL || d < p.dim) *(uintx2*)(p.out + (row * p.dim + d) * 2) = uintx2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
+    if (d == 0 && p.lse) p.lse[row] = tot == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(tot)) * kLn2;
   }
 }
 
@@ -529,6 +616,7 @@ int compute_units() {
 struct Plan {
   int dt, lists, group, tiles, part_heads;
   int64_t streams, waves;
+  int group_waves;  // of a group's work-group; 0: the waves share all streams
   bool joins;
   int64_t ends_bytes, bytes;
 };
@@ -545,6 +633,20 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
   const int64_t tiles = std::max<int64_t>(1, (max_tokens + (lists ? 0 : 7) + kTile - 1) / kTile);
   if (tiles + kStart > 0x7FFFFFFF / std::max<int64_t>(1, batch * a.streams)) throw std::invalid_argument("batch x heads x tokens is too large");
   const int64_t resident = std::min(kWaves, compute_units() * (a.dt == 256 ? 4 : 8));
+  // A group spares the second kernel, but a wave of it waits 1.4 us for each
+  // tile while most of the GPU idles where there are few streams. Of 8 key
+  // heads of 128 fp16 values, group against shared, us: one sequence of 100
+  // tokens 5.2 / 8.4, 300 7.9 / 8.5, 700 10.8 / 8.9; four of 500 9.2 / 10.1, of
+  // 1000 17.1 / 12.5; 16 of 1000 20.4 / 21.5; 64 of 1000 45.7 / 54.4; 512 of 128
+  // 48.7 / 57.2. Longer tables may hold sequences too unlike for it.
+  const int64_t all = batch * a.streams;
+  const int most = std::min(group_waves(a.dt), kGroupLds / std::max(a.part_heads * (a.dt + 2) * 4, kGroupStage * 8));
+  const bool grouped = all > 0 && tiles <= most * (2 * all >= compute_units() ? 4 : 2);
+  a.group_waves = grouped ? (int)std::clamp<int64_t>(resident / all, 1, std::min<int64_t>(most, tiles)) : 0;
+  if (a.group_waves) {
+    a.joins = false, a.waves = 0, a.ends_bytes = 0, a.bytes = 0;
+    return a;
+  }
   a.waves = std::min(batch * a.streams * (tiles + kStart), resident);
   a.joins = tiles > 1;
   a.ends_bytes = (batch * a.streams * 8 + 15) / 16 * 16;
@@ -555,6 +657,14 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
 template <typename T, bool F8, int DT>
 void launch(const Params& p, const Plan& plan, bool listed, hipStream_t s) {
   const bool full = p.dim == DT;
+  if (plan.group_waves) {
+    auto kernel = listed ? (full ? attend_group_kernel<T, F8, DT, true, true> : attend_group_kernel<T, F8, DT, true, false>)
+                         : (full ? attend_group_kernel<T, F8, DT, false, true> : attend_group_kernel<T, F8, DT, false, false>);
+    const size_t lds = (size_t)plan.group_waves * std::max(plan.part_heads * (DT + 2) * 4, kGroupStage * 8);
+    kernel<<<(unsigned)(p.batch * plan.streams), 64 * plan.group_waves, lds, s>>>(p);
+    hip_check(hipGetLastError(), "attention");
+    return;
+  }
   auto kernel = listed ? (full ? attend_kernel<T, F8, DT, true, true> : attend_kernel<T, F8, DT, true, false>)
                        : (full ? attend_kernel<T, F8, DT, false, true> : attend_kernel<T, F8, DT, false, false>);
   kernel<<<(unsigned)plan.waves, 64, 0, s>>>(p);
@@ -586,7 +696,7 @@ void attend(const AttendArgs& a, const KvPages& pages, hipStream_t s) {
   p.limit = pages.pages ? (int)std::min<int64_t>({a.max_len, width, 0x7FFFFF00}) : 0;
   const int64_t most = listed ? a.first + a.last + a.count : a.last < 0 ? a.max_len : std::min(a.max_len, a.last);
   const Plan plan = plan_of(a.batch, a.q.heads, pages, most, a.lists);
-  if (a.workspace_bytes < plan.bytes || !a.workspace || ((uintptr_t)a.workspace & 15u))
+  if (plan.bytes && (a.workspace_bytes < plan.bytes || !a.workspace || ((uintptr_t)a.workspace & 15u)))
     throw std::invalid_argument("workspace must be 16-byte aligned and hold " + std::to_string(plan.bytes) + " bytes");
   p.q = (const char*)a.q.p, p.q_stride = a.q.stride, p.q_head = a.q.head_stride;
   p.k = pages.k, p.v = pages.v;

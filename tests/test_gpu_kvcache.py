@@ -686,3 +686,23 @@ def test_empty_calls(jasper):
     out = jasper.decode_attention(randn((1, 4, 64), F16, 1), empty, empty, torch.zeros((1, 4), dtype=torch.int32, device="cuda"),
                                   torch.tensor([9], dtype=torch.int32, device="cuda"))
     assert (out == 0).all()
+
+
+SHORT = [0, 1, 5, 8, 17, 31, 32, 33, 64, 100, 129, 255, 300, 500]
+
+
+@pytest.mark.parametrize("hq,heads,dim,page,dtype,cache", [
+    (8, 2, 128, 16, F16, F16), (32, 8, 128, 16, BF16, BF16), (20, 1, 128, 16, BF16, F8), (5, 5, 64, 32, F16, F16),
+    (16, 1, 64, 8, F16, F16), (3, 3, 80, 16, F16, F8), (16, 1, 96, 8, BF16, BF16), (12, 4, 256, 16, F16, F16),
+    (17, 1, 256, 8, BF16, F8), (6, 2, 200, 64, BF16, BF16), (2, 1, 8, 128, F16, F16), (4, 2, 16, 8, BF16, F8)])
+@pytest.mark.parametrize("repeat", [1, 20])
+def test_decode_short(jasper, hq, heads, dim, page, dtype, cache, repeat):
+    """Tables that hold few tokens; few sequences, and many."""
+    lens = SHORT * repeat
+    kp, vp, tables, keys, values = build_cache(lens, heads, page, dim, cache, 180)
+    tables = tables[:, :-(-500 // page)]  # rows of a wider table
+    ks, vs = f8_scales(heads, cache, 181)
+    q = randn((len(lens), hq, dim), dtype, 182, 2.0)
+    ref = ref_attention(q, keys, values, dim ** -0.5, lambda i, j: torch.arange(lens[i]), dtype, ks, vs)
+    tens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    check(jasper.decode_attention(q, kp, vp, tables, tens, k_scale=ks, v_scale=vs, return_lse=True), ref)
