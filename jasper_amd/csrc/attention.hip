@@ -554,6 +554,16 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
   const float* const own = p.parts + ((int64_t)range.x * 2 + 1) * size;  // the part that begins the stream
   const float* const rest = own - size;                                   // part i > 0: 2 * size * i from here
   const auto part = [&](int i) { return i ? rest + (int64_t)i * 2 * size : own; };
+  const int d = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
+  floatx4 y[kBatch];
+  const auto fetch = [&](int i0) {
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) {
+      const int i = i0 + e * kRows;
+      if (i < parts) y[e] = *(const floatx4*)(part(i) + n * DT + 4 * d);
+    }
+  };
+  fetch(row);  // on their way while the weights are found
   float top = -__builtin_inff();
   for (int i = threadIdx.x; i < parts; i += kJoin) {
     const float m = part(i)[stats];
@@ -575,15 +585,9 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
   if (lane == 0) tots[wave] = tot;
   __syncthreads();
   tot = (tots[0] + tots[1]) + (tots[2] + tots[3]);
-  const int d = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
   floatx4 acc = {0, 0, 0, 0};
   for (int i0 = row; i0 < parts; i0 += kRows * kBatch) {
-    floatx4 y[kBatch];
-#pragma unroll
-    for (int e = 0; e < kBatch; ++e) {
-      const int i = i0 + e * kRows;
-      y[e] = *(const floatx4*)(part(i < parts ? i : i0) + n * DT + 4 * d);
-    }
+    if (i0 != row) fetch(i0);
 #pragma unroll
     for (int e = 0; e < kBatch; ++e) {
       const int i = i0 + e * kRows;
@@ -638,10 +642,14 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
   // heads of 128 fp16 values, group against shared, us: one sequence of 100
   // tokens 5.2 / 8.4, 300 7.9 / 8.5, 700 10.8 / 8.9; four of 500 9.2 / 10.1, of
   // 1000 17.1 / 12.5; 16 of 1000 20.4 / 21.5; 64 of 1000 45.7 / 54.4; 512 of 128
-  // 48.7 / 57.2. Longer tables may hold sequences too unlike for it.
+  // 48.7 / 57.2. Longer tables may hold sequences too unlike for it; lists are
+  // alike, and are grouped up to eight tiles a wave where there is one for
+  // three in four compute units: 1,068 tokens in 128 lists 29.3 / 26.3, in 256
+  // 30.2 / 37.7, in 512 54.1 / 64.2.
   const int64_t all = batch * a.streams;
   const int most = std::min(group_waves(a.dt), kGroupLds / std::max(a.part_heads * (a.dt + 2) * 4, kGroupStage * 8));
-  const bool grouped = all > 0 && tiles <= most * (2 * all >= compute_units() ? 4 : 2);
+  const int each = lists && 4 * all >= 3 * compute_units() ? 8 : 2 * all >= compute_units() ? 4 : 2;
+  const bool grouped = all > 0 && tiles <= most * each;
   a.group_waves = grouped ? (int)std::clamp<int64_t>(resident / all, 1, std::min<int64_t>(most, tiles)) : 0;
   if (a.group_waves) {
     a.joins = false, a.waves = 0, a.ends_bytes = 0, a.bytes = 0;

@@ -269,9 +269,10 @@ def test_copy_pages(jasper, cache, layers, heads, page, dim, layout):
 
 
 @pytest.mark.parametrize("moves,sequences,width", [(1, 1, 1), (513, 5, 77), (1025, 64, 130), (2500, 300, 33)])
-def test_copy_pages_moves_tables(jasper, moves, sequences, width):
+@pytest.mark.parametrize("heads,page,dim", [(1, 8, 16), (3, 8, 40), (2, 64, 64)])
+def test_copy_pages_moves_tables(jasper, moves, sequences, width, heads, page, dim):
     pages = 2 * moves + 100
-    kp, vp = make_pages(pages, 1, 8, 16, F16, seed=30)
+    kp, vp = make_pages(pages, heads, page, dim, F16, seed=30)
     before = kp.clone()
     order = torch.randperm(pages)
     src, dst = order[:moves].int(), order[moves:2 * moves].int()
