@@ -7,6 +7,7 @@
 #include "kvtypes.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <stdexcept>
 #include <type_traits>
 
@@ -534,9 +535,10 @@ __global__ __launch_bounds__(64 * group_waves(DT)) void attend_group_kernel(Para
 }
 
 // Joins the parts of a stream that several waves had: a work-group per
-// sequence, stream and head. The parts' weights go to LDS, then a thread has
-// four dims of every kRows-th part, eight loads in flight.
-template <typename T, int DT>
+// sequence, stream and head, and for streams of many parts per DIMS dims of
+// it. The parts' weights go to LDS, then a thread has four dims of every
+// kRows-th part, eight loads in flight.
+template <typename T, int DT, int DIMS>
 __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
   const int streams = p.lists * p.tiles;
   const int b = blockIdx.x / streams, x = blockIdx.x % streams, n = blockIdx.y;
@@ -545,7 +547,7 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
   const int2 range = p.ends[blockIdx.x];
   const int parts = range.y - range.x + 1;
   if (parts == 1) return;
-  constexpr int kLanes = DT / 4, kRows = kJoin / kLanes, kBatch = 8;
+  constexpr int kLanes = DIMS / 4, kRows = kJoin / kLanes, kBatch = 8;
   __shared__ float weight[kWaves];
   __shared__ float tops[kJoin / 64], tots[kJoin / 64];
   __shared__ floatx4 sums[kRows][kLanes];
@@ -554,13 +556,13 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
   const float* const own = p.parts + ((int64_t)range.x * 2 + 1) * size;  // the part that begins the stream
   const float* const rest = own - size;                                   // part i > 0: 2 * size * i from here
   const auto part = [&](int i) { return i ? rest + (int64_t)i * 2 * size : own; };
-  const int d = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
+  const int lane4 = threadIdx.x % kLanes, row = threadIdx.x / kLanes, d = blockIdx.z * DIMS + 4 * lane4;
   floatx4 y[kBatch];
   const auto fetch = [&](int i0) {
 #pragma unroll
     for (int e = 0; e < kBatch; ++e) {
       const int i = i0 + e * kRows;
-      if (i < parts) y[e] = *(const floatx4*)(part(i) + n * DT + 4 * d);
+      if (i < parts) y[e] = *(const floatx4*)(part(i) + n * DT + d);
     }
   };
   fetch(row);  // on their way while the weights are found
@@ -594,15 +596,15 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
       if (i < parts) acc += y[e] * weight[i];
     }
   }
-  sums[row][d] = acc;
+  sums[row][lane4] = acc;
   __syncthreads();
   if (row) return;
-  for (int r = 1; r < kRows; ++r) acc += sums[r][d];
+  for (int r = 1; r < kRows; ++r) acc += sums[r][lane4];
   const int64_t at = (int64_t)b * p.q_heads + list * p.group + head0 + n;
   const float inv = (p.v_scale ? p.v_scale[list * p.heads / p.lists] : 1.f) / tot;
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc[e] = tot == 0.f ? 0.f : acc[e] * inv;
-  if (4 * d < p.dim) *(uintx2*)(p.out + (at * p.dim + 4 * d) * 2) = uintx2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
+  if (d < p.dim) *(uintx2*)(p.out + (at * p.dim + d) * 2) = uintx2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
   if (d == 0 && p.lse) p.lse[at] = tot == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(tot)) * kLn2;
 }
 
@@ -655,7 +657,14 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
     a.joins = false, a.waves = 0, a.ends_bytes = 0, a.bytes = 0;
     return a;
   }
-  a.waves = std::min(batch * a.streams * (tiles + kStart), resident);
+  // Fewer waves where there is little for each, by what was measured of small
+  // calls in us: a tile more costs a wave 1.2, a part more the join of its
+  // stream 0.02, a wave more the call 0.003. One sequence of 16,000 tokens 24.9
+  // -> 19.6 (2048 waves before), 131,072 under one key head 58.9 -> 22.8.
+  const double units = (double)all * (tiles + kStart);
+  const double wave_cost = (0.02 / all + 0.003) * std::max(1.0, a.part_heads / 8.0);
+  const int64_t worth = std::max<int64_t>(1, (int64_t)std::sqrt(1.2 * units / wave_cost));
+  a.waves = std::min({(int64_t)units, resident, worth});
   a.joins = tiles > 1;
   a.ends_bytes = (batch * a.streams * 8 + 15) / 16 * 16;
   a.bytes = a.ends_bytes + a.waves * 2 * a.part_heads * (a.dt + 2) * 4;
@@ -678,7 +687,11 @@ void launch(const Params& p, const Plan& plan, bool listed, hipStream_t s) {
   kernel<<<(unsigned)plan.waves, 64, 0, s>>>(p);
   hip_check(hipGetLastError(), "attention");
   if (plan.joins) {
-    join_kernel<T, DT><<<dim3((unsigned)(p.batch * plan.streams), (unsigned)plan.part_heads), kJoin, 0, s>>>(p);
+    const int64_t all = p.batch * plan.streams;
+    if (plan.waves > 32 * all)
+      join_kernel<T, DT, 32><<<dim3((unsigned)all, (unsigned)plan.part_heads, DT / 32), kJoin, 0, s>>>(p);
+    else
+      join_kernel<T, DT, DT><<<dim3((unsigned)all, (unsigned)plan.part_heads), kJoin, 0, s>>>(p);
     hip_check(hipGetLastError(), "attention join");
   }
 }

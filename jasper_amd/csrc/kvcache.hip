@@ -123,22 +123,19 @@ void launch_token(const TokenParams& p, int P, hipStream_t s) {
   if (p.n == 0 || all == 0) return;
   const int chunks = p.dim / (2 * P);
   if (chunks > 1024) throw std::invalid_argument("a head is too large");
-  // Few tokens: a thread per chunk of a head, so that a token is as many
-  // waves as it has work. Many: half a wave per token, whose threads keep
-  // their cosines for several heads (8192 tokens of 32 + 8 heads of 128: 37.5
-  // us, 42.0 with a wave, 43.5 with two waves to a token).
-  const int wide = std::max(1, 256 / chunks);
-  dim3 block, grid;
-  if (p.n < 1024) {
-    block = dim3(chunks, std::min(all, wide), 1);
-    grid = dim3((unsigned)p.n, (all + (int)block.y - 1) / (int)block.y);
-  } else {
-    block = dim3(chunks, std::max(1, 32 / chunks), 1);
-    block.z = std::max(1u, 256u / (block.x * block.y));
-    const int64_t blocks = (p.n + block.z - 1) / block.z;
-    if (blocks > 0x7FFFFFFF) throw std::invalid_argument("too many tokens (too large)");
-    grid = dim3((unsigned)blocks, 1);
-  }
+  // A thread per chunk of a head where that is all there is to do; with more,
+  // threads keep their cosines for several heads, up to 12: 512 work-items for
+  // each compute unit come first. 445 tokens of 64 + 2 x 8 heads of 256 values
+  // 14.4 us (25.3 with a thread each), 6007 of 32 + 2 x 8 of 128 31.5 (33.4 with
+  // 10 heads to a thread, 43.8 with 24).
+  const int64_t items = p.n * all * chunks;
+  const int per = (int)std::clamp<int64_t>(items / 131072, 1, 12), lanes = (all + per - 1) / per;
+  dim3 block(chunks, std::min(lanes, std::max(1, 256 / chunks)), 1), grid;
+  grid.y = (lanes + block.y - 1) / block.y;
+  if (grid.y == 1) block.z = std::max(1u, 256u / (block.x * block.y));
+  const int64_t blocks = (p.n + block.z - 1) / block.z;
+  if (blocks > 0x7FFFFFFF) throw std::invalid_argument("too many tokens (too large)");
+  grid.x = (unsigned)blocks;
   auto kernel = P == 8 ? token_kernel<T, CT, 8, APPEND> : P == 4 ? token_kernel<T, CT, 4, APPEND>
                                                                  : token_kernel<T, CT, 1, APPEND>;
   kernel<<<grid, block, 0, s>>>(p);
