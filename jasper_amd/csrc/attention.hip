@@ -19,6 +19,7 @@ constexpr int kTile = 32;    // tokens a wave takes at once
 constexpr int kHeads = 16;   // query heads of a matrix instruction
 constexpr int kStart = 2;    // what beginning a stream costs a wave, in tiles
 constexpr int kWaves = 2048;  // at most; of a call
+constexpr int kStage = 512;   // row offsets of a wave, in LDS
 constexpr int kJoin = 256;   // threads of a joining work-group
 constexpr int kGroupStage = 256;        // row offsets of a wave of a group, in LDS
 constexpr int kGroupLds = 64 << 10;     // bytes at most
@@ -41,7 +42,8 @@ struct Params {
   float* parts;
   int2* ends;
   float scale;  // times log2(e)
-  int batch, heads, q_heads, lists, group, tiles, count;  // tiles: of 16 heads per list
+  int batch, heads, q_heads, lists, group, count;
+  int head_tiles, side;  // 16s of a list's query heads, and how many of them share a work-group
   int part_heads;
   int page_shift, pages, dim;
   int limit, first, last;  // tokens; last: -1 for all
@@ -139,7 +141,7 @@ struct Share {
 // before that sequence. -1: there is no work for it.
 template <bool LISTED>
 __device__ int find_sequence(const Params& p, int streams, Share& share, int& before) {
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63;
   const int run = (p.batch + 63) / 64;
   const int b0 = min(lane * run, p.batch), b1 = min(b0 + run, p.batch);
   int mine = 0;
@@ -187,8 +189,8 @@ struct Stream {
   int b, list, heads, q_head, kv_head;
 };
 
-__device__ __forceinline__ Stream stream_of(const Params& p, int b, int x) {
-  const int list = x / p.tiles, head0 = (x % p.tiles) * kHeads;
+__device__ __forceinline__ Stream stream_of(const Params& p, int b, int list, int head_tile) {
+  const int head0 = head_tile * kHeads;
   return {b, list, min(kHeads, p.group - head0), list * p.group + head0, list * p.heads / p.lists};
 }
 
@@ -433,12 +435,20 @@ __device__ __forceinline__ Sums<DT> attend_tiles(const Params& p, const Span& sp
 // other. A stream that one wave has whole is finished here, the others' parts
 // go to the workspace: a wave has at most one that an earlier wave began (slot
 // 0) and one that it begins itself (slot 1).
+//
+// More than 16 query heads to a list are further waves of the work-group,
+// which take the same rows at about the same time and find them in the caches:
+// 64 sequences of 8192 tokens, one key head of 128 values under 64 heads, 104
+// us (183 with a work-group for each 16; under 32 heads 75 and 101).
+constexpr int side_of(int dt) { return dt == 256 ? 4 : 8; }
+
 template <typename T, bool F8, int DT, bool LISTED, bool FULL>
-__global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p) {
-  constexpr int VD = DT / 16, kStage = 512;
-  __shared__ int64_t rows[kStage];
-  const int lane = threadIdx.x, g = lane >> 4, i = lane & 15;
-  const int streams = p.lists * p.tiles;
+__global__ __launch_bounds__(64 * (FULL ? 1 : side_of(DT)), DT == 256 ? 1 : 2) void attend_kernel(Params p) {
+  constexpr int VD = DT / 16;
+  extern __shared__ int64_t lds[];
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  const int wave = FULL ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per_list = (p.head_tiles + p.side - 1) / p.side, streams = p.lists * per_list;
   Share share;
   int before;
   int b = find_sequence<LISTED>(p, streams, share, before);
@@ -454,11 +464,14 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
       x = 0;
       sp = span_of<LISTED>(p, ++b);
     }
+    const int list = x / per_list, head_tile = x % per_list * p.side + wave;
     const int c = max(0, pos - kStart), c1 = max(0, min(sp.cost, pos + (u1 - u)) - kStart);
-    if (c1 == c) continue;
-    const Stream at = stream_of(p, b, x);
-    const Sums<DT> s = attend_tiles<T, F8, DT, LISTED, FULL, kStage>(p, sp, at, c, c1, rows);
-    if (c == 0 && lane == 0) p.ends[(int64_t)b * streams + x] = int2{(int)blockIdx.x, share.owner(u - pos + sp.cost - 1)};
+    if (c1 == c || head_tile >= p.head_tiles) continue;
+    const Stream at = stream_of(p, b, list, head_tile);
+    const Sums<DT> s = attend_tiles<T, F8, DT, LISTED, FULL, kStage>(p, sp, at, c, c1, lds + wave * kStage);
+    if (c == 0 && lane == 0)
+      p.ends[((int64_t)b * p.lists + list) * p.head_tiles + head_tile] =
+          int2{(int)blockIdx.x, share.owner(u - pos + sp.cost - 1)};
     if (i >= at.heads) continue;
     if (c == 0 && c1 == sp.tiles) {
       const int64_t row = (int64_t)b * p.q_heads + at.q_head + i;
@@ -476,7 +489,7 @@ __global__ __launch_bounds__(64, DT == 256 ? 1 : 2) void attend_kernel(Params p)
       }
       if (g == 0 && p.lse) p.lse[row] = s.sum == 0.f ? -__builtin_inff() : (s.ref + __builtin_amdgcn_logf(s.sum)) * kLn2;
     } else {
-      float* part = p.parts + ((int64_t)blockIdx.x * 2 + (c == 0 ? 1 : 0)) * p.part_heads * (DT + 2);
+      float* part = p.parts + (((int64_t)blockIdx.x * 2 + (c == 0 ? 1 : 0)) * p.side + wave) * p.part_heads * (DT + 2);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -495,10 +508,10 @@ __global__ __launch_bounds__(64 * group_waves(DT)) void attend_group_kernel(Para
   extern __shared__ int64_t lds[];
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int streams = p.lists * p.tiles;
-  const int b = blockIdx.x / streams;
+  const int head_tile = blockIdx.x % p.head_tiles, list = blockIdx.x / p.head_tiles % p.lists;
+  const int b = blockIdx.x / p.head_tiles / p.lists;
   const Span sp = span_of<LISTED>(p, b);
-  const Stream at = stream_of(p, b, blockIdx.x % streams);
+  const Stream at = stream_of(p, b, list, head_tile);
   const Sums<DT> s = attend_tiles<T, F8, DT, LISTED, FULL, kGroupStage>(
       p, sp, at, sp.tiles * wave / waves, sp.tiles * (wave + 1) / waves, lds + wave * kGroupStage);
   __syncthreads();  // the rows' offsets make room for the waves' sums
@@ -540,9 +553,8 @@ __global__ __launch_bounds__(64 * group_waves(DT)) void attend_group_kernel(Para
 // kRows-th part, eight loads in flight.
 template <typename T, int DT, int DIMS>
 __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
-  const int streams = p.lists * p.tiles;
-  const int b = blockIdx.x / streams, x = blockIdx.x % streams, n = blockIdx.y;
-  const int list = x / p.tiles, head0 = (x % p.tiles) * kHeads;
+  const int head_tile = blockIdx.x % p.head_tiles, list = blockIdx.x / p.head_tiles % p.lists, n = blockIdx.y;
+  const int b = blockIdx.x / p.head_tiles / p.lists, head0 = head_tile * kHeads;
   if (n >= p.group - head0) return;
   const int2 range = p.ends[blockIdx.x];
   const int parts = range.y - range.x + 1;
@@ -553,9 +565,10 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
   __shared__ floatx4 sums[kRows][kLanes];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int size = p.part_heads * (DT + 2), stats = p.part_heads * DT + 2 * n;
-  const float* const own = p.parts + ((int64_t)range.x * 2 + 1) * size;  // the part that begins the stream
-  const float* const rest = own - size;                                   // part i > 0: 2 * size * i from here
-  const auto part = [&](int i) { return i ? rest + (int64_t)i * 2 * size : own; };
+  // the part that begins the stream, and what part i > 0 is i steps from
+  const float* const own = p.parts + (((int64_t)range.x * 2 + 1) * p.side + head_tile % p.side) * size;
+  const float* const rest = own - p.side * size;
+  const auto part = [&](int i) { return i ? rest + (int64_t)i * 2 * p.side * size : own; };
   const int lane4 = threadIdx.x % kLanes, row = threadIdx.x / kLanes, d = blockIdx.z * DIMS + 4 * lane4;
   floatx4 y[kBatch];
   const auto fetch = [&](int i0) {
@@ -620,8 +633,8 @@ int compute_units() {
 
 // How a call's work is laid out, from its sizes alone.
 struct Plan {
-  int dt, lists, group, tiles, part_heads;
-  int64_t streams, waves;
+  int dt, lists, group, head_tiles, side, part_heads;
+  int64_t streams, work_groups;
   int group_waves;  // of a group's work-group; 0: the waves share all streams
   bool joins;
   int64_t ends_bytes, bytes;
@@ -632,9 +645,10 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
   a.dt = pages.dim <= 64 ? 64 : pages.dim <= 128 ? 128 : 256;
   a.lists = (int)(lists ? lists : pages.heads);
   a.group = (int)(q_heads / a.lists);
-  a.tiles = (a.group + kHeads - 1) / kHeads;
+  a.head_tiles = (a.group + kHeads - 1) / kHeads;
+  a.side = std::min(a.head_tiles, side_of(a.dt));
   a.part_heads = std::min(a.group, kHeads);
-  a.streams = (int64_t)a.lists * a.tiles;
+  a.streams = (int64_t)a.lists * a.head_tiles;
   // a window's first group of 8 rows may start 7 tokens early
   const int64_t tiles = std::max<int64_t>(1, (max_tokens + (lists ? 0 : 7) + kTile - 1) / kTile);
   if (tiles + kStart > 0x7FFFFFFF / std::max<int64_t>(1, batch * a.streams)) throw std::invalid_argument("batch x heads x tokens is too large");
@@ -654,20 +668,21 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
   const bool grouped = all > 0 && tiles <= most * each;
   a.group_waves = grouped ? (int)std::clamp<int64_t>(resident / all, 1, std::min<int64_t>(most, tiles)) : 0;
   if (a.group_waves) {
-    a.joins = false, a.waves = 0, a.ends_bytes = 0, a.bytes = 0;
+    a.joins = false, a.work_groups = 0, a.ends_bytes = 0, a.bytes = 0;
     return a;
   }
   // Fewer waves where there is little for each, by what was measured of small
   // calls in us: a tile more costs a wave 1.2, a part more the join of its
   // stream 0.02, a wave more the call 0.003. One sequence of 16,000 tokens 24.9
   // -> 19.6 (2048 waves before), 131,072 under one key head 58.9 -> 22.8.
-  const double units = (double)all * (tiles + kStart);
-  const double wave_cost = (0.02 / all + 0.003) * std::max(1.0, a.part_heads / 8.0);
-  const int64_t worth = std::max<int64_t>(1, (int64_t)std::sqrt(1.2 * units / wave_cost));
-  a.waves = std::min({(int64_t)units, resident, worth});
+  const int64_t shared = batch * a.lists * ((a.head_tiles + a.side - 1) / a.side);
+  const double units = (double)shared * (tiles + kStart);
+  const double cost = (0.02 / shared + 0.003 * a.side) * std::max(1.0, a.part_heads / 8.0);
+  const int64_t worth = std::max<int64_t>(1, (int64_t)std::sqrt(1.2 * units / cost));
+  a.work_groups = std::min({(int64_t)units, resident / a.side, worth});
   a.joins = tiles > 1;
   a.ends_bytes = (batch * a.streams * 8 + 15) / 16 * 16;
-  a.bytes = a.ends_bytes + a.waves * 2 * a.part_heads * (a.dt + 2) * 4;
+  a.bytes = a.ends_bytes + a.work_groups * 2 * a.side * a.part_heads * (a.dt + 2) * 4;
   return a;
 }
 
@@ -682,13 +697,14 @@ void launch(const Params& p, const Plan& plan, bool listed, hipStream_t s) {
     hip_check(hipGetLastError(), "attention");
     return;
   }
-  auto kernel = listed ? (full ? attend_kernel<T, F8, DT, true, true> : attend_kernel<T, F8, DT, true, false>)
-                       : (full ? attend_kernel<T, F8, DT, false, true> : attend_kernel<T, F8, DT, false, false>);
-  kernel<<<(unsigned)plan.waves, 64, 0, s>>>(p);
+  const bool alone = full && plan.side == 1;
+  auto kernel = listed ? (alone ? attend_kernel<T, F8, DT, true, true> : attend_kernel<T, F8, DT, true, false>)
+                       : (alone ? attend_kernel<T, F8, DT, false, true> : attend_kernel<T, F8, DT, false, false>);
+  kernel<<<(unsigned)plan.work_groups, 64 * plan.side, plan.side * kStage * 8, s>>>(p);
   hip_check(hipGetLastError(), "attention");
   if (plan.joins) {
     const int64_t all = p.batch * plan.streams;
-    if (plan.waves > 32 * all)
+    if (plan.work_groups > 32 * all)
       join_kernel<T, DT, 32><<<dim3((unsigned)all, (unsigned)plan.part_heads, DT / 32), kJoin, 0, s>>>(p);
     else
       join_kernel<T, DT, DT><<<dim3((unsigned)all, (unsigned)plan.part_heads), kJoin, 0, s>>>(p);
@@ -728,7 +744,7 @@ void attend(const AttendArgs& a, const KvPages& pages, hipStream_t s) {
   p.ends = (int2*)a.workspace, p.parts = (float*)((char*)a.workspace + plan.ends_bytes);
   p.scale = a.scale * 1.4426950408889634f;
   p.batch = (int)a.batch, p.heads = pages.heads, p.q_heads = a.q.heads;
-  p.lists = plan.lists, p.group = plan.group, p.tiles = plan.tiles, p.count = pages.pages ? a.count : 0;
+  p.lists = plan.lists, p.group = plan.group, p.head_tiles = plan.head_tiles, p.side = plan.side, p.count = pages.pages ? a.count : 0;
   p.page_shift = pages.page_shift, p.pages = pages.pages, p.dim = pages.dim;
   p.first = (int)a.first, p.last = (int)std::min<int64_t>(a.last, 0x7FFFFF00), p.part_heads = plan.part_heads;
   if (pages.type == kE4M3) {

@@ -689,6 +689,24 @@ def test_empty_calls(jasper):
     assert (out == 0).all()
 
 
+@pytest.mark.parametrize("hq,heads,dim,dtype,cache", [
+    (130, 1, 128, F16, F16), (64, 2, 64, BF16, F8), (130, 1, 256, BF16, BF16), (66, 2, 96, F16, F16), (33, 1, 16, F16, F8)])
+def test_many_heads_to_a_key_head(jasper, hq, heads, dim, dtype, cache):
+    lens = [3000, 0, 1, 900, 4100]
+    kp, vp, tables, keys, values = build_cache(lens, heads, 16, dim, cache, 190)
+    ks, vs = f8_scales(heads, cache, 191)
+    q = randn((len(lens), hq, dim), dtype, 192, 2.0)
+    tens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ref = ref_attention(q, keys, values, dim ** -0.5, lambda i, j: torch.arange(lens[i]), dtype, ks, vs)
+    check(jasper.decode_attention(q, kp, vp, tables, tens, k_scale=ks, v_scale=vs, return_lse=True), ref)
+    ids = torch.arange(3500, dtype=torch.int32, device="cuda").flip(0).expand(len(lens), heads, 3500).contiguous()
+    ref = ref_attention(q, keys, values, dim ** -0.5,
+                        lambda i, j: torch.tensor([t for t in range(lens[i]) if t < 3500 or t >= lens[i] - 7], dtype=torch.int64),
+                        dtype, ks, vs)
+    check(jasper.retrieved_attention(q, kp, vp, tables, tens, ids, first=1, last=7, k_scale=ks, v_scale=vs,
+                                     return_lse=True), ref)
+
+
 SHORT = [0, 1, 5, 8, 17, 31, 32, 33, 64, 100, 129, 255, 300, 500]
 
 
