@@ -64,16 +64,17 @@ def main(argv=None):
     ap.add_argument("--k", type=int, default=100, help="tokens retrieved per query head")
     ap.add_argument("--first", type=int, default=4)
     ap.add_argument("--last", type=int, default=64)
-    ap.add_argument("--topics", type=int, default=512)
+    ap.add_argument("--topics", type=int, default=0, help="0: one per 64 tokens")
     ap.add_argument("--exact", action="store_true", help="search by brute force, not through a graph")
     ap.add_argument("--quiet", action="store_true")
     a = ap.parse_args(argv)
     g = torch.Generator(device="cuda").manual_seed(1)
     rand = lambda *shape: torch.randn(shape, device="cuda", generator=g)  # noqa: E731
-    topics = rand(a.topics, a.dim)
+    n_topics = a.topics or max(1, a.tokens // 64)
+    topics = 1.8 * rand(n_topics, a.dim)
 
     def tokens(n, noise):  # keys of n tokens: a topic each, and the rest of the layer's projections
-        topic = torch.randint(0, a.topics, (n, a.kv_heads), device="cuda", generator=g)
+        topic = torch.randint(0, n_topics, (n, a.kv_heads), device="cuda", generator=g)
         k = (topics[topic] + noise * rand(n, a.kv_heads, a.dim)).half()
         q = topics[topic.repeat_interleave(a.q_heads // a.kv_heads, dim=1)] + noise * rand(n, a.q_heads, a.dim)
         return q.half(), k, rand(n, a.kv_heads, a.dim).half()

@@ -171,19 +171,6 @@ __device__ int find_sequence(const Params& p, int streams, Share& share, int& be
   return __builtin_amdgcn_readlane(b, src);
 }
 
-// S = K Q^T and O^T = V^T P^T on 16x16x32 instructions, all in registers. With
-// g = lane / 16, i = lane % 16 and 8 tokens to a group, a tile of 32 tokens is
-//  K  two operands' rows i: token 8 (i / 4) + i % 4 (+ 4 in the second); so
-//  S  comes out with lane (g, i) holding head i's scores of group g's eight
-//     tokens, which is where P has to be as the operand of the second product:
-//     nothing crosses lanes.
-//  V  lane (g, i) loads VD dims of group g's eight tokens, in blocks of up to
-//     16 bytes of which 16 lanes read a contiguous run: dims BD i on, and 16
-//     BD further in each next block. The 8 x VD values are turned with byte
-//     permutes into VD operands, product j giving the j-th dims of all lanes.
-//  O  lane (g, i): head i, of dims that lane 4 g + r loads the j-th in o[j][r].
-// Heads past the group's are zero queries: the loads bound the kernel, not
-// the products (32 instructions of 16 cycles per 16 KB of a wave).
 // A stream: the tokens of one sequence under up to 16 query heads of a list.
 struct Stream {
   int b, list, heads, q_head, kv_head;
@@ -217,6 +204,21 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 // One wave over tiles [c, c1) of a stream; rows: STAGE offsets in LDS.
+//
+// S = K Q^T and O^T = V^T P^T on 16x16x32 instructions, all in registers. With
+// g = lane / 16, i = lane % 16 and 8 tokens to a group, a tile of 32 tokens is
+//  K  two operands' rows i: token 8 (i / 4) + i % 4 (+ 4 in the second); so
+//  S  comes out with lane (g, i) holding head i's scores of group g's eight
+//     tokens, which is where P has to be as the operand of the second product:
+//     nothing crosses lanes.
+//  V  lane (g, i) loads VD dims of group g's eight tokens, in blocks of up to
+//     16 bytes of which 16 lanes read a contiguous run: dims BD i on, and 16
+//     BD further in each next block. The 8 x VD values are turned with byte
+//     permutes into VD operands, product j giving the j-th dims of all lanes.
+//  O  lane (g, i): head i, of dims that lane 4 g + r loads the j-th in o[j][r].
+// Heads past the group's are zero queries: the loads bound the kernel, not the
+// products (of fp16 rows of 128 values 24 instructions of 16 cycles for the 16
+// KB of a tile; weights of one term would spare 8 of them, and 1 us of 71).
 template <typename T, bool F8, int DT, bool LISTED, bool FULL, int STAGE>
 __device__ __forceinline__ Sums<DT> attend_tiles(const Params& p, const Span& sp, const Stream& at, int c, int c1,
                                                  int64_t* rows) {
@@ -548,8 +550,7 @@ __global__ __launch_bounds__(64 * group_waves(DT)) void attend_group_kernel(Para
 }
 
 // Joins the parts of a stream that several waves had: a work-group per
-// sequence, stream and head, and for streams of many parts per DIMS dims of
-// it. The parts' weights go to LDS, then a thread has four dims of every
+// sequence, stream, head and DIMS dims. The parts' weights go to LDS, then a thread has four dims of every
 // kRows-th part, eight loads in flight.
 template <typename T, int DT, int DIMS>
 __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
@@ -704,7 +705,10 @@ void launch(const Params& p, const Plan& plan, bool listed, hipStream_t s) {
   hip_check(hipGetLastError(), "attention");
   if (plan.joins) {
     const int64_t all = p.batch * plan.streams;
-    if (plan.work_groups > 32 * all)
+    // Few streams: more work-groups with 32 dims each (131,072 tokens under one
+    // key head 22.8 us, 27.7 without; of 32 streams under 8 heads, where there
+    // are work-groups enough, 189 and 176).
+    if (4 * all * plan.part_heads <= compute_units())
       join_kernel<T, DT, 32><<<dim3((unsigned)all, (unsigned)plan.part_heads, DT / 32), kJoin, 0, s>>>(p);
     else
       join_kernel<T, DT, DT><<<dim3((unsigned)all, (unsigned)plan.part_heads), kJoin, 0, s>>>(p);

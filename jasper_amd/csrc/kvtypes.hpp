@@ -1,5 +1,5 @@
-// kvtypes.hpp -- the value types of the cache's kernels: fp16, bf16 and OCP
-// e4m3, widened to fp32 and rounded from it (to nearest even).
+// kvtypes.hpp -- the value types of the cache's kernels: fp16 and bf16, widened
+// to fp32 and rounded from it (to nearest even), and OCP e4m3, rounded to.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -26,23 +26,8 @@ struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Pack {
 
 template <typename T, int N>
 __device__ __forceinline__ void widen(const Pack<T, N>& p, float* out) {
-  if constexpr (sizeof(T) == 1) {
-    static_assert(N % 4 == 0 || N == 1, "bytes come in words");
-    if constexpr (N == 1) {
-      out[0] = __builtin_amdgcn_cvt_f32_fp8((int)p.v[0].bits, 0);
-    } else {
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
 #pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
-        const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
-        const floatx2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-        out[4 * i] = a.x, out[4 * i + 1] = a.y, out[4 * i + 2] = b.x, out[4 * i + 3] = b.y;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = (float)p.v[i];
-  }
+  for (int i = 0; i < N; ++i) out[i] = (float)p.v[i];
 }
 
 // A stored e4m3 value saturates at +-448 (the type has no infinity); NaN stays.

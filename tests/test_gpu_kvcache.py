@@ -725,3 +725,54 @@ def test_decode_short(jasper, hq, heads, dim, page, dtype, cache, repeat):
     ref = ref_attention(q, keys, values, dim ** -0.5, lambda i, j: torch.arange(lens[i]), dtype, ks, vs)
     tens = torch.tensor(lens, dtype=torch.int32, device="cuda")
     check(jasper.decode_attention(q, kp, vp, tables, tens, k_scale=ks, v_scale=vs, return_lse=True), ref)
+
+
+def test_rotary_gradient_of_broadcast_rows(jasper):
+    """One key head seen by four: their gradients add up in it."""
+    n, dim = 9, 32
+    cos, sin = jasper.rotary_table(64, dim)
+    pos = torch.arange(n, device="cuda") * 5
+    q = randn((n, 4, dim), BF16, 200)
+    one = randn((n, 1, dim), BF16, 201).requires_grad_()
+    g = randn((n, 4, dim), BF16, 202)
+    _, k = jasper.rotary(q, one.expand(n, 4, dim), pos, cos, sin)
+    want, _ = ref_rotary(one.detach().expand(n, 4, dim), pos, cos, sin, False)
+    near(k.detach(), want, rotary_tol(want, want.abs() * 2, BF16))
+    got, = torch.autograd.grad(k, one, g)
+    each, size = ref_rotary(g, pos, cos, sin, False, back=True)
+    # four rounded gradients, added with three roundings
+    tol = rotary_tol(each, size, BF16).sum(1, keepdim=True) + 3 * UNIT[BF16] * each.abs().sum(1, keepdim=True)
+    near(got, each.sum(1, keepdim=True), tol)
+    flat = randn((1, 4, dim), BF16, 203).requires_grad_()  # one row for all positions
+    out, _ = jasper.rotary(flat.expand(n, 4, dim), None, pos, cos, sin)
+    got, = torch.autograd.grad(out, flat, g)
+    tol = rotary_tol(each, size, BF16).sum(0, keepdim=True) + n * UNIT[BF16] * each.abs().sum(0, keepdim=True)
+    near(got, each.sum(0, keepdim=True), tol)
+
+
+@pytest.mark.parametrize("scale", [-0.4, 0.0, 1e-6])
+def test_decode_scales(jasper, scale):
+    lens = [1500, 70, 1]
+    kp, vp, tables, keys, values = build_cache(lens, 2, 16, 128, BF16, 210)
+    q = randn((3, 6, 128), BF16, 211, 2.0)
+    ref = ref_attention(q, keys, values, scale, lambda i, j: torch.arange(lens[i]), BF16)
+    tens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    check(jasper.decode_attention(q, kp, vp, tables, tens, scale=scale, return_lse=True), ref)
+
+
+def test_flat_softmax_over_many_tokens_keeps_its_tail(jasper):
+    """One token far above 100,000 equal ones whose weights are 2^-26 of its: together 0.15% of the sum."""
+    n = 100_001
+    kp, vp, tables, keys, values = build_cache([n], 1, 16, 64, F16, 220)
+    kp.zero_()
+    keys[0].zero_()
+    page = tables[0, 5000 // 16].item()
+    kp[page, 0, 5000 % 16, 0] = 26 * math.log(2.0)
+    keys[0][0, 5000, 0] = kp[page, 0, 5000 % 16, 0].double().cpu()
+    q = torch.zeros((1, 1, 64), dtype=F16, device="cuda")
+    q[0, 0, 0] = 1.0
+    vp.copy_(vp.abs() + 1.0)
+    values[0].copy_(vp.float()[tables[0, :-(-n // 16)].long()].transpose(0, 1).reshape(1, -1, 64)[:, :n].double().cpu())
+    ref = ref_attention(q, keys, values, 1.0, lambda i, j: torch.arange(n), F16)
+    tens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    check(jasper.decode_attention(q, kp, vp, tables, tens, scale=1.0, return_lse=True), ref)
