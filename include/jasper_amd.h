@@ -416,7 +416,7 @@ int64_t jasperx_retrieved_attention(const jasperx_head_rows* q, int32_t type, in
                                     int64_t count, int64_t first, int64_t last, double scale, void* out, float* lse,
                                     void* workspace, int64_t workspace_bytes, void* stream);
 /* Scratch bytes of the two calls above for their sizes (pages: sizes and type
- * only). max_tokens: the tokens one head reads at most, min(max_len, window)
+ * only); 0: none is needed, and workspace may be NULL. max_tokens: the tokens one head reads at most, min(max_len, window)
  * or first + last + count; lists 0: decode_attention. */
 int64_t jasperx_attention_workspace(int64_t batch, int64_t q_heads, const jasperx_kv_pages* pages,
                                     int64_t max_tokens, int64_t lists);

@@ -776,3 +776,26 @@ def test_flat_softmax_over_many_tokens_keeps_its_tail(jasper):
     ref = ref_attention(q, keys, values, 1.0, lambda i, j: torch.arange(n), F16)
     tens = torch.tensor([n], dtype=torch.int32, device="cuda")
     check(jasper.decode_attention(q, kp, vp, tables, tens, scale=1.0, return_lse=True), ref)
+
+
+@pytest.mark.parametrize("batch,window", [(65, 0), (130, 0), (700, 0), (700, 50), (2000, 0)])
+def test_many_unlike_sequences(jasper, batch, window):
+    """Tables wide enough that the waves share out all sequences' tokens among them: runs of short sequences, of
+    empty ones, and long ones between."""
+    g = torch.Generator().manual_seed(230)
+    lens = torch.randint(0, 90, (batch,), generator=g)
+    lens[torch.rand(batch, generator=g) < 0.2] = 0
+    lens[batch // 3], lens[-1], lens[batch // 2:batch // 2 + 20] = 9000, 4321, 0
+    lens = lens.tolist()
+    kp, vp, tables, keys, values = build_cache(lens, 2, 16, 64, F16, 231)
+    q = randn((batch, 4, 64), F16, 232, 2.0)
+    tens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ref = ref_attention(q, keys, values, 0.125, lambda i, j: torch.arange(max(0, lens[i] - window) if window else 0, lens[i]),
+                        F16)
+    check(jasper.decode_attention(q, kp, vp, tables, tens, window=window, return_lse=True), ref)
+    ids = torch.arange(7000, dtype=torch.int32, device="cuda").expand(3, 2, 7000).contiguous()
+    few = torch.tensor([0, batch // 3, batch - 1], device="cuda")
+    rows = few.tolist()
+    ref = ref_attention(q[few], [keys[i] for i in rows], [values[i] for i in rows], 0.125,
+                        lambda i, j: torch.arange(min(7000, lens[rows[i]])), F16)
+    check(jasper.retrieved_attention(q[few], kp, vp, tables[few], tens[few], ids, return_lse=True), ref)
