@@ -799,3 +799,16 @@ def test_many_unlike_sequences(jasper, batch, window):
     ref = ref_attention(q[few], [keys[i] for i in rows], [values[i] for i in rows], 0.125,
                         lambda i, j: torch.arange(min(7000, lens[rows[i]])), F16)
     check(jasper.retrieved_attention(q[few], kp, vp, tables[few], tens[few], ids, return_lse=True), ref)
+
+
+def test_copy_pages_in_several_launches(jasper):
+    """More than 32 GB are copied in several launches (here of pages that are all the same memory), and the table
+    entries of every part are rewritten."""
+    kp, vp = (randn((1, 64, 256, 256), F16, 240 + i).expand(5000, -1, -1, -1) for i in range(2))
+    before = kp[0].clone(), vp[0].clone()
+    src = torch.arange(2100, dtype=torch.int32, device="cuda")
+    tables = torch.arange(5000, dtype=torch.int32, device="cuda").flip(0).contiguous()
+    jasper.copy_pages(kp, vp, src, src + 2500, tables=tables)
+    want = torch.arange(5000, device="cuda").flip(0)
+    assert torch.equal(tables.long(), torch.where(want < 2100, want + 2500, want))
+    assert torch.equal(kp[0], before[0]) and torch.equal(vp[0], before[1])
