@@ -660,8 +660,9 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
   const int64_t tiles = std::max<int64_t>(1, (max_tokens + (lists ? 0 : 7) + kTile - 1) / kTile);
   if (tiles + kStart > 0x7FFFFFFF / std::max<int64_t>(1, batch * a.streams)) throw std::invalid_argument("batch x heads x tokens is too large");
   const int64_t resident = std::min(kWaves, compute_units() * (a.dt == 256 ? 4 : 8));
-  // A group spares the second kernel, but a wave of it waits 1.4 us for each
-  // tile while most of the GPU idles where there are few streams. Of 8 key
+  // A group spares the second kernel, but its compute unit reads a tile of each
+  // wave in 1.4 us (90 GB/s) while most of the GPU idles where there are few
+  // streams. Of 8 key
   // heads of 128 fp16 values, group against shared, us: one sequence of 100
   // tokens 5.2 / 8.4, 300 7.9 / 8.5, 700 10.8 / 8.9; four of 500 9.2 / 10.1, of
   // 1000 17.1 / 12.5; 16 of 1000 20.4 / 21.5; 64 of 1000 45.7 / 54.4; 512 of 128
