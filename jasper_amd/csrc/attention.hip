@@ -82,8 +82,12 @@ __device__ __forceinline__ floatx2 unpack2(uint32_t w) {
 // Two of a word's four e4m3 bytes as two values of T (exact in both types).
 template <typename T>
 __device__ __forceinline__ uint32_t from_e4m3(uint32_t w, bool high) {
-  const floatx2 a = high ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
-  return pack2<T>(a.x, a.y);
+  if constexpr (std::is_same_v<T, f16>)
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true)
+                                             : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+  else
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true)
+                                             : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
 }
 
 // Rows are read once, past the caches (four sequences of 131k tokens: 175 us,

@@ -169,6 +169,9 @@ def test_rotary_table_scalings():
 def test_library_is_required_to_be_on_the_gpu():
     """Every operator refuses CPU tensors: there is no CPU form of them."""
     import jasper_amd
+    from jasper_amd import build_lib
+    if not build_lib.BINDING.exists():
+        build_lib.build(verbose=False)
     x = torch.zeros((2, 2, 64), dtype=torch.float16)
     pages = torch.zeros((2, 2, 16, 64), dtype=torch.float16)
     i32, i64 = torch.zeros((2, 1), dtype=torch.int32), torch.zeros(2, dtype=torch.int64)
