@@ -86,7 +86,8 @@ def rotary_table(n_positions: int, rot_dim: int, base: float = 10000.0, scaling:
             return rot_dim * math.log(original / (2 * math.pi * turns)) / (2 * math.log(base))
 
         low = max(0, math.floor(at(beta_fast)))
-        high = min(rot_dim // 2 - 1, math.ceil(at(beta_slow)))
+        # past the last pair where even that turns more often: the blend then ends there, undivided
+        high = min(rot_dim - 1, math.ceil(at(beta_slow)))
         ramp = ((pair / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)
         freq = freq / factor * ramp + freq * (1 - ramp)
         size = 0.1 * math.log(factor) + 1.0

@@ -183,3 +183,28 @@ def test_library_is_required_to_be_on_the_gpu():
               lambda: jasper_amd.retrieved_attention(x, pages, pages, i32, i32[:, 0], i32[:, :, None])):
         with pytest.raises(ValueError, match="CUDA tensor"):
             f()
+
+
+@pytest.mark.parametrize("rot,base,original,factor", [
+    (64, 10000.0, 131072, 4.0), (128, 10000.0, 131072, 4.0), (16, 10000.0, 32768, 4.0), (64, 10000.0, 2048, 16.0),
+    (128, 500000.0, 8192, 8.0), (96, 10000.0, 10 ** 7, 2.0)])
+def test_yarn_blends_between_its_two_bounds(rot, base, original, factor):
+    """Every pair's frequency against the formula. The blend ends at the pair that turns beta_slow times within the
+    original context, also where that is past the last pair: then no pair is divided outright."""
+    cos, sin = rotary_table(2, rot, base=base, scaling="yarn", factor=factor, original=original, device="cpu")
+    size = 1 + 0.1 * math.log(factor)
+
+    def place(turns):  # where original * base^(-2i / rot) = 2 pi turns
+        return rot / 2 * math.log(original / (2 * math.pi * turns), base)
+
+    low, high = max(math.floor(place(32)), 0), min(math.ceil(place(1)), rot - 1)
+    for i in range(rot // 2):
+        plain = base ** (-2 * i / rot)
+        divided = 0.0 if i <= low else 1.0 if i >= high else (i - low) / (high - low)
+        want = plain * (1 - divided) + plain / factor * divided
+        # sine and cosine of position 1 are rounded to 32 bits, 2^-24 of each: twice that in the angle's tangent
+        got = math.atan2(sin[1, i].item(), cos[1, i].item())
+        assert abs(got - want) <= 2.0 ** -22 * want, i
+        assert abs(math.hypot(sin[1, i].item(), cos[1, i].item()) - size) <= 2.0 ** -23 * size
+        if original * plain / (2 * math.pi) > 1:
+            assert got > plain / factor * (1 + 2.0 ** -20), i
