@@ -417,7 +417,7 @@ int64_t jasperx_retrieved_attention(const jasperx_head_rows* q, int32_t type, in
                                     void* workspace, int64_t workspace_bytes, void* stream);
 /* Scratch bytes of the two calls above for their sizes (pages: sizes and type
  * only); 0: none is needed, and workspace may be NULL. max_tokens: the tokens one head reads at most, min(max_len, window)
- * or first + last + count; lists 0: decode_attention. */
+ * or first + last + count; lists 0: decode_attention, else as in the call. */
 int64_t jasperx_attention_workspace(int64_t batch, int64_t q_heads, const jasperx_kv_pages* pages,
                                     int64_t max_tokens, int64_t lists);
 /* Library build identifier (git-independent), for load checks. */

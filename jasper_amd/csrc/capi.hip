@@ -1041,8 +1041,9 @@ extern "C" int64_t jasperx_attention_workspace(int64_t batch, int64_t q_heads, c
     jasperx_kv_pages sizes = pages ? *pages : jasperx_kv_pages{};
     sizes.k = sizes.v = nullptr, sizes.pages = 0;
     const KvPages p = kv_pages(&sizes);
-    if (batch < 0 || batch > 65535 || q_heads < 1 || q_heads % p.heads || max_tokens < 0 || lists < 0)
+    if (batch < 0 || batch > 65535 || q_heads < 1 || q_heads > 65535 || q_heads % p.heads || max_tokens < 0 || lists < 0)
       throw std::invalid_argument("bad sizes");
+    if (lists && lists != q_heads && lists != p.heads) throw std::invalid_argument("lists must be 0, the query heads or the cache's heads");
     return attend_workspace(batch, q_heads, p, max_tokens, lists);
   });
 }
