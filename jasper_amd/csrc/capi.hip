@@ -1025,8 +1025,9 @@ extern "C" int64_t jasperx_retrieved_attention(const jasperx_head_rows* q, int32
     AttendArgs a = attend_args(q, type, batch, p, tables, table_stride, table_width, lens, scale, out, lse, workspace,
                                workspace_bytes);
     if (lists != a.q.heads && lists != p.heads) throw std::invalid_argument("lists must be the query heads or the cache's heads");
-    if (count < 0 || first < 0 || last < 0 || first + last + count > 0x3FFFFFFF)
-      throw std::invalid_argument("first, last and count must be at least 0, at most 2^30 in sum");
+    const int64_t most = 0x3FFFFFFF;
+    if (std::min({count, first, last}) < 0 || std::max({count, first, last}) > most || first + last + count > most)
+      throw std::invalid_argument("first, last and count must be at least 0, below 2^30 in sum");
     if (batch && count && !ids) throw std::invalid_argument("null ids");
     a.max_len = (int64_t)1 << 31;
     a.ids = ids, a.lists = (int32_t)lists, a.count = (int32_t)count, a.first = first, a.last = last;

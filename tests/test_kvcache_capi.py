@@ -53,3 +53,21 @@ def test_workspace_refuses_lists_of_no_kind(lib, lists):
 def test_workspace_refuses_query_heads_that_the_calls_refuse(lib, q_heads):
     assert lib.jasperx_attention_workspace(4, q_heads, ctypes.byref(pages()), 1000, 8 if q_heads == 2 ** 35 else 0) < 0
     assert b"bad sizes" in lib.jasper_last_error()
+
+
+BIG = 2 ** 63 - 1
+
+
+@pytest.mark.parametrize("count,first,last", [
+    (0, BIG, BIG), (2, BIG, BIG), (2 ** 31, BIG, 2 ** 63 - 2 ** 31), (BIG, 1, 0), (0, 2 ** 30, 0), (5, 0, 2 ** 62), (-1, 4, 4),
+    (4, -1, 4), (4, 4, -1)])
+def test_retrieved_refuses_sums_past_64_bits(lib, count, first, last):
+    """The three numbers' sum counts a list's tokens; past 64 bits it wraps to a small one. (The addresses are never
+    read: the call ends before.)"""
+    somewhere = 4096
+    p = pages()
+    p.k = p.v = somewhere
+    q = Rows(somewhere, 32 * 128, 128, 32)
+    r = lib.jasperx_retrieved_attention(ctypes.byref(q), 0, 4, ctypes.byref(p), somewhere, 8, 8, somewhere, somewhere, 8,
+                                        count, first, last, 1.0, somewhere, None, None, 0, None)
+    assert r < 0 and b"first, last and count must be" in lib.jasper_last_error()
