@@ -661,7 +661,7 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
   a.part_heads = std::min(a.group, kHeads);
   a.streams = (int64_t)a.lists * a.head_tiles;
   // a window's first group of 8 rows may start 7 tokens early
-  const int64_t tiles = std::max<int64_t>(1, (max_tokens + (lists ? 0 : 7) + kTile - 1) / kTile);
+  const int64_t tiles = std::max<int64_t>(1, max_tokens / kTile + (max_tokens % kTile + (lists ? 0 : 7) + kTile - 1) / kTile);
   if (tiles + kStart > 0x7FFFFFFF / std::max<int64_t>(1, batch * a.streams)) throw std::invalid_argument("batch x heads x tokens is too large");
   const int64_t resident = std::min(kWaves, compute_units() * (a.dt == 256 ? 4 : 8));
   // A group spares the second kernel, but its compute unit reads a tile of each

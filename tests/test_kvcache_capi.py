@@ -71,3 +71,9 @@ def test_retrieved_refuses_sums_past_64_bits(lib, count, first, last):
     r = lib.jasperx_retrieved_attention(ctypes.byref(q), 0, 4, ctypes.byref(p), somewhere, 8, 8, somewhere, somewhere, 8,
                                         count, first, last, 1.0, somewhere, None, None, 0, None)
     assert r < 0 and b"first, last and count must be" in lib.jasper_last_error()
+
+
+@pytest.mark.parametrize("tokens", [BIG, BIG - 6, BIG - 38, 2 ** 62])
+def test_workspace_of_more_tokens_than_64_bits_round_up(lib, tokens):
+    assert lib.jasperx_attention_workspace(4, 32, ctypes.byref(pages()), tokens, 0) < 0
+    assert b"too large" in lib.jasper_last_error()
