@@ -25,6 +25,9 @@ constexpr int kGroupStage = 256;        // row offsets of a wave of a group, in 
 constexpr int kGroupLds = 64 << 10;     // bytes at most
 // waves of a group at most: what a compute unit has registers for
 constexpr int group_waves(int dt) { return dt == 64 ? 16 : dt == 128 ? 8 : 4; }
+// A wave's sums in the workspace: dt floats and two for each of its heads, and
+// what keeps the next one's on 16 bytes.
+__host__ __device__ constexpr int part_size(int heads, int dt) { return (heads * (dt + 2) + 3) / 4 * 4; }
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -500,7 +503,7 @@ __global__ __launch_bounds__(64 * (FULL ? 1 : side_of(DT)), DT == 256 ? 1 : 2) v
       }
       if (g == 0 && p.lse) p.lse[row] = s.sum == 0.f ? -__builtin_inff() : (s.ref + __builtin_amdgcn_logf(s.sum)) * kLn2;
     } else {
-      float* part = p.parts + (((int64_t)blockIdx.x * 2 + (c == 0 ? 1 : 0)) * p.side + wave) * p.part_heads * (DT + 2);
+      float* part = p.parts + (((int64_t)blockIdx.x * 2 + (c == 0 ? 1 : 0)) * p.side + wave) * part_size(p.part_heads, DT);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -575,7 +578,7 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Params p) {
   __shared__ float tops[kJoin / 64], tots[kJoin / 64];
   __shared__ floatx4 sums[kRows][kLanes];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int size = p.part_heads * (DT + 2), stats = p.part_heads * DT + 2 * n;
+  const int size = part_size(p.part_heads, DT), stats = p.part_heads * DT + 2 * n;
   // the part that begins the stream, and what part i > 0 is i steps from
   const float* const own = p.parts + (((int64_t)range.x * 2 + 1) * p.side + head_tile % p.side) * size;
   const float* const rest = own - p.side * size;
@@ -694,7 +697,7 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
   a.work_groups = std::min({(int64_t)units, resident / a.side, worth});
   a.joins = tiles > 1;
   a.ends_bytes = (batch * a.streams * 8 + 15) / 16 * 16;
-  a.bytes = a.ends_bytes + a.work_groups * 2 * a.side * a.part_heads * (a.dt + 2) * 4;
+  a.bytes = a.ends_bytes + a.work_groups * 2 * a.side * part_size(a.part_heads, a.dt) * 4;
   return a;
 }
 

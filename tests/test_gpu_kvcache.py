@@ -812,3 +812,28 @@ def test_copy_pages_in_several_launches(jasper):
     want = torch.arange(5000, device="cuda").flip(0)
     assert torch.equal(tables.long(), torch.where(want < 2100, want + 2500, want))
     assert torch.equal(kp[0], before[0]) and torch.equal(vp[0], before[1])
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 8, 15, 16])
+@pytest.mark.parametrize("heads", [1, 8])
+def test_parts_of_a_stream_start_on_16_bytes(jasper, group, heads):
+    """What a wave leaves for the join is written and read 16 bytes at a time. The workspace is a list of ends, whole
+    16s, then two parts to a work-group. As many work-groups are taken for 64 values as for 128, so the difference
+    tells their number: 64 values more per query head and part."""
+    import ctypes
+    from tests.test_kvcache_capi import I64, Pages
+    lib = ctypes.CDLL(str(jasper.library_path()))
+    fn = lib.jasperx_attention_workspace
+    fn.restype, fn.argtypes = I64, [I64, I64, ctypes.POINTER(Pages), I64, I64]
+    sizes = []
+    for dim in (64, 128):
+        p = Pages(layers=1, pages=4, heads=heads, page_size=16, dim=dim, type=0, row_stride=dim, head_stride=16 * dim,
+                  page_stride=heads * 16 * dim)
+        sizes.append(fn(1, heads * group, ctypes.byref(p), 100_000, 0))
+    ends = -(-heads * 8 // 16) * 16
+    work_groups, rest = divmod(sizes[1] - sizes[0], 2 * 64 * 4 * group)
+    assert rest == 0 and work_groups > 0
+    for dim, size in zip((64, 128), sizes):
+        values = group * (dim + 2)
+        part = -(-values // 4) * 16
+        assert size == ends + work_groups * 2 * part
