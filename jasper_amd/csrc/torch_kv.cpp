@@ -116,6 +116,14 @@ void check_alike(const char* name, const Tensor& t, const Tensor& like) {
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+bool wants_grad(const OptTensor& t) { return t && wants_grad(*t); }
+
+// What has no gradient is refused where one is asked for, rather than taken as a constant.
+template <typename... Ts>
+bool asks_grad(const Ts&... given) {
+  return at::GradMode::is_enabled() && (wants_grad(given) || ...);
+}
+
 // ---- rotary positions ----
 
 // q and k turned; either may be undefined. The arguments are checked.
@@ -193,6 +201,7 @@ py::tuple rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, c
   TORCH_CHECK_VALUE(at.sizes() == q.sizes().slice(0, q.dim() - 2), "positions must be ",
                     q.sizes().slice(0, q.dim() - 2), ", got ", at.sizes());
   TORCH_CHECK_VALUE(cos && sin, "cos and sin are needed");
+  TORCH_CHECK_VALUE(!asks_grad(cos, sin), "rotary has no gradient for cos and sin: detach them");
   TORCH_CHECK_VALUE(table_of(cos, sin, q).rot <= q.size(-1), "the tables rotate more values than a head has");
   const auto [q_out, k_out] = Rotary::turn(q, k ? *k : Tensor(), at, *cos, *sin, interleaved, false);
   return py::make_tuple(q_out, k ? py::cast(k_out) : py::none());

@@ -837,3 +837,15 @@ def test_parts_of_a_stream_start_on_16_bytes(jasper, group, heads):
         values = group * (dim + 2)
         part = -(-values // 4) * 16
         assert size == ends + work_groups * 2 * part
+
+
+def test_rotary_refuses_tables_that_require_a_gradient(jasper):
+    cos, sin = jasper.rotary_table(16, 64)
+    q = randn((3, 2, 64), F16, 250)
+    pos = torch.arange(3, device="cuda")
+    for c, s in ((cos.clone().requires_grad_(), sin), (cos, sin.clone().requires_grad_())):
+        for rows in (q, q.clone().requires_grad_()):
+            with pytest.raises(ValueError, match="no gradient for cos and sin"):
+                jasper.rotary(rows, None, pos, c, s)
+        with torch.no_grad():
+            assert torch.equal(jasper.rotary(q, None, pos, c, s)[0], jasper.rotary(q, None, pos, cos, sin)[0])
