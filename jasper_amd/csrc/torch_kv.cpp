@@ -221,7 +221,7 @@ OptTensor append_tokens(const OptTensor& q, const Tensor& k, const Tensor& v, co
   check_alike("v", v, k);
   TORCH_CHECK_VALUE(v.size(1) == pages.heads, "v must be [n, ", pages.heads, ", ", pages.dim, "]");
   if (q) check_alike("q", *q, k);
-  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(wants_grad(k) || wants_grad(v) || (q && wants_grad(*q))),
+  TORCH_CHECK_VALUE(!asks_grad(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale),
                     "append_tokens has no gradient: use rotary, or torch.no_grad()");
   const int64_t n = k.size(0);
   Tensor rows = indexes("slots", slots, k), at;
@@ -251,6 +251,7 @@ OptTensor append_tokens(const OptTensor& q, const Tensor& k, const Tensor& v, co
 void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& src, const Tensor& dst,
                 const OptTensor& tables) {
   const jasperx_kv_pages pages = pages_of(k_pages, v_pages, {}, {}, true);
+  TORCH_CHECK_VALUE(!asks_grad(k_pages, v_pages), "copy_pages has no gradient: use torch.no_grad()");
   for (const Tensor* t : {&src, &dst})
     TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->dim() == 1 && t->device() == k_pages.device() &&
                           t->is_contiguous(),

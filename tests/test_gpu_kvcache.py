@@ -849,3 +849,27 @@ def test_rotary_refuses_tables_that_require_a_gradient(jasper):
                 jasper.rotary(rows, None, pos, c, s)
         with torch.no_grad():
             assert torch.equal(jasper.rotary(q, None, pos, c, s)[0], jasper.rotary(q, None, pos, cos, sin)[0])
+
+
+def test_append_and_copy_refuse_what_requires_a_gradient(jasper):
+    """Rows, tables, pages and scales alike; without gradients they are what they always were."""
+    heads, page, dim = 2, 16, 64
+    given = dict(zip(("q", "k", "v"), (randn((3, h, dim), F16, 260 + h) for h in (4, heads, heads))))
+    given["cos"], given["sin"] = jasper.rotary_table(16, dim)
+    at = torch.arange(3, device="cuda")
+    pair = torch.tensor([0], dtype=torch.int32, device="cuda")
+    for cache in (F16, F8):
+        given["k_pages"], given["v_pages"] = make_pages(4, heads, page, dim, F16)
+        if cache == F8:
+            given |= {"k_scale": torch.ones(heads, device="cuda"), "v_scale": torch.ones(heads, device="cuda")}
+            given["k_pages"], given["v_pages"] = make_pages(4, heads, page, dim, F8)
+        want = jasper.append_tokens(positions=at, slots=at, **given)
+        for name in given:
+            asked = given | {name: given[name].detach().clone().requires_grad_()}
+            with pytest.raises(ValueError, match="append_tokens has no gradient"):
+                jasper.append_tokens(positions=at, slots=at, **asked)
+            if name.endswith("pages"):
+                with pytest.raises(ValueError, match="copy_pages has no gradient"):
+                    jasper.copy_pages(asked["k_pages"], asked["v_pages"], pair, pair + 1)
+            with torch.no_grad():
+                assert torch.equal(jasper.append_tokens(positions=at, slots=at, **asked), want), name
