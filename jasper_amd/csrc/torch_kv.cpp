@@ -287,7 +287,7 @@ struct Attention {
     TORCH_CHECK_VALUE(q.dim() == 3 && q.size(2) == pages.dim && q.size(1) > 0 && pages.heads > 0 &&
                           q.size(1) % pages.heads == 0 && q.device() == device,
                       "q must be [batch, a multiple of ", pages.heads, " heads, ", pages.dim, "] on ", device);
-    TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !q.requires_grad(),
+    TORCH_CHECK_VALUE(!asks_grad(q, k_pages, v_pages, k_scale, v_scale),
                       "attention over the cache has no gradient: use torch.no_grad()");
     batch = q.size(0);
     TORCH_CHECK_VALUE(tables.scalar_type() == at::kInt && tables.dim() == 2 && tables.size(0) == batch &&

@@ -873,3 +873,23 @@ def test_append_and_copy_refuse_what_requires_a_gradient(jasper):
                     jasper.copy_pages(asked["k_pages"], asked["v_pages"], pair, pair + 1)
             with torch.no_grad():
                 assert torch.equal(jasper.append_tokens(positions=at, slots=at, **asked), want), name
+
+
+def test_attention_refuses_what_requires_a_gradient(jasper):
+    tables = torch.tensor([[2, 1, 0], [3, 0, 0]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([40, 9], dtype=torch.int32, device="cuda")
+    ids = torch.arange(12, dtype=torch.int32, device="cuda").view(2, 2, 3)
+    for cache in (F16, F8):
+        given = {"q": randn((2, 4, 64), F16, 270)}
+        given["k_pages"], given["v_pages"] = make_pages(4, 2, 16, 64, cache, seed=271)
+        if cache == F8:
+            given |= {"k_scale": torch.full((2,), 0.03, device="cuda"), "v_scale": torch.full((2,), 0.03, device="cuda")}
+        for f in (lambda **x: jasper.decode_attention(tables=tables, lens=lens, **x),
+                  lambda **x: jasper.retrieved_attention(tables=tables, lens=lens, ids=ids, first=1, **x)):
+            want = f(**given)
+            for name in given:
+                asked = given | {name: given[name].detach().clone().requires_grad_()}
+                with pytest.raises(ValueError, match="has no gradient"):
+                    f(**asked)
+                with torch.no_grad():
+                    assert torch.equal(f(**asked), want), name
