@@ -118,6 +118,10 @@ bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 bool wants_grad(const OptTensor& t) { return t && wants_grad(*t); }
 
+// Forward mode: a tensor that carries a tangent (it need not require a gradient).
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
+
 // What has no gradient is refused where one is asked for, rather than taken as a constant.
 template <typename... Ts>
 bool asks_grad(const Ts&... given) {
@@ -180,9 +184,18 @@ struct Rotary : torch::autograd::Function<Rotary> {
     return out;
   }
 
-  // differentiable where something asks for it
+  // differentiable where something asks for it; the tangents are turned like the rows
   static std::pair<Tensor, Tensor> turn(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& cos,
                                         const Tensor& sin, bool interleaved, bool back) {
+    if (has_tangent(q) || has_tangent(k)) {
+      const auto value = [](const Tensor& t) { return t.defined() ? t._fw_primal(0) : t; };
+      const auto tangent = [](const Tensor& t) { return t.defined() ? t._fw_grad(0) : t; };
+      const auto out = turn(value(q), value(k), positions, cos, sin, interleaved, back);
+      const auto moved = turn(tangent(q), tangent(k), positions, cos, sin, interleaved, back);
+      if (moved.first.defined()) out.first._set_fw_grad(moved.first, 0, false);
+      if (moved.second.defined()) out.second._set_fw_grad(moved.second, 0, false);
+      return out;
+    }
     if (!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k)))
       return rotate(q, k, positions, cos, sin, interleaved, back);
     const auto given = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
@@ -201,7 +214,8 @@ py::tuple rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, c
   TORCH_CHECK_VALUE(at.sizes() == q.sizes().slice(0, q.dim() - 2), "positions must be ",
                     q.sizes().slice(0, q.dim() - 2), ", got ", at.sizes());
   TORCH_CHECK_VALUE(cos && sin, "cos and sin are needed");
-  TORCH_CHECK_VALUE(!asks_grad(cos, sin), "rotary has no gradient for cos and sin: detach them");
+  TORCH_CHECK_VALUE(!asks_grad(cos, sin) && !has_tangent(cos) && !has_tangent(sin),
+                    "rotary has no gradient for cos and sin: detach them");
   TORCH_CHECK_VALUE(table_of(cos, sin, q).rot <= q.size(-1), "the tables rotate more values than a head has");
   const auto [q_out, k_out] = Rotary::turn(q, k ? *k : Tensor(), at, *cos, *sin, interleaved, false);
   return py::make_tuple(q_out, k ? py::cast(k_out) : py::none());

@@ -101,9 +101,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos
     first 2 * cos.size(1) values of every head are turned in pairs by the
     angles in row positions[...] of the tables (`rotary_table`), the rest is
     as it was. Pairs are (i, i + rot_dim / 2), or neighbours when interleaved.
-    Differentiable in q and k (tables that require a gradient are refused). k
-    may be None. A position outside the tables gives NaN. Sums are in 32 bits,
-    rounded once.
+    Differentiable in q and k, backward and forward (tables that require a
+    gradient or carry a tangent are refused). k may be None. A position
+    outside the tables gives NaN. Sums are in 32 bits, rounded once.
     """
     return _kv().rotary(q, k, positions, cos, sin, interleaved)
 

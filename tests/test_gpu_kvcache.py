@@ -893,3 +893,43 @@ def test_attention_refuses_what_requires_a_gradient(jasper):
                     f(**asked)
                 with torch.no_grad():
                     assert torch.equal(f(**asked), want), name
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_forward_mode(jasper, interleaved, grad):
+    """The map is linear: the tangent of the result is the rotation of the tangent. With rows that require a gradient
+    too, the tangent is differentiable as the result is."""
+    import torch.autograd.forward_ad as fwd
+    n, dim, rot = 19, 96, 48
+    cos, sin = jasper.rotary_table(300, rot)
+    pos = torch.randint(0, 300, (n,), device="cuda")
+    q, k = randn((n, 6, dim), F16, 280), randn((n, 2, dim), F16, 281)
+    tq, tk = randn((n, 6, dim), F16, 282), randn((n, 2, dim), F16, 283)
+    plain = jasper.rotary(q, k, pos, cos, sin, interleaved=interleaved)
+    if grad:
+        q, k, tq = q.requires_grad_(), k.requires_grad_(), tq.requires_grad_()
+    wants = [ref_rotary(t.detach(), pos, cos, sin, interleaved) for t in (tq, tk)]
+    with fwd.dual_level():
+        dq, dk = fwd.make_dual(q, tq), fwd.make_dual(k, tk)
+        out = jasper.rotary(dq, dk, pos, cos, sin, interleaved=interleaved)
+        for y, same, (want, size) in zip(out, plain, wants):
+            value, tangent = fwd.unpack_dual(y)
+            assert torch.equal(value, same)
+            near(tangent.detach(), want, rotary_tol(want, size, F16))
+        only_k = jasper.rotary(q, dk, pos, cos, sin, interleaved=interleaved)
+        assert fwd.unpack_dual(only_k[0]).tangent is None
+        assert torch.equal(fwd.unpack_dual(only_k[1]).tangent, fwd.unpack_dual(out[1]).tangent)
+        alone, none = jasper.rotary(dq, None, pos, cos, sin, interleaved=interleaved)
+        assert none is None and torch.equal(fwd.unpack_dual(alone).tangent, fwd.unpack_dual(out[0]).tangent)
+        if grad:
+            g = randn((n, 6, dim), F16, 284)
+            value, tangent = fwd.unpack_dual(out[0])
+            want, size = ref_rotary(g, pos, cos, sin, interleaved, back=True)
+            for y, x in ((value, q), (tangent, tq)):
+                near(torch.autograd.grad(y, x, g, retain_graph=True)[0], want, rotary_tol(want, size, F16))
+        for c, s in ((fwd.make_dual(cos, sin), sin), (cos, fwd.make_dual(sin, cos))):
+            with pytest.raises(ValueError, match="no gradient for cos and sin"):
+                jasper.rotary(q, k, pos, c, s)
+    again = jasper.rotary(q, k, pos, cos, sin, interleaved=interleaved)
+    assert all(torch.equal(a, b) for a, b in zip(again, plain))
