@@ -125,7 +125,7 @@ bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
 // What has no gradient is refused where one is asked for, rather than taken as a constant.
 template <typename... Ts>
 bool asks_grad(const Ts&... given) {
-  return at::GradMode::is_enabled() && (wants_grad(given) || ...);
+  return (at::GradMode::is_enabled() && (wants_grad(given) || ...)) || (has_tangent(given) || ...);
 }
 
 // ---- rotary positions ----
@@ -214,8 +214,7 @@ py::tuple rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, c
   TORCH_CHECK_VALUE(at.sizes() == q.sizes().slice(0, q.dim() - 2), "positions must be ",
                     q.sizes().slice(0, q.dim() - 2), ", got ", at.sizes());
   TORCH_CHECK_VALUE(cos && sin, "cos and sin are needed");
-  TORCH_CHECK_VALUE(!asks_grad(cos, sin) && !has_tangent(cos) && !has_tangent(sin),
-                    "rotary has no gradient for cos and sin: detach them");
+  TORCH_CHECK_VALUE(!asks_grad(cos, sin), "rotary has no gradient for cos and sin: detach them");
   TORCH_CHECK_VALUE(table_of(cos, sin, q).rot <= q.size(-1), "the tables rotate more values than a head has");
   const auto [q_out, k_out] = Rotary::turn(q, k ? *k : Tensor(), at, *cos, *sin, interleaved, false);
   return py::make_tuple(q_out, k ? py::cast(k_out) : py::none());
@@ -236,7 +235,7 @@ OptTensor append_tokens(const OptTensor& q, const Tensor& k, const Tensor& v, co
   TORCH_CHECK_VALUE(v.size(1) == pages.heads, "v must be [n, ", pages.heads, ", ", pages.dim, "]");
   if (q) check_alike("q", *q, k);
   TORCH_CHECK_VALUE(!asks_grad(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale),
-                    "append_tokens has no gradient: use rotary, or torch.no_grad()");
+                    "append_tokens has no gradient: use rotary, or detached tensors or torch.no_grad()");
   const int64_t n = k.size(0);
   Tensor rows = indexes("slots", slots, k), at;
   TORCH_CHECK_VALUE(rows.dim() == 1 && rows.size(0) == n, "slots must be [", n, "]");
@@ -265,7 +264,7 @@ OptTensor append_tokens(const OptTensor& q, const Tensor& k, const Tensor& v, co
 void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& src, const Tensor& dst,
                 const OptTensor& tables) {
   const jasperx_kv_pages pages = pages_of(k_pages, v_pages, {}, {}, true);
-  TORCH_CHECK_VALUE(!asks_grad(k_pages, v_pages), "copy_pages has no gradient: use torch.no_grad()");
+  TORCH_CHECK_VALUE(!asks_grad(k_pages, v_pages), "copy_pages has no gradient: use detached tensors or torch.no_grad()");
   for (const Tensor* t : {&src, &dst})
     TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->dim() == 1 && t->device() == k_pages.device() &&
                           t->is_contiguous(),
@@ -302,7 +301,7 @@ struct Attention {
                           q.size(1) % pages.heads == 0 && q.device() == device,
                       "q must be [batch, a multiple of ", pages.heads, " heads, ", pages.dim, "] on ", device);
     TORCH_CHECK_VALUE(!asks_grad(q, k_pages, v_pages, k_scale, v_scale),
-                      "attention over the cache has no gradient: use torch.no_grad()");
+                      "attention over the cache has no gradient: use detached tensors or torch.no_grad()");
     batch = q.size(0);
     TORCH_CHECK_VALUE(tables.scalar_type() == at::kInt && tables.dim() == 2 && tables.size(0) == batch &&
                           tables.device() == device && (tables.size(1) <= 1 || tables.stride(1) == 1),

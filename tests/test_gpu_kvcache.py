@@ -933,3 +933,30 @@ def test_rotary_forward_mode(jasper, interleaved, grad):
                 jasper.rotary(q, k, pos, c, s)
     again = jasper.rotary(q, k, pos, cos, sin, interleaved=interleaved)
     assert all(torch.equal(a, b) for a, b in zip(again, plain))
+
+
+def test_tangents_are_refused_where_none_come_out(jasper):
+    """append_tokens, copy_pages and the attentions have no forward-mode derivative either, with gradients on or off."""
+    import torch.autograd.forward_ad as fwd
+    q, k = randn((2, 4, 64), F16, 290), randn((2, 2, 64), F16, 291)
+    kp, vp = make_pages(4, 2, 16, 64, F16, seed=292)
+    cos, sin = jasper.rotary_table(16, 64)
+    at = torch.arange(2, device="cuda")
+    i32 = torch.arange(2, dtype=torch.int32, device="cuda")
+    with fwd.dual_level(), torch.no_grad():
+        def dual(x):
+            return fwd.make_dual(x, torch.ones_like(x))
+        for rows in ((dual(q), k, k), (q, dual(k), k), (q, k, dual(k))):
+            with pytest.raises(ValueError, match="append_tokens has no gradient"):
+                jasper.append_tokens(*rows, at, at, cos, sin, kp, vp)
+        with pytest.raises(ValueError, match="append_tokens has no gradient"):
+            jasper.append_tokens(q, k, k, at, at, dual(cos), sin, kp, vp)
+        with pytest.raises(ValueError, match="copy_pages has no gradient"):
+            jasper.copy_pages(kp, dual(vp), i32, i32 + 2)
+        for pages, rows in (((kp, vp), dual(q)), ((dual(kp), vp), q), ((kp, dual(vp)), q)):
+            with pytest.raises(ValueError, match="has no gradient"):
+                jasper.decode_attention(rows, *pages, i32[:, None], i32)
+            with pytest.raises(ValueError, match="has no gradient"):
+                jasper.retrieved_attention(rows, *pages, i32[:, None], i32, i32.expand(2, 2, 2).contiguous())
+        plain = jasper.decode_attention(q, kp, vp, i32[:, None], i32)
+        assert torch.equal(jasper.decode_attention(dual(q).detach(), kp, vp, i32[:, None], i32), plain)
