@@ -128,6 +128,12 @@ bool asks_grad(const Ts&... given) {
   return (at::GradMode::is_enabled() && (wants_grad(given) || ...)) || (has_tangent(given) || ...);
 }
 
+// A tensor was written in place: autograd refuses what it saved of it before
+// (inference tensors keep no count).
+void mark_written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ---- rotary positions ----
 
 // q and k turned; either may be undefined. The arguments are checked.
@@ -253,11 +259,13 @@ OptTensor append_tokens(const OptTensor& q, const Tensor& k, const Tensor& v, co
   jasperx_head_rows q_rows{};
   if (q) out = at::empty(q->sizes(), q->options()), q_rows = rows_of(*q, q_held);
   const jasperx_head_rows k_rows = rows_of(k, k_held), v_rows = rows_of(v, v_held);
-  if (n)
+  if (n) {
     check(jasperx_append_tokens(&q_rows, &k_rows, &v_rows, type_of(k), n, table.rot ? at.data_ptr() : nullptr,
                                 rows.data_ptr(), (int32_t)rows.element_size(), table.cos, table.sin, table.rows,
                                 table.rot, interleaved ? JASPERX_ROTARY_INTERLEAVED : 0u, &pages,
                                 out ? out->data_ptr() : nullptr, current_stream(k.get_device())));
+    mark_written(k_pages), mark_written(v_pages);
+  }
   return out;
 }
 
@@ -274,10 +282,13 @@ void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& src,
                                 tables->device() == k_pages.device()),
                     "tables must be a contiguous int32 tensor on ", k_pages.device());
   const c10::DeviceGuard guard(k_pages.device());
-  if (src.size(0))
+  if (src.size(0)) {
     check(jasperx_copy_pages(&pages, (const int32_t*)src.data_ptr(), (const int32_t*)dst.data_ptr(), src.size(0),
                              tables ? (int32_t*)tables->data_ptr() : nullptr, tables ? tables->numel() : 0,
                              current_stream(k_pages.get_device())));
+    mark_written(k_pages), mark_written(v_pages);
+    if (tables) mark_written(*tables);
+  }
 }
 
 // ---- attention of one new token ----

@@ -960,3 +960,39 @@ def test_tangents_are_refused_where_none_come_out(jasper):
                 jasper.retrieved_attention(rows, *pages, i32[:, None], i32, i32.expand(2, 2, 2).contiguous())
         plain = jasper.decode_attention(q, kp, vp, i32[:, None], i32)
         assert torch.equal(jasper.decode_attention(dual(q).detach(), kp, vp, i32[:, None], i32), plain)
+
+
+def test_writes_in_place_are_counted(jasper):
+    """Autograd has to know that pages and tables changed: what it saved of them before is stale."""
+    store = [torch.zeros((2, 4, 2, 16, 64), dtype=F16, device="cuda") for _ in range(2)]
+    kp, vp = store[0][1], store[1][1]  # a layer of larger tensors
+    k = randn((2, 2, 64), F16, 300)
+    at = torch.arange(2, device="cuda")
+    src, dst = (torch.tensor([i], dtype=torch.int32, device="cuda") for i in (0, 3))
+    tables = torch.zeros((2, 3), dtype=torch.int32, device="cuda")
+    w = randn(kp.shape, F16, 301).requires_grad_()
+    tensors = [*store, kp, vp, tables]
+
+    def counts():
+        return [t._version for t in tensors]
+
+    saved, before = (kp * w).sum(), counts()
+    jasper.append_tokens(None, k, k, None, at, None, None, kp, vp)
+    assert [b > a for a, b in zip(before, counts())] == [True] * 4 + [False]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()
+    for given, moved in ((None, False), (tables, True)):
+        saved, before = (vp * w).sum(), counts()
+        jasper.copy_pages(*store, src, dst, tables=given)
+        assert [b > a for a, b in zip(before, counts())] == [True] * 4 + [moved]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            saved.backward()
+    saved, before = (vp * w).sum(), counts()
+    jasper.decode_attention(randn((2, 4, 64), F16, 302), kp, vp, tables, dst.expand(2).contiguous())
+    assert counts() == before
+    saved.backward()
+    with torch.inference_mode():  # such tensors are not counted, and still written
+        free = torch.zeros_like(kp), torch.zeros_like(vp)
+    jasper.append_tokens(None, k, k, None, at, None, None, *free)
+    jasper.copy_pages(*free, src, dst)
+    assert torch.equal(free[0][0, :, :2], k.transpose(0, 1)) and torch.equal(free[1][3], free[1][0])
