@@ -996,3 +996,24 @@ def test_writes_in_place_are_counted(jasper):
     jasper.append_tokens(None, k, k, None, at, None, None, *free)
     jasper.copy_pages(*free, src, dst)
     assert torch.equal(free[0][0, :, :2], k.transpose(0, 1)) and torch.equal(free[1][3], free[1][0])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_append_e4m3_quotients_are_a_division_s(jasper, dtype):
+    """Every value of the type over ordinary scales, tiny, huge, infinite and zero ones: the bits of a division in 32
+    bits, saturated and rounded, the sign of a zero among them."""
+    scales = [0.001, 1 / 3, -0.02, 7.3, 448.0, 2.0 ** -79, 2.0 ** 79, 1.3 * 2.0 ** -81, 1.7 * 2.0 ** 81, 2.0 ** -126,
+              2.0 ** -127, 2.0 ** -129, 3 * 2.0 ** -134, 3e38, math.inf, 0.0]
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    k = bits.view(256, 1, 256).expand(256, len(scales), 256)
+    scale = torch.tensor(scales, dtype=torch.float32)
+    kp, vp = make_pages(32, len(scales), 8, 256, F8)
+    jasper.append_tokens(None, k.cuda(), k.cuda(), None, torch.arange(256, device="cuda"), None, None, kp, vp,
+                         k_scale=scale.cuda(), v_scale=scale.cuda())
+    want = (k.float() / scale[None, :, None]).clamp(-448, 448).to(F8)
+    for store in (kp, vp):
+        got = store.transpose(1, 2).reshape(want.shape).cpu()
+        nan = want.float().isnan()
+        assert torch.equal(got.float().isnan(), nan)
+        off = (got.view(torch.uint8) != want.view(torch.uint8)) & ~nan
+        assert not off.any(), [(scales[i], int(n)) for i, n in enumerate(off.sum((0, 2)).tolist()) if n]
