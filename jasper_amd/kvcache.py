@@ -413,15 +413,19 @@ class PagedCache:
                                    **options)
 
     def keys(self, layer: int, seq: int) -> torch.Tensor:
-        """The keys of a sequence as they are held, [kv_heads, length, dim], contiguous: rows for an index."""
+        """The keys of a sequence, [kv_heads, length, dim], contiguous float16 rows for an index (`Graph`,
+        `bruteforce_knn`), whatever the pages' type: what they hold (times k_scale), rounded once; finite values past
+        float16's range are its ends, +-65504."""
         n = self.length(seq)
         own, = self._upload(self.table.pages[seq, :-(-n // self.table.page_size)])
         store = self.k_pages[layer]
         rows = store.view(torch.uint8)[own].view(store.dtype) if store.dtype == _F8 else store[own]
         heads, dim = store.size(1), store.size(3)
         rows = rows.transpose(0, 1).reshape(heads, -1, dim)[:, :n]
-        if store.dtype == _F8:
-            rows = rows.to(torch.float16)
+        if store.dtype != torch.float16:
+            rows = rows.float()
             if self.k_scale is not None:
-                rows = (rows.float() * self.k_scale[layer][:, None, None]).to(torch.float16)
+                rows = rows * self.k_scale[layer][:, None, None]
+            most = torch.finfo(torch.float16).max
+            rows = torch.where(rows.isfinite(), rows.clamp(-most, most), rows).to(torch.float16)
         return rows.contiguous()

@@ -143,3 +143,42 @@ def test_example(jasper, exact):
     # every token read: the full attention itself, but for the types' rounding
     weight, error = example.main(args + ["--last", "4000"])
     assert abs(weight - 1) < 1e-4 and error < 2.0 ** -9
+
+
+@pytest.mark.parametrize("dtype", [F16, torch.bfloat16, F8])
+def test_keys_are_rows_for_an_index(jasper, dtype):
+    """Whatever type the pages have, the index takes the keys: the search finds what the rows' products say."""
+    heads, dim, n = 2, 64, 700
+    rows_type = F16 if dtype == F8 else dtype
+    scale = torch.tensor([[0.02, 0.03]], device="cuda") if dtype == F8 else None
+    cache = jasper.PagedCache(50, 1, heads, dim, dtype=dtype, k_scale=scale)
+    g = torch.Generator(device="cuda").manual_seed(11)
+    k = torch.randn((n, heads, dim), device="cuda", generator=g).to(rows_type)
+    seq = cache.new()
+    cache.append(0, cache.extend([seq], n), None, k, k)
+    keys = cache.keys(0, seq)
+    assert keys.dtype == F16 and keys.shape == (heads, n, dim) and keys.is_contiguous()
+    held = k.double().transpose(0, 1)
+    if dtype == F8:  # to 4 bits of 448 scales' worth, then to fp16
+        assert ((keys.double() - held).abs() <= held.abs() * (2.0 ** -4 + 2.0 ** -10) + 0.03 * 2.0 ** -9).all()
+    else:  # bf16's 8 bits fit fp16's 11 but below its smallest normal value
+        assert ((keys.double() - held).abs() <= 2.0 ** -25).all()
+    q = torch.randn((5, dim), device="cuda", generator=g).half()
+    for h in range(heads):
+        found = jasper.bruteforce_knn(keys[h], q, 10, distance="ip")[0]
+        products = q.double() @ keys[h].double().T
+        best = products.topk(10, dim=1).values
+        # products of 64 terms, summed in 32 bits and held in 16
+        assert (products.gather(1, found.long()) >= best[:, -1:] - 2.0 ** -9 * best.abs().amax()).all()
+        graph = jasper.Graph.build(keys[h], n_neighbors=32, distance="ip")
+        assert graph.search(q, k=10)[0].shape == (5, 10)
+
+
+def test_keys_past_the_range_of_float16(jasper):
+    """bf16 keys reach further: rows for the index stay finite; what is no number stays so."""
+    cache = jasper.PagedCache(4, 1, 1, 8, dtype=torch.bfloat16)
+    k = torch.tensor([[1e38, -1e38, 65504.0, 66000.0, -70000.0, math.inf, -math.inf, math.nan]], device="cuda").bfloat16()
+    seq = cache.new()
+    cache.append(0, cache.extend([seq], 1), None, k[:, None], k[:, None])
+    got = cache.keys(0, seq)[0, 0].tolist()
+    assert got[:7] == [65504.0, -65504.0, 65504.0, 65504.0, -65504.0, math.inf, -math.inf] and math.isnan(got[7])
