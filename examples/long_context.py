@@ -9,7 +9,9 @@ built over the keys of every key head, and then, for every new token,
   3. retrieved_attention reads the first tokens, the latest ones and those
      found, decode_attention all of them.
 
-Two continuations share the document's pages (a fork). Printed: the share of
+The index holds the document; the tokens that came after it are all read, as the
+window grows with them (a much longer answer would append them to an index of its
+own). Two continuations share the document's pages (a fork). Printed: the share of
 the full softmax's weight that the retrieved tokens carry, how far the output
 is off, and the time of either attention. The data are synthetic: keys of
 --topics topics with noise, every new query near one of them.
@@ -63,7 +65,7 @@ def main(argv=None):
     ap.add_argument("--dim", type=int, default=128)
     ap.add_argument("--k", type=int, default=100, help="tokens retrieved per query head")
     ap.add_argument("--first", type=int, default=4)
-    ap.add_argument("--last", type=int, default=64)
+    ap.add_argument("--last", type=int, default=64, help="at least; all tokens after the document in any case")
     ap.add_argument("--topics", type=int, default=0, help="0: one per 64 tokens")
     ap.add_argument("--exact", action="store_true", help="search by brute force, not through a graph")
     ap.add_argument("--quiet", action="store_true")
@@ -97,13 +99,14 @@ def main(argv=None):
         found = [search(q[:, h * group:(h + 1) * group].reshape(-1, a.dim), a.k).view(len(answers), group, a.k)
                  for h, search in enumerate(searches)]
         ids = torch.cat(found, dim=1).contiguous()
-        out, lse = cache.retrieved(0, step, q, ids, first=a.first, last=a.last, return_lse=True)
+        last = max(a.last, step.max_len - a.tokens)  # what the index does not hold
+        out, lse = cache.retrieved(0, step, q, ids, first=a.first, last=last, return_lse=True)
         full, full_lse = cache.decode(0, step, q, return_lse=True)
         weights.append(torch.exp(lse - full_lse).mean().item())
         errors.append(((out.float() - full.float()).norm() / full.float().norm()).item())
-    us = [timed(lambda: cache.retrieved(0, step, q, ids, first=a.first, last=a.last)), timed(lambda: cache.decode(0, step, q))]
+    us = [timed(lambda: cache.retrieved(0, step, q, ids, first=a.first, last=last)), timed(lambda: cache.decode(0, step, q))]
     if not a.quiet:
-        print(f"{a.tokens} tokens, {a.first} + {a.k} + {a.last} read per query head: "
+        print(f"{a.tokens} tokens, {a.first} + {a.k} + {last} read per query head: "
               f"{100 * sum(weights) / a.steps:.1f}% of the weight, output off by {100 * sum(errors) / a.steps:.2f}%; "
               f"attention {us[0]:.1f} us of the retrieved, {us[1]:.1f} us of all")
     cache.free(answers)

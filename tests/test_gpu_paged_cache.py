@@ -182,3 +182,14 @@ def test_keys_past_the_range_of_float16(jasper):
     cache.append(0, cache.extend([seq], 1), None, k[:, None], k[:, None])
     got = cache.keys(0, seq)[0, 0].tolist()
     assert got[:7] == [65504.0, -65504.0, 65504.0, 65504.0, -65504.0, math.inf, -math.inf] and math.isnan(got[7])
+
+
+@pytest.mark.parametrize("exact", [False, True])
+def test_example_reads_every_token_after_the_document(jasper, exact):
+    """An answer longer than the window: with the whole document retrieved, nothing may be missing."""
+    spec = importlib.util.spec_from_file_location("long_context", Path(__file__).parent.parent / "examples/long_context.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    weight, error = example.main(["--tokens", "100", "--k", "100", "--first", "100", "--last", "2", "--steps", "40",
+                                  "--topics", "2", "--quiet"] + (["--exact"] if exact else []))
+    assert abs(weight - 1) < 1e-4 and error < 2.0 ** -9
