@@ -1017,3 +1017,31 @@ def test_append_e4m3_quotients_are_a_division_s(jasper, dtype):
         assert torch.equal(got.float().isnan(), nan)
         off = (got.view(torch.uint8) != want.view(torch.uint8)) & ~nan
         assert not off.any(), [(scales[i], int(n)) for i, n in enumerate(off.sum((0, 2)).tolist()) if n]
+
+
+def test_every_page_of_several_launches_is_copied(jasper):
+    """2,100 pages of 8 MB of keys and as much of values: 2,048 go in the first launch, the others in the second.
+    No page shares memory with another, and each holds its own numbers."""
+    torch.cuda.empty_cache()
+    moves, shape = 2100, (4201, 64, 256, 256)
+    kp, vp = (torch.empty(shape, dtype=F16, device="cuda") for _ in range(2))
+    words = [x.view(torch.int64).view(shape[0], -1) for x in (kp, vp)]
+    g = torch.Generator(device="cuda").manual_seed(310)
+    for x in words:
+        x.random_(generator=g)
+    sums = [x.sum(1) for x in words]
+    order = torch.randperm(shape[0], device="cuda", generator=g)
+    src, dst, spare = order[:moves], order[moves:2 * moves], order[2 * moves:]
+    tables = order.flip(0).int().contiguous()
+    jasper.copy_pages(kp, vp, src.int(), dst.int(), tables=tables)
+    for x, before in zip(words, sums):
+        for i in range(0, moves, 70):
+            assert torch.equal(x[dst[i:i + 70]], x[src[i:i + 70]]), i
+        after = x.sum(1)
+        assert torch.equal(after[dst], before[src]) and torch.equal(after[src], before[src])
+        assert torch.equal(after[spare], before[spare])
+    to = torch.arange(shape[0], device="cuda")
+    to[src] = dst
+    assert torch.equal(tables.long(), to[order.flip(0)])
+    del kp, vp, words, x
+    torch.cuda.empty_cache()
