@@ -886,7 +886,8 @@ void check_type(int32_t type) {
 KvPages kv_pages(const jasperx_kv_pages* p) {
   if (!p) throw std::invalid_argument("null pages");
   if (p->type < kF16 || p->type > kE4M3) throw std::invalid_argument("page type must be 0 (fp16), 1 (bf16) or 2 (e4m3)");
-  if (p->layers < 1 || p->pages < 0 || p->heads < 1) throw std::invalid_argument("bad cache sizes");
+  if (p->layers < 1 || p->pages < 0 || p->heads < 1)
+    throw std::invalid_argument("a cache must be of at least one layer and one head, and not of fewer than no pages");
   if (p->page_size < 8 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
     throw std::invalid_argument("page_size must be a power of two from 8 to 256");
   const int64_t bytes = kv_bytes(p->type), unit = 16 / bytes;

@@ -1045,3 +1045,14 @@ def test_every_page_of_several_launches_is_copied(jasper):
     assert torch.equal(tables.long(), to[order.flip(0)])
     del kp, vp, words, x
     torch.cuda.empty_cache()
+
+
+def test_caches_without_layers_or_heads_are_refused_as_arguments(jasper):
+    kp, vp = (torch.zeros((0, 4, 2, 16, 64), dtype=F16, device="cuda") for _ in range(2))
+    one = torch.zeros(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="at least one layer"):
+        jasper.copy_pages(kp, vp, one, one + 1)
+    kp, vp = (torch.zeros((4, 0, 16, 64), dtype=F16, device="cuda") for _ in range(2))
+    rows = torch.zeros((1, 0, 64), dtype=F16, device="cuda")
+    with pytest.raises(ValueError, match="one head"):
+        jasper.append_tokens(None, rows, rows, None, one, None, None, kp, vp)
