@@ -923,7 +923,7 @@ RotaryArgs rotary_args(const jasperx_head_rows* q, const jasperx_head_rows* k, i
   if (rot_dim < 0 || rot_dim > dim || rot_dim % 2) throw std::invalid_argument("rot_dim must be even, up to dim");
   if (index_bytes != 4 && index_bytes != 8) throw std::invalid_argument("index_bytes must be 4 or 8");
   if (flags & ~(JASPERX_ROTARY_INTERLEAVED | JASPERX_ROTARY_INVERSE)) throw std::invalid_argument("unknown rotary flags");
-  if (n && rot_dim && (!positions || !cos || !sin || table_rows < 0)) throw std::invalid_argument("null positions or tables");
+  if (n && rot_dim && (!positions || table_rows < 0 || (table_rows && (!cos || !sin)))) throw std::invalid_argument("null positions or tables");
   RotaryArgs a;
   a.q = head_rows(q), a.k = head_rows(k);
   a.positions = positions, a.pos64 = index_bytes == 8;

@@ -1056,3 +1056,10 @@ def test_caches_without_layers_or_heads_are_refused_as_arguments(jasper):
     rows = torch.zeros((1, 0, 64), dtype=F16, device="cuda")
     with pytest.raises(ValueError, match="one head"):
         jasper.append_tokens(None, rows, rows, None, one, None, None, kp, vp)
+
+
+def test_every_position_is_outside_of_empty_tables(jasper):
+    cos, sin = jasper.rotary_table(0, 32)
+    q = randn((3, 2, 48), F16, 320)
+    y, _ = jasper.rotary(q, None, torch.arange(3, device="cuda"), cos, sin)
+    assert y[..., :32].isnan().all() and torch.equal(y[..., 32:], q[..., 32:])
