@@ -17,12 +17,14 @@ Pages are [n_pages, kv_heads, page_size, dim] (with a leading layer dimension
 where said) in float16, bfloat16 or float8_e4m3fn, any strides that keep a
 row's dim values together and rows on 16 bytes. Calls run on the current
 stream of the tensors' device, synchronize nothing and may be captured in a
-graph (PagedCache's bookkeeping is on the host and is not captured).
+graph (PagedCache's bookkeeping is on the host and is not captured). They take
+tensors with memory, and are not operators registered with torch:
+torch.compile runs them as they are, between the graphs before and after, and
+vmap, torch.func's grad and jvp, export and fake tensors end in an error.
 """
 
 from __future__ import annotations
 
-import functools
 import importlib.machinery
 import importlib.util
 import math
@@ -34,9 +36,16 @@ _TYPES = (torch.float16, torch.bfloat16, torch.float8_e4m3fn)
 _F8 = torch.float8_e4m3fn
 
 
-@functools.lru_cache(maxsize=None)
+_module = None
+
+
 def _kv():
     """The module that takes tensors to the HIP library's calls (csrc/torch_kv.cpp)."""
+    return _module or _load_kv()
+
+
+def _load_kv():
+    global _module
     from . import _load_lib, library_path
     _load_lib()
     path = library_path().parent / "_kv.so"
@@ -46,6 +55,7 @@ def _kv():
     loader = importlib.machinery.ExtensionFileLoader("jasper_amd._kv", str(path))
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader("jasper_amd._kv", loader))
     loader.exec_module(module)
+    _module = module
     return module
 
 

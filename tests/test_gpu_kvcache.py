@@ -1063,3 +1063,33 @@ def test_every_position_is_outside_of_empty_tables(jasper):
     q = randn((3, 2, 48), F16, 320)
     y, _ = jasper.rotary(q, None, torch.arange(3, device="cuda"), cos, sin)
     assert y[..., :32].isnan().all() and torch.equal(y[..., 32:], q[..., 32:])
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_what_has_no_memory_is_refused_and_compiled_code_calls_through(jasper):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    q, k = randn((3, 4, 64), F16, 330), randn((3, 2, 64), F16, 331)
+    kp, vp = make_pages(4, 2, 16, 64, F16, seed=332)
+    at = torch.arange(3, device="cuda")
+    cos, sin = jasper.rotary_table(8, 64)
+    tables, lens = torch.zeros((3, 1), dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    ids = torch.zeros((3, 2, 1), dtype=torch.int32, device="cuda")
+    calls = [lambda q, k: jasper.rotary(q, k, at, cos, sin)[0],
+             lambda q, k: jasper.append_tokens(q, k, k, at, at, cos, sin, kp, vp),
+             lambda q, k: jasper.decode_attention(q, kp, vp, tables, lens),
+             lambda q, k: jasper.retrieved_attention(q, kp, vp, tables, lens, ids)]
+    module = jasper.kvcache._kv()
+    for f in calls:
+        want = f(q, k)
+        twice = torch.compile(lambda q, k, f=f: 2 * f(q, k), backend="eager")
+        assert torch.equal(twice(q, k), 2 * want)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(torch.stack([q, q]), torch.stack([k, k]))
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.func.jvp(lambda q, f=f: f(q, k), (q,), (q,))
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.func.grad(lambda q, f=f: f(q, k).float().sum())(q)
+        with FakeTensorMode() as mode, pytest.raises((RuntimeError, ValueError)):
+            f(mode.from_tensor(q), mode.from_tensor(k))
+    assert jasper.kvcache._kv() is module
+    torch.cuda.synchronize()
