@@ -1093,3 +1093,81 @@ def test_what_has_no_memory_is_refused_and_compiled_code_calls_through(jasper):
             f(mode.from_tensor(q), mode.from_tensor(k))
     assert jasper.kvcache._kv() is module
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("batch,heads,count,dim,cache", [(64, 8, 1300, 128, F16), (128, 8, 1700, 128, F8), (200, 4, 3000, 64, F16),
+                                                         (130, 4, 900, 256, BF16)])
+def test_lists_longer_than_a_wave_stages_at_once(jasper, batch, heads, count, dim, cache):
+    """So many lists that a wave of a group has more tiles than it keeps row offsets of."""
+    g = torch.Generator().manual_seed(340)
+    lens = torch.randint(count, 2 * count, (batch,), generator=g).tolist()
+    lens[3], lens[7] = 0, 40
+    dtype = F16 if cache == F8 else cache
+    pages = [-(-n // 16) for n in lens]
+    total = sum(pages) + 1
+    kp, vp = make_pages(total, heads, 16, dim, cache, seed=341)
+    order = torch.randperm(total, generator=g)
+    tables = torch.zeros((batch, max(pages)), dtype=torch.int32)
+    for i, n in enumerate(pages):
+        tables[i, :n] = order[sum(pages[:i]):sum(pages[:i]) + n].int()
+    ks, vs = f8_scales(heads, cache, 342)
+    q = randn((batch, heads, dim), dtype, 343, 2.0)
+    ids = torch.stack([torch.stack([torch.randperm(max(lens), generator=g)[:count] for _ in range(heads)])
+                       for _ in range(batch)]).int()
+    out = jasper.retrieved_attention(q, kp, vp, tables.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), ids.cuda(),
+                                     first=3, last=30, k_scale=ks, v_scale=vs, return_lse=True)
+    some = [0, 3, 7, batch // 2, batch - 1]
+    keys, values = [], []
+    for i in some:
+        mine = tables[i, :pages[i]].long().cuda()
+        for held, store in ((keys, kp), (values, vp)):
+            held.append(raw(store)[mine].view(cache).transpose(0, 1).reshape(heads, -1, dim)[:, :lens[i]].double().cpu())
+
+    def choose(i, j):
+        n = lens[some[i]]
+        a, z = min(3, n), max(n - 30, min(3, n))
+        mine = ids[some[i], j].long()
+        return torch.cat([torch.arange(a), torch.arange(z, n), mine[(mine >= a) & (mine < z)]])
+
+    at = torch.tensor(some, device="cuda")
+    check([x[at] for x in out], ref_attention(q[at], keys, values, dim ** -0.5, choose, dtype, ks, vs, heads))
+
+
+def test_threads_with_streams_of_their_own(jasper):
+    import threading
+    cos, sin = jasper.rotary_table(4000, 128)
+    errors = []
+
+    def work(x):
+        try:
+            lens = [3000 + x, 5, 700]
+            kp, vp, tables, _, _ = build_cache(lens, 2, 16, 128, F16, 350 + x)
+            q = randn((3, 8, 128), F16, 360 + x, 2.0)
+            tens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+            ids = torch.randint(0, 700, (3, 2, 90), dtype=torch.int32, device="cuda")
+            pos = tens.long() - 1
+
+            def step():
+                turned, _ = jasper.rotary(q, None, pos, cos, sin)
+                return (turned, *jasper.decode_attention(turned, kp, vp, tables, tens, return_lse=True),
+                        *jasper.retrieved_attention(turned, kp, vp, tables, tens, ids, first=2, last=9, return_lse=True))
+
+            want = step()
+            torch.cuda.current_stream().synchronize()
+            stream = torch.cuda.Stream()
+            for _ in range(30):
+                with torch.cuda.stream(stream):
+                    got = step()
+                    with pytest.raises(ValueError):
+                        jasper.decode_attention(q, kp, vp, tables[:1], tens)
+                stream.synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except Exception as e:  # noqa: BLE001  a thread's own error is told below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(x,)) for x in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
