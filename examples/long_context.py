@@ -11,10 +11,10 @@ built over the keys of every key head, and then, for every new token,
 
 The index holds the document; the tokens that came after it are all read, as the
 window grows with them (a much longer answer would append them to an index of its
-own). Two continuations share the document's pages (a fork). Printed: the share of
-the full softmax's weight that the retrieved tokens carry, how far the output
-is off, and the time of either attention. The data are synthetic: keys of
---topics topics with noise, every new query near one of them.
+own). Two continuations share the document's pages (a fork). Printed: the share
+of the full softmax's weight that the retrieved tokens carry, how far the output
+is off, and the time of either attention and of the searches. The data are
+synthetic: keys of --topics topics with noise, every new query near one of them.
 
     python examples/long_context.py --tokens 65536
 """
@@ -42,6 +42,15 @@ def build_indexes(cache, seq, exact):
             graph = jasper_amd.Graph.build(keys, n_neighbors=32, distance="ip")
             searches.append(lambda q, k, graph=graph: graph.search(q, k=k, beam_width=max(64, 2 * k))[0])
     return searches
+
+
+def retrieve(searches, q, k):
+    """The ids [sequences, heads, k] that each query head's search of its key head's index returns."""
+    n, heads, dim = q.shape
+    group = heads // len(searches)
+    found = [search(q[:, h * group:(h + 1) * group].reshape(-1, dim), k).view(n, group, k)
+             for h, search in enumerate(searches)]
+    return torch.cat(found, dim=1).contiguous()
 
 
 def timed(f, repeats=20):
@@ -91,24 +100,23 @@ def main(argv=None):
     searches = build_indexes(cache, document, a.exact)
     answers = [document, cache.fork(document)]
 
-    group, weights, errors = a.q_heads // a.kv_heads, [], []
+    weights, errors = [], []
     for _ in range(a.steps):
         step = cache.extend(answers, 1)
         q, k, v = tokens(len(answers), 0.5)
         q = cache.append(0, step, q, k, v, cos, sin)
-        found = [search(q[:, h * group:(h + 1) * group].reshape(-1, a.dim), a.k).view(len(answers), group, a.k)
-                 for h, search in enumerate(searches)]
-        ids = torch.cat(found, dim=1).contiguous()
+        ids = retrieve(searches, q, a.k)
         last = max(a.last, step.max_len - a.tokens)  # what the index does not hold
         out, lse = cache.retrieved(0, step, q, ids, first=a.first, last=last, return_lse=True)
         full, full_lse = cache.decode(0, step, q, return_lse=True)
         weights.append(torch.exp(lse - full_lse).mean().item())
         errors.append(((out.float() - full.float()).norm() / full.float().norm()).item())
-    us = [timed(lambda: cache.retrieved(0, step, q, ids, first=a.first, last=last)), timed(lambda: cache.decode(0, step, q))]
+    us = [timed(lambda: cache.retrieved(0, step, q, ids, first=a.first, last=last)), timed(lambda: cache.decode(0, step, q)),
+          timed(lambda: retrieve(searches, q, a.k))]
     if not a.quiet:
         print(f"{a.tokens} tokens, {a.first} + {a.k} + {last} read per query head: "
               f"{100 * sum(weights) / a.steps:.1f}% of the weight, output off by {100 * sum(errors) / a.steps:.2f}%; "
-              f"attention {us[0]:.1f} us of the retrieved, {us[1]:.1f} us of all")
+              f"attention {us[0]:.1f} us of the retrieved, after {us[2]:.1f} us of searches; {us[1]:.1f} us of all")
     cache.free(answers)
     return sum(weights) / a.steps, sum(errors) / a.steps
 
