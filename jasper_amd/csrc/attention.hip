@@ -232,9 +232,10 @@ __device__ __forceinline__ Sums<DT> attend_tiles(const Params& p, const Span& sp
   constexpr int VD = DT / 16, KS = DT / 32, ES = F8 ? 1 : 2;
   constexpr int BD = VD * ES > 16 ? 16 / ES : VD;  // dims of a lane that lie together
   typedef std::conditional_t<F8, f16, T> PT;  // e4m3 values are exact in fp16, where weights keep more bits
+  // The reference is moved once a score is 2^3 above the one it was set for.
   // fp16 weights are 2^12 larger, so that those far below the largest are not
-  // lost; the reference is moved once a score is 2^3 above it
-  constexpr float kTop = std::is_same_v<PT, f16> ? 12.f : 0.f, kLag = 3.f;
+  // lost; bf16's are at most 1, as V may reach fp32's end.
+  constexpr float kLag = 3.f, kTop = std::is_same_v<PT, f16> ? 12.f : -kLag;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
   const char* kb = p.k + at.kv_head * p.head_stride * ES;
   const char* vb = p.v + at.kv_head * p.head_stride * ES;

@@ -1171,3 +1171,26 @@ def test_threads_with_streams_of_their_own(jasper):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+@pytest.mark.parametrize("width", [8, 4000])
+@pytest.mark.parametrize("step", [1.0, 2.0, 5.0])
+def test_large_bf16_values_stay_finite(jasper, width, step):
+    """Values near bf16's end, the later ones with the higher scores: no weight may be over one. So many sequences that
+    a wave has several tiles of one, under short tables (a work-group to a stream) and wide ones."""
+    n, batch = 120, 3000
+    kp, vp = (torch.zeros((9, 1, 16, 64), dtype=BF16, device="cuda") for _ in range(2))
+    tables = torch.zeros((batch, width), dtype=torch.int32, device="cuda")
+    tables[:, :8] = torch.arange(1, 9)
+    for i, t in enumerate((3, 50, 90)):
+        page, row = 1 + t // 16, t % 16
+        kp[page, 0, row, 0] = step * i
+        vp[page, 0, row] = 1e38 * (1 - 0.1 * i)
+    q = torch.zeros((batch, 2, 64), dtype=BF16, device="cuda")
+    q[:, :, 0] = 1.0
+    keys, values = ([x[1:].float().transpose(0, 1).reshape(1, -1, 64)[:, :n].double().cpu()] for x in (kp, vp))
+    ref = ref_attention(q[:1], keys, values, 1.0, lambda i, j: torch.arange(n), BF16)
+    out, lse = jasper.decode_attention(q, kp, vp, tables, torch.full((batch,), n, dtype=torch.int32, device="cuda"), scale=1.0,
+                                       return_lse=True)
+    for i in range(0, batch, 99):
+        check((out[i:i + 1], lse[i:i + 1]), ref)
