@@ -140,9 +140,9 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     """Copies pages src[i] to dst[i] (int32) of k_pages and v_pages, [n_pages,
     kv_heads, page_size, dim] or with a leading layer dimension, all layers in
     one launch. With `tables` (int32, any shape, contiguous) it moves them:
-    entries equal to src[i] become dst[i]. No page may be a source and a
-    destination, or the destination of two. Pairs with an id outside the
-    cache are skipped."""
+    entries equal to src[i] become dst[i], and no page may be listed in src
+    twice. No page may be a source and a destination, or the destination of
+    two. Pairs with an id outside the cache are skipped."""
     _kv().copy_pages(k_pages, v_pages, src, dst, tables)
 
 
@@ -161,9 +161,10 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     Returns out [batch, heads, dim] in q's type, and with return_lse the
     logarithm of the sum of exp(scores) in float32 [batch, heads]; a sequence
     without tokens gives 0 and -inf. Whatever the rows past a sequence's end
-    hold is not seen, nor are tokens whose table entry is no page. max_len: no
-    sequence is longer (default: what tables can hold); the work is laid out
-    for it, and tokens past it are not read.
+    hold is not seen, nor are tokens whose table entry is no page. A row of
+    v_pages that is read and holds an infinity gives an infinity or NaN.
+    max_len: no sequence is longer (default: what tables can hold); the work
+    is laid out for it, and tokens past it are not read.
     """
     return _kv().decode_attention(q, k_pages, v_pages, tables, lens, scale, window, k_scale, v_scale, max_len, return_lse)
 
@@ -328,11 +329,12 @@ class PagedCache:
             raise ValueError("page_size must be a power of two from 8 to 256")
         if n_layers < 1 or kv_heads < 1 or dim < 1 or dim > 256 or dim % (16 if dtype == _F8 else 8):
             raise ValueError("n_layers and kv_heads must be at least 1, dim up to 256 and a multiple of 16 bytes")
-        self.table = PageTable(n_pages, page_size, max_sequences, max_pages or n_pages)
+        max_pages = n_pages if max_pages is None else max_pages
+        self.table = PageTable(n_pages, page_size, max_sequences, max_pages)
         shape = (n_layers, n_pages, kv_heads, page_size, dim)
         self.k_pages = torch.empty(shape, dtype=dtype, device=device)
         self.v_pages = torch.empty(shape, dtype=dtype, device=device)
-        self.tables = torch.full((max_sequences, max_pages or n_pages), -1, dtype=torch.int32, device=device)
+        self.tables = torch.full((max_sequences, max_pages), -1, dtype=torch.int32, device=device)
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
             if t is not None and (dtype != _F8 or t.shape != (n_layers, kv_heads)):
                 raise ValueError(f"{name} must be [{n_layers}, {kv_heads}] with float8_e4m3fn pages")

@@ -208,3 +208,12 @@ def test_yarn_blends_between_its_two_bounds(rot, base, original, factor):
         assert abs(math.hypot(sin[1, i].item(), cos[1, i].item()) - size) <= 2.0 ** -23 * size
         if original * plain / (2 * math.pi) > 1:
             assert got > plain / factor * (1 + 2.0 ** -20), i
+
+
+def test_cache_refuses_tables_of_no_pages():
+    """max_pages 0 is no default."""
+    from jasper_amd import PagedCache
+    for bad in (0, -1):
+        with pytest.raises(ValueError, match="max_pages"):
+            PagedCache(4, 1, 2, 64, max_pages=bad, device="cpu")
+    assert PagedCache(4, 1, 2, 64, device="cpu").tables.shape == (64, 4)
