@@ -23,7 +23,9 @@ constexpr int kStage = 512;   // row offsets of a wave, in LDS
 constexpr int kJoin = 256;   // threads of a joining work-group
 constexpr int kGroupStage = 256;        // row offsets of a wave of a group, in LDS
 constexpr int kGroupLds = 64 << 10;     // bytes at most
-// waves of a group at most: what a compute unit has registers for
+// waves of a group at most. A compute unit has registers for 16 and more of 64
+// values, for four of 256; of 128 for eight of the largest form (169 of a lane)
+// and for 12 to 16 of the others, which was not tried
 constexpr int group_waves(int dt) { return dt == 64 ? 16 : dt == 128 ? 8 : 4; }
 // A wave's sums in the workspace: dt floats and two for each of its heads, and
 // what keeps the next one's on 16 bytes.
@@ -460,7 +462,7 @@ constexpr int side_of(int dt) { return dt == 256 ? 4 : 8; }
 template <typename T, bool F8, int DT, bool LISTED, bool FULL>
 __global__ __launch_bounds__(64 * (FULL ? 1 : side_of(DT)), DT == 256 ? 1 : 2) void attend_kernel(Params p) {
   constexpr int VD = DT / 16;
-  extern __shared__ int64_t lds[];
+  extern __shared__ __attribute__((aligned(16))) int64_t lds[];
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
   const int wave = FULL ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per_list = (p.head_tiles + p.side - 1) / p.side, streams = p.lists * per_list;
@@ -520,7 +522,7 @@ __global__ __launch_bounds__(64 * (FULL ? 1 : side_of(DT)), DT == 256 ? 1 : 2) v
 template <typename T, bool F8, int DT, bool LISTED, bool FULL>
 __global__ __launch_bounds__(64 * group_waves(DT)) void attend_group_kernel(Params p) {
   constexpr int VD = DT / 16;
-  extern __shared__ int64_t lds[];
+  extern __shared__ __attribute__((aligned(16))) int64_t lds[];
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int head_tile = blockIdx.x % p.head_tiles, list = blockIdx.x / p.head_tiles % p.lists;
@@ -677,7 +679,12 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_t
   // 48.7 / 57.2. Longer tables may hold sequences too unlike for it; lists are
   // alike, and are grouped up to eight tiles a wave where there is one for
   // three in four compute units: 1,068 tokens in 128 lists 29.3 / 26.3, in 256
-  // 30.2 / 37.7, in 512 54.1 / 64.2.
+  // 30.2 / 37.7, in 512 54.1 / 64.2; 1,272 tokens in 192 lists 28.6 / 33. Between
+  // 128 and 192 neither was measured: the cut may lie lower (near 165, if the
+  // times change evenly). The waves are counted as the shared kernel's, eight to
+  // a compute unit; groups of 64 values have room for twice as many, not tried:
+  // 204 streams of up to 1000 tokens get ten waves each, with up to four tiles
+  // in a row, 11.8 us.
   const int64_t all = batch * a.streams;
   const int most = std::min(group_waves(a.dt), kGroupLds / std::max(a.part_heads * (a.dt + 2) * 4, kGroupStage * 8));
   const int each = lists && 4 * all >= 3 * compute_units() ? 8 : 2 * all >= compute_units() ? 4 : 2;
