@@ -377,6 +377,16 @@ typedef struct jasperx_head_rows {
 int64_t jasperx_rotary(const jasperx_head_rows* q, const jasperx_head_rows* k, int32_t type, int64_t n, int64_t dim,
                        const void* positions, int32_t index_bytes, const float* cos, const float* sin,
                        int64_t table_rows, int64_t rot_dim, uint32_t flags, void* q_out, void* k_out, void* stream);
+/* The same with positions of several axes (time, height and width of an
+ * image's tokens): positions [axes][n], 1 to 4 axes; sections[a] pairs are
+ * turned by axis a's position, axis after axis, or with cyclic dealt to the
+ * axes in turn, each until it has its share. They are rot_dim / 2 in sum. Pair
+ * i reads column i of its axis's table row; a position outside the table makes
+ * its axis's pairs NaN. */
+int64_t jasperx_rotary_by_axes(const jasperx_head_rows* q, const jasperx_head_rows* k, int32_t type, int64_t n,
+                               int64_t dim, const void* positions, int32_t index_bytes, const int32_t* sections,
+                               int32_t axes, int32_t cyclic, const float* cos, const float* sin, int64_t table_rows,
+                               int64_t rot_dim, uint32_t flags, void* q_out, void* k_out, void* stream);
 /* The tokens of a step into the cache: q rotated to q_out, k rotated (as
  * above; rot_dim 0: not at all) and v to row slots[i] % page_size of page
  * slots[i] / page_size. The cache has q's type or e4m3 (values divided by
@@ -387,12 +397,71 @@ int64_t jasperx_append_tokens(const jasperx_head_rows* q, const jasperx_head_row
                               int32_t index_bytes, const float* cos, const float* sin, int64_t table_rows,
                               int64_t rot_dim, uint32_t flags, const jasperx_kv_pages* pages, void* q_out,
                               void* stream);
+/* The same with positions of several axes, as jasperx_rotary_by_axes. */
+int64_t jasperx_append_tokens_by_axes(const jasperx_head_rows* q, const jasperx_head_rows* k,
+                                      const jasperx_head_rows* v, int32_t type, int64_t n, const void* positions,
+                                      const void* slots, int32_t index_bytes, const int32_t* sections, int32_t axes,
+                                      int32_t cyclic, const float* cos, const float* sin, int64_t table_rows,
+                                      int64_t rot_dim, uint32_t flags, const jasperx_kv_pages* pages, void* q_out,
+                                      void* stream);
 /* Pages src[i] to dst[i], K and V of every layer. With tables (NULL: none),
  * each of table_entries entries that equals src[i] becomes dst[i]. A page may
  * be the source of several copies (not with tables) and the destination of
  * one, not both. Pairs with an id outside the cache are skipped. */
 int64_t jasperx_copy_pages(const jasperx_kv_pages* pages, const int32_t* src, const int32_t* dst, int64_t n,
                            int32_t* tables, int64_t table_entries, void* stream);
+/* Which pages the sequences of a cache have, kept on the GPU so that a step
+ * that grows them can be captured in a graph. tables [sequences][width]: a
+ * sequence's pages in order, -1 behind them; lens [sequences]: its tokens; refs
+ * [pages]: how many sequences have a page; free_bits [(pages + 31) / 32]: bit p
+ * % 32 of word p / 32 is set where no sequence has page p. page_size: a power
+ * of two, 8 to 256; width * page_size below 2^31. At first: entries -1, lens
+ * and refs 0, all bits set. */
+typedef struct jasperx_page_table {
+  int32_t* tables;
+  int32_t* lens;
+  int32_t* refs;
+  uint32_t* free_bits;
+  int32_t sequences, width, pages, page_size;
+} jasperx_page_table;
+
+/* Room for counts[i] more tokens of sequences seqs[i], i < n: new pages, the
+ * lowest free ones, to the requests in order; a request that grows in a page
+ * which others have too first gets one for a copy of it (the last of them that
+ * grows keeps it). Written: for the tokens in order positions and slots (page *
+ * page_size + row) [n_tokens], 0 and -1 behind the last; starts [n + 1], where a
+ * request's tokens begin; the sequences' tables step_tables [n][width] and
+ * lengths step_lens [n]; the pages to copy before the tokens are stored, src and
+ * dst [n] (-1: none), as jasperx_copy_pages takes them. missing [1]: 0; or the
+ * pages that were missing, or -1 where a request cannot be: a sequence listed
+ * twice, a count below 0, a sequence past width entries, more than n_tokens
+ * tokens. Then nothing has changed, and the outputs are those of no new tokens.
+ * Ids outside [0, sequences) are left out (padding: -1). */
+int64_t jasperx_extend_tables(const jasperx_page_table* table, const int32_t* seqs, const int32_t* counts, int64_t n,
+                              int64_t n_tokens, int64_t width, int64_t* positions, int64_t* slots, int32_t* starts,
+                              int32_t* step_tables, int32_t* step_lens, int32_t* src, int32_t* dst, int32_t* missing,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+/* Scratch bytes of the call above. */
+int64_t jasperx_extend_workspace(int64_t n, int64_t pages);
+/* Sequences seqs[i] cut back to to[i] tokens (0: given up; longer than it is, or
+ * below 0: left as it is), pages that no sequence has any more freed. Of a
+ * sequence listed twice the first counts; ids outside are left out. */
+int64_t jasperx_truncate_tables(const jasperx_page_table* table, const int32_t* seqs, const int32_t* to, int64_t n,
+                                void* stream);
+/* Sequences into[i], empty until now, get the tokens of seqs[i], on the same
+ * pages. Pairs with an id outside, with an into that is not empty, that is
+ * listed before or that stands in the other list too are left out. */
+int64_t jasperx_fork_tables(const jasperx_page_table* table, const int32_t* seqs, const int32_t* into, int64_t n,
+                            void* stream);
+/* Neighbours in a batch that begin with the same pages: sequence b joins the one before it where
+ * both have at least max(1, least) tokens in the same whole pages. groups
+ * [batch + 1]: where the groups begin, batch behind the last; shared [batch]:
+ * the tokens in whole pages that all of a group share, 0 for one by itself. */
+int64_t jasperx_shared_prefixes(const int32_t* tables, int64_t table_stride, int64_t table_width, const int32_t* lens,
+                                int64_t batch, int64_t page_size, int64_t least, int32_t* groups, int32_t* shared,
+                                void* workspace, int64_t workspace_bytes, void* stream);
+/* Scratch bytes of the call above. */
+int64_t jasperx_prefixes_workspace(int64_t batch);
 /* Attention of one new token per sequence: with t over the last `window` (0:
  * all) of the lens[b] tokens of sequence b, s_t = scale * <q, k_t>, out =
  * sum softmax(s)_t v_t and lse = log sum exp s_t (NULL: not written); no

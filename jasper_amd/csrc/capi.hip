@@ -24,6 +24,7 @@
 #include "directional_api.hpp"
 #include "graph.hpp"
 #include "kvcache.hpp"
+#include "pagetable.hpp"
 #include "rabitq.hpp"
 #include "search.hpp"
 
@@ -933,6 +934,17 @@ RotaryArgs rotary_args(const jasperx_head_rows* q, const jasperx_head_rows* k, i
   return a;
 }
 
+void set_axes(RotaryArgs& a, const int32_t* sections, int32_t axes, bool cyclic) {
+  if (axes < 1 || axes > 4 || !sections) throw std::invalid_argument("axes must be 1 to 4, with the pairs of each");
+  int64_t pairs = 0;
+  for (int i = 0; i < axes; ++i) {
+    if (sections[i] < 0) throw std::invalid_argument("the axes' pairs must be at least 0");
+    pairs += sections[i];
+  }
+  if (pairs != a.half) throw std::invalid_argument("the axes' pairs must be rot_dim / 2 in sum");
+  if (pairs) a.axes = rotary_axes(sections, axes, cyclic);
+}
+
 AttendArgs attend_args(const jasperx_head_rows* q, int32_t type, int64_t batch, const KvPages& pages,
                        const int32_t* tables, int64_t table_stride, int64_t table_width, const int32_t* lens,
                        double scale, void* out, float* lse, void* workspace, int64_t workspace_bytes) {
@@ -955,17 +967,63 @@ AttendArgs attend_args(const jasperx_head_rows* q, int32_t type, int64_t batch, 
 
 }  // namespace
 
+namespace {
+
+int64_t rotary_call(const jasperx_head_rows* q, const jasperx_head_rows* k, int32_t type, int64_t n, int64_t dim,
+                    const void* positions, int32_t index_bytes, const int32_t* sections, int32_t axes, bool cyclic,
+                    const float* cos, const float* sin, int64_t table_rows, int64_t rot_dim, uint32_t flags, void* q_out,
+                    void* k_out, void* stream) {
+  RotaryArgs a = rotary_args(q, k, type, n, dim, positions, index_bytes, cos, sin, table_rows, rot_dim, flags);
+  if (axes) set_axes(a, sections, axes, cyclic);
+  if (n && ((a.q.heads && (!a.q.p || !q_out)) || (a.k.heads && (!a.k.p || !k_out))))
+    throw std::invalid_argument("null rows");
+  if (((uintptr_t)q_out & 15u) || ((uintptr_t)k_out & 15u)) throw std::invalid_argument("outputs must be 16-byte aligned");
+  rotary(a, q_out, k_out, (hipStream_t)stream);
+  return 0;
+}
+
+int64_t append_call(const jasperx_head_rows* q, const jasperx_head_rows* k, const jasperx_head_rows* v, int32_t type,
+                    int64_t n, const void* positions, const void* slots, int32_t index_bytes, const int32_t* sections,
+                    int32_t axes, bool cyclic, const float* cos, const float* sin, int64_t table_rows, int64_t rot_dim,
+                    uint32_t flags, const jasperx_kv_pages* pages, void* q_out, void* stream) {
+  const KvPages p = kv_pages(pages);
+  RotaryArgs a = rotary_args(q, k, type, n, p.dim, positions, index_bytes, cos, sin, table_rows, rot_dim, flags);
+  if (axes) set_axes(a, sections, axes, cyclic);
+  const HeadRows vr = head_rows(v);
+  if (a.k.heads != p.heads || vr.heads != p.heads) throw std::invalid_argument("keys and values must be of the cache's heads");
+  if (p.type != kE4M3 && p.type != type) throw std::invalid_argument("pages must be of the keys' type or e4m3");
+  if (p.layers != 1) throw std::invalid_argument("pages must be of one layer");
+  if (n && (!a.k.p || !vr.p || !slots || (a.q.heads && (!a.q.p || !q_out)))) throw std::invalid_argument("null argument");
+  if ((uintptr_t)q_out & 15u) throw std::invalid_argument("outputs must be 16-byte aligned");
+  append_tokens(a, vr, slots, index_bytes == 8, p, q_out, (hipStream_t)stream);
+  return 0;
+}
+
+int32_t some_axes(int32_t axes) {
+  if (axes < 1) throw std::invalid_argument("axes must be 1 to 4, with the pairs of each");
+  return axes;
+}
+
+}  // namespace
+
 extern "C" int64_t jasperx_rotary(const jasperx_head_rows* q, const jasperx_head_rows* k, int32_t type, int64_t n,
                                   int64_t dim, const void* positions, int32_t index_bytes, const float* cos,
                                   const float* sin, int64_t table_rows, int64_t rot_dim, uint32_t flags, void* q_out,
                                   void* k_out, void* stream) {
   return guarded([&]() -> int64_t {
-    const RotaryArgs a = rotary_args(q, k, type, n, dim, positions, index_bytes, cos, sin, table_rows, rot_dim, flags);
-    if (n && ((a.q.heads && (!a.q.p || !q_out)) || (a.k.heads && (!a.k.p || !k_out))))
-      throw std::invalid_argument("null rows");
-    if (((uintptr_t)q_out & 15u) || ((uintptr_t)k_out & 15u)) throw std::invalid_argument("outputs must be 16-byte aligned");
-    rotary(a, q_out, k_out, (hipStream_t)stream);
-    return 0;
+    return rotary_call(q, k, type, n, dim, positions, index_bytes, nullptr, 0, false, cos, sin, table_rows, rot_dim, flags,
+                       q_out, k_out, stream);
+  });
+}
+
+extern "C" int64_t jasperx_rotary_by_axes(const jasperx_head_rows* q, const jasperx_head_rows* k, int32_t type, int64_t n,
+                                          int64_t dim, const void* positions, int32_t index_bytes,
+                                          const int32_t* sections, int32_t axes, int32_t cyclic, const float* cos,
+                                          const float* sin, int64_t table_rows, int64_t rot_dim, uint32_t flags,
+                                          void* q_out, void* k_out, void* stream) {
+  return guarded([&]() -> int64_t {
+    return rotary_call(q, k, type, n, dim, positions, index_bytes, sections, some_axes(axes), cyclic, cos, sin, table_rows,
+                       rot_dim, flags, q_out, k_out, stream);
   });
 }
 
@@ -975,16 +1033,21 @@ extern "C" int64_t jasperx_append_tokens(const jasperx_head_rows* q, const jaspe
                                          int64_t table_rows, int64_t rot_dim, uint32_t flags,
                                          const jasperx_kv_pages* pages, void* q_out, void* stream) {
   return guarded([&]() -> int64_t {
-    const KvPages p = kv_pages(pages);
-    const RotaryArgs a = rotary_args(q, k, type, n, p.dim, positions, index_bytes, cos, sin, table_rows, rot_dim, flags);
-    const HeadRows vr = head_rows(v);
-    if (a.k.heads != p.heads || vr.heads != p.heads) throw std::invalid_argument("keys and values must be of the cache's heads");
-    if (p.type != kE4M3 && p.type != type) throw std::invalid_argument("pages must be of the keys' type or e4m3");
-    if (p.layers != 1) throw std::invalid_argument("pages must be of one layer");
-    if (n && (!a.k.p || !vr.p || !slots || (a.q.heads && (!a.q.p || !q_out)))) throw std::invalid_argument("null argument");
-    if ((uintptr_t)q_out & 15u) throw std::invalid_argument("outputs must be 16-byte aligned");
-    append_tokens(a, vr, slots, index_bytes == 8, p, q_out, (hipStream_t)stream);
-    return 0;
+    return append_call(q, k, v, type, n, positions, slots, index_bytes, nullptr, 0, false, cos, sin, table_rows, rot_dim,
+                       flags, pages, q_out, stream);
+  });
+}
+
+extern "C" int64_t jasperx_append_tokens_by_axes(const jasperx_head_rows* q, const jasperx_head_rows* k,
+                                                 const jasperx_head_rows* v, int32_t type, int64_t n,
+                                                 const void* positions, const void* slots, int32_t index_bytes,
+                                                 const int32_t* sections, int32_t axes, int32_t cyclic,
+                                                 const float* cos, const float* sin, int64_t table_rows,
+                                                 int64_t rot_dim, uint32_t flags, const jasperx_kv_pages* pages,
+                                                 void* q_out, void* stream) {
+  return guarded([&]() -> int64_t {
+    return append_call(q, k, v, type, n, positions, slots, index_bytes, sections, some_axes(axes), cyclic, cos, sin,
+                       table_rows, rot_dim, flags, pages, q_out, stream);
   });
 }
 
@@ -1047,6 +1110,96 @@ extern "C" int64_t jasperx_attention_workspace(int64_t batch, int64_t q_heads, c
       throw std::invalid_argument("bad sizes");
     if (lists && lists != q_heads && lists != p.heads) throw std::invalid_argument("lists must be 0, the query heads or the cache's heads");
     return attend_workspace(batch, q_heads, p, max_tokens, lists);
+  });
+}
+
+namespace {
+
+int32_t page_shift(int64_t page_size) {
+  if (page_size < 8 || page_size > 256 || (page_size & (page_size - 1)))
+    throw std::invalid_argument("page_size must be a power of two from 8 to 256");
+  return __builtin_ctz((unsigned)page_size);
+}
+
+PageState page_state(const jasperx_page_table* t, const int32_t* seqs, const int32_t* other, int64_t n) {
+  if (!t) throw std::invalid_argument("null page table");
+  PageState r;
+  r.page_shift = page_shift(t->page_size);
+  if (t->sequences < 0 || t->width < 0 || t->pages < 0 || ((int64_t)t->width << r.page_shift) > 0x7FFFFFFF)
+    throw std::invalid_argument("sequences, width and pages must be at least 0, and width * page_size below 2^31");
+  if ((t->sequences && !t->lens) || (t->sequences && t->width && !t->tables) || (t->pages && (!t->refs || !t->free_bits)) ||
+      (n > 0 && (!seqs || !other)))
+    throw std::invalid_argument("null argument");
+  r.tables = t->tables, r.lens = t->lens, r.refs = t->refs, r.free = t->free_bits;
+  r.sequences = t->sequences, r.width = t->width, r.pages = t->pages;
+  return r;
+}
+
+}  // namespace
+
+extern "C" int64_t jasperx_extend_tables(const jasperx_page_table* table, const int32_t* seqs, const int32_t* counts,
+                                         int64_t n, int64_t n_tokens, int64_t width, int64_t* positions, int64_t* slots,
+                                         int32_t* starts, int32_t* step_tables, int32_t* step_lens, int32_t* src,
+                                         int32_t* dst, int32_t* missing, void* workspace, int64_t workspace_bytes,
+                                         void* stream) {
+  return guarded([&]() -> int64_t {
+    const PageState st = page_state(table, seqs, counts, n);
+    if (n_tokens < 0 || width < 0 || (width << st.page_shift) > 0x7FFFFFFF || width > 0x7FFFFFFF)
+      throw std::invalid_argument("n_tokens and width must be at least 0, and width * page_size below 2^31");
+    if (!starts || !missing || (n > 0 && (!step_lens || !src || !dst || (width && !step_tables))) ||
+        (n_tokens && (!positions || !slots)))
+      throw std::invalid_argument("null argument");
+    ExtendArgs a;
+    a.seqs = seqs, a.counts = counts, a.n = n, a.n_tokens = n_tokens, a.width = (int32_t)width;
+    a.positions = positions, a.slots = slots, a.starts = starts, a.step_tables = step_tables, a.step_lens = step_lens;
+    a.src = src, a.dst = dst, a.missing = missing, a.workspace = workspace, a.workspace_bytes = workspace_bytes;
+    extend_tables(st, a, (hipStream_t)stream);
+    return 0;
+  });
+}
+
+extern "C" int64_t jasperx_extend_workspace(int64_t n, int64_t pages) {
+  return guarded([&]() -> int64_t {
+    if (n < 0 || n > 65535 || pages < 0 || pages > 0x7FFFFFFF) throw std::invalid_argument("requests must be 0 to 65535, pages at least 0");
+    return extend_workspace(n, pages);
+  });
+}
+
+extern "C" int64_t jasperx_truncate_tables(const jasperx_page_table* table, const int32_t* seqs, const int32_t* to,
+                                           int64_t n, void* stream) {
+  return guarded([&]() -> int64_t {
+    truncate_tables(page_state(table, seqs, to, n), seqs, to, n, (hipStream_t)stream);
+    return 0;
+  });
+}
+
+extern "C" int64_t jasperx_fork_tables(const jasperx_page_table* table, const int32_t* seqs, const int32_t* into,
+                                       int64_t n, void* stream) {
+  return guarded([&]() -> int64_t {
+    fork_tables(page_state(table, seqs, into, n), seqs, into, n, (hipStream_t)stream);
+    return 0;
+  });
+}
+
+extern "C" int64_t jasperx_shared_prefixes(const int32_t* tables, int64_t table_stride, int64_t table_width,
+                                           const int32_t* lens, int64_t batch, int64_t page_size, int64_t least,
+                                           int32_t* groups, int32_t* shared, void* workspace, int64_t workspace_bytes,
+                                           void* stream) {
+  return guarded([&]() -> int64_t {
+    const int32_t shift = page_shift(page_size);
+    if (table_width < 0 || table_width > (0x7FFFFFFF >> shift)) throw std::invalid_argument("width * page_size must be below 2^31");
+    if (least < 0) throw std::invalid_argument("least must be at least 0");
+    if (!groups || (batch > 0 && (!lens || !shared || (table_width && !tables)))) throw std::invalid_argument("null argument");
+    shared_prefixes(tables, table_stride, table_width, lens, batch, shift, least, groups, shared, workspace,
+                    workspace_bytes, (hipStream_t)stream);
+    return 0;
+  });
+}
+
+extern "C" int64_t jasperx_prefixes_workspace(int64_t batch) {
+  return guarded([&]() -> int64_t {
+    if (batch < 0 || batch > 65535) throw std::invalid_argument("batch must be 0 to 65535");
+    return prefixes_workspace(batch);
   });
 }
 

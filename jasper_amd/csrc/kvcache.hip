@@ -27,6 +27,7 @@ struct TokenParams {
   char *q_out, *k_out;
   KvPages pages;
   int64_t rows;  // of the cache: pages * page size
+  RotaryAxes axes;
 };
 
 __device__ __forceinline__ int64_t index_at(const void* p, bool wide, int64_t i) {
@@ -52,6 +53,17 @@ __device__ __forceinline__ bool quotient_fits(float d) {
   return __builtin_fabsf(d) > 0x1p-80f && __builtin_fabsf(d) < 0x1p80f;
 }
 
+// The axis of pair i. x % count without a division: count is 1 to 4 and x below
+// 1024, so (x * ceil(2^16 / count)) >> 16 is x / count.
+__device__ __forceinline__ int axis_of(const RotaryAxes& a, int i) {
+  int begin = 0, count = a.count[0], list = a.list[0];
+#pragma unroll
+  for (int r = 1; r < 4; ++r)
+    if (i >= a.begin[r]) begin = a.begin[r], count = a.count[r], list = a.list[r];
+  const int x = i - begin, inverse = count == 1 ? 65536 : count == 2 ? 32768 : count == 3 ? 21846 : 16384;
+  return list >> 2 * (x - (x * inverse >> 16) * count) & 3;
+}
+
 // A thread has one chunk of 2 * P values of a head (threadIdx.x) and walks
 // the heads of its token (threadIdx.y on) with the chunk's P cosines and
 // sines in registers. In the half layout the chunk is P values of each half,
@@ -60,7 +72,10 @@ __device__ __forceinline__ bool quotient_fits(float d) {
 // same bits as the formula in fp32 operations. Bound by memory: 8192 tokens of
 // 32 + 8 heads of 128 bf16 values 38 us (4.4 TB/s read and written; a large copy
 // 4.7), 6007 of 32 + 2 x 8 into e4m3 pages 32 us (4.3); one token 3.6 us.
-template <typename T, typename CT, int P, bool APPEND>
+//
+// AXES: a pair's position is its axis's. Chunks of one axis load their angles
+// as before, those that several axes have a part of pair by pair.
+template <typename T, typename CT, int P, bool APPEND, bool AXES>
 __global__ void token_kernel(TokenParams a) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
   if (i >= a.n) return;
@@ -70,7 +85,34 @@ __global__ void token_kernel(TokenParams a) {
   const int at = split ? c * P : c * 2 * P;
   const int to = split ? a.half + at : at + P;
   float co[P], si[P];
-  if (turn) {
+  if (AXES && turn) {
+    int64_t at_axis[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      at_axis[x] = x < a.axes.axes ? index_at(a.positions, a.pos64, x * a.n + i) : 0;
+      if (at_axis[x] < 0 || at_axis[x] >= a.table_rows) at_axis[x] = -1;
+    }
+    const auto position = [&](int x) { return x == 0 ? at_axis[0] : x == 1 ? at_axis[1] : x == 2 ? at_axis[2] : at_axis[3]; };
+    int axis[P];
+    bool same = true;
+#pragma unroll
+    for (int e = 0; e < P; ++e) axis[e] = axis_of(a.axes, c * P + e), same = same && axis[e] == axis[0];
+    if (same) {
+      const int64_t pos = position(axis[0]), row = max(pos, (int64_t)0) * a.half + c * P;
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        co[e] = pos >= 0 ? a.cos[row + e] : __builtin_nanf("");
+        si[e] = pos >= 0 ? (a.back ? -a.sin[row + e] : a.sin[row + e]) : __builtin_nanf("");
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        const int64_t pos = position(axis[e]), row = max(pos, (int64_t)0) * a.half + c * P + e;
+        co[e] = pos >= 0 ? a.cos[row] : __builtin_nanf("");
+        si[e] = pos >= 0 ? (a.back ? -a.sin[row] : a.sin[row]) : __builtin_nanf("");
+      }
+    }
+  } else if (turn) {
     const int64_t pos = index_at(a.positions, a.pos64, i);
     const bool known = pos >= 0 && pos < a.table_rows;
     const int64_t row = known ? pos * a.half + c * P : 0;
@@ -151,8 +193,13 @@ void launch_token(const TokenParams& p, int P, hipStream_t s) {
   const int64_t blocks = (p.n + block.z - 1) / block.z;
   if (blocks > 0x7FFFFFFF) throw std::invalid_argument("too many tokens (too large)");
   grid.x = (unsigned)blocks;
-  auto kernel = P == 8 ? token_kernel<T, CT, 8, APPEND> : P == 4 ? token_kernel<T, CT, 4, APPEND>
-                                                                 : token_kernel<T, CT, 1, APPEND>;
+  auto kernel = P == 8   ? token_kernel<T, CT, 8, APPEND, false>
+                : P == 4 ? token_kernel<T, CT, 4, APPEND, false>
+                         : token_kernel<T, CT, 1, APPEND, false>;
+  if (p.axes.axes)
+    kernel = P == 8   ? token_kernel<T, CT, 8, APPEND, true>
+             : P == 4 ? token_kernel<T, CT, 4, APPEND, true>
+                      : token_kernel<T, CT, 1, APPEND, true>;
   kernel<<<grid, block, 0, s>>>(p);
   hip_check(hipGetLastError(), "rotary");
 }
@@ -167,7 +214,7 @@ TokenParams token_params(const RotaryArgs& a) {
   p.q = (const char*)a.q.p, p.q_stride = a.q.stride, p.q_head = a.q.head_stride, p.q_heads = a.q.heads;
   p.k = (const char*)a.k.p, p.k_stride = a.k.stride, p.k_head = a.k.head_stride, p.k_heads = a.k.heads;
   p.positions = a.positions, p.pos64 = a.pos64, p.cos = a.cos, p.sin = a.sin, p.n = a.n, p.table_rows = a.table_rows;
-  p.dim = a.dim, p.half = a.half, p.interleaved = a.interleaved, p.back = a.back;
+  p.dim = a.dim, p.half = a.half, p.interleaved = a.interleaved, p.back = a.back, p.axes = a.axes;
   return p;
 }
 
@@ -185,6 +232,26 @@ int chunk_of(const TokenParams& p, int type) {
 }
 
 }  // namespace
+
+RotaryAxes rotary_axes(const int32_t* sections, int32_t axes, bool cyclic) {
+  RotaryAxes r;
+  r.axes = axes;
+  int32_t left[4] = {0, 0, 0, 0};
+  std::copy(sections, sections + axes, left);
+  int runs = 0;
+  for (int32_t at = 0;; ++runs) {
+    // a run: the next axis with pairs, or in turn all that have some, as many rounds as the least of them has
+    int32_t list = 0, count = 0, rounds = 0;
+    for (int a = 0; a < axes && (cyclic || !count); ++a)
+      if (left[a]) list |= a << 2 * count++, rounds = rounds ? std::min(rounds, left[a]) : left[a];
+    if (!count) break;
+    for (int k = 0; k < count; ++k) left[list >> 2 * k & 3] -= rounds;
+    r.begin[runs] = at, r.count[runs] = count, r.list[runs] = list;
+    at += count * rounds;
+  }
+  for (; runs < 4; ++runs) r.begin[runs] = 0x7FFFFFFF;
+  return r;
+}
 
 void rotary(const RotaryArgs& a, void* q_out, void* k_out, hipStream_t s) {
   TokenParams p = token_params(a);

@@ -36,6 +36,17 @@ struct HeadRows {
   int32_t heads = 0;
 };
 
+// Positions of several axes: which axis a pair of values is turned by. The
+// pairs come in up to four runs; pair i of run r, which begins at begin[r], has
+// the axis in place (i - begin[r]) % count[r] of list[r], two bits each. One
+// axis after the other is runs of one axis, axes in turn one run of all and,
+// where some have fewer pairs, further ones of those that are left.
+struct RotaryAxes {
+  int32_t axes = 0;  // 0: one position for all pairs
+  int32_t begin[4] = {0, 0, 0, 0}, count[4] = {1, 1, 1, 1}, list[4] = {0, 0, 0, 0};
+};
+RotaryAxes rotary_axes(const int32_t* sections, int32_t axes, bool cyclic);
+
 // q and k (heads 0: absent) with the first 2 * half values of every head
 // turned by the angles of their positions' table rows, to contiguous q_out,
 // k_out. back: by the opposite angles (the gradient). Rows whose position is
@@ -48,6 +59,7 @@ struct RotaryArgs {
   const float* sin = nullptr;
   int64_t n = 0, table_rows = 0;
   int32_t dim = 0, half = 0, type = kF16;
+  RotaryAxes axes;  // with axes: positions are [axes][n]
 };
 void rotary(const RotaryArgs& a, void* q_out, void* k_out, hipStream_t s);
 

@@ -136,9 +136,41 @@ void mark_written(const Tensor& t) {
 
 // ---- rotary positions ----
 
+// Positions of several axes: the pairs of each; none: one position for all.
+struct Axes {
+  std::vector<int32_t> sections;
+  bool cyclic = false;
+  int64_t count() const { return (int64_t)sections.size(); }
+};
+
+Axes axes_of(const std::optional<std::vector<int64_t>>& sections, bool cyclic, int64_t rot) {
+  Axes a;
+  a.cyclic = cyclic;
+  if (!sections) {
+    TORCH_CHECK_VALUE(!cyclic, "cyclic needs sections");
+    return a;
+  }
+  TORCH_CHECK_VALUE(!sections->empty() && sections->size() <= 4, "sections must be of 1 to 4 axes, got ", sections->size());
+  int64_t pairs = 0;
+  for (const int64_t s : *sections) {
+    TORCH_CHECK_VALUE(s >= 0 && s <= 1024, "a section must be of 0 to 1024 pairs, got ", s);
+    a.sections.push_back((int32_t)s), pairs += s;
+  }
+  TORCH_CHECK_VALUE(2 * pairs == rot, "sections must be ", rot / 2, " pairs in sum (half of what the tables rotate), got ", pairs);
+  return a;
+}
+
+// The sizes of positions for rows with these leading sizes.
+std::vector<int64_t> position_sizes(const Axes& axes, at::IntArrayRef leading) {
+  std::vector<int64_t> r;
+  if (axes.count()) r.push_back(axes.count());
+  r.insert(r.end(), leading.begin(), leading.end());
+  return r;
+}
+
 // q and k turned; either may be undefined. The arguments are checked.
 std::pair<Tensor, Tensor> rotate(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& cos,
-                                 const Tensor& sin, bool interleaved, bool back) {
+                                 const Tensor& sin, bool interleaved, bool back, const Axes& axes) {
   const Tensor& first = q.defined() ? q : k;
   const c10::DeviceGuard guard(first.device());
   const Table table = table_of(cos, sin, first);
@@ -146,13 +178,21 @@ std::pair<Tensor, Tensor> rotate(const Tensor& q, const Tensor& k, const Tensor&
   jasperx_head_rows q_rows{}, k_rows{};
   if (q.defined()) q_out = at::empty(q.sizes(), q.options()), q_rows = rows_of(q, q_held);
   if (k.defined()) k_out = at::empty(k.sizes(), k.options()), k_rows = rows_of(k, k_held);
-  const int64_t n = positions.numel();
-  if (n)
-    check(jasperx_rotary(&q_rows, &k_rows, type_of(first), n, first.size(-1), positions.data_ptr(),
-                         (int32_t)positions.element_size(), table.cos, table.sin, table.rows, table.rot,
-                         (interleaved ? JASPERX_ROTARY_INTERLEAVED : 0u) | (back ? JASPERX_ROTARY_INVERSE : 0u),
-                         q.defined() ? q_out.data_ptr() : nullptr, k.defined() ? k_out.data_ptr() : nullptr,
-                         current_stream(first.get_device())));
+  const int64_t n = positions.numel() / std::max<int64_t>(1, axes.count());
+  if (n) {
+    const uint32_t flags = (interleaved ? JASPERX_ROTARY_INTERLEAVED : 0u) | (back ? JASPERX_ROTARY_INVERSE : 0u);
+    void* const q_to = q.defined() ? q_out.data_ptr() : nullptr;
+    void* const k_to = k.defined() ? k_out.data_ptr() : nullptr;
+    const int32_t type = type_of(first), bytes = (int32_t)positions.element_size();
+    void* const stream = current_stream(first.get_device());
+    if (axes.count())
+      check(jasperx_rotary_by_axes(&q_rows, &k_rows, type, n, first.size(-1), positions.data_ptr(), bytes,
+                                   axes.sections.data(), (int32_t)axes.count(), axes.cyclic, table.cos, table.sin,
+                                   table.rows, table.rot, flags, q_to, k_to, stream));
+    else
+      check(jasperx_rotary(&q_rows, &k_rows, type, n, first.size(-1), positions.data_ptr(), bytes, table.cos, table.sin,
+                           table.rows, table.rot, flags, q_to, k_to, stream));
+  }
   return {q_out, k_out};
 }
 
@@ -161,14 +201,18 @@ std::pair<Tensor, Tensor> rotate(const Tensor& q, const Tensor& k, const Tensor&
 struct Rotary : torch::autograd::Function<Rotary> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const OptTensor& q,
                                                 const OptTensor& k, const Tensor& positions, const Tensor& cos,
-                                                const Tensor& sin, bool interleaved, bool back) {
+                                                const Tensor& sin, bool interleaved, bool back, Axes axes) {
     ctx->save_for_backward({positions, cos, sin});
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["back"] = back;
     ctx->saved_data["q"] = q.has_value();
     ctx->saved_data["k"] = k.has_value();
+    if (axes.count()) {
+      ctx->saved_data["sections"] = std::vector<int64_t>(axes.sections.begin(), axes.sections.end());
+      ctx->saved_data["cyclic"] = axes.cyclic;
+    }
     ctx->set_materialize_grads(false);
-    const auto [q_out, k_out] = rotate(q.value_or(Tensor()), k.value_or(Tensor()), positions, cos, sin, interleaved, back);
+    const auto [q_out, k_out] = rotate(q.value_or(Tensor()), k.value_or(Tensor()), positions, cos, sin, interleaved, back, axes);
     torch::autograd::variable_list out;
     if (q) out.push_back(q_out);
     if (k) out.push_back(k_out);
@@ -182,47 +226,55 @@ struct Rotary : torch::autograd::Function<Rotary> {
     Tensor gq, gk;
     if (has_q && ctx->needs_input_grad(0)) gq = grads[0];
     if (has_k && ctx->needs_input_grad(at_k)) gk = grads[at_k];
-    torch::autograd::variable_list out(7);
+    torch::autograd::variable_list out(8);
     if (!gq.defined() && !gk.defined()) return out;
     const auto saved = ctx->get_saved_variables();
     const bool interleaved = ctx->saved_data["interleaved"].toBool(), back = ctx->saved_data["back"].toBool();
-    std::tie(out[0], out[1]) = turn(gq, gk, saved[0], saved[1], saved[2], interleaved, !back);
+    Axes axes;
+    const auto sections = ctx->saved_data.find("sections");
+    if (sections != ctx->saved_data.end()) {
+      for (const int64_t s : sections->second.toIntVector()) axes.sections.push_back((int32_t)s);
+      axes.cyclic = ctx->saved_data["cyclic"].toBool();
+    }
+    std::tie(out[0], out[1]) = turn(gq, gk, saved[0], saved[1], saved[2], interleaved, !back, axes);
     return out;
   }
 
   // differentiable where something asks for it; the tangents are turned like the rows
   static std::pair<Tensor, Tensor> turn(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& cos,
-                                        const Tensor& sin, bool interleaved, bool back) {
+                                        const Tensor& sin, bool interleaved, bool back, const Axes& axes) {
     if (has_tangent(q) || has_tangent(k)) {
       const auto value = [](const Tensor& t) { return t.defined() ? t._fw_primal(0) : t; };
       const auto tangent = [](const Tensor& t) { return t.defined() ? t._fw_grad(0) : t; };
-      const auto out = turn(value(q), value(k), positions, cos, sin, interleaved, back);
-      const auto moved = turn(tangent(q), tangent(k), positions, cos, sin, interleaved, back);
+      const auto out = turn(value(q), value(k), positions, cos, sin, interleaved, back, axes);
+      const auto moved = turn(tangent(q), tangent(k), positions, cos, sin, interleaved, back, axes);
       if (moved.first.defined()) out.first._set_fw_grad(moved.first, 0, false);
       if (moved.second.defined()) out.second._set_fw_grad(moved.second, 0, false);
       return out;
     }
     if (!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k)))
-      return rotate(q, k, positions, cos, sin, interleaved, back);
+      return rotate(q, k, positions, cos, sin, interleaved, back, axes);
     const auto given = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
-    const auto out = Rotary::apply(given(q), given(k), positions, cos, sin, interleaved, back);
+    const auto out = Rotary::apply(given(q), given(k), positions, cos, sin, interleaved, back, axes);
     return {q.defined() ? out[0] : Tensor(), k.defined() ? out[q.defined() ? 1 : 0] : Tensor()};
   }
 };
 
 py::tuple rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, const OptTensor& cos,
-                 const OptTensor& sin, bool interleaved) {
+                 const OptTensor& sin, bool interleaved, const std::optional<std::vector<int64_t>>& sections, bool cyclic) {
   TORCH_CHECK_VALUE(is_row_type(q), "q must be float16 or bfloat16, got ", q.dtype());
   TORCH_CHECK_VALUE(q.is_cuda(), "q must be a CUDA tensor");
   TORCH_CHECK_VALUE(q.dim() >= 2 && q.size(-1) % 2 == 0, "q must be [..., heads, dim] with an even dim");
   if (k) check_alike("k", *k, q);
   const Tensor at = indexes("positions", positions, q);
-  TORCH_CHECK_VALUE(at.sizes() == q.sizes().slice(0, q.dim() - 2), "positions must be ",
-                    q.sizes().slice(0, q.dim() - 2), ", got ", at.sizes());
   TORCH_CHECK_VALUE(cos && sin, "cos and sin are needed");
   TORCH_CHECK_VALUE(!asks_grad(cos, sin), "rotary has no gradient for cos and sin: detach them");
-  TORCH_CHECK_VALUE(table_of(cos, sin, q).rot <= q.size(-1), "the tables rotate more values than a head has");
-  const auto [q_out, k_out] = Rotary::turn(q, k ? *k : Tensor(), at, *cos, *sin, interleaved, false);
+  const int64_t rot = table_of(cos, sin, q).rot;
+  TORCH_CHECK_VALUE(rot <= q.size(-1), "the tables rotate more values than a head has");
+  const Axes axes = axes_of(sections, cyclic, rot);
+  const auto sizes = position_sizes(axes, q.sizes().slice(0, q.dim() - 2));
+  TORCH_CHECK_VALUE(at.sizes() == at::IntArrayRef(sizes), "positions must be ", at::IntArrayRef(sizes), ", got ", at.sizes());
+  const auto [q_out, k_out] = Rotary::turn(q, k ? *k : Tensor(), at, *cos, *sin, interleaved, false, axes);
   return py::make_tuple(q_out, k ? py::cast(k_out) : py::none());
 }
 
@@ -230,7 +282,8 @@ py::tuple rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, c
 
 OptTensor append_tokens(const OptTensor& q, const Tensor& k, const Tensor& v, const OptTensor& positions,
                         const Tensor& slots, const OptTensor& cos, const OptTensor& sin, const Tensor& k_pages,
-                        const Tensor& v_pages, bool interleaved, const OptTensor& k_scale, const OptTensor& v_scale) {
+                        const Tensor& v_pages, bool interleaved, const OptTensor& k_scale, const OptTensor& v_scale,
+                        const std::optional<std::vector<int64_t>>& sections, bool cyclic) {
   const jasperx_kv_pages pages = pages_of(k_pages, v_pages, k_scale, v_scale, false);
   TORCH_CHECK_VALUE(is_row_type(k) && (pages.type == 2 || pages.type == type_of(k)),
                     "k must be float16 or bfloat16 and the pages of its type or float8_e4m3fn, got ", k.dtype(), " and ",
@@ -247,10 +300,12 @@ OptTensor append_tokens(const OptTensor& q, const Tensor& k, const Tensor& v, co
   TORCH_CHECK_VALUE(rows.dim() == 1 && rows.size(0) == n, "slots must be [", n, "]");
   const Table table = table_of(cos, sin, k);
   TORCH_CHECK_VALUE(table.rot <= pages.dim, "the tables rotate more values than a head has");
+  const Axes axes = axes_of(sections, cyclic, table.rot);
   if (table.rot) {
     TORCH_CHECK_VALUE(positions, "positions are needed with cos and sin");
     at = indexes("positions", *positions, k);
-    TORCH_CHECK_VALUE(at.dim() == 1 && at.size(0) == n, "positions must be [", n, "]");
+    const auto sizes = position_sizes(axes, {n});
+    TORCH_CHECK_VALUE(at.sizes() == at::IntArrayRef(sizes), "positions must be ", at::IntArrayRef(sizes), ", got ", at.sizes());
     if (at.scalar_type() != rows.scalar_type()) at = at.to(at::kLong), rows = rows.to(at::kLong);
   }
   const c10::DeviceGuard guard(k.device());
@@ -260,10 +315,18 @@ OptTensor append_tokens(const OptTensor& q, const Tensor& k, const Tensor& v, co
   if (q) out = at::empty(q->sizes(), q->options()), q_rows = rows_of(*q, q_held);
   const jasperx_head_rows k_rows = rows_of(k, k_held), v_rows = rows_of(v, v_held);
   if (n) {
-    check(jasperx_append_tokens(&q_rows, &k_rows, &v_rows, type_of(k), n, table.rot ? at.data_ptr() : nullptr,
-                                rows.data_ptr(), (int32_t)rows.element_size(), table.cos, table.sin, table.rows,
-                                table.rot, interleaved ? JASPERX_ROTARY_INTERLEAVED : 0u, &pages,
-                                out ? out->data_ptr() : nullptr, current_stream(k.get_device())));
+    const void* const at_ptr = table.rot ? at.data_ptr() : nullptr;
+    const uint32_t flags = interleaved ? JASPERX_ROTARY_INTERLEAVED : 0u;
+    const int32_t bytes = (int32_t)rows.element_size();
+    void* const q_to = out ? out->data_ptr() : nullptr;
+    void* const stream = current_stream(k.get_device());
+    if (axes.count())
+      check(jasperx_append_tokens_by_axes(&q_rows, &k_rows, &v_rows, type_of(k), n, at_ptr, rows.data_ptr(), bytes,
+                                          axes.sections.data(), (int32_t)axes.count(), axes.cyclic, table.cos, table.sin,
+                                          table.rows, table.rot, flags, &pages, q_to, stream));
+    else
+      check(jasperx_append_tokens(&q_rows, &k_rows, &v_rows, type_of(k), n, at_ptr, rows.data_ptr(), bytes, table.cos,
+                                  table.sin, table.rows, table.rot, flags, &pages, q_to, stream));
     mark_written(k_pages), mark_written(v_pages);
   }
   return out;
@@ -289,6 +352,105 @@ void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& src,
     mark_written(k_pages), mark_written(v_pages);
     if (tables) mark_written(*tables);
   }
+}
+
+// ---- page tables on the GPU ----
+
+void check_ints(const char* name, const Tensor& t, int64_t dims, c10::Device device) {
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == dims && t.is_contiguous() && t.device() == device, name,
+                    " must be a contiguous ", dims, "D int32 tensor on ", device);
+}
+
+struct PageTable {
+  jasperx_page_table table{};
+  c10::Device device;
+
+  PageTable(const Tensor& tables, const Tensor& lens, const Tensor& refs, const Tensor& free, int64_t page_size)
+      : device(tables.device()) {
+    TORCH_CHECK_VALUE(tables.is_cuda(), "tables must be a CUDA tensor");
+    check_ints("tables", tables, 2, device), check_ints("lens", lens, 1, device);
+    check_ints("refs", refs, 1, device), check_ints("free", free, 1, device);
+    for (const Tensor* t : {&tables, &lens, &refs, &free})
+      for (const int64_t size : t->sizes()) TORCH_CHECK_VALUE(size <= INT32_MAX, "the page table is too large");
+    TORCH_CHECK_VALUE(lens.size(0) == tables.size(0), "lens must be [", tables.size(0), "], a length for each table");
+    TORCH_CHECK_VALUE(free.size(0) == (refs.size(0) + 31) / 32, "free must be [", (refs.size(0) + 31) / 32,
+                      "], a bit for each of ", refs.size(0), " pages");
+    TORCH_CHECK_VALUE(page_size > 0 && page_size <= 256, "page_size must be a power of two from 8 to 256, got ", page_size);
+    table.tables = (int32_t*)tables.data_ptr(), table.lens = (int32_t*)lens.data_ptr();
+    table.refs = (int32_t*)refs.data_ptr(), table.free_bits = (uint32_t*)free.data_ptr();
+    table.sequences = (int32_t)tables.size(0), table.width = (int32_t)tables.size(1);
+    table.pages = (int32_t)refs.size(0), table.page_size = (int32_t)page_size;
+  }
+
+  void pair(const char* name_a, const Tensor& a, const char* name_b, const Tensor& b) const {
+    check_ints(name_a, a, 1, device), check_ints(name_b, b, 1, device);
+    TORCH_CHECK_VALUE(a.size(0) == b.size(0), name_a, " and ", name_b, " must have the same length");
+  }
+};
+
+py::tuple extend_tables(const Tensor& tables, const Tensor& lens, const Tensor& refs, const Tensor& free,
+                        const Tensor& seqs, const Tensor& counts, int64_t page_size, int64_t n_tokens,
+                        std::optional<int64_t> width) {
+  const PageTable t(tables, lens, refs, free, page_size);
+  t.pair("seqs", seqs, "counts", counts);
+  const int64_t wide = width.value_or(tables.size(1)), n = seqs.size(0);
+  TORCH_CHECK_VALUE(n_tokens >= 0 && wide >= 0 && n_tokens <= INT32_MAX && wide <= INT32_MAX,
+                    "n_tokens and width must be at least 0 and below 2^31");
+  const c10::DeviceGuard guard(t.device);
+  const auto longs = tables.options().dtype(at::kLong);
+  const Tensor positions = at::empty({n_tokens}, longs), slots = at::empty({n_tokens}, longs);
+  const Tensor starts = at::empty({n + 1}, tables.options()), step = at::empty({n, wide}, tables.options());
+  const Tensor step_lens = at::empty({n}, tables.options()), src = at::empty({n}, tables.options());
+  const Tensor dst = at::empty({n}, tables.options()), missing = at::empty({1}, tables.options());
+  const int64_t size = jasperx_extend_workspace(n, refs.size(0));
+  check(size);
+  const Tensor scratch = at::empty({std::max<int64_t>(size, 16)}, tables.options().dtype(at::kByte));
+  const auto ints = [](const Tensor& x) { return (int32_t*)x.data_ptr(); };
+  check(jasperx_extend_tables(&t.table, ints(seqs), ints(counts), n, n_tokens, wide, (int64_t*)positions.data_ptr(),
+                              (int64_t*)slots.data_ptr(), ints(starts), ints(step), ints(step_lens), ints(src), ints(dst),
+                              ints(missing), scratch.data_ptr(), size, current_stream(tables.get_device())));
+  for (const Tensor* x : {&tables, &lens, &refs, &free}) mark_written(*x);
+  return py::make_tuple(positions, slots, starts, step, step_lens, src, dst, missing);
+}
+
+void truncate_tables(const Tensor& tables, const Tensor& lens, const Tensor& refs, const Tensor& free,
+                     const Tensor& seqs, const Tensor& to, int64_t page_size) {
+  const PageTable t(tables, lens, refs, free, page_size);
+  t.pair("seqs", seqs, "to", to);
+  const c10::DeviceGuard guard(t.device);
+  check(jasperx_truncate_tables(&t.table, (const int32_t*)seqs.data_ptr(), (const int32_t*)to.data_ptr(), seqs.size(0),
+                                current_stream(tables.get_device())));
+  for (const Tensor* x : {&tables, &lens, &refs, &free}) mark_written(*x);
+}
+
+void fork_tables(const Tensor& tables, const Tensor& lens, const Tensor& refs, const Tensor& free, const Tensor& seqs,
+                 const Tensor& into, int64_t page_size) {
+  const PageTable t(tables, lens, refs, free, page_size);
+  t.pair("seqs", seqs, "into", into);
+  const c10::DeviceGuard guard(t.device);
+  check(jasperx_fork_tables(&t.table, (const int32_t*)seqs.data_ptr(), (const int32_t*)into.data_ptr(), seqs.size(0),
+                            current_stream(tables.get_device())));
+  for (const Tensor* x : {&tables, &lens, &refs}) mark_written(*x);
+}
+
+py::tuple shared_prefixes(const Tensor& tables, const Tensor& lens, int64_t page_size, int64_t least) {
+  TORCH_CHECK_VALUE(tables.is_cuda() && tables.scalar_type() == at::kInt && tables.dim() == 2 &&
+                        (tables.size(1) <= 1 || tables.stride(1) == 1),
+                    "tables must be a CUDA int32 [batch, pages] tensor with contiguous rows");
+  TORCH_CHECK_VALUE(lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.size(0) == tables.size(0) &&
+                        lens.device() == tables.device(),
+                    "lens must be int32 [", tables.size(0), "] on ", tables.device());
+  const c10::DeviceGuard guard(tables.device());
+  const int64_t n = tables.size(0);
+  const Tensor held = lens.contiguous();
+  const Tensor groups = at::empty({n + 1}, held.options()), shared = at::empty({n}, held.options());
+  const int64_t size = jasperx_prefixes_workspace(n);
+  check(size);
+  const Tensor scratch = at::empty({size}, held.options().dtype(at::kByte));
+  check(jasperx_shared_prefixes((const int32_t*)tables.data_ptr(), tables.stride(0), tables.size(1),
+                                (const int32_t*)held.data_ptr(), n, page_size, least, (int32_t*)groups.data_ptr(),
+                                (int32_t*)shared.data_ptr(), scratch.data_ptr(), size, current_stream(tables.get_device())));
+  return py::make_tuple(groups, shared);
 }
 
 // ---- attention of one new token ----
@@ -401,6 +563,10 @@ PYBIND11_MODULE(_kv, m) {
   m.def("rotary", &rotary);
   m.def("append_tokens", &append_tokens);
   m.def("copy_pages", &copy_pages);
+  m.def("extend_tables", &extend_tables);
+  m.def("truncate_tables", &truncate_tables);
+  m.def("fork_tables", &fork_tables);
+  m.def("shared_prefixes", &shared_prefixes);
   m.def("decode_attention", &decode_attention);
   m.def("retrieved_attention", &retrieved_attention);
 }

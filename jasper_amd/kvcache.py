@@ -12,12 +12,17 @@ reference counterpart.
   decode_attention        one new token per sequence over its whole cache
   retrieved_attention     over the first, the last and the retrieved tokens
   PagedCache              pages, sequences, forks and compaction put together
+  extend_tables, truncate_tables, fork_tables
+                          which sequence has which pages, kept on the GPU
+  shared_prefixes         which sequences of a batch begin with the same pages
+  GpuPagedCache           a PagedCache of which every step can be captured
 
 Pages are [n_pages, kv_heads, page_size, dim] (with a leading layer dimension
 where said) in float16, bfloat16 or float8_e4m3fn, any strides that keep a
 row's dim values together and rows on 16 bytes. Calls run on the current
 stream of the tensors' device, synchronize nothing and may be captured in a
-graph (PagedCache's bookkeeping is on the host and is not captured). They take
+graph (PagedCache's bookkeeping is on the host and is not captured,
+GpuPagedCache's is). They take
 tensors with memory, and are not operators registered with torch:
 torch.compile runs them as they are, between the graphs before and after, and
 vmap, torch.func's grad and jvp, export and fake tensors end in an error.
@@ -28,6 +33,7 @@ from __future__ import annotations
 import importlib.machinery
 import importlib.util
 import math
+from collections.abc import Sequence
 
 import numpy as np
 import torch
@@ -106,7 +112,7 @@ def rotary_table(n_positions: int, rot_dim: int, base: float = 10000.0, scaling:
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
-           interleaved: bool = False):
+           interleaved: bool = False, sections: Sequence[int] | None = None, cyclic: bool = False):
     """(q, k) [..., heads, dim] (fp16 or bf16) with rotary positions: the
     first 2 * cos.size(1) values of every head are turned in pairs by the
     angles in row positions[...] of the tables (`rotary_table`), the rest is
@@ -114,8 +120,16 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos
     Differentiable in q and k, backward and forward (tables that require a
     gradient or carry a tangent are refused). k may be None. A position
     outside the tables gives NaN. Sums are in 32 bits, rounded once.
+
+    sections: positions have up to four axes (time, height and width of an
+    image's or a video's tokens), positions [axes, ...], and sections[a] pairs
+    are turned by axis a's: axis after axis or, when cyclic, dealt to the axes
+    in turn, each until it has its share (sections (2, 1, 1): axes 0 1 2 0).
+    They are cos.size(1) in sum. Pair i reads column i of its axis's row, so
+    tables put together from several (`torch.cat`) give each axis frequencies
+    of its own.
     """
-    return _kv().rotary(q, k, positions, cos, sin, interleaved)
+    return _kv().rotary(q, k, positions, cos, sin, interleaved, sections, cyclic)
 
 
 # ---- the cache ----
@@ -123,16 +137,19 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos
 def append_tokens(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor | None,
                   slots: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None, k_pages: torch.Tensor,
                   v_pages: torch.Tensor, interleaved: bool = False, k_scale: torch.Tensor | None = None,
-                  v_scale: torch.Tensor | None = None) -> torch.Tensor | None:
+                  v_scale: torch.Tensor | None = None, sections: Sequence[int] | None = None,
+                  cyclic: bool = False) -> torch.Tensor | None:
     """Stores k (rotated as `rotary` does) and v [n, kv_heads, dim] to rows
     slots [n] of the pages (page * page_size + row; a slot outside the cache,
     such as -1, stores nothing) and returns q [n, heads, dim] rotated. q may
     be None; cos and sin None: nothing is rotated. float8_e4m3fn pages hold
     values divided by k_scale, v_scale [kv_heads] (float32, or None),
     rounded to nearest and saturated at +-448. No two tokens may have one
-    slot. q, k and v may be slices of one projection's output.
+    slot. q, k and v may be slices of one projection's output. sections and
+    cyclic: positions [axes, n] of several axes, as in `rotary`.
     """
-    return _kv().append_tokens(q, k, v, positions, slots, cos, sin, k_pages, v_pages, interleaved, k_scale, v_scale)
+    return _kv().append_tokens(q, k, v, positions, slots, cos, sin, k_pages, v_pages, interleaved, k_scale, v_scale,
+                               sections, cyclic)
 
 
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
@@ -181,6 +198,60 @@ def retrieved_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     last tokens are there already. An id listed twice counts twice."""
     return _kv().retrieved_attention(q, k_pages, v_pages, tables, lens, ids, first, last, scale, k_scale, v_scale,
                                      return_lse)
+
+
+# ---- page tables on the GPU ----
+
+def extend_tables(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, free: torch.Tensor,
+                  seqs: torch.Tensor, counts: torch.Tensor, page_size: int, n_tokens: int, width: int | None = None):
+    """Room for counts[i] more tokens of sequences seqs[i] (int32 [n]), decided
+    on the GPU from its own state: tables [sequences, max_pages] (a sequence's
+    pages in order, -1 behind them), lens [sequences], refs [n_pages] (how many
+    sequences have a page) and free [ceil(n_pages / 32)] (bit p % 32 of word
+    p / 32 where none has page p), all int32 and updated in place; at first -1,
+    0, 0 and the bits of all pages. The lowest free pages go to the requests in
+    order. One that grows inside a page which other sequences have too gets a
+    page for a copy of it first; the last that has it keeps it.
+
+    Returns positions and slots (int64 [n_tokens]; the tokens request after
+    request, then position 0 and slot -1), starts (int32 [n + 1], where each
+    request's begin), the sequences' tables [n, width] (default: max_pages) and
+    lens [n], the pages to copy before tokens are stored, src and dst [n] (-1:
+    none; `copy_pages` takes them), and missing [1]: 0, or the number of pages
+    that are not there, or -1 where a request cannot be: a sequence listed
+    twice, a count below 0, a sequence past width or max_pages, more than
+    n_tokens tokens. Nothing has changed then, and the outputs are those of no
+    new tokens. Ids outside the tables, such as -1, are left out.
+    """
+    return _kv().extend_tables(tables, lens, refs, free, seqs, counts, page_size, n_tokens, width)
+
+
+def truncate_tables(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, free: torch.Tensor,
+                    seqs: torch.Tensor, to: torch.Tensor, page_size: int) -> None:
+    """Cuts sequences seqs[i] back to to[i] tokens (int32 [n]; 0 gives one up, a
+    number below 0 or past its length leaves it), and frees the pages that no
+    sequence has any more. State as in `extend_tables`. Of a sequence listed
+    twice the first counts; ids outside the tables are left out."""
+    _kv().truncate_tables(tables, lens, refs, free, seqs, to, page_size)
+
+
+def fork_tables(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, free: torch.Tensor, seqs: torch.Tensor,
+                into: torch.Tensor, page_size: int) -> None:
+    """Gives the sequences into[i], empty until now, the tokens of seqs[i]
+    (int32 [n]), on the same pages. State as in `extend_tables`. A sequence may
+    be forked several times. Pairs are left out whose ids are outside the
+    tables, and whose into is not empty, is listed before, or stands in seqs
+    too."""
+    _kv().fork_tables(tables, lens, refs, free, seqs, into, page_size)
+
+
+def shared_prefixes(tables: torch.Tensor, lens: torch.Tensor, page_size: int, least: int = 1):
+    """(groups, shared) int32 [batch + 1] and [batch] of a batch's tables [batch, pages] and lens [batch] (int32): a
+    sequence is of its predecessor's group where both have at least `least`
+    tokens in the same whole pages, and a group shares the whole pages that all
+    of it have. Sequences with a prefix in common should be neighbours. Behind
+    the last group, groups is batch and shared 0."""
+    return _kv().shared_prefixes(tables, lens, page_size, least)
 
 
 # ---- pages and sequences ----
@@ -298,9 +369,10 @@ class Step:
     """The new tokens of some sequences (PagedCache.extend): where they go,
     and the sequences' tables and lengths with them. All layers use one."""
 
-    def __init__(self, seqs, positions, slots, tables, lens, max_len):
+    def __init__(self, seqs, positions, slots, tables, lens, max_len, starts=None, missing=None):
         self.seqs, self.positions, self.slots = seqs, positions, slots
         self.tables, self.lens, self.max_len = tables, lens, max_len
+        self.starts, self.missing = starts, missing  # GpuPagedCache's
 
 
 class PagedCache:
@@ -406,11 +478,13 @@ class PagedCache:
         return self.k_pages[layer], self.v_pages[layer], scales
 
     def append(self, layer: int, step: Step, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
-               cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, interleaved: bool = False):
-        """append_tokens for the step's tokens."""
+               cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, interleaved: bool = False,
+               positions: torch.Tensor | None = None, sections: Sequence[int] | None = None, cyclic: bool = False):
+        """append_tokens for the step's tokens. positions: other ones than their places in the sequences, as with
+        several axes."""
         k_pages, v_pages, scales = self._layer(layer)
-        return append_tokens(q, k, v, step.positions, step.slots, cos, sin, k_pages, v_pages, interleaved=interleaved,
-                             **scales)
+        return append_tokens(q, k, v, step.positions if positions is None else positions, step.slots, cos, sin, k_pages,
+                             v_pages, interleaved=interleaved, sections=sections, cyclic=cyclic, **scales)
 
     def decode(self, layer: int, step: Step, q: torch.Tensor, **options):
         """decode_attention for the step's sequences, q [sequences, heads, dim]."""
@@ -424,12 +498,21 @@ class PagedCache:
         return retrieved_attention(q, k_pages, v_pages, step.tables, step.lens, ids, first=first, last=last, **scales,
                                    **options)
 
+    def prefixes(self, step: Step, least: int = 1):
+        """shared_prefixes of the step's sequences. Forks should be neighbours in it."""
+        return shared_prefixes(step.tables, step.lens, self.k_pages.size(3), least)
+
+    def _own(self, seq: int):
+        """A sequence's length and its pages."""
+        n = self.length(seq)
+        own, = self._upload(self.table.pages[seq, :-(-n // self.table.page_size)])
+        return n, own
+
     def keys(self, layer: int, seq: int) -> torch.Tensor:
         """The keys of a sequence, [kv_heads, length, dim], contiguous float16 rows for an index (`Graph`,
         `bruteforce_knn`), whatever the pages' type: what they hold (times k_scale), rounded once; finite values past
         float16's range are its ends, +-65504."""
-        n = self.length(seq)
-        own, = self._upload(self.table.pages[seq, :-(-n // self.table.page_size)])
+        n, own = self._own(seq)
         store = self.k_pages[layer]
         rows = store.view(torch.uint8)[own].view(store.dtype) if store.dtype == _F8 else store[own]
         heads, dim = store.size(1), store.size(3)
@@ -441,3 +524,85 @@ class PagedCache:
             most = torch.finfo(torch.float16).max
             rows = torch.where(rows.isfinite(), rows.clamp(-most, most), rows).to(torch.float16)
         return rows.contiguous()
+
+
+class GpuPagedCache(PagedCache):
+    """A PagedCache whose bookkeeping is on the GPU as well, so that a step --
+    sequences that grow, are cut back, forked and given up, their tokens
+    appended and attended to -- synchronizes nothing and can be captured in a
+    graph and replayed.
+
+    Sequences are rows 0 to max_sequences - 1 of the tables, all empty at
+    first; which of them a program uses is its own affair. Where pages run out
+    nothing is stored, and step.missing says so (extend_tables), to be read
+    when it suits.
+
+        step = cache.extend(seqs, counts, n_tokens)       # int32 tensors
+        for layer in range(n_layers):
+            q = cache.append(layer, step, q, k, v, cos, sin)
+            out = cache.decode(layer, step, q)
+        cache.truncate(seqs, accepted)
+    """
+
+    def __init__(self, n_pages: int, n_layers: int, kv_heads: int, dim: int, page_size: int = 16,
+                 dtype: torch.dtype = torch.float16, max_sequences: int = 64, max_pages: int | None = None,
+                 device: str = "cuda", k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
+        super().__init__(n_pages, n_layers, kv_heads, dim, page_size, dtype, max_sequences, max_pages, device, k_scale,
+                         v_scale)
+        del self.table  # nothing is kept on the host
+        self.page_size, place = page_size, self.k_pages.device
+        self.lens = torch.zeros(max_sequences, dtype=torch.int32, device=place)
+        self.refs = torch.zeros(n_pages, dtype=torch.int32, device=place)
+        bits = np.packbits(np.arange(-(-n_pages // 32) * 32) < n_pages, bitorder="little").view(np.int32)
+        self.free_bits = torch.from_numpy(bits).to(place)
+
+    def _state(self):
+        return self.tables, self.lens, self.refs, self.free_bits
+
+    def new(self):
+        raise NotImplementedError("sequences of a GpuPagedCache are the rows of its tables, empty until they are extended")
+
+    def compact(self):
+        raise NotImplementedError("a GpuPagedCache takes the lowest free pages and is not compacted")
+
+    def length(self, seq: int) -> int:
+        """Waits for the GPU."""
+        if not 0 <= seq < self.lens.size(0):
+            raise ValueError(f"no such sequence: {seq}")
+        return int(self.lens[seq])
+
+    @property
+    def n_free(self) -> int:
+        """Pages that no sequence has. Waits for the GPU."""
+        return int((self.refs == 0).sum())
+
+    def extend(self, seqs: torch.Tensor, counts: torch.Tensor, n_tokens: int, max_len: int | None = None) -> Step:
+        """extend_tables, and the copies of pages that are shared no longer, in all layers. n_tokens: the counts' sum,
+        or more (the rest are tokens without a slot). max_len: no sequence is longer than that now."""
+        width = self.tables.size(1)
+        longest = width * self.page_size
+        if max_len is not None:
+            if max_len < 0:
+                raise ValueError("max_len must be at least 0")
+            longest = min(longest, max_len)
+            width = -(-longest // self.page_size)
+        positions, slots, starts, tables, lens, src, dst, missing = extend_tables(
+            *self._state(), seqs, counts, self.page_size, n_tokens, width)
+        copy_pages(self.k_pages, self.v_pages, src, dst)
+        return Step(seqs, positions, slots, tables, lens, longest, starts, missing)
+
+    def truncate(self, seqs: torch.Tensor, to: torch.Tensor) -> None:
+        """truncate_tables."""
+        truncate_tables(*self._state(), seqs, to, self.page_size)
+
+    def free(self, seqs: torch.Tensor) -> None:
+        """Gives up the sequences, and the pages that only they have."""
+        self.truncate(seqs, torch.zeros_like(seqs))
+
+    def fork(self, seqs: torch.Tensor, into: torch.Tensor) -> None:
+        """fork_tables."""
+        fork_tables(*self._state(), seqs, into, self.page_size)
+
+    def _own(self, seq: int):
+        n = self.length(seq)
+        return n, self.tables[seq, :-(-n // self.page_size)].long()
