@@ -897,7 +897,7 @@ def save_groundtruth(path: str, indices: torch.Tensor, distances: torch.Tensor):
 from .groundtruth import bruteforce_knn, generate_groundtruth  # noqa: E402
 from .kvcache import (GpuPagedCache, PagedCache, append_tokens, copy_pages, decode_attention,  # noqa: E402
                       extend_tables, fork_tables, retrieved_attention, rotary, rotary_table, shared_prefixes,
-                     , truncate_tables)
+                      truncate_tables)
 
 __all__ = [
     "Graph", "DistanceFunc", "DataType", "JasperError", "read_bin", "read_groundtruth",
