@@ -453,7 +453,8 @@ int64_t jasperx_truncate_tables(const jasperx_page_table* table, const int32_t* 
  * listed before or that stands in the other list too are left out. */
 int64_t jasperx_fork_tables(const jasperx_page_table* table, const int32_t* seqs, const int32_t* into, int64_t n,
                             void* stream);
-/* Neighbours in a batch that begin with the same pages: sequence b joins the one before it where
+/* Neighbours in a batch that begin with the same pages, as
+ * jasperx_shared_attention takes them: sequence b joins the one before it where
  * both have at least max(1, least) tokens in the same whole pages. groups
  * [batch + 1]: where the groups begin, batch behind the last; shared [batch]:
  * the tokens in whole pages that all of a group share, 0 for one by itself. */
@@ -489,6 +490,19 @@ int64_t jasperx_retrieved_attention(const jasperx_head_rows* q, int32_t type, in
  * or first + last + count; lists 0: decode_attention, else as in the call. */
 int64_t jasperx_attention_workspace(int64_t batch, int64_t q_heads, const jasperx_kv_pages* pages,
                                     int64_t max_tokens, int64_t lists);
+/* jasperx_decode_attention (window 0) for a batch whose neighbours share their
+ * first tokens, which are read once: sequences groups[g] to groups[g + 1] - 1
+ * (rising, [n_groups + 1], n_groups at most batch) have their first shared[g]
+ * tokens in common; they are read from the table of the first that is as long.
+ * A shorter one, and one in no group, reads its own. max_len below 2^31. */
+int64_t jasperx_shared_attention(const jasperx_head_rows* q, int32_t type, int64_t batch,
+                                 const jasperx_kv_pages* pages, const int32_t* tables, int64_t table_stride,
+                                 int64_t table_width, const int32_t* lens, int64_t max_len, const int32_t* groups,
+                                 const int32_t* shared, int64_t n_groups, double scale, void* out, float* lse,
+                                 void* workspace, int64_t workspace_bytes, void* stream);
+/* Scratch bytes of the call above (pages: sizes and type only). */
+int64_t jasperx_shared_workspace(int64_t batch, int64_t q_heads, const jasperx_kv_pages* pages, int64_t max_len,
+                                 int64_t n_groups);
 /* Library build identifier (git-independent), for load checks. */
 const char* jasperx_version(void);
 

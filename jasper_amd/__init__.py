@@ -896,15 +896,15 @@ def save_groundtruth(path: str, indices: torch.Tensor, distances: torch.Tensor):
 
 from .groundtruth import bruteforce_knn, generate_groundtruth  # noqa: E402
 from .kvcache import (GpuPagedCache, PagedCache, append_tokens, copy_pages, decode_attention,  # noqa: E402
-                      extend_tables, fork_tables, retrieved_attention, rotary, rotary_table, shared_prefixes,
-                      truncate_tables)
+                      extend_tables, fork_tables, retrieved_attention, rotary, rotary_table, shared_attention,
+                      shared_prefixes, truncate_tables)
 
 __all__ = [
     "Graph", "DistanceFunc", "DataType", "JasperError", "read_bin", "read_groundtruth",
     "get_recall", "generate_groundtruth", "bruteforce_knn", "save_groundtruth", "parse_storage_size",
     "last_build_stats", "last_scale_stats", "last_diskann_stats", "diskann_assign", "library_path",
     "rotary_table", "rotary", "append_tokens", "copy_pages", "decode_attention", "retrieved_attention",
-    "extend_tables", "truncate_tables", "fork_tables", "shared_prefixes",
+    "shared_attention", "extend_tables", "truncate_tables", "fork_tables", "shared_prefixes",
     "PagedCache", "GpuPagedCache",
 ]
 

@@ -1100,6 +1100,38 @@ extern "C" int64_t jasperx_retrieved_attention(const jasperx_head_rows* q, int32
   });
 }
 
+extern "C" int64_t jasperx_shared_attention(const jasperx_head_rows* q, int32_t type, int64_t batch,
+                                            const jasperx_kv_pages* pages, const int32_t* tables,
+                                            int64_t table_stride, int64_t table_width, const int32_t* lens,
+                                            int64_t max_len, const int32_t* groups, const int32_t* shared,
+                                            int64_t n_groups, double scale, void* out, float* lse, void* workspace,
+                                            int64_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int64_t {
+    const KvPages p = kv_pages(pages);
+    AttendArgs a = attend_args(q, type, batch, p, tables, table_stride, table_width, lens, scale, out, lse, workspace,
+                               workspace_bytes);
+    if (max_len < 0 || max_len > 0x7FFFFFFF) throw std::invalid_argument("max_len must be at least 0 and below 2^31");
+    if (n_groups < 0 || n_groups > batch) throw std::invalid_argument("groups must be 0 to batch");
+    if (batch && (!groups || (n_groups && !shared))) throw std::invalid_argument("null groups");
+    a.max_len = max_len;
+    shared_attend(a, groups, shared, n_groups, p, (hipStream_t)stream);
+    return 0;
+  });
+}
+
+extern "C" int64_t jasperx_shared_workspace(int64_t batch, int64_t q_heads, const jasperx_kv_pages* pages,
+                                            int64_t max_len, int64_t n_groups) {
+  return guarded([&]() -> int64_t {
+    jasperx_kv_pages sizes = pages ? *pages : jasperx_kv_pages{};
+    sizes.k = sizes.v = nullptr, sizes.pages = 0;
+    const KvPages p = kv_pages(&sizes);
+    if (batch < 0 || batch > 65535 || q_heads < 1 || q_heads > 65535 || q_heads % p.heads || max_len < 0 ||
+        max_len > 0x7FFFFFFF || n_groups < 0 || n_groups > batch)
+      throw std::invalid_argument("bad sizes (too large, or below 0)");
+    return shared_workspace(batch, q_heads, p, max_len, n_groups);
+  });
+}
+
 extern "C" int64_t jasperx_attention_workspace(int64_t batch, int64_t q_heads, const jasperx_kv_pages* pages,
                                                int64_t max_tokens, int64_t lists) {
   return guarded([&]() -> int64_t {

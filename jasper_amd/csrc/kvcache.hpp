@@ -1,6 +1,6 @@
 // kvcache.hpp -- a paged cache of keys and values: its layout, the kernels
 // that fill and move it (kvcache.hip) and the attention of one new token that
-// reads it (attention.hip).
+// reads it (attention.hip, shared.hip).
 //
 // K and V are each [layers][pages][kv heads][page size][dim]; a sequence's
 // token t lies in row t % page_size of page table[t / page_size]. The heads
@@ -101,5 +101,12 @@ struct AttendArgs {
 // 0: no ids).
 int64_t attend_workspace(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_tokens, int64_t lists);
 void attend(const AttendArgs& a, const KvPages& pages, hipStream_t s);
+
+// Attention of one new token per sequence, where sequences groups[g] to
+// groups[g + 1] - 1 have their first shared[g] tokens in common. max_len is
+// what the workspace was sized for.
+int64_t shared_workspace(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_len, int64_t n_groups);
+void shared_attend(const AttendArgs& a, const int32_t* groups, const int32_t* shared, int64_t n_groups, const KvPages& pages,
+                   hipStream_t s);
 
 }  // namespace jasper_amd

@@ -1,0 +1,717 @@
+// shared.hip -- attention of one new token per sequence where groups of
+// sequences begin with the same tokens, which are read once for all of them.
+//
+// With n sequences of a group and gh query heads to a key head, the scores of
+// the group's first S tokens are one product of M = n gh query rows with S key
+// rows, and softmax statistics put what a row saw of them together with what it
+// saw of its own tokens: out = sum_i 2^(ref_i - ref) o_i / sum_i 2^(ref_i -
+// ref) sum_i over the parts i. So the work is streams of tokens under some
+// query rows, shared out evenly over the work-groups:
+//  wide  a group's prefix under more than 16 rows: a work-group takes tiles of
+//        tokens into LDS, its waves 32 rows each (or the same rows and other
+//        tokens of the tile), on 32x32x16 products;
+//  thin  a group's prefix under up to 16 rows, and
+//  own   what a sequence reads by itself: a wave each, past LDS (attend.hpp).
+// A second kernel joins the parts of every row.
+#include "kvcache.hpp"
+
+#include "attend.hpp"
+#include "graph.hpp"
+#include "kvtypes.hpp"
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+namespace jasper_amd {
+
+namespace {
+
+using namespace attention;
+
+constexpr int kBatch = 1024;     // sequences of a launch
+constexpr int kGroups = 256;     // work-groups at most
+constexpr int kStage = 512;      // row offsets of a wave, in LDS
+constexpr int kJoin = 256;       // threads of a joining work-group
+constexpr int kWideStart = 8;    // what beginning a wide stream and a tile of it
+constexpr int kWideTile = 4;     // cost, in tiles of 32 tokens of a wave
+
+constexpr int waves_of(int dt) { return dt == 256 ? 4 : 8; }    // of a work-group
+constexpr int tokens_of(int dt) { return dt == 256 ? 64 : 128; }  // of a wide tile
+__host__ __device__ constexpr int part_row(int dt) { return dt + 4; }  // floats: sums of V, ref, sum
+
+struct Shared {
+  Params a;  // lists: the key heads
+  const int32_t *groups, *shared;
+  int n_groups;
+  int first, count;  // sequences of this launch
+  int4* prefix_ends;  // [count * q_heads]: work-groups (or waves) that have parts, first and last, the row in them, 1 wide 0 thin; first -1: none
+  int2* own_ends;     // [count * q_heads]: waves, first and last
+  float *prefix_first, *own_first;  // [count * q_heads] part rows: the parts that begin a stream
+  float *wide_rest;   // [work-groups][rows of a wide tile]: parts that go on with one
+  float *wave_rest;   // [waves][16]
+};
+
+// What every work-group finds out for itself, in LDS. Of group members only the
+// first and last that have the whole prefix count, as leader and last, at the
+// place of the group's first sequence. wide, thin, own: units before.
+struct Layout {
+  int from[kBatch];  // tokens that a sequence leaves to its group
+  int leader[kBatch], last[kBatch];
+  int wide[kBatch], thin[kBatch], own[kBatch];
+  int totals[3];
+  int part[3][16];
+};
+
+__device__ __forceinline__ int length_of(const Shared& p, int i) { return min(max(p.a.lens[p.first + i], 0), p.a.limit); }
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+template <int NW>
+__device__ __forceinline__ int block_scan(int x, int* part, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int incl = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 63) part[wave] = incl;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w == wave) before = total;
+    total += part[w];
+  }
+  return before + incl - x;
+}
+
+template <int NW, int R, int TT>
+__device__ void lay_out(const Shared& p, Layout& l) {
+  constexpr int kThreads = NW * 64, kRun = kBatch / kThreads;
+  const int t = threadIdx.x, gh = p.a.group;
+  for (int i = t; i < kBatch; i += kThreads) l.leader[i] = 0x7FFFFFFF, l.last[i] = -1, l.from[i] = 0, l.own[i] = 0;
+  __syncthreads();
+  for (int i = t; i < p.count; i += kThreads) {
+    const int b = p.first + i;
+    int lo = 0, hi = p.n_groups + 1;  // the last group that begins at or before b
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (p.groups[mid] <= b) lo = mid + 1;
+      else hi = mid;
+    }
+    const int g = lo - 1;
+    if (g < 0 || g >= p.n_groups) continue;
+    const int shared = p.shared[g], slot = max(p.groups[g] - p.first, 0);
+    if (shared <= 0 || length_of(p, i) < shared) continue;
+    l.from[i] = shared, l.own[i] = slot;
+    atomicMin(&l.leader[slot], i);
+    atomicMax(&l.last[slot], i);
+  }
+  __syncthreads();
+  int wide = 0, thin = 0, own = 0;
+  int each[3][kRun];
+#pragma unroll
+  for (int k = 0; k < kRun; ++k) {
+    const int i = t * kRun + k;
+    each[0][k] = wide, each[1][k] = thin, each[2][k] = own;
+    if (i >= p.count) continue;
+    if (l.leader[i] < l.last[i]) {
+      const int shared = l.from[l.leader[i]], m = (l.last[i] - l.leader[i] + 1) * gh;
+      if (m > kHeads) wide += p.a.heads * ceil_div(m, R) * (kWideStart + ceil_div(shared, TT) * kWideTile);
+      else thin += p.a.heads * (kStart + ceil_div(shared, kTile));
+    }
+    const int slot = l.own[i];
+    const bool alone = l.leader[slot] >= l.last[slot];
+    const int from = alone ? 0 : l.from[i];
+    own += p.a.heads * p.a.head_tiles * (kStart + max(1, ceil_div(length_of(p, i) - (from & ~7), kTile)));
+  }
+  int total[3];
+  const int before[3] = {block_scan<NW>(wide, l.part[0], total[0]), block_scan<NW>(thin, l.part[1], total[1]),
+                         block_scan<NW>(own, l.part[2], total[2])};
+#pragma unroll
+  for (int k = 0; k < kRun; ++k) {
+    const int i = t * kRun + k;
+    const int slot = l.own[i];
+    if (l.leader[slot] >= l.last[slot]) l.from[i] = 0;  // alone with its prefix; nobody else reads this place
+    l.wide[i] = before[0] + each[0][k], l.thin[i] = before[1] + each[1][k], l.own[i] = before[2] + each[2][k];
+  }
+  if (t == 0) l.totals[0] = total[0], l.totals[1] = total[1], l.totals[2] = total[2];
+  __syncthreads();
+}
+
+// The last i with at[i] <= u.
+__device__ __forceinline__ int find(const int* at, int n, int u) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (at[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ floatx16 mfma32(Frag a, Frag b, floatx16 c) {
+  typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
+  if constexpr (std::is_same_v<T, f16>)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
+}
+
+// Lane i of 16 gives the address of four values in row i / 4 of a 4 x 16 block
+// of LDS, its columns 4 (i % 4) on, and gets column i.
+__device__ __forceinline__ uintx2 read_column(const char* p) {
+  return __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                        (__attribute__((address_space(3))) shortx4*)(uintptr_t)(p)));
+}
+
+// A stretch of a wide stream.
+struct WidePart {
+  int leader;  // the group's first sequence here
+  int head, row0, rows, tokens;
+  int c, c1;  // its tiles
+};
+
+// One work-group over tiles [c, c1) of a wide stream; the sums end up in the
+// waves of the tile's first tokens. LDS: two tiles of K and V.
+//
+// S^T = K Q^T and O^T = V^T P^T on 32x32x16 products, hi = lane / 32. Lane's
+// column is a query row all the way: S comes out with the scores of rows 8 a + 4
+// hi + c of K in register 4 a + c, so K's rows are put into LDS with bits 2 and
+// 3 of the token exchanged, and registers 8 k on hold tokens 16 k + 8 hi on, as P
+// has to be as the operand of the second product: nothing crosses lanes. V^T is
+// read from V's rows by LDS reads that transpose. K's 16-byte chunks are
+// exchanged by the low bits of the row and V's by twice those of the token, so
+// that lanes read from different banks.
+template <typename T, bool F8, int DT, bool FULL, int NW, int RW>
+struct Wide {
+  typedef std::conditional_t<F8, f16, T> PT;
+  static constexpr int TT = tokens_of(DT), TW = NW / RW, TPW = TT / TW, NB = TPW / 32;
+  static constexpr int RB = DT * 2, CH = RB / 16, KEY = CH < 16 ? CH - 1 : 15;
+  static constexpr int kThreads = NW * 64, kTileBytes = TT * RB;
+  static constexpr int UNITS = F8 ? CH / 2 : CH, ITER = TT * UNITS / kThreads;  // 16-byte loads of a row, of a thread
+  static constexpr int KS = DT / 16, DB = DT / 32;
+  static constexpr float kLag = 3.f, kTop = std::is_same_v<PT, f16> ? 12.f : -kLag;  // as in attend_tiles
+  static constexpr int kLds = 4 * kTileBytes;
+  static_assert(NB >= 1 && ITER >= 1, "a tile is too small");
+  static_assert((TW - 1) * RW * (DB * 16 + 2) * 64 * 4 <= kLds, "the waves' sums do not fit");
+
+  const Shared& p;
+  char* const lds;
+  uint8_t (*const ok)[TT];
+  int (*const bad)[NW];
+  const int lane = threadIdx.x & 63, hi = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = wave % RW, tw = wave / RW;
+
+  Frag q[KS];
+  floatx16 o[DB];
+  float ref, use, sum;
+  uintx4 kr[ITER], vr[ITER];
+  uint32_t row_ok;
+
+  __device__ char* k_tile(int b) const { return lds + b * 2 * kTileBytes; }
+  __device__ char* v_tile(int b) const { return lds + b * 2 * kTileBytes + kTileBytes; }
+
+  __device__ __forceinline__ void fetch(const WidePart& w, int tile) {
+    constexpr int ES = F8 ? 1 : 2;
+    const Params& a = p.a;
+    const int32_t* const table = a.tables + (p.first + w.leader) * a.table_stride;
+    row_ok = 0;
+#pragma unroll
+    for (int e = 0; e < ITER; ++e) {
+      const int idx = e * kThreads + threadIdx.x, row = idx / UNITS, unit = idx % UNITS;
+      const int t = tile * TT + row;
+      kr[e] = vr[e] = uintx4{0, 0, 0, 0};
+      if (t >= w.tokens) continue;
+      const int32_t page = table[t >> a.page_shift];
+      if (page < 0 || page >= a.pages) continue;
+      row_ok |= 1u << e;
+      if (!FULL && unit * (16 / ES) >= a.dim) continue;
+      const int64_t off = (page * a.page_stride + w.head * a.head_stride + (t & ((1 << a.page_shift) - 1)) * a.row_stride) * ES + unit * 16;
+      kr[e] = *(const uintx4*)(a.k + off);
+      vr[e] = *(const uintx4*)(a.v + off);
+    }
+  }
+
+  __device__ __forceinline__ void store(int b) {
+    bool all = true;
+#pragma unroll
+    for (int e = 0; e < ITER; ++e) {
+      const int idx = e * kThreads + threadIdx.x, row = idx / UNITS, unit = idx % UNITS;
+      const int m = (row & ~12) | (row & 4) << 1 | (row & 8) >> 1;
+      char* const kd = k_tile(b) + m * RB;
+      char* const vd = v_tile(b) + row * RB;
+      const int kx = m & KEY, vx = (row & 3) << 1;
+      if constexpr (F8) {
+        const uintx4 k = kr[e], v = vr[e];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t k0 = h ? k.z : k.x, k1 = h ? k.w : k.y, v0 = h ? v.z : v.x, v1 = h ? v.w : v.y;
+          *(uintx4*)(kd + ((2 * unit + h) ^ kx) * 16) = uintx4{from_e4m3<T>(k0, false), from_e4m3<T>(k0, true), from_e4m3<T>(k1, false), from_e4m3<T>(k1, true)};
+          *(uintx4*)(vd + ((2 * unit + h) ^ vx) * 16) = uintx4{from_e4m3<PT>(v0, false), from_e4m3<PT>(v0, true), from_e4m3<PT>(v1, false), from_e4m3<PT>(v1, true)};
+        }
+      } else {
+        *(uintx4*)(kd + (unit ^ kx) * 16) = kr[e];
+        *(uintx4*)(vd + (unit ^ vx) * 16) = vr[e];
+      }
+      const bool in = row_ok >> e & 1;
+      if (unit == 0) ok[b][row] = in;
+      all = all && in;
+    }
+    const bool any_bad = __any(!all);
+    if (lane == 0) bad[b][wave] = any_bad;
+  }
+
+  __device__ __forceinline__ void compute(int b, float cs) {
+    const char* const kt = k_tile(b) + (tw * TPW + (lane & 31)) * RB;
+    floatx16 s[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[n][r] = 0;
+#pragma unroll
+      for (int e = 0; e < KS; ++e)
+        s[n] = mfma32<T>(*(const Frag*)(kt + n * 32 * RB + ((2 * e + hi) ^ (lane & KEY)) * 16), q[e], s[n]);
+    }
+    int any_bad = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) any_bad |= bad[b][w];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) s[n] *= cs;
+    if (any_bad) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!ok[b][tw * TPW + n * 32 + 16 * (r / 8) + 8 * hi + r % 8]) s[n][r] = -__builtin_inff();
+      }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+    if (__any(top > ref + (kTop + kLag))) {
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float now = fmaxf(ref, top - kTop);
+      const float to = now == -__builtin_inff() ? 0.f : now;
+      const float keep = __builtin_amdgcn_exp2f(ref - to);
+      sum *= keep;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= keep;
+      ref = now, use = to;
+    }
+    // lane's place in the 4 x 16 blocks that it reads with 15 others
+    const int i = lane & 15, g1 = lane >> 4 & 1, x = 2 * (i / 4);
+    const char* const vt = v_tile(b) + (tw * TPW + 8 * hi + i / 4) * RB + 8 * (i & 1);
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        Frag wh, wl;
+#pragma unroll
+        for (int r = 0; r < 8; r += 2) {
+          const float a = __builtin_amdgcn_exp2f(s[n][8 * k + r] - use), c = __builtin_amdgcn_exp2f(s[n][8 * k + r + 1] - use);
+          sum += a + c;
+          wh[r / 2] = pack2<PT>(a, c);
+          const floatx2 back = unpack2<PT>(wh[r / 2]);
+          wl[r / 2] = pack2<PT>(a - back.x, c - back.y);
+        }
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const char* const at = vt + (n * 32 + 16 * k) * RB + ((4 * d + 2 * g1 + (i % 4) / 2) ^ x) * 16;
+          const uintx2 v0 = read_column(at), v1 = read_column(at + 4 * RB);
+          const Frag f = {v0.x, v0.y, v1.x, v1.y};
+          o[d] = mfma32<PT>(f, wh, o[d]);
+          o[d] = mfma32<PT>(f, wl, o[d]);
+        }
+      }
+  }
+
+  __device__ void run(const WidePart& w) {
+    const Params& a = p.a;
+    const int row = rw * 32 + (lane & 31), at = w.row0 + row;
+    const int member = w.leader + at / a.group, q_head = w.head * a.group + at % a.group;
+    const char* const q_row = a.q + ((p.first + member) * a.q_stride + q_head * a.q_head) * 2;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = 16 * s + 8 * hi;
+      q[s] = Frag{0, 0, 0, 0};
+      if (row < w.rows && (FULL || d < a.dim)) q[s] = *(const Frag*)(q_row + d * 2);
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0;
+    ref = -__builtin_inff(), use = 0.f, sum = 0.f;
+    const float cs = a.scale * (a.k_scale ? a.k_scale[w.head] : 1.f);
+    fetch(w, w.c);
+    __syncthreads();  // what was in LDS before has been read
+    store(0);
+    for (int t = w.c; t < w.c1; ++t) {
+      const int b = (t - w.c) & 1;
+      __syncthreads();
+      if (t + 1 < w.c1) fetch(w, t + 1);
+      compute(b, cs);
+      if (t + 1 < w.c1) store(b ^ 1);
+    }
+    sum += __shfl_xor(sum, 32, 64);
+    if constexpr (TW > 1) {
+      constexpr int kOne = (DB * 16 + 2) * 64;
+      float* const all = (float*)lds;
+      __syncthreads();
+      if (tw) {
+        float* const mine = all + ((tw - 1) * RW + rw) * kOne + lane;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mine[(d * 16 + r) * 64] = o[d][r];
+        mine[DB * 16 * 64] = ref, mine[(DB * 16 + 1) * 64] = sum;
+      }
+      __syncthreads();
+      if (tw == 0) {
+#pragma unroll 1
+        for (int other = 0; other < TW - 1; ++other) {
+          const float* const its = all + (other * RW + rw) * kOne + lane;
+          const float its_ref = its[DB * 16 * 64], now = fmaxf(ref, its_ref);
+          // without scores so far the sums are zero (or NaN)
+          const float mine = ref == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ref - now);
+          const float theirs = its_ref == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(its_ref - now);
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * mine + its[(d * 16 + r) * 64] * theirs;
+          sum = sum * mine + its[(DB * 16 + 1) * 64] * theirs;
+          ref = now;
+        }
+      }
+    }
+  }
+
+  // The sums to the workspace; range: the work-groups that have parts of the stream.
+  __device__ void write(const WidePart& w, int2 range, const Layout& l) {
+    if (tw) return;
+    const Params& a = p.a;
+    const int row = rw * 32 + (lane & 31), at = w.row0 + row;
+    if (row >= w.rows) return;
+    const int member = w.leader + at / a.group;
+    const int64_t out = (int64_t)member * a.q_heads + w.head * a.group + at % a.group;
+    float* const part = w.c == 0 ? p.prefix_first + out * part_row(DT)
+                                 : p.wide_rest + ((int64_t)blockIdx.x * 32 * RW + row) * part_row(DT);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *(floatx4*)(part + 32 * d + 2 * r + 4 * hi) = floatx4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+    if (hi == 0) {
+      *(floatx2*)(part + DT) = floatx2{ref, sum};
+      if (w.c == 0 && l.from[member]) p.prefix_ends[out] = int4{range.x, range.y, row, 1};
+    }
+  }
+};
+
+template <typename T, bool F8, int DT, bool FULL, int NW, int RW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void shared_kernel(Shared p) {
+  typedef Wide<T, F8, DT, FULL, NW, RW> W;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ Layout l;
+  __shared__ uint8_t ok[2][W::TT];
+  __shared__ int bad[2][NW];
+  const Params& a = p.a;
+  lay_out<NW, 32 * RW, W::TT>(p, l);
+  const int wides = l.totals[0], thins = l.totals[1], total = wides + thins + l.totals[2];
+  Share share;
+  // a work-group has units for all of its waves, and at least a wide tile's: so
+  // that within a stream each has a part
+  share.waves = min(max(1, total / max(NW, kWideTile)), (int)gridDim.x);
+  share.each = total / share.waves;
+  share.more = total % share.waves;
+  if ((int)blockIdx.x >= share.waves) return;
+  const int u0 = share.begin(blockIdx.x), u1 = share.begin(blockIdx.x + 1);
+
+  for (int u = u0; u < min(u1, wides);) {
+    const int i = __builtin_amdgcn_readfirstlane(find(l.wide, p.count, u));
+    WidePart w;
+    w.leader = __builtin_amdgcn_readfirstlane(l.leader[i]);
+    w.tokens = __builtin_amdgcn_readfirstlane(l.from[w.leader]);
+    const int m = (__builtin_amdgcn_readfirstlane(l.last[i]) - w.leader + 1) * a.group, row_tiles = ceil_div(m, 32 * RW);
+    const int tiles = ceil_div(w.tokens, W::TT), cost = kWideStart + tiles * kWideTile;
+    const int x = (u - l.wide[i]) / cost, pos = (u - l.wide[i]) % cost, begin = u - pos;
+    w.head = __builtin_amdgcn_readfirstlane(x / row_tiles);
+    w.row0 = __builtin_amdgcn_readfirstlane(x % row_tiles * 32 * RW);
+    w.rows = min(32 * RW, m - w.row0);
+    const int end = min(cost, pos + (u1 - u));
+    w.c = __builtin_amdgcn_readfirstlane(ceil_div(max(0, pos - kWideStart), kWideTile));
+    w.c1 = __builtin_amdgcn_readfirstlane(ceil_div(max(0, end - kWideStart), kWideTile));
+    if (w.c < w.c1) {
+      W wide{p, lds, ok, bad};
+      wide.run(w);
+      wide.write(w, int2{(int)blockIdx.x, share.owner(begin + kWideStart + (tiles - 1) * kWideTile)}, l);
+    }
+    u += cost - pos;
+  }
+  __syncthreads();
+
+  // the waves' shares of the rest
+  constexpr int VD = DT / 16;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int x0 = max(u0, wides), span = u1 - x0;
+  if (span <= 0) return;
+  // n units go to the last min(n, NW) waves of a work-group: only where the wide
+  // streams end there are fewer than NW, and the next one's first wave goes on
+  // with what the last of them began
+  const auto wave_begin = [&](int64_t n, int k) { return (int)(n * k / min(n, (int64_t)NW)); };
+  const auto owner = [&](int u) {  // the wave that has unit u
+    const int group = share.owner(u), begin = max(share.begin(group), wides), n = share.begin(group + 1) - begin;
+    int k = (int)((int64_t)(u - begin) * min(n, NW) / n);
+    while (wave_begin(n, k + 1) <= u - begin) ++k;
+    return group * NW + NW - min(n, NW) + k;
+  };
+  const int mine = wave - (NW - min(span, NW));
+  if (mine < 0) return;
+  const int me = blockIdx.x * NW + wave, a1 = x0 + wave_begin(span, mine + 1);
+  for (int u = x0 + wave_begin(span, mine); u < a1;) {
+    Span sp{};
+    Stream at;
+    const char* q_row;
+    int pos, i;
+    const bool thin = u < wides + thins;
+    if (thin) {
+      i = find(l.thin, p.count, u - wides);
+      const int leader = __builtin_amdgcn_readfirstlane(l.leader[i]);
+      sp.end = __builtin_amdgcn_readfirstlane(l.from[leader]);
+      sp.tiles = ceil_div(sp.end, kTile), sp.cost = kStart + sp.tiles;
+      const int in = u - wides - __builtin_amdgcn_readfirstlane(l.thin[i]), head = in / sp.cost;
+      pos = in % sp.cost;
+      at = Stream{p.first + leader, head, (__builtin_amdgcn_readfirstlane(l.last[i]) - leader + 1) * a.group, head * a.group, head};
+      q_row = a.q + ((at.b + i16 / a.group) * a.q_stride + (at.q_head + i16 % a.group) * a.q_head) * 2;
+    } else {
+      i = __builtin_amdgcn_readfirstlane(find(l.own, p.count, u - wides - thins));
+      sp.begin = __builtin_amdgcn_readfirstlane(l.from[i]), sp.base = sp.begin & ~7, sp.end = length_of(p, i);
+      sp.tiles = max(1, ceil_div(sp.end - sp.base, kTile)), sp.cost = kStart + sp.tiles;
+      const int in = u - wides - thins - __builtin_amdgcn_readfirstlane(l.own[i]), x = in / sp.cost;
+      pos = in % sp.cost;
+      at = stream_of(a, p.first + i, x / a.head_tiles, x % a.head_tiles);
+      q_row = query_of(a, at, i16);
+    }
+    const int c = max(0, pos - kStart), c1 = max(0, min(sp.cost, pos + (a1 - u)) - kStart);
+    if (c < c1) {
+      const Sums<DT> s = attend_tiles<T, F8, DT, false, FULL, kStage>(p.a, sp, at, q_row, c, c1, (int64_t*)lds + wave * kStage);
+      if (i16 < at.heads) {
+        const int seq = at.b - p.first + (thin ? i16 / a.group : 0);
+        const int64_t out = (int64_t)seq * a.q_heads + at.q_head + (thin ? i16 % a.group : i16);
+        float* const part = c ? p.wave_rest + ((int64_t)me * kHeads + i16) * part_row(DT)
+                              : (thin ? p.prefix_first : p.own_first) + out * part_row(DT);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < VD; j += 4)
+            *(floatx4*)(part + dim_of<F8, DT>(g, j, r)) = floatx4{s.o[j][r], s.o[j + 1][r], s.o[j + 2][r], s.o[j + 3][r]};
+        if (g == 0) {
+          *(floatx2*)(part + DT) = floatx2{s.ref, s.sum};
+          if (c == 0) {
+            const int last = owner(u - pos + sp.cost - 1);
+            if (!thin) p.own_ends[out] = int2{me, last};
+            if (thin && l.from[seq]) p.prefix_ends[out] = int4{me, last, i16, 0};
+            if (!thin && sp.begin == 0) p.prefix_ends[out] = int4{-1, -2, 0, 0};
+          }
+        }
+      }
+    }
+    u += sp.cost - pos;
+  }
+}
+
+// Joins the parts of a query row: a thread has four dims of every kRows-th part.
+template <typename T, int DT, int R>
+__global__ __launch_bounds__(kJoin) void join_kernel(Shared p) {
+  constexpr int kLanes = DT / 4, kRows = kJoin / kLanes, kLoads = 8;
+  __shared__ float weight[kGroups * (1 + 2 * waves_of(DT))];
+  __shared__ float tops[kJoin / 64], tots[kJoin / 64];
+  __shared__ floatx4 sums[kRows][kLanes];
+  const Params& a = p.a;
+  const int64_t out = blockIdx.x;
+  const int4 prefix = p.prefix_ends[out];
+  const int2 own = p.own_ends[out];
+  const int n_prefix = prefix.y - prefix.x + 1, parts = n_prefix + own.y - own.x + 1;
+  const int head = (int)(out % a.q_heads);
+  const auto part = [&](int i) -> const float* {
+    if (i < n_prefix) {
+      if (i == 0) return p.prefix_first + out * part_row(DT);
+      return prefix.w ? p.wide_rest + ((int64_t)(prefix.x + i) * R + prefix.z) * part_row(DT)
+                      : p.wave_rest + ((int64_t)(prefix.x + i) * kHeads + prefix.z) * part_row(DT);
+    }
+    i -= n_prefix;
+    if (i == 0) return p.own_first + out * part_row(DT);
+    return p.wave_rest + ((int64_t)(own.x + i) * kHeads + head % a.group % kHeads) * part_row(DT);
+  };
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane4 = threadIdx.x % kLanes, row = threadIdx.x / kLanes, d = 4 * lane4;
+  floatx4 y[kLoads];
+  const auto fetch = [&](int i0) {
+#pragma unroll
+    for (int e = 0; e < kLoads; ++e)
+      if (i0 + e * kRows < parts) y[e] = *(const floatx4*)(part(i0 + e * kRows) + d);
+  };
+  fetch(row);  // on their way while the weights are found
+  float top = -__builtin_inff();
+  for (int i = threadIdx.x; i < parts; i += kJoin) {
+    const float m = part(i)[DT];
+    weight[i] = m;
+    top = fmaxf(top, m);
+  }
+  for (int m = 32; m; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  float tot = 0;
+  for (int i = threadIdx.x; i < parts; i += kJoin) {
+    const float m = weight[i];
+    const float f = m == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - top);  // then its sums are zero (or NaN)
+    weight[i] = f;
+    tot += f * part(i)[DT + 1];
+  }
+  for (int m = 32; m; m >>= 1) tot += __shfl_xor(tot, m, 64);
+  if (lane == 0) tots[wave] = tot;
+  __syncthreads();
+  tot = (tots[0] + tots[1]) + (tots[2] + tots[3]);
+  floatx4 acc = {0, 0, 0, 0};
+  for (int i0 = row; i0 < parts; i0 += kRows * kLoads) {
+    if (i0 != row) fetch(i0);
+#pragma unroll
+    for (int e = 0; e < kLoads; ++e) {
+      const int i = i0 + e * kRows;
+      if (i < parts) acc += y[e] * weight[i];
+    }
+  }
+  sums[row][lane4] = acc;
+  __syncthreads();
+  if (row) return;
+  for (int r = 1; r < kRows; ++r) acc += sums[r][lane4];
+  const int64_t at = (int64_t)p.first * a.q_heads + out;
+  const float inv = (a.v_scale ? a.v_scale[head / a.group] : 1.f) / tot;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] = tot == 0.f ? 0.f : acc[e] * inv;
+  if (d < a.dim) *(uintx2*)(a.out + (at * a.dim + d) * 2) = uintx2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
+  if (d == 0 && a.lse) a.lse[at] = tot == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(tot)) * kLn2;
+}
+
+int compute_units() {
+  static const int n = [] {
+    int device = 0, v = 0;
+    hip_check(hipGetDevice(&device), "get device");
+    hip_check(hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, device), "device attribute");
+    return v > 0 ? v : 256;
+  }();
+  return n;
+}
+
+// How a call's work is laid out, from its sizes alone.
+struct Plan {
+  int dt, group, head_tiles, row_waves;
+  int64_t work_groups;
+  int64_t ends, firsts, wide_rest, wave_rest, bytes;  // of the workspace: bytes of each
+};
+
+Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_len, int64_t n_groups) {
+  Plan a;
+  a.dt = pages.dim <= 64 ? 64 : pages.dim <= 128 ? 128 : 256;
+  a.group = (int)(q_heads / pages.heads);
+  a.head_tiles = (a.group + kHeads - 1) / kHeads;
+  const int64_t count = std::min<int64_t>(batch, kBatch);
+  // units of a launch, at most
+  const int64_t tiles = max_len / kTile + 2 + kStart + 2 * kWideStart;
+  const int64_t per_seq = pages.heads * (2 * (int64_t)a.head_tiles + a.group / 32 + 2);
+  if (tiles > 0x7FFFFFFF / std::max<int64_t>(1, count * per_seq)) throw std::invalid_argument("batch x heads x tokens is too large");
+  a.row_waves = count * a.group > 64 * std::max<int64_t>(1, std::min(n_groups, count)) ? 4 : 2;
+  a.work_groups = std::min<int64_t>({kGroups, compute_units(), std::max<int64_t>(1, count * pages.heads * a.head_tiles * tiles)});
+  const int64_t rows = count * q_heads, row = part_row(a.dt) * 4;
+  a.ends = rows * 24, a.firsts = rows * row;
+  a.wide_rest = a.work_groups * 32 * a.row_waves * row;
+  a.wave_rest = a.work_groups * waves_of(a.dt) * kHeads * row;
+  a.bytes = (a.ends + 15) / 16 * 16 + 2 * a.firsts + a.wide_rest + a.wave_rest;
+  return a;
+}
+
+template <typename T, bool F8, int DT, bool FULL, int RW>
+void launch(const Shared& p, const Plan& plan, hipStream_t s) {
+  constexpr int NW = waves_of(DT);
+  auto kernel = shared_kernel<T, F8, DT, FULL, NW, RW>;
+  constexpr int lds = std::max(Wide<T, F8, DT, FULL, NW, RW>::kLds, NW * kStage * 8);
+  hip_check(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "shared attention");
+  kernel<<<(unsigned)plan.work_groups, 64 * NW, lds, s>>>(p);
+  hip_check(hipGetLastError(), "shared attention");
+  join_kernel<T, DT, 32 * RW><<<(unsigned)(p.count * p.a.q_heads), kJoin, 0, s>>>(p);
+  hip_check(hipGetLastError(), "shared attention join");
+}
+
+template <typename T, bool F8, int DT>
+void launch_rows(const Shared& p, const Plan& plan, hipStream_t s) {
+  const bool full = p.a.dim == DT;
+  if (plan.row_waves == 4) full ? launch<T, F8, DT, true, 4>(p, plan, s) : launch<T, F8, DT, false, 4>(p, plan, s);
+  else full ? launch<T, F8, DT, true, 2>(p, plan, s) : launch<T, F8, DT, false, 2>(p, plan, s);
+}
+
+template <typename T, bool F8>
+void launch_dim(const Shared& p, const Plan& plan, hipStream_t s) {
+  if (plan.dt == 64) launch_rows<T, F8, 64>(p, plan, s);
+  else if (plan.dt == 128) launch_rows<T, F8, 128>(p, plan, s);
+  else launch_rows<T, F8, 256>(p, plan, s);
+}
+
+}  // namespace
+
+int64_t shared_workspace(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_len, int64_t n_groups) {
+  return batch ? plan_of(batch, q_heads, pages, max_len, n_groups).bytes : 0;
+}
+
+void shared_attend(const AttendArgs& a, const int32_t* groups, const int32_t* shared, int64_t n_groups, const KvPages& pages,
+                   hipStream_t s) {
+  if (a.batch == 0) return;
+  const int64_t width = (int64_t)a.table_width << pages.page_shift;
+  Shared p{};
+  Params& r = p.a;
+  r.limit = pages.pages ? (int)std::min<int64_t>({a.max_len, width, 0x7FFFFF00}) : 0;
+  const Plan plan = plan_of(a.batch, a.q.heads, pages, a.max_len, n_groups);
+  if (a.workspace_bytes < plan.bytes || !a.workspace || ((uintptr_t)a.workspace & 15u))
+    throw std::invalid_argument("workspace must be 16-byte aligned and hold " + std::to_string(plan.bytes) + " bytes");
+  r.q = (const char*)a.q.p, r.q_stride = a.q.stride, r.q_head = a.q.head_stride;
+  r.k = pages.k, r.v = pages.v;
+  r.page_stride = pages.page_stride, r.head_stride = pages.head_stride, r.row_stride = pages.row_stride;
+  r.tables = a.tables, r.table_stride = a.table_stride, r.lens = a.lens;
+  r.k_scale = pages.k_scale, r.v_scale = pages.v_scale;
+  r.out = (char*)a.out, r.lse = a.lse;
+  r.scale = a.scale * 1.4426950408889634f;
+  r.batch = (int)a.batch, r.heads = pages.heads, r.q_heads = a.q.heads, r.lists = pages.heads;
+  r.group = plan.group, r.head_tiles = plan.head_tiles, r.side = 1;
+  r.page_shift = pages.page_shift, r.pages = pages.pages, r.dim = pages.dim;
+  p.groups = groups, p.shared = shared, p.n_groups = (int)n_groups;
+  char* w = (char*)a.workspace;
+  const int64_t rows = plan.ends / 24;
+  p.prefix_ends = (int4*)w, p.own_ends = (int2*)(w + rows * 16);
+  w += (plan.ends + 15) / 16 * 16;
+  p.prefix_first = (float*)w, p.own_first = (float*)(w + plan.firsts);
+  p.wide_rest = (float*)(w + 2 * plan.firsts), p.wave_rest = (float*)(w + 2 * plan.firsts + plan.wide_rest);
+  for (p.first = 0; p.first < a.batch; p.first += kBatch) {
+    p.count = (int)std::min<int64_t>(kBatch, a.batch - p.first);
+    if (pages.type == kE4M3) {
+      if (a.type == kF16) launch_dim<f16, true>(p, plan, s);
+      else launch_dim<bf16, true>(p, plan, s);
+    } else if (a.type == kF16) {
+      launch_dim<f16, false>(p, plan, s);
+    } else {
+      launch_dim<bf16, false>(p, plan, s);
+    }
+  }
+}
+
+}  // namespace jasper_amd

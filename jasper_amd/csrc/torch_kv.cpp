@@ -489,9 +489,13 @@ struct Attention {
     scale = scale_in ? *scale_in : 1.0 / std::sqrt((double)pages.dim);
   }
 
-  int64_t allocate(bool return_lse, int64_t max_tokens, int64_t lists) {
+  void allocate_outputs(bool return_lse) {
     out = at::empty(q.sizes(), q.options());
     if (return_lse) lse = at::empty({batch, q.size(1)}, q.options().dtype(at::kFloat));
+  }
+
+  int64_t allocate(bool return_lse, int64_t max_tokens, int64_t lists) {
+    allocate_outputs(return_lse);
     int64_t size = 0;
     if (batch) {
       size = jasperx_attention_workspace(batch, q.size(1), &pages, max_tokens, lists);
@@ -550,6 +554,33 @@ py::object retrieved_attention(const Tensor& q, const Tensor& k_pages, const Ten
   return a.result();
 }
 
+py::object shared_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables,
+                            const Tensor& lens, const Tensor& groups, const Tensor& shared, std::optional<double> scale,
+                            const OptTensor& k_scale, const OptTensor& v_scale, std::optional<int64_t> max_len,
+                            bool return_lse) {
+  Attention a(q, k_pages, v_pages, tables, lens, scale, k_scale, v_scale);
+  TORCH_CHECK_VALUE(!max_len || *max_len >= 0, "max_len must be at least 0");
+  check_ints("groups", groups, 1, k_pages.device()), check_ints("shared", shared, 1, k_pages.device());
+  const int64_t n = shared.size(0);
+  TORCH_CHECK_VALUE(groups.size(0) == n + 1 && n <= a.batch, "groups must be [n_groups + 1] and shared [n_groups], of at most ",
+                    a.batch, " groups, got ", groups.size(0), " and ", n);
+  const c10::DeviceGuard guard(k_pages.device());
+  int64_t most = tables.size(1) * a.pages.page_size;
+  if (max_len) most = std::min(most, *max_len);
+  a.allocate_outputs(return_lse);
+  if (a.batch) {
+    const int64_t size = jasperx_shared_workspace(a.batch, q.size(1), &a.pages, most, n);
+    check(size);
+    a.scratch = at::empty({size}, a.q.options().dtype(at::kByte));
+    check(jasperx_shared_attention(&a.rows, type_of(a.q), a.batch, &a.pages, (const int32_t*)tables.data_ptr(),
+                                   tables.stride(0), tables.size(1), (const int32_t*)a.lens.data_ptr(), most,
+                                   (const int32_t*)groups.data_ptr(), (const int32_t*)shared.data_ptr(), n, a.scale,
+                                   a.out.data_ptr(), a.lse_ptr(), a.scratch.data_ptr(), size,
+                                   current_stream(k_pages.get_device())));
+  }
+  return a.result();
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_kv, m) {
@@ -569,4 +600,5 @@ PYBIND11_MODULE(_kv, m) {
   m.def("shared_prefixes", &shared_prefixes);
   m.def("decode_attention", &decode_attention);
   m.def("retrieved_attention", &retrieved_attention);
+  m.def("shared_attention", &shared_attention);
 }

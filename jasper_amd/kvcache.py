@@ -11,6 +11,7 @@ reference counterpart.
   copy_pages              pages copied or moved, in all layers
   decode_attention        one new token per sequence over its whole cache
   retrieved_attention     over the first, the last and the retrieved tokens
+  shared_attention        over the whole cache, where sequences share a prefix
   PagedCache              pages, sequences, forks and compaction put together
   extend_tables, truncate_tables, fork_tables
                           which sequence has which pages, kept on the GPU
@@ -200,6 +201,26 @@ def retrieved_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
                                      return_lse)
 
 
+def shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
+                     lens: torch.Tensor, groups: torch.Tensor, shared: torch.Tensor, scale: float | None = None,
+                     k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                     max_len: int | None = None, return_lse: bool = False):
+    """decode_attention for a batch whose neighbours share their first tokens,
+    which are then read once for all of them. Sequences groups[g] to
+    groups[g + 1] - 1 (int32 [n_groups + 1], rising; n_groups at most batch)
+    have their first shared[g] tokens (int32 [n_groups]) in common, in the same
+    pages or in others with the same rows: they are read where the first of
+    them has them. tables and lens are those of whole sequences, as for
+    decode_attention, and `shared_prefixes` gives groups and shared for them.
+    A sequence that is shorter than its group's prefix reads its own pages, and
+    so does one that is in no group. Groups are best as large as they come:
+    every group costs as much as a sequence, and 16 query heads of one key head
+    fill a matrix instruction.
+    """
+    return _kv().shared_attention(q, k_pages, v_pages, tables, lens, groups, shared, scale, k_scale, v_scale, max_len,
+                                  return_lse)
+
+
 # ---- page tables on the GPU ----
 
 def extend_tables(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, free: torch.Tensor,
@@ -246,7 +267,8 @@ def fork_tables(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, fr
 
 
 def shared_prefixes(tables: torch.Tensor, lens: torch.Tensor, page_size: int, least: int = 1):
-    """(groups, shared) int32 [batch + 1] and [batch] of a batch's tables [batch, pages] and lens [batch] (int32): a
+    """(groups, shared) int32 [batch + 1] and [batch], as shared_attention takes
+    them, of a batch's tables [batch, pages] and lens [batch] (int32): a
     sequence is of its predecessor's group where both have at least `least`
     tokens in the same whole pages, and a group shares the whole pages that all
     of it have. Sequences with a prefix in common should be neighbours. Behind
@@ -499,8 +521,14 @@ class PagedCache:
                                    **options)
 
     def prefixes(self, step: Step, least: int = 1):
-        """shared_prefixes of the step's sequences. Forks should be neighbours in it."""
+        """shared_prefixes of the step's sequences, for `shared` in all layers. Forks should be neighbours in it."""
         return shared_prefixes(step.tables, step.lens, self.k_pages.size(3), least)
+
+    def shared(self, layer: int, step: Step, q: torch.Tensor, prefixes, **options):
+        """shared_attention for the step's sequences: decode, with what `prefixes` found in common read once."""
+        k_pages, v_pages, scales = self._layer(layer)
+        return shared_attention(q, k_pages, v_pages, step.tables, step.lens, *prefixes, max_len=step.max_len, **scales,
+                                **options)
 
     def _own(self, seq: int):
         """A sequence's length and its pages."""
@@ -538,9 +566,10 @@ class GpuPagedCache(PagedCache):
     when it suits.
 
         step = cache.extend(seqs, counts, n_tokens)       # int32 tensors
+        prefixes = cache.prefixes(step)
         for layer in range(n_layers):
             q = cache.append(layer, step, q, k, v, cos, sin)
-            out = cache.decode(layer, step, q)
+            out = cache.shared(layer, step, q, prefixes)
         cache.truncate(seqs, accepted)
     """
 
