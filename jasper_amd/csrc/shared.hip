@@ -180,16 +180,26 @@ struct WidePart {
   int c, c1;  // its tiles
 };
 
+// A wave's 64 times 16 bytes from memory to LDS at `to` on, in the lanes' order,
+// past the registers; lanes that do not take part leave theirs out. Waited for by
+// loads_done. (In LDS the compiler does not see these writes coming: they go to
+// the tile that nobody reads before the next barrier.)
+__device__ __forceinline__ void load_lds(const void* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "memory");
+}
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
 // One work-group over tiles [c, c1) of a wide stream; the sums end up in the
-// waves of the tile's first tokens. LDS: two tiles of K and V.
+// waves of the tile's first tokens. LDS: two tiles of K and V, of which one is
+// filled while the other is used.
 //
-// S^T = K Q^T and O^T = V^T P^T on 32x32x16 products, hi = lane / 32. Lane's
+// S^T = K Q^T and O^T = V^T P^T on 32x32x16 products, hi = lane / 32. A lane's
 // column is a query row all the way: S comes out with the scores of rows 8 a + 4
-// hi + c of K in register 4 a + c, so K's rows are put into LDS with bits 2 and
+// hi + c of K in register 4 a + c, so the rows are put into LDS with bits 2 and
 // 3 of the token exchanged, and registers 8 k on hold tokens 16 k + 8 hi on, as P
 // has to be as the operand of the second product: nothing crosses lanes. V^T is
-// read from V's rows by LDS reads that transpose. K's 16-byte chunks are
-// exchanged by the low bits of the row and V's by twice those of the token, so
+// read from V's rows by LDS reads that transpose. The 16-byte chunks of a row of
+// K are exchanged by the row's low bits, those of V by twice its lowest two, so
 // that lanes read from different banks.
 template <typename T, bool F8, int DT, bool FULL, int NW, int RW>
 struct Wide {
@@ -214,62 +224,77 @@ struct Wide {
   Frag q[KS];
   floatx16 o[DB];
   float ref, use, sum;
-  uintx4 kr[ITER], vr[ITER];
-  uint32_t row_ok;
+  int32_t pages[ITER];
+  uintx4 kr[F8 ? ITER : 1], vr[F8 ? ITER : 1];
 
   __device__ char* k_tile(int b) const { return lds + b * 2 * kTileBytes; }
   __device__ char* v_tile(int b) const { return lds + b * 2 * kTileBytes + kTileBytes; }
 
-  __device__ __forceinline__ void fetch(const WidePart& w, int tile) {
-    constexpr int ES = F8 ? 1 : 2;
-    const Params& a = p.a;
-    const int32_t* const table = a.tables + (p.first + w.leader) * a.table_stride;
-    row_ok = 0;
+  // The row of LDS that a thread's e-th 16 bytes are in, and the token that is in it.
+  __device__ static __forceinline__ int row_of(int e) { return (e * kThreads + (int)threadIdx.x) / UNITS; }
+  __device__ static __forceinline__ int token_of(int m) { return (m & ~12) | (m & 4) << 1 | (m & 8) >> 1; }
+
+  // The pages of a tile's tokens, -1 where there is none.
+  __device__ __forceinline__ void look(const WidePart& w, int tile) {
+    const int32_t* const table = p.a.tables + (p.first + w.leader) * p.a.table_stride;
 #pragma unroll
     for (int e = 0; e < ITER; ++e) {
-      const int idx = e * kThreads + threadIdx.x, row = idx / UNITS, unit = idx % UNITS;
-      const int t = tile * TT + row;
-      kr[e] = vr[e] = uintx4{0, 0, 0, 0};
-      if (t >= w.tokens) continue;
-      const int32_t page = table[t >> a.page_shift];
-      if (page < 0 || page >= a.pages) continue;
-      row_ok |= 1u << e;
-      if (!FULL && unit * (16 / ES) >= a.dim) continue;
-      const int64_t off = (page * a.page_stride + w.head * a.head_stride + (t & ((1 << a.page_shift) - 1)) * a.row_stride) * ES + unit * 16;
-      kr[e] = *(const uintx4*)(a.k + off);
-      vr[e] = *(const uintx4*)(a.v + off);
+      const int t = tile * TT + token_of(row_of(e));
+      pages[e] = t < w.tokens ? table[t >> p.a.page_shift] : -1;
     }
   }
 
-  __device__ __forceinline__ void store(int b) {
+  // Sends for a tile whose pages are known: to buffer b, or (e4m3, which is
+  // widened on the way) to registers.
+  __device__ __forceinline__ void fetch(const WidePart& w, int tile, int b) {
+    constexpr int ES = F8 ? 1 : 2;
+    const Params& a = p.a;
     bool all = true;
 #pragma unroll
     for (int e = 0; e < ITER; ++e) {
-      const int idx = e * kThreads + threadIdx.x, row = idx / UNITS, unit = idx % UNITS;
-      const int m = (row & ~12) | (row & 4) << 1 | (row & 8) >> 1;
-      char* const kd = k_tile(b) + m * RB;
-      char* const vd = v_tile(b) + row * RB;
-      const int kx = m & KEY, vx = (row & 3) << 1;
+      const int m = row_of(e), t = tile * TT + token_of(m), slot = (e * kThreads + (int)threadIdx.x) % UNITS;
+      const int32_t page = pages[e];
+      const bool in = page >= 0 && page < a.pages;
+      const int64_t off = (page * a.page_stride + w.head * a.head_stride + (t & ((1 << a.page_shift) - 1)) * a.row_stride) * ES;
       if constexpr (F8) {
-        const uintx4 k = kr[e], v = vr[e];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t k0 = h ? k.z : k.x, k1 = h ? k.w : k.y, v0 = h ? v.z : v.x, v1 = h ? v.w : v.y;
-          *(uintx4*)(kd + ((2 * unit + h) ^ kx) * 16) = uintx4{from_e4m3<T>(k0, false), from_e4m3<T>(k0, true), from_e4m3<T>(k1, false), from_e4m3<T>(k1, true)};
-          *(uintx4*)(vd + ((2 * unit + h) ^ vx) * 16) = uintx4{from_e4m3<PT>(v0, false), from_e4m3<PT>(v0, true), from_e4m3<PT>(v1, false), from_e4m3<PT>(v1, true)};
-        }
+        kr[e] = vr[e] = uintx4{0, 0, 0, 0};
+        if (in && (FULL || slot * 16 < a.dim)) kr[e] = *(const uintx4*)(a.k + off + slot * 16), vr[e] = *(const uintx4*)(a.v + off + slot * 16);
       } else {
-        *(uintx4*)(kd + (unit ^ kx) * 16) = kr[e];
-        *(uintx4*)(vd + (unit ^ vx) * 16) = vr[e];
+        const int kc = slot ^ (m & KEY), vc = slot ^ (m & 3) << 1, at = (e * kThreads + (int)threadIdx.x) * 16;
+        // a wave's 64 places are a run
+        const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)k_tile(b) + (e * kThreads + wave * 64) * 16);
+        if (in && (FULL || kc * 8 < a.dim)) load_lds(a.k + off + kc * 16, to);
+        else *(uintx4*)(k_tile(b) + at) = uintx4{0, 0, 0, 0};
+        if (in && (FULL || vc * 8 < a.dim)) load_lds(a.v + off + vc * 16, to + kTileBytes);
+        else *(uintx4*)(v_tile(b) + at) = uintx4{0, 0, 0, 0};
       }
-      const bool in = row_ok >> e & 1;
-      if (unit == 0) ok[b][row] = in;
+      if (slot == 0) ok[b][m] = in;
       all = all && in;
     }
     const bool any_bad = __any(!all);
     if (lane == 0) bad[b][wave] = any_bad;
   }
 
+  // e4m3: from the registers to buffer b.
+  __device__ __forceinline__ void store(int b) {
+    if constexpr (F8) {
+#pragma unroll
+      for (int e = 0; e < ITER; ++e) {
+        const int m = row_of(e), slot = (e * kThreads + (int)threadIdx.x) % UNITS;
+        char* const kd = k_tile(b) + m * RB;
+        char* const vd = v_tile(b) + m * RB;
+        const uintx4 k = kr[e], v = vr[e];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t k0 = h ? k.z : k.x, k1 = h ? k.w : k.y, v0 = h ? v.z : v.x, v1 = h ? v.w : v.y;
+          *(uintx4*)(kd + ((2 * slot + h) ^ (m & KEY)) * 16) = uintx4{from_e4m3<T>(k0, false), from_e4m3<T>(k0, true), from_e4m3<T>(k1, false), from_e4m3<T>(k1, true)};
+          *(uintx4*)(vd + ((2 * slot + h) ^ (m & 3) << 1) * 16) = uintx4{from_e4m3<PT>(v0, false), from_e4m3<PT>(v0, true), from_e4m3<PT>(v1, false), from_e4m3<PT>(v1, true)};
+        }
+      }
+    }
+  }
+
+  // A wave's tokens of buffer b under its rows. cs > 0.
   __device__ __forceinline__ void compute(int b, float cs) {
     const char* const kt = k_tile(b) + (tw * TPW + (lane & 31)) * RB;
     floatx16 s[NB];
@@ -281,24 +306,23 @@ struct Wide {
       for (int e = 0; e < KS; ++e)
         s[n] = mfma32<T>(*(const Frag*)(kt + n * 32 * RB + ((2 * e + hi) ^ (lane & KEY)) * 16), q[e], s[n]);
     }
-    int any_bad = 0;
+    int some = 0;  // of the tile's tokens are none
 #pragma unroll
-    for (int w = 0; w < NW; ++w) any_bad |= bad[b][w];
+    for (int x = 0; x < NW; ++x) some |= bad[b][x];
+    if (__builtin_amdgcn_readfirstlane(some)) {
+      asm volatile("");  // a branch, not selects in every tile
 #pragma unroll
-    for (int n = 0; n < NB; ++n) s[n] *= cs;
-    if (any_bad) {
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (!ok[b][tw * TPW + n * 32 + 16 * (r / 8) + 8 * hi + r % 8]) s[n][r] = -__builtin_inff();
-      }
+          if (!ok[b][tw * TPW + n * 32 + 8 * (r / 4) + 4 * hi + r % 4]) s[n][r] = -__builtin_inff();
     }
     float top = s[0][0];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+    top *= cs;
     if (__any(top > ref + (kTop + kLag))) {
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const float now = fmaxf(ref, top - kTop);
@@ -311,27 +335,24 @@ struct Wide {
     }
     // lane's place in the 4 x 16 blocks that it reads with 15 others
     const int i = lane & 15, g1 = lane >> 4 & 1, x = 2 * (i / 4);
-    const char* const vt = v_tile(b) + (tw * TPW + 8 * hi + i / 4) * RB + 8 * (i & 1);
+    const char* const vt = v_tile(b) + (tw * TPW + 4 * hi + i / 4) * RB + 8 * (i & 1);
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        Frag wh, wl;
+        Frag w;
 #pragma unroll
         for (int r = 0; r < 8; r += 2) {
-          const float a = __builtin_amdgcn_exp2f(s[n][8 * k + r] - use), c = __builtin_amdgcn_exp2f(s[n][8 * k + r + 1] - use);
-          sum += a + c;
-          wh[r / 2] = pack2<PT>(a, c);
-          const floatx2 back = unpack2<PT>(wh[r / 2]);
-          wl[r / 2] = pack2<PT>(a - back.x, c - back.y);
+          const float z0 = s[n][8 * k + r], z1 = s[n][8 * k + r + 1];
+          const float y0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z0, cs, -use)), y1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z1, cs, -use));
+          sum += y0 + y1;
+          w[r / 2] = pack2<PT>(y0, y1);
         }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           const char* const at = vt + (n * 32 + 16 * k) * RB + ((4 * d + 2 * g1 + (i % 4) / 2) ^ x) * 16;
-          const uintx2 v0 = read_column(at), v1 = read_column(at + 4 * RB);
-          const Frag f = {v0.x, v0.y, v1.x, v1.y};
-          o[d] = mfma32<PT>(f, wh, o[d]);
-          o[d] = mfma32<PT>(f, wl, o[d]);
+          const uintx2 v0 = read_column(at), v1 = read_column(at + 8 * RB);
+          o[d] = mfma32<PT>(Frag{v0.x, v0.y, v1.x, v1.y}, w, o[d]);
         }
       }
   }
@@ -352,14 +373,24 @@ struct Wide {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = 0;
     ref = -__builtin_inff(), use = 0.f, sum = 0.f;
-    const float cs = a.scale * (a.k_scale ? a.k_scale[w.head] : 1.f);
-    fetch(w, w.c);
+    float cs = a.scale * (a.k_scale ? a.k_scale[w.head] : 1.f);
+    if (cs < 0.f) {  // the queries take the sign, so that the largest score is the largest product's
+      cs = -cs;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) q[s] ^= 0x80008000u;
+    }
+    if (cs == 0.f) cs = 0x1p-126f;  // a masked score, -inf, times it stays that
+    look(w, w.c);
     __syncthreads();  // what was in LDS before has been read
+    fetch(w, w.c, 0);
+    if (w.c + 1 < w.c1) look(w, w.c + 1);
     store(0);
     for (int t = w.c; t < w.c1; ++t) {
       const int b = (t - w.c) & 1;
+      loads_done();
       __syncthreads();
-      if (t + 1 < w.c1) fetch(w, t + 1);
+      if (t + 1 < w.c1) fetch(w, t + 1, b ^ 1);
+      if (t + 2 < w.c1) look(w, t + 2);
       compute(b, cs);
       if (t + 1 < w.c1) store(b ^ 1);
     }
