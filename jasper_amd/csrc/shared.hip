@@ -33,17 +33,19 @@ constexpr int kBatch = 1024;     // sequences of a launch
 constexpr int kGroups = 256;     // work-groups at most
 constexpr int kStage = 512;      // row offsets of a wave, in LDS
 constexpr int kJoin = 256;       // threads of a joining work-group
-constexpr int kWideStart = 8;    // what beginning a wide stream and a tile of it
-constexpr int kWideTile = 4;     // cost, in tiles of 32 tokens of a wave
+constexpr int kWideStart = 8;    // what beginning a wide stream and a tile of it cost,
+constexpr int wide_tile(int dt) { return 256 / dt; }  // in tiles of 32 tokens of a wave
 
 constexpr int waves_of(int dt) { return dt == 256 ? 4 : 8; }    // of a work-group
-constexpr int tokens_of(int dt) { return dt == 256 ? 64 : 128; }  // of a wide tile
+constexpr int tokens_of(int dt) { return 8192 / dt; }             // of a wide tile: 16 KB of K
+constexpr int kRows = 128;       // query rows of a work-group
 __host__ __device__ constexpr int part_row(int dt) { return dt + 4; }  // floats: sums of V, ref, sum
 
 struct Shared {
   Params a;  // lists: the key heads
   const int32_t *groups, *shared;
   int n_groups;
+  bool far;  // rows of a page are more than 2^31 bytes apart
   int first, count;  // sequences of this launch
   int4* prefix_ends;  // [count * q_heads]: work-groups (or waves) that have parts, first and last, the row in them, 1 wide 0 thin; first -1: none
   int2* own_ends;     // [count * q_heads]: waves, first and last
@@ -88,9 +90,9 @@ __device__ __forceinline__ int block_scan(int x, int* part, int& total) {
   return before + incl - x;
 }
 
-template <int NW, int R, int TT>
+template <int NW, int DT>
 __device__ void lay_out(const Shared& p, Layout& l) {
-  constexpr int kThreads = NW * 64, kRun = kBatch / kThreads;
+  constexpr int kThreads = NW * 64, kRun = kBatch / kThreads, R = kRows, TT = tokens_of(DT), kWideTile = wide_tile(DT);
   const int t = threadIdx.x, gh = p.a.group;
   for (int i = t; i < kBatch; i += kThreads) l.leader[i] = 0x7FFFFFFF, l.last[i] = -1, l.from[i] = 0, l.own[i] = 0;
   __syncthreads();
@@ -181,135 +183,168 @@ struct WidePart {
 };
 
 // A wave's 64 times 16 bytes from memory to LDS at `to` on, in the lanes' order,
-// past the registers; lanes that do not take part leave theirs out. Waited for by
-// loads_done. (In LDS the compiler does not see these writes coming: they go to
-// the tile that nobody reads before the next barrier.)
+// past the registers; lanes that do not take part leave theirs out. They arrive
+// in order and are waited for by loads_left. (The compiler does not see these
+// writes to LDS coming: they go to tiles that nobody reads before a barrier.)
 __device__ __forceinline__ void load_lds(const void* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "memory");
 }
-__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+__device__ __forceinline__ void load_lds(const char* base, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(to) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void loads_left() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
 
 // One work-group over tiles [c, c1) of a wide stream; the sums end up in the
-// waves of the tile's first tokens. LDS: two tiles of K and V, of which one is
-// filled while the other is used.
+// waves of the tile's first tokens. LDS holds four tiles of K and V: while the
+// weights of one are found and multiplied with its values, the next one's scores
+// are multiplied, and two more are on their way. Waves are four times 32 query
+// rows, and as many for other tokens of the tile as there are more.
 //
 // S^T = K Q^T and O^T = V^T P^T on 32x32x16 products, hi = lane / 32. A lane's
 // column is a query row all the way: S comes out with the scores of rows 8 a + 4
 // hi + c of K in register 4 a + c, so the rows are put into LDS with bits 2 and
 // 3 of the token exchanged, and registers 8 k on hold tokens 16 k + 8 hi on, as P
 // has to be as the operand of the second product: nothing crosses lanes. V^T is
-// read from V's rows by LDS reads that transpose. The 16-byte chunks of a row of
-// K are exchanged by the row's low bits, those of V by twice its lowest two, so
-// that lanes read from different banks.
-template <typename T, bool F8, int DT, bool FULL, int NW, int RW>
+// read from V's rows by LDS reads that transpose. The 16-byte chunks of a row are
+// exchanged by bits of the row so that lanes read from different banks: of reads
+// of 16 bytes 16 lanes at once (8.6 cycles a read of a wave, 10.5 otherwise), of
+// those that transpose 16 and 32 lanes (5.6 cycles, 8.1 without).
+template <typename T, bool F8, int DT, bool FULL>
 struct Wide {
   typedef std::conditional_t<F8, f16, T> PT;
-  static constexpr int TT = tokens_of(DT), TW = NW / RW, TPW = TT / TW, NB = TPW / 32;
-  static constexpr int RB = DT * 2, CH = RB / 16, KEY = CH < 16 ? CH - 1 : 15;
-  static constexpr int kThreads = NW * 64, kTileBytes = TT * RB;
-  static constexpr int UNITS = F8 ? CH / 2 : CH, ITER = TT * UNITS / kThreads;  // 16-byte loads of a row, of a thread
-  static constexpr int KS = DT / 16, DB = DT / 32;
+  static constexpr int NW = waves_of(DT), TT = tokens_of(DT), TW = NW / 4, TPW = TT / TW, NB = TPW / 32;
+  static constexpr int RB = DT * 2, CH = RB / 16;
+  static constexpr int kThreads = NW * 64, kTileBytes = TT * RB, kBuffers = 4;
+  // 16-byte loads of a row; of a thread for a tile of K; rows of a wave's load
+  static constexpr int UNITS = F8 ? CH / 2 : CH, ITER = TT * UNITS / kThreads, RPL = 64 / UNITS;
+  static constexpr int KS = DT / 16, DB = DT / 32, ES = F8 ? 1 : 2;
   static constexpr float kLag = 3.f, kTop = std::is_same_v<PT, f16> ? 12.f : -kLag;  // as in attend_tiles
-  static constexpr int kLds = 4 * kTileBytes;
+  static constexpr int kLds = kBuffers * 2 * kTileBytes;
   static_assert(NB >= 1 && ITER >= 1, "a tile is too small");
-  static_assert((TW - 1) * RW * (DB * 16 + 2) * 64 * 4 <= kLds, "the waves' sums do not fit");
+  static_assert((TW - 1) * 4 * (DB * 16 + 2) * 64 * 4 <= kLds, "the waves' sums do not fit");
+
+  typedef floatx16 Scores[NB];
+  struct Staged {
+    uintx4 k[F8 ? ITER : 1], v[F8 ? ITER : 1];
+  };
 
   const Shared& p;
   char* const lds;
   uint8_t (*const ok)[TT];
-  int (*const bad)[NW];
   const int lane = threadIdx.x & 63, hi = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rw = wave % RW, tw = wave / RW;
+  const int rw = wave / TW, tw = wave % TW;
 
   Frag q[KS];
   floatx16 o[DB];
-  float ref, use, sum;
-  int32_t pages[ITER];
-  uintx4 kr[F8 ? ITER : 1], vr[F8 ? ITER : 1];
+  float ref, use, sum, cs;
+  bool holes;  // tokens without a page, or strides past 32 bits
+  int32_t page_a[ITER], page_b[ITER];  // of a wave's loads: the pages of their first and second eight tokens
+  uint32_t k_off[ITER], v_off[ITER];
 
   __device__ char* k_tile(int b) const { return lds + b * 2 * kTileBytes; }
   __device__ char* v_tile(int b) const { return lds + b * 2 * kTileBytes + kTileBytes; }
 
-  // The row of LDS that a thread's e-th 16 bytes are in, and the token that is in it.
+  // The row of LDS that a thread's e-th 16 bytes are in, their place in it, and the token that is in a row.
   __device__ static __forceinline__ int row_of(int e) { return (e * kThreads + (int)threadIdx.x) / UNITS; }
+  __device__ static __forceinline__ int slot_of(int e) { return (e * kThreads + (int)threadIdx.x) % UNITS; }
   __device__ static __forceinline__ int token_of(int m) { return (m & ~12) | (m & 4) << 1 | (m & 8) >> 1; }
+  __device__ static __forceinline__ int k_key(int m) { return CH == 8 ? m >> 1 & 7 : m & 15; }
+  __device__ static __forceinline__ int v_key(int m) { return CH == 8 ? (m & 3) << 1 : (m & 3) << 1 | (m & 1) << 3; }
 
-  // The pages of a tile's tokens, -1 where there is none.
+  __device__ __forceinline__ bool whole(const WidePart& w, int tile) const { return !holes && (tile + 1) * TT <= w.tokens; }
+
+  // The pages of a tile's tokens, by scalar loads.
   __device__ __forceinline__ void look(const WidePart& w, int tile) {
-    const int32_t* const table = p.a.tables + (p.first + w.leader) * p.a.table_stride;
+    typedef __attribute__((address_space(4))) const int32_t* Table;
+    const Table table = (Table)(uintptr_t)(p.a.tables + (p.first + w.leader) * p.a.table_stride);
+    const int last = w.tokens - 1;
 #pragma unroll
     for (int e = 0; e < ITER; ++e) {
-      const int t = tile * TT + token_of(row_of(e));
-      pages[e] = t < w.tokens ? table[t >> p.a.page_shift] : -1;
+      const int m = (e * NW + wave) * RPL;  // the first row of the wave's load
+      const int t = tile * TT + (RPL >= 8 ? m & ~15 : token_of(m) & ~7);
+      page_a[e] = table[min(t, last) >> p.a.page_shift];
+      if constexpr (RPL >= 8) page_b[e] = table[min(t + 8, last) >> p.a.page_shift];
     }
   }
 
   // Sends for a tile whose pages are known: to buffer b, or (e4m3, which is
   // widened on the way) to registers.
-  __device__ __forceinline__ void fetch(const WidePart& w, int tile, int b) {
-    constexpr int ES = F8 ? 1 : 2;
+  __device__ __forceinline__ void fetch(const WidePart& w, int tile, int b, Staged& st) {
     const Params& a = p.a;
-    bool all = true;
+    const int64_t at = w.head * a.head_stride + (int64_t)(tile * TT & ((1 << a.page_shift) - 1)) * a.row_stride;
+    const bool all = whole(w, tile);
 #pragma unroll
     for (int e = 0; e < ITER; ++e) {
-      const int m = row_of(e), t = tile * TT + token_of(m), slot = (e * kThreads + (int)threadIdx.x) % UNITS;
-      const int32_t page = pages[e];
-      const bool in = page >= 0 && page < a.pages;
-      const int64_t off = (page * a.page_stride + w.head * a.head_stride + (t & ((1 << a.page_shift) - 1)) * a.row_stride) * ES;
-      if constexpr (F8) {
-        kr[e] = vr[e] = uintx4{0, 0, 0, 0};
-        if (in && (FULL || slot * 16 < a.dim)) kr[e] = *(const uintx4*)(a.k + off + slot * 16), vr[e] = *(const uintx4*)(a.v + off + slot * 16);
-      } else {
-        const int kc = slot ^ (m & KEY), vc = slot ^ (m & 3) << 1, at = (e * kThreads + (int)threadIdx.x) * 16;
-        // a wave's 64 places are a run
-        const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)k_tile(b) + (e * kThreads + wave * 64) * 16);
-        if (in && (FULL || kc * 8 < a.dim)) load_lds(a.k + off + kc * 16, to);
-        else *(uintx4*)(k_tile(b) + at) = uintx4{0, 0, 0, 0};
-        if (in && (FULL || vc * 8 < a.dim)) load_lds(a.v + off + vc * 16, to + kTileBytes);
-        else *(uintx4*)(v_tile(b) + at) = uintx4{0, 0, 0, 0};
+      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)k_tile(b) + (e * kThreads + wave * 64) * 16;
+      if (!F8 && RPL < 8 && all) {
+        const int64_t off = (page_a[e] * a.page_stride + at) * ES;
+        if (FULL || (slot_of(e) ^ k_key(row_of(e))) * 8 < a.dim) load_lds(a.k + off, k_off[e], to);
+        if (FULL || (slot_of(e) ^ v_key(row_of(e))) * 8 < a.dim) load_lds(a.v + off, v_off[e], to + kTileBytes);
+        continue;
       }
-      if (slot == 0) ok[b][m] = in;
-      all = all && in;
+      const int m = row_of(e), slot = slot_of(e), r = token_of(m);
+      const int32_t page = RPL >= 8 && m & 4 ? page_b[e] : page_a[e];
+      const bool in = all || (page >= 0 && page < a.pages && tile * TT + r < w.tokens);
+      const char* const row = (const char*)((page * a.page_stride + at + (int64_t)(r & ((1 << a.page_shift) - 1)) * a.row_stride) * ES);
+      if constexpr (F8) {
+        st.k[e] = st.v[e] = uintx4{0, 0, 0, 0};
+        if (in && (FULL || slot * 16 < a.dim)) {
+          st.k[e] = *(const uintx4*)(a.k + (intptr_t)row + slot * 16);
+          st.v[e] = *(const uintx4*)(a.v + (intptr_t)row + slot * 16);
+        }
+      } else {
+        const int kc = slot ^ k_key(m), vc = slot ^ v_key(m), place = (e * kThreads + (int)threadIdx.x) * 16;
+        if (in && (FULL || kc * 8 < a.dim)) load_lds(a.k + (intptr_t)row + kc * 16, to);
+        else if (!all) *(uintx4*)(k_tile(b) + place) = uintx4{0, 0, 0, 0};
+        if (in && (FULL || vc * 8 < a.dim)) load_lds(a.v + (intptr_t)row + vc * 16, to + kTileBytes);
+        else if (!all) *(uintx4*)(v_tile(b) + place) = uintx4{0, 0, 0, 0};
+      }
+      if (!all && slot == 0) ok[b][m] = in;
     }
-    const bool any_bad = __any(!all);
-    if (lane == 0) bad[b][wave] = any_bad;
   }
 
   // e4m3: from the registers to buffer b.
-  __device__ __forceinline__ void store(int b) {
-    if constexpr (F8) {
+  __device__ __forceinline__ void store(int b, const Staged& st) {
 #pragma unroll
-      for (int e = 0; e < ITER; ++e) {
-        const int m = row_of(e), slot = (e * kThreads + (int)threadIdx.x) % UNITS;
-        char* const kd = k_tile(b) + m * RB;
-        char* const vd = v_tile(b) + m * RB;
-        const uintx4 k = kr[e], v = vr[e];
+    for (int e = 0; e < ITER; ++e) {
+      const int m = row_of(e), slot = slot_of(e);
+      char* const kd = k_tile(b) + m * RB;
+      char* const vd = v_tile(b) + m * RB;
+      const uintx4 k = st.k[e], v = st.v[e];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t k0 = h ? k.z : k.x, k1 = h ? k.w : k.y, v0 = h ? v.z : v.x, v1 = h ? v.w : v.y;
-          *(uintx4*)(kd + ((2 * slot + h) ^ (m & KEY)) * 16) = uintx4{from_e4m3<T>(k0, false), from_e4m3<T>(k0, true), from_e4m3<T>(k1, false), from_e4m3<T>(k1, true)};
-          *(uintx4*)(vd + ((2 * slot + h) ^ (m & 3) << 1) * 16) = uintx4{from_e4m3<PT>(v0, false), from_e4m3<PT>(v0, true), from_e4m3<PT>(v1, false), from_e4m3<PT>(v1, true)};
-        }
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t k0 = h ? k.z : k.x, k1 = h ? k.w : k.y, v0 = h ? v.z : v.x, v1 = h ? v.w : v.y;
+        *(uintx4*)(kd + ((2 * slot + h) ^ k_key(m)) * 16) = uintx4{from_e4m3<T>(k0, false), from_e4m3<T>(k0, true), from_e4m3<T>(k1, false), from_e4m3<T>(k1, true)};
+        *(uintx4*)(vd + ((2 * slot + h) ^ v_key(m)) * 16) = uintx4{from_e4m3<PT>(v0, false), from_e4m3<PT>(v0, true), from_e4m3<PT>(v1, false), from_e4m3<PT>(v1, true)};
       }
     }
   }
 
-  // A wave's tokens of buffer b under its rows. cs > 0.
-  __device__ __forceinline__ void compute(int b, float cs) {
+  // A wave's tokens of buffer b as operands of the first product.
+  __device__ __forceinline__ void read_keys(int b, Frag (&f)[NB * KS]) const {
     const char* const kt = k_tile(b) + (tw * TPW + (lane & 31)) * RB;
-    floatx16 s[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < KS; ++e) f[n * KS + e] = *(const Frag*)(kt + n * 32 * RB + ((2 * e + hi) ^ k_key(lane & 31)) * 16);
+  }
+
+  __device__ __forceinline__ void scores(const Frag (&f)[NB * KS], Scores& s) const {
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[n][r] = 0;
 #pragma unroll
-      for (int e = 0; e < KS; ++e)
-        s[n] = mfma32<T>(*(const Frag*)(kt + n * 32 * RB + ((2 * e + hi) ^ (lane & KEY)) * 16), q[e], s[n]);
+      for (int e = 0; e < KS; ++e) s[n] = mfma32<T>(f[n * KS + e], q[e], s[n]);
     }
-    int some = 0;  // of the tile's tokens are none
-#pragma unroll
-    for (int x = 0; x < NW; ++x) some |= bad[b][x];
-    if (__builtin_amdgcn_readfirstlane(some)) {
+  }
+
+  // Scores that are none left out; the reference moved where one is too large for it.
+  __device__ __forceinline__ void settle(const WidePart& w, int tile, int b, Scores& s) {
+    if (!whole(w, tile)) {
       asm volatile("");  // a branch, not selects in every tile
 #pragma unroll
       for (int n = 0; n < NB; ++n)
@@ -333,28 +368,88 @@ struct Wide {
       for (int d = 0; d < DB; ++d) o[d] *= keep;
       ref = now, use = to;
     }
-    // lane's place in the 4 x 16 blocks that it reads with 15 others
-    const int i = lane & 15, g1 = lane >> 4 & 1, x = 2 * (i / 4);
-    const char* const vt = v_tile(b) + (tw * TPW + 4 * hi + i / 4) * RB + 8 * (i & 1);
+  }
+
+  // The weights of scores, rounded to their type once: a second term of them is
+  // half again as many products, and takes bf16's error from 0.0019 to the
+  // output's own 0.0017.
+  __device__ __forceinline__ void weigh(const Scores& s, Frag (&w)[NB * 2]) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int n = 0; n < NB * 2; ++n)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        Frag w;
-#pragma unroll
-        for (int r = 0; r < 8; r += 2) {
-          const float z0 = s[n][8 * k + r], z1 = s[n][8 * k + r + 1];
-          const float y0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z0, cs, -use)), y1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z1, cs, -use));
-          sum += y0 + y1;
-          w[r / 2] = pack2<PT>(y0, y1);
-        }
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const char* const at = vt + (n * 32 + 16 * k) * RB + ((4 * d + 2 * g1 + (i % 4) / 2) ^ x) * 16;
-          const uintx2 v0 = read_column(at), v1 = read_column(at + 8 * RB);
-          o[d] = mfma32<PT>(Frag{v0.x, v0.y, v1.x, v1.y}, w, o[d]);
-        }
+      for (int r = 0; r < 8; r += 2) {
+        const float y0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 2][n % 2 * 8 + r], cs, -use));
+        const float y1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 2][n % 2 * 8 + r + 1], cs, -use));
+        sum += y0 + y1;
+        w[n][r / 2] = pack2<PT>(y0, y1);
       }
+  }
+
+  // Sixteen tokens, n * 16 on, of a wave's in buffer b as operands of the second product.
+  __device__ __forceinline__ void read_values(int b, int n, Frag (&f)[DB]) const {
+    // lane's place in the 4 x 16 blocks that it reads with 15 others
+    const int i = lane & 15, g1 = lane >> 4 & 1;
+    const char* const vt = v_tile(b) + (tw * TPW + n * 16 + 4 * hi + i / 4) * RB + 8 * (i & 1);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const char* const at = vt + ((4 * d + 2 * g1 + (i % 4) / 2) ^ v_key(i / 4)) * 16;
+      const uintx2 v0 = read_column(at), v1 = read_column(at + 8 * RB);
+      f[d] = Frag{v0.x, v0.y, v1.x, v1.y};
+    }
+  }
+
+  __device__ __forceinline__ void add_values(const Frag (&f)[DB], Frag w) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = mfma32<PT>(f[d], w, o[d]);
+  }
+
+  __device__ __forceinline__ void values(int b, const Frag (&w)[NB * 2]) {
+    Frag f[2][DB];
+    read_values(b, 0, f[0]);
+#pragma unroll
+    for (int n = 0; n < NB * 2; ++n) {
+      if (n + 1 < NB * 2) read_values(b, n + 1, f[n + 1 & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      add_values(f[n & 1], w[n]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // Tile t's weights and values with tile t + 1's scores: what is on its way then is t + 2 and t + 3.
+  __device__ __forceinline__ void step(const WidePart& w, int t, const Scores& now, Scores& next, Staged& st) {
+    const int b = t - w.c;
+    if constexpr (F8) {
+      __syncthreads();
+      if (t + 2 < w.c1) store((b + 2) & 3, st);
+      if (t + 4 < w.c1) fetch(w, t + 4, (b + 4) & 3, st);
+      if (t + 5 < w.c1) look(w, t + 5);
+    } else {
+      if (t + 2 < w.c1 && whole(w, t + 2)) loads_left<2 * ITER>();
+      else loads_left<0>();
+      __syncthreads();
+      if (t + 3 < w.c1) fetch(w, t + 3, (b + 3) & 3, st);
+      if (t + 4 < w.c1) look(w, t + 4);
+    }
+    // The order matters, and the compiler would put every read right before its
+    // product: keys are read while weights are found, the first values while the
+    // keys are multiplied.
+    Frag kf[NB * KS], wf[NB * 2], vf[2][DB];
+    read_keys((b + 1) & 3, kf);
+    __builtin_amdgcn_sched_barrier(0);
+    weigh(now, wf);
+    __builtin_amdgcn_sched_barrier(0);
+    read_values(b & 3, 0, vf[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    scores(kf, next);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < NB * 2; ++n) {
+      if (n + 1 < NB * 2) read_values(b & 3, n + 1, vf[n + 1 & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      add_values(vf[n & 1], wf[n]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    settle(w, t + 1, (b + 1) & 3, next);
   }
 
   __device__ void run(const WidePart& w) {
@@ -373,7 +468,7 @@ struct Wide {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = 0;
     ref = -__builtin_inff(), use = 0.f, sum = 0.f;
-    float cs = a.scale * (a.k_scale ? a.k_scale[w.head] : 1.f);
+    cs = a.scale * (a.k_scale ? a.k_scale[w.head] : 1.f);
     if (cs < 0.f) {  // the queries take the sign, so that the largest score is the largest product's
       cs = -cs;
 #pragma unroll
@@ -381,26 +476,66 @@ struct Wide {
     }
     if (cs == 0.f) cs = 0x1p-126f;  // a masked score, -inf, times it stays that
     look(w, w.c);
-    __syncthreads();  // what was in LDS before has been read
-    fetch(w, w.c, 0);
-    if (w.c + 1 < w.c1) look(w, w.c + 1);
-    store(0);
-    for (int t = w.c; t < w.c1; ++t) {
-      const int b = (t - w.c) & 1;
-      loads_done();
-      __syncthreads();
-      if (t + 1 < w.c1) fetch(w, t + 1, b ^ 1);
-      if (t + 2 < w.c1) look(w, t + 2);
-      compute(b, cs);
-      if (t + 1 < w.c1) store(b ^ 1);
+    bool hole = p.far;
+    const int first = w.c * TT >> a.page_shift, last = (min(w.c1 * TT, w.tokens) - 1) >> a.page_shift;
+    for (int i = first + (int)threadIdx.x; i <= last; i += kThreads) {
+      const int32_t page = a.tables[(p.first + w.leader) * a.table_stride + i];
+      hole = hole || page < 0 || page >= a.pages;
     }
+    holes = __syncthreads_or(hole);  // and what was in LDS before has been read
+#pragma unroll
+    for (int e = 0; e < ITER; ++e) {
+      const int m = row_of(e), slot = slot_of(e);
+      const uint32_t r = (uint32_t)((token_of(m) & ((1 << a.page_shift) - 1)) * a.row_stride * ES);
+      k_off[e] = r + (slot ^ k_key(m)) * 16, v_off[e] = r + (slot ^ v_key(m)) * 16;
+      if (!FULL && !F8 && (slot ^ k_key(m)) * 8 >= a.dim)
+        for (int b = 0; b < kBuffers; ++b) *(uintx4*)(k_tile(b) + (e * kThreads + (int)threadIdx.x) * 16) = uintx4{0, 0, 0, 0};
+    }
+    Staged st[2];
+    Scores s[2];
+    const int n = w.c1 - w.c;
+    if constexpr (F8) {
+      fetch(w, w.c, 0, st[0]);
+      if (n > 1) look(w, w.c + 1), fetch(w, w.c + 1, 1, st[1]);
+      store(0, st[0]);
+      if (n > 2) look(w, w.c + 2), fetch(w, w.c + 2, 2, st[0]);
+      if (n > 1) store(1, st[1]);
+      if (n > 3) look(w, w.c + 3), fetch(w, w.c + 3, 3, st[1]);
+      if (n > 4) look(w, w.c + 4);
+    } else {
+      for (int b = 0; b < min(n, 3); ++b) {
+        if (b) look(w, w.c + b);
+        fetch(w, w.c + b, b, st[0]);
+      }
+      if (n > 3) look(w, w.c + 3);
+      if (n > 2 && whole(w, w.c + 2)) loads_left<4 * ITER>();
+      else loads_left<0>();
+    }
+    __syncthreads();
+    Frag kf[NB * KS], wf[NB * 2];
+    read_keys(0, kf);
+    scores(kf, s[0]);
+    settle(w, w.c, 0, s[0]);
+    int t = w.c;
+    for (; t + 2 < w.c1; t += 2) {
+      step(w, t, s[0], s[1], st[0]);
+      step(w, t + 1, s[1], s[0], st[1]);
+    }
+    if (t + 1 < w.c1) {
+      step(w, t, s[0], s[1], st[0]);
+      weigh(s[1], wf);
+      ++t;
+    } else {
+      weigh(s[0], wf);
+    }
+    values((t - w.c) & 3, wf);
     sum += __shfl_xor(sum, 32, 64);
     if constexpr (TW > 1) {
       constexpr int kOne = (DB * 16 + 2) * 64;
       float* const all = (float*)lds;
       __syncthreads();
       if (tw) {
-        float* const mine = all + ((tw - 1) * RW + rw) * kOne + lane;
+        float* const mine = all + ((tw - 1) * 4 + rw) * kOne + lane;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -411,17 +546,17 @@ struct Wide {
       if (tw == 0) {
 #pragma unroll 1
         for (int other = 0; other < TW - 1; ++other) {
-          const float* const its = all + (other * RW + rw) * kOne + lane;
-          const float its_ref = its[DB * 16 * 64], now = fmaxf(ref, its_ref);
+          const float* const its = all + (other * 4 + rw) * kOne + lane;
+          const float its_ref = its[DB * 16 * 64], top = fmaxf(ref, its_ref);
           // without scores so far the sums are zero (or NaN)
-          const float mine = ref == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ref - now);
-          const float theirs = its_ref == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(its_ref - now);
+          const float mine = ref == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ref - top);
+          const float theirs = its_ref == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(its_ref - top);
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * mine + its[(d * 16 + r) * 64] * theirs;
           sum = sum * mine + its[(DB * 16 + 1) * 64] * theirs;
-          ref = now;
+          ref = top;
         }
       }
     }
@@ -436,7 +571,7 @@ struct Wide {
     const int member = w.leader + at / a.group;
     const int64_t out = (int64_t)member * a.q_heads + w.head * a.group + at % a.group;
     float* const part = w.c == 0 ? p.prefix_first + out * part_row(DT)
-                                 : p.wide_rest + ((int64_t)blockIdx.x * 32 * RW + row) * part_row(DT);
+                                 : p.wide_rest + ((int64_t)blockIdx.x * kRows + row) * part_row(DT);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -449,15 +584,15 @@ struct Wide {
   }
 };
 
-template <typename T, bool F8, int DT, bool FULL, int NW, int RW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void shared_kernel(Shared p) {
-  typedef Wide<T, F8, DT, FULL, NW, RW> W;
+template <typename T, bool F8, int DT, bool FULL>
+__global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_kernel(Shared p) {
+  typedef Wide<T, F8, DT, FULL> W;
+  constexpr int NW = W::NW, kWideTile = wide_tile(DT);
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ Layout l;
-  __shared__ uint8_t ok[2][W::TT];
-  __shared__ int bad[2][NW];
+  __shared__ uint8_t ok[W::kBuffers][W::TT];
   const Params& a = p.a;
-  lay_out<NW, 32 * RW, W::TT>(p, l);
+  lay_out<NW, DT>(p, l);
   const int wides = l.totals[0], thins = l.totals[1], total = wides + thins + l.totals[2];
   Share share;
   // a work-group has units for all of its waves, and at least a wide tile's: so
@@ -473,17 +608,17 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void shared_kernel(Shared p) {
     WidePart w;
     w.leader = __builtin_amdgcn_readfirstlane(l.leader[i]);
     w.tokens = __builtin_amdgcn_readfirstlane(l.from[w.leader]);
-    const int m = (__builtin_amdgcn_readfirstlane(l.last[i]) - w.leader + 1) * a.group, row_tiles = ceil_div(m, 32 * RW);
+    const int m = (__builtin_amdgcn_readfirstlane(l.last[i]) - w.leader + 1) * a.group, row_tiles = ceil_div(m, kRows);
     const int tiles = ceil_div(w.tokens, W::TT), cost = kWideStart + tiles * kWideTile;
     const int x = (u - l.wide[i]) / cost, pos = (u - l.wide[i]) % cost, begin = u - pos;
     w.head = __builtin_amdgcn_readfirstlane(x / row_tiles);
-    w.row0 = __builtin_amdgcn_readfirstlane(x % row_tiles * 32 * RW);
-    w.rows = min(32 * RW, m - w.row0);
+    w.row0 = __builtin_amdgcn_readfirstlane(x % row_tiles * kRows);
+    w.rows = min(kRows, m - w.row0);
     const int end = min(cost, pos + (u1 - u));
     w.c = __builtin_amdgcn_readfirstlane(ceil_div(max(0, pos - kWideStart), kWideTile));
     w.c1 = __builtin_amdgcn_readfirstlane(ceil_div(max(0, end - kWideStart), kWideTile));
     if (w.c < w.c1) {
-      W wide{p, lds, ok, bad};
+      W wide{p, lds, ok};
       wide.run(w);
       wide.write(w, int2{(int)blockIdx.x, share.owner(begin + kWideStart + (tiles - 1) * kWideTile)}, l);
     }
@@ -562,13 +697,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void shared_kernel(Shared p) {
   }
 }
 
-// Joins the parts of a query row: a thread has four dims of every kRows-th part.
-template <typename T, int DT, int R>
+// Joins the parts of a query row: a thread has four dims of every kAtOnce-th part.
+template <typename T, int DT>
 __global__ __launch_bounds__(kJoin) void join_kernel(Shared p) {
-  constexpr int kLanes = DT / 4, kRows = kJoin / kLanes, kLoads = 8;
+  constexpr int kLanes = DT / 4, kAtOnce = kJoin / kLanes, kLoads = 8;
   __shared__ float weight[kGroups * (1 + 2 * waves_of(DT))];
   __shared__ float tops[kJoin / 64], tots[kJoin / 64];
-  __shared__ floatx4 sums[kRows][kLanes];
+  __shared__ floatx4 sums[kAtOnce][kLanes];
   const Params& a = p.a;
   const int64_t out = blockIdx.x;
   const int4 prefix = p.prefix_ends[out];
@@ -578,7 +713,7 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Shared p) {
   const auto part = [&](int i) -> const float* {
     if (i < n_prefix) {
       if (i == 0) return p.prefix_first + out * part_row(DT);
-      return prefix.w ? p.wide_rest + ((int64_t)(prefix.x + i) * R + prefix.z) * part_row(DT)
+      return prefix.w ? p.wide_rest + ((int64_t)(prefix.x + i) * kRows + prefix.z) * part_row(DT)
                       : p.wave_rest + ((int64_t)(prefix.x + i) * kHeads + prefix.z) * part_row(DT);
     }
     i -= n_prefix;
@@ -591,7 +726,7 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Shared p) {
   const auto fetch = [&](int i0) {
 #pragma unroll
     for (int e = 0; e < kLoads; ++e)
-      if (i0 + e * kRows < parts) y[e] = *(const floatx4*)(part(i0 + e * kRows) + d);
+      if (i0 + e * kAtOnce < parts) y[e] = *(const floatx4*)(part(i0 + e * kAtOnce) + d);
   };
   fetch(row);  // on their way while the weights are found
   float top = -__builtin_inff();
@@ -616,18 +751,18 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Shared p) {
   __syncthreads();
   tot = (tots[0] + tots[1]) + (tots[2] + tots[3]);
   floatx4 acc = {0, 0, 0, 0};
-  for (int i0 = row; i0 < parts; i0 += kRows * kLoads) {
+  for (int i0 = row; i0 < parts; i0 += kAtOnce * kLoads) {
     if (i0 != row) fetch(i0);
 #pragma unroll
     for (int e = 0; e < kLoads; ++e) {
-      const int i = i0 + e * kRows;
+      const int i = i0 + e * kAtOnce;
       if (i < parts) acc += y[e] * weight[i];
     }
   }
   sums[row][lane4] = acc;
   __syncthreads();
   if (row) return;
-  for (int r = 1; r < kRows; ++r) acc += sums[r][lane4];
+  for (int r = 1; r < kAtOnce; ++r) acc += sums[r][lane4];
   const int64_t at = (int64_t)p.first * a.q_heads + out;
   const float inv = (a.v_scale ? a.v_scale[head / a.group] : 1.f) / tot;
 #pragma unroll
@@ -648,7 +783,7 @@ int compute_units() {
 
 // How a call's work is laid out, from its sizes alone.
 struct Plan {
-  int dt, group, head_tiles, row_waves;
+  int dt, group, head_tiles;
   int64_t work_groups;
   int64_t ends, firsts, wide_rest, wave_rest, bytes;  // of the workspace: bytes of each
 };
@@ -663,40 +798,31 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_l
   const int64_t tiles = max_len / kTile + 2 + kStart + 2 * kWideStart;
   const int64_t per_seq = pages.heads * (2 * (int64_t)a.head_tiles + a.group / 32 + 2);
   if (tiles > 0x7FFFFFFF / std::max<int64_t>(1, count * per_seq)) throw std::invalid_argument("batch x heads x tokens is too large");
-  a.row_waves = count * a.group > 64 * std::max<int64_t>(1, std::min(n_groups, count)) ? 4 : 2;
   a.work_groups = std::min<int64_t>({kGroups, compute_units(), std::max<int64_t>(1, count * pages.heads * a.head_tiles * tiles)});
   const int64_t rows = count * q_heads, row = part_row(a.dt) * 4;
   a.ends = rows * 24, a.firsts = rows * row;
-  a.wide_rest = a.work_groups * 32 * a.row_waves * row;
+  a.wide_rest = a.work_groups * kRows * row;
   a.wave_rest = a.work_groups * waves_of(a.dt) * kHeads * row;
   a.bytes = (a.ends + 15) / 16 * 16 + 2 * a.firsts + a.wide_rest + a.wave_rest;
   return a;
 }
 
-template <typename T, bool F8, int DT, bool FULL, int RW>
-void launch(const Shared& p, const Plan& plan, hipStream_t s) {
-  constexpr int NW = waves_of(DT);
-  auto kernel = shared_kernel<T, F8, DT, FULL, NW, RW>;
-  constexpr int lds = std::max(Wide<T, F8, DT, FULL, NW, RW>::kLds, NW * kStage * 8);
-  hip_check(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "shared attention");
-  kernel<<<(unsigned)plan.work_groups, 64 * NW, lds, s>>>(p);
-  hip_check(hipGetLastError(), "shared attention");
-  join_kernel<T, DT, 32 * RW><<<(unsigned)(p.count * p.a.q_heads), kJoin, 0, s>>>(p);
-  hip_check(hipGetLastError(), "shared attention join");
-}
-
 template <typename T, bool F8, int DT>
-void launch_rows(const Shared& p, const Plan& plan, hipStream_t s) {
-  const bool full = p.a.dim == DT;
-  if (plan.row_waves == 4) full ? launch<T, F8, DT, true, 4>(p, plan, s) : launch<T, F8, DT, false, 4>(p, plan, s);
-  else full ? launch<T, F8, DT, true, 2>(p, plan, s) : launch<T, F8, DT, false, 2>(p, plan, s);
+void launch(const Shared& p, const Plan& plan, hipStream_t s) {
+  auto kernel = p.a.dim == DT ? shared_kernel<T, F8, DT, true> : shared_kernel<T, F8, DT, false>;
+  constexpr int lds = std::max(Wide<T, F8, DT, true>::kLds, waves_of(DT) * kStage * 8);
+  hip_check(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "shared attention");
+  kernel<<<(unsigned)plan.work_groups, 64 * waves_of(DT), lds, s>>>(p);
+  hip_check(hipGetLastError(), "shared attention");
+  join_kernel<T, DT><<<(unsigned)(p.count * p.a.q_heads), kJoin, 0, s>>>(p);
+  hip_check(hipGetLastError(), "shared attention join");
 }
 
 template <typename T, bool F8>
 void launch_dim(const Shared& p, const Plan& plan, hipStream_t s) {
-  if (plan.dt == 64) launch_rows<T, F8, 64>(p, plan, s);
-  else if (plan.dt == 128) launch_rows<T, F8, 128>(p, plan, s);
-  else launch_rows<T, F8, 256>(p, plan, s);
+  if (plan.dt == 64) launch<T, F8, 64>(p, plan, s);
+  else if (plan.dt == 128) launch<T, F8, 128>(p, plan, s);
+  else launch<T, F8, 256>(p, plan, s);
 }
 
 }  // namespace
@@ -726,6 +852,7 @@ void shared_attend(const AttendArgs& a, const int32_t* groups, const int32_t* sh
   r.group = plan.group, r.head_tiles = plan.head_tiles, r.side = 1;
   r.page_shift = pages.page_shift, r.pages = pages.pages, r.dim = pages.dim;
   p.groups = groups, p.shared = shared, p.n_groups = (int)n_groups;
+  p.far = pages.row_stride > 0x3FFFFFFF / pages.page;
   char* w = (char*)a.workspace;
   const int64_t rows = plan.ends / 24;
   p.prefix_ends = (int4*)w, p.own_ends = (int2*)(w + rows * 16);
