@@ -29,12 +29,14 @@ namespace {
 
 using namespace attention;
 
-constexpr int kBatch = 1024;     // sequences of a launch
+constexpr int kBatch = 512;      // sequences of a launch
 constexpr int kGroups = 256;     // work-groups at most
 constexpr int kStage = 512;      // row offsets of a wave, in LDS
 constexpr int kJoin = 256;       // threads of a joining work-group
-constexpr int kWideStart = 8;    // what beginning a wide stream and a tile of it cost,
-constexpr int wide_tile(int dt) { return 256 / dt; }  // in tiles of 32 tokens of a wave
+constexpr int kPages = 1024;     // of a wide stream's table, in LDS
+constexpr int kTeam = 8;         // work-groups of a team at most
+constexpr int kWideStart = 8;    // what beginning a wide stream and a tile of it
+constexpr int kWideTile = 3;     // cost, in tiles of 32 tokens of a wave
 
 constexpr int waves_of(int dt) { return dt == 256 ? 4 : 8; }    // of a work-group
 constexpr int tokens_of(int dt) { return 8192 / dt; }             // of a wide tile: 16 KB of K
@@ -47,8 +49,8 @@ struct Shared {
   int n_groups;
   bool far;  // rows of a page are more than 2^31 bytes apart
   int first, count;  // sequences of this launch
-  int4* prefix_ends;  // [count * q_heads]: work-groups (or waves) that have parts, first and last, the row in them, 1 wide 0 thin; first -1: none
-  int2* own_ends;     // [count * q_heads]: waves, first and last
+  int4* prefix_ends;  // [count * q_heads]: the work-group that begins the prefix, how many have parts, the row in them, the step from one to the next (0: they are waves)
+  int2* own_ends;     // [count * q_heads]: the wave that begins what a sequence has itself, how many have parts
   float *prefix_first, *own_first;  // [count * q_heads] part rows: the parts that begin a stream
   float *wide_rest;   // [work-groups][rows of a wide tile]: parts that go on with one
   float *wave_rest;   // [waves][16]
@@ -61,98 +63,145 @@ struct Layout {
   int from[kBatch];  // tokens that a sequence leaves to its group
   int leader[kBatch], last[kBatch];
   int wide[kBatch], thin[kBatch], own[kBatch];
+  int len[kBatch];
   int totals[3];
-  int part[3][16];
+  int part[3][8];
 };
 
 __device__ __forceinline__ int length_of(const Shared& p, int i) { return min(max(p.a.lens[p.first + i], 0), p.a.limit); }
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-template <int NW>
-__device__ __forceinline__ int block_scan(int x, int* part, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int incl = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(incl, d, 64);
-    if (lane >= d) incl += o;
-  }
-  if (lane == 63) part[wave] = incl;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    if (w == wave) before = total;
-    total += part[w];
-  }
-  return before + incl - x;
+// The sum of x over the lanes up to this one, without LDS.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // rows of 16 lanes, shifted by 1, 2, 4 and 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // lane 15 of a row to the next one
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // lane 31 to the last two
+  return x;
 }
 
+// For three numbers at once: their sums over the threads before, and over all.
+template <int NW>
+__device__ __forceinline__ void block_scan(const int (&x)[3], int (&before)[3], int (&total)[3], int (&part)[3][8]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int incl[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    incl[k] = wave_scan(x[k]);
+    if (lane == 63) part[k][wave] = incl[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    before[k] = incl[k] - x[k], total[k] = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w == wave) before[k] += total[k];
+      total[k] += part[k][w];
+    }
+  }
+}
+
+// The row tiles of a wide group, as blocks of a team.
+__device__ __forceinline__ int blocks_of(int rows, int team) { return ceil_div(ceil_div(rows, kRows), team); }
+
+// Work-groups form teams: those of one take the same tokens under different
+// rows, on one XCD, so that its L2 reads them from memory once (512 rows over
+// 65,536 tokens of 8 heads: 252 us without, and 185 with no loads at all). Groups
+// of unlike size might leave members without rows; then there are no teams.
+// Returns the work-groups of a team.
 template <int NW, int DT>
-__device__ void lay_out(const Shared& p, Layout& l) {
-  constexpr int kThreads = NW * 64, kRun = kBatch / kThreads, R = kRows, TT = tokens_of(DT), kWideTile = wide_tile(DT);
+__device__ int lay_out(const Shared& p, Layout& l) {
+  constexpr int kThreads = NW * 64, kRun = kBatch / kThreads, TT = tokens_of(DT);
   const int t = threadIdx.x, gh = p.a.group;
   for (int i = t; i < kBatch; i += kThreads) l.leader[i] = 0x7FFFFFFF, l.last[i] = -1, l.from[i] = 0, l.own[i] = 0;
+  // the groups' first sequences and prefixes, where there is room for them
+  const bool held = p.n_groups <= kBatch;
+  if (held)
+    for (int i = t; i < p.n_groups; i += kThreads) l.wide[i] = p.groups[i], l.thin[i] = p.shared[i];
+  const int end = p.groups[p.n_groups];
   __syncthreads();
   for (int i = t; i < p.count; i += kThreads) {
-    const int b = p.first + i;
-    int lo = 0, hi = p.n_groups + 1;  // the last group that begins at or before b
+    const int b = p.first + i, len = length_of(p, i);
+    l.len[i] = len;
+    int lo = 0, hi = p.n_groups;  // the last group that begins at or before b
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
-      if (p.groups[mid] <= b) lo = mid + 1;
+      if ((held ? l.wide[mid] : p.groups[mid]) <= b) lo = mid + 1;
       else hi = mid;
     }
     const int g = lo - 1;
-    if (g < 0 || g >= p.n_groups) continue;
-    const int shared = p.shared[g], slot = max(p.groups[g] - p.first, 0);
-    if (shared <= 0 || length_of(p, i) < shared) continue;
+    if (g < 0 || b >= end) continue;
+    const int shared = held ? l.thin[g] : p.shared[g], slot = max((held ? l.wide[g] : p.groups[g]) - p.first, 0);
+    if (shared <= 0 || len < shared) continue;
     l.from[i] = shared, l.own[i] = slot;
     atomicMin(&l.leader[slot], i);
     atomicMax(&l.last[slot], i);
   }
   __syncthreads();
-  int wide = 0, thin = 0, own = 0;
+  const auto rows_of = [&](int i) { return l.leader[i] < l.last[i] ? (l.last[i] - l.leader[i] + 1) * gh : 0; };
+  // the team that the largest group would have, and what all groups would make of it
+  int most = 0, team = 1;
+  for (int i = t; i < p.count; i += kThreads) most = max(most, ceil_div(rows_of(i), kRows));
+  if (__syncthreads_or(most > 1)) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) most = max(most, __shfl_xor(most, d, 64));
+    if ((t & 63) == 0) l.part[0][t >> 6] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) most = max(most, l.part[0][w]);
+    __syncthreads();
+    team = min(ceil_div(most, ceil_div(most, kTeam)), (int)(gridDim.x % 8 ? gridDim.x : gridDim.x / 8));
+    int used[3] = {0, 0, 0}, unused[3], all[3];
+    for (int i = t; i < p.count; i += kThreads) {
+      const int rows = rows_of(i);
+      if (rows <= kHeads) continue;
+      const int tiles = ceil_div(l.from[l.leader[i]], TT);
+      used[0] += ceil_div(rows, kRows) * tiles, used[1] += blocks_of(rows, team) * team * tiles;
+    }
+    block_scan<NW>(used, unused, all, l.part);
+    if (all[1] > all[0] + all[0] / 4) team = 1;
+    __syncthreads();
+  }
+  const int wide_tile = kWideTile * team, wide_start = kWideStart * team;
+  int units[3] = {0, 0, 0}, before[3], total[3];
   int each[3][kRun];
 #pragma unroll
   for (int k = 0; k < kRun; ++k) {
     const int i = t * kRun + k;
-    each[0][k] = wide, each[1][k] = thin, each[2][k] = own;
+    each[0][k] = units[0], each[1][k] = units[1], each[2][k] = units[2];
     if (i >= p.count) continue;
-    if (l.leader[i] < l.last[i]) {
-      const int shared = l.from[l.leader[i]], m = (l.last[i] - l.leader[i] + 1) * gh;
-      if (m > kHeads) wide += p.a.heads * ceil_div(m, R) * (kWideStart + ceil_div(shared, TT) * kWideTile);
-      else thin += p.a.heads * (kStart + ceil_div(shared, kTile));
+    const int rows = rows_of(i);
+    if (rows) {
+      const int shared = l.from[l.leader[i]];
+      if (rows > kHeads) units[0] += p.a.heads * blocks_of(rows, team) * (wide_start + ceil_div(shared, TT) * wide_tile);
+      else units[1] += p.a.heads * (kStart + ceil_div(shared, kTile));
     }
-    const int slot = l.own[i];
-    const bool alone = l.leader[slot] >= l.last[slot];
-    const int from = alone ? 0 : l.from[i];
-    own += p.a.heads * p.a.head_tiles * (kStart + max(1, ceil_div(length_of(p, i) - (from & ~7), kTile)));
+    const int slot = l.own[i], from = l.leader[slot] >= l.last[slot] ? 0 : l.from[i];
+    units[2] += p.a.heads * p.a.head_tiles * (kStart + max(1, ceil_div(l.len[i] - (from & ~7), kTile)));
   }
-  int total[3];
-  const int before[3] = {block_scan<NW>(wide, l.part[0], total[0]), block_scan<NW>(thin, l.part[1], total[1]),
-                         block_scan<NW>(own, l.part[2], total[2])};
+  block_scan<NW>(units, before, total, l.part);
 #pragma unroll
   for (int k = 0; k < kRun; ++k) {
-    const int i = t * kRun + k;
-    const int slot = l.own[i];
+    const int i = t * kRun + k, slot = l.own[i];
     if (l.leader[slot] >= l.last[slot]) l.from[i] = 0;  // alone with its prefix; nobody else reads this place
     l.wide[i] = before[0] + each[0][k], l.thin[i] = before[1] + each[1][k], l.own[i] = before[2] + each[2][k];
   }
   if (t == 0) l.totals[0] = total[0], l.totals[1] = total[1], l.totals[2] = total[2];
   __syncthreads();
+  return __builtin_amdgcn_readfirstlane(team);
 }
 
-// The last i with at[i] <= u.
+// The last i with at[i] <= u, of n <= kBatch; for a whole wave.
 __device__ __forceinline__ int find(const int* at, int n, int u) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (at[mid] <= u) lo = mid;
-    else hi = mid;
-  }
-  return lo;
+  constexpr int kRun = kBatch / 64;
+  const int lane = threadIdx.x & 63;
+  const int run = __popcll(__ballot(lane * kRun < n && at[lane * kRun] <= u)) - 1;
+  const int i = run * kRun + lane;
+  return run * kRun + __popcll(__ballot(lane < kRun && i < n && at[i] <= u)) - 1;
 }
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
@@ -187,9 +236,13 @@ struct WidePart {
 // in order and are waited for by loads_left. (The compiler does not see these
 // writes to LDS coming: they go to tiles that nobody reads before a barrier.)
 __device__ __forceinline__ void load_lds(const void* from, uint32_t to) {
+  to = __builtin_amdgcn_readfirstlane(to);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "memory");
 }
 __device__ __forceinline__ void load_lds(const char* base, uint32_t offset, uint32_t to) {
+  const uint64_t at = (uint64_t)base;
+  base = (const char*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at));
+  to = __builtin_amdgcn_readfirstlane(to);
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(to) : "memory");
 }
 template <int N>
@@ -217,7 +270,7 @@ struct Wide {
   typedef std::conditional_t<F8, f16, T> PT;
   static constexpr int NW = waves_of(DT), TT = tokens_of(DT), TW = NW / 4, TPW = TT / TW, NB = TPW / 32;
   static constexpr int RB = DT * 2, CH = RB / 16;
-  static constexpr int kThreads = NW * 64, kTileBytes = TT * RB, kBuffers = 4;
+  static constexpr int kThreads = NW * 64, kTileBytes = TT * RB, kBuffers = 4, kAhead = F8 ? 4 : 3;
   // 16-byte loads of a row; of a thread for a tile of K; rows of a wave's load
   static constexpr int UNITS = F8 ? CH / 2 : CH, ITER = TT * UNITS / kThreads, RPL = 64 / UNITS;
   static constexpr int KS = DT / 16, DB = DT / 32, ES = F8 ? 1 : 2;
@@ -234,7 +287,8 @@ struct Wide {
   const Shared& p;
   char* const lds;
   uint8_t (*const ok)[TT];
-  const int lane = threadIdx.x & 63, hi = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int32_t* const held;  // kPages pages of the table, from page0 on
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = wave / TW, tw = wave % TW;
 
   Frag q[KS];
@@ -243,66 +297,118 @@ struct Wide {
   bool holes;  // tokens without a page, or strides past 32 bits
   int32_t page_a[ITER], page_b[ITER];  // of a wave's loads: the pages of their first and second eight tokens
   uint32_t k_off[ITER], v_off[ITER];
+  int page0;
+  int tid, lane, hi;
+
+  // What is worked out from a thread's index from here on is worked out from here
+  // on: kept from further up in the kernel it would take most of the registers.
+  __device__ __forceinline__ void place() {
+    tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    lane = tid & 63, hi = lane >> 5;
+  }
 
   __device__ char* k_tile(int b) const { return lds + b * 2 * kTileBytes; }
   __device__ char* v_tile(int b) const { return lds + b * 2 * kTileBytes + kTileBytes; }
 
+  __device__ static __forceinline__ uint32_t lds_at(const char* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+  }
+
   // The row of LDS that a thread's e-th 16 bytes are in, their place in it, and the token that is in a row.
-  __device__ static __forceinline__ int row_of(int e) { return (e * kThreads + (int)threadIdx.x) / UNITS; }
-  __device__ static __forceinline__ int slot_of(int e) { return (e * kThreads + (int)threadIdx.x) % UNITS; }
+  __device__ static __forceinline__ int row_of(int e, int t) { return (e * kThreads + t) / UNITS; }
+  __device__ static __forceinline__ int slot_of(int e, int t) { return (e * kThreads + t) % UNITS; }
   __device__ static __forceinline__ int token_of(int m) { return (m & ~12) | (m & 4) << 1 | (m & 8) >> 1; }
   __device__ static __forceinline__ int k_key(int m) { return CH == 8 ? m >> 1 & 7 : m & 15; }
   __device__ static __forceinline__ int v_key(int m) { return CH == 8 ? (m & 3) << 1 : (m & 3) << 1 | (m & 1) << 3; }
 
+  // The chunk of a row in memory that a thread's e-th place has.
+  __device__ static __forceinline__ int chunk_of(int e, int t, bool of_k) {
+    const int m = row_of(e, t), slot = slot_of(e, t);
+    return F8 ? slot : slot ^ (of_k ? k_key(m) : v_key(m));
+  }
+
   __device__ __forceinline__ bool whole(const WidePart& w, int tile) const { return !holes && (tile + 1) * TT <= w.tokens; }
 
-  // The pages of a tile's tokens, by scalar loads.
+  // The pages of a tile's tokens, from LDS (scalar loads from the table itself
+  // would wait for memory every few tiles, and LDS reads with them).
   __device__ __forceinline__ void look(const WidePart& w, int tile) {
-    typedef __attribute__((address_space(4))) const int32_t* Table;
-    const Table table = (Table)(uintptr_t)(p.a.tables + (p.first + w.leader) * p.a.table_stride);
     const int last = w.tokens - 1;
 #pragma unroll
     for (int e = 0; e < ITER; ++e) {
       const int m = (e * NW + wave) * RPL;  // the first row of the wave's load
       const int t = tile * TT + (RPL >= 8 ? m & ~15 : token_of(m) & ~7);
-      page_a[e] = table[min(t, last) >> p.a.page_shift];
-      if constexpr (RPL >= 8) page_b[e] = table[min(t + 8, last) >> p.a.page_shift];
+      page_a[e] = held[(min(t, last) >> p.a.page_shift) - page0];
+      if constexpr (RPL >= 8) page_b[e] = held[(min(t + 8, last) >> p.a.page_shift) - page0];
     }
   }
 
   // Sends for a tile whose pages are known: to buffer b, or (e4m3, which is
-  // widened on the way) to registers.
-  __device__ __forceinline__ void fetch(const WidePart& w, int tile, int b, Staged& st) {
+  // widened on the way) to registers. This for a whole tile, and PART of 4 of it, as
+  // the loads of all waves at once would stand in each other's way: a wave's four
+  // took 500 to 790 of a step's 3000 cycles.
+  template <int PART>
+  __device__ __forceinline__ void fetch_part(const WidePart& w, int tile, int b, Staged& st) {
     const Params& a = p.a;
     const int64_t at = w.head * a.head_stride + (int64_t)(tile * TT & ((1 << a.page_shift) - 1)) * a.row_stride;
-    const bool all = whole(w, tile);
+#pragma unroll
+    for (int j = PART * 2 * ITER / 4; j < (PART + 1) * 2 * ITER / 4; ++j) {
+      const int e = j / 2;
+      const bool of_k = j % 2 == 0;
+      const char* const base = of_k ? a.k : a.v;
+      const int32_t pa = __builtin_amdgcn_readfirstlane(page_a[e]);
+      const uint32_t off = of_k || F8 ? k_off[e] : v_off[e];
+      const bool mine = FULL || chunk_of(e, tid, of_k) * (16 / ES) < a.dim;
+      const char* from = base + (pa * a.page_stride + at) * ES;
+      if constexpr (RPL >= 8) {
+        const int32_t pb = __builtin_amdgcn_readfirstlane(page_b[e]);
+        from = row_of(e, tid) & 4 ? base + (pb * a.page_stride + at) * ES : from;
+      }
+      if constexpr (F8) {
+        uintx4& staged = of_k ? st.k[e] : st.v[e];
+        if constexpr (!FULL) staged = uintx4{0, 0, 0, 0};
+        if (mine) staged = *(const uintx4*)(from + off);
+      } else {
+        const uint32_t to = lds_at(of_k ? k_tile(b) : v_tile(b)) + (e * kThreads + wave * 64) * 16;
+        if constexpr (RPL < 8) {
+          if (mine) load_lds(from, off, to);
+        } else {
+          if (mine) load_lds(from + off, to);
+        }
+      }
+    }
+  }
+
+  // The same for any tile, all of it. What is not there is zero, and not ok.
+  __device__ __forceinline__ void fetch(const WidePart& w, int tile, int b, Staged& st) {
+    if (whole(w, tile)) {
+      fetch_part<0>(w, tile, b, st), fetch_part<1>(w, tile, b, st);
+      fetch_part<2>(w, tile, b, st), fetch_part<3>(w, tile, b, st);
+      return;
+    }
+    const Params& a = p.a;
+    const int64_t at = w.head * a.head_stride + (int64_t)(tile * TT & ((1 << a.page_shift) - 1)) * a.row_stride;
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));  // this is rare: not worth registers through every step
 #pragma unroll
     for (int e = 0; e < ITER; ++e) {
-      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)k_tile(b) + (e * kThreads + wave * 64) * 16;
-      if (!F8 && RPL < 8 && all) {
-        const int64_t off = (page_a[e] * a.page_stride + at) * ES;
-        if (FULL || (slot_of(e) ^ k_key(row_of(e))) * 8 < a.dim) load_lds(a.k + off, k_off[e], to);
-        if (FULL || (slot_of(e) ^ v_key(row_of(e))) * 8 < a.dim) load_lds(a.v + off, v_off[e], to + kTileBytes);
-        continue;
-      }
-      const int m = row_of(e), slot = slot_of(e), r = token_of(m);
+      const int m = row_of(e, thread), r = token_of(m), place = (e * kThreads + thread) * 16;
       const int32_t page = RPL >= 8 && m & 4 ? page_b[e] : page_a[e];
-      const bool in = all || (page >= 0 && page < a.pages && tile * TT + r < w.tokens);
-      const char* const row = (const char*)((page * a.page_stride + at + (int64_t)(r & ((1 << a.page_shift) - 1)) * a.row_stride) * ES);
+      const bool in = page >= 0 && page < a.pages && tile * TT + r < w.tokens;
+      const int64_t row = (page * a.page_stride + at + (int64_t)(r & ((1 << a.page_shift) - 1)) * a.row_stride) * ES;
+      const int kc = chunk_of(e, thread, true), vc = chunk_of(e, thread, false);
+      const bool k_in = in && (FULL || kc * (16 / ES) < a.dim), v_in = in && (FULL || vc * (16 / ES) < a.dim);
       if constexpr (F8) {
         st.k[e] = st.v[e] = uintx4{0, 0, 0, 0};
-        if (in && (FULL || slot * 16 < a.dim)) {
-          st.k[e] = *(const uintx4*)(a.k + (intptr_t)row + slot * 16);
-          st.v[e] = *(const uintx4*)(a.v + (intptr_t)row + slot * 16);
-        }
+        if (k_in) st.k[e] = *(const uintx4*)(a.k + row + kc * 16), st.v[e] = *(const uintx4*)(a.v + row + vc * 16);
       } else {
-        const int kc = slot ^ k_key(m), vc = slot ^ v_key(m), place = (e * kThreads + (int)threadIdx.x) * 16;
-        if (in && (FULL || kc * 8 < a.dim)) load_lds(a.k + (intptr_t)row + kc * 16, to);
-        else if (!all) *(uintx4*)(k_tile(b) + place) = uintx4{0, 0, 0, 0};
-        if (in && (FULL || vc * 8 < a.dim)) load_lds(a.v + (intptr_t)row + vc * 16, to + kTileBytes);
-        else if (!all) *(uintx4*)(v_tile(b) + place) = uintx4{0, 0, 0, 0};
+        const uint32_t run = (e * kThreads + wave * 64) * 16;
+        if (k_in) load_lds(a.k + row + kc * 16, lds_at(k_tile(b)) + run);
+        else *(uintx4*)(k_tile(b) + place) = uintx4{0, 0, 0, 0};
+        if (v_in) load_lds(a.v + row + vc * 16, lds_at(v_tile(b)) + run);
+        else *(uintx4*)(v_tile(b) + place) = uintx4{0, 0, 0, 0};
       }
-      if (!all && slot == 0) ok[b][m] = in;
+      if (slot_of(e, thread) == 0) ok[b][m] = in;
     }
   }
 
@@ -310,7 +416,7 @@ struct Wide {
   __device__ __forceinline__ void store(int b, const Staged& st) {
 #pragma unroll
     for (int e = 0; e < ITER; ++e) {
-      const int m = row_of(e), slot = slot_of(e);
+      const int m = row_of(e, tid), slot = slot_of(e, tid);
       char* const kd = k_tile(b) + m * RB;
       char* const vd = v_tile(b) + m * RB;
       const uintx4 k = st.k[e], v = st.v[e];
@@ -343,8 +449,8 @@ struct Wide {
   }
 
   // Scores that are none left out; the reference moved where one is too large for it.
-  __device__ __forceinline__ void settle(const WidePart& w, int tile, int b, Scores& s) {
-    if (!whole(w, tile)) {
+  __device__ __forceinline__ void settle(bool all, int b, Scores& s) {
+    if (!all) {
       asm volatile("");  // a branch, not selects in every tile
 #pragma unroll
       for (int n = 0; n < NB; ++n)
@@ -415,45 +521,130 @@ struct Wide {
     }
   }
 
-  // Tile t's weights and values with tile t + 1's scores: what is on its way then is t + 2 and t + 3.
-  __device__ __forceinline__ void step(const WidePart& w, int t, const Scores& now, Scores& next, Staged& st) {
-    const int b = t - w.c;
-    if constexpr (F8) {
-      __syncthreads();
-      if (t + 2 < w.c1) store((b + 2) & 3, st);
-      if (t + 4 < w.c1) fetch(w, t + 4, (b + 4) & 3, st);
-      if (t + 5 < w.c1) look(w, t + 5);
-    } else {
-      if (t + 2 < w.c1 && whole(w, t + 2)) loads_left<2 * ITER>();
-      else loads_left<0>();
-      __syncthreads();
-      if (t + 3 < w.c1) fetch(w, t + 3, (b + 3) & 3, st);
-      if (t + 4 < w.c1) look(w, t + 4);
-    }
-    // The order matters, and the compiler would put every read right before its
-    // product: keys are read while weights are found, the first values while the
-    // keys are multiplied.
+  // Tile t's values with tile t + 1's scores: what is on its way then is t + 2 and
+  // t + 3. Reads of LDS go out well before their products and loads between
+  // products; the compiler would put every read right before its product, and is
+  // kept from it. Nothing here may spill: reading it back would wait for all loads.
+  // STEADY: what is sent for is a whole tile. (To have the two waves of a SIMD take
+  // turns, one with the vector units and one with the matrix cores, by barriers at
+  // different places, gave nothing.)
+  template <bool STEADY>
+  __device__ __forceinline__ void step(const WidePart& w, int t, Scores& s, Staged& st) {
+    const int b = t - w.c, to = (b + kAhead) & 3;
     Frag kf[NB * KS], wf[NB * 2], vf[2][DB];
+    const auto apart = [] { __builtin_amdgcn_sched_barrier(0); };
+    const auto send = [&](auto part) {
+      if constexpr (STEADY) fetch_part<decltype(part)::value>(w, t + kAhead, to, st);
+      apart();
+    };
+    if constexpr (!F8) {
+      if (STEADY || (t + 2 < w.c1 && whole(w, t + 2))) loads_left<2 * ITER>();
+      else loads_left<0>();
+    }
+    __syncthreads();
     read_keys((b + 1) & 3, kf);
-    __builtin_amdgcn_sched_barrier(0);
-    weigh(now, wf);
-    __builtin_amdgcn_sched_barrier(0);
+    apart();
+    weigh(s, wf);
+    apart();
+    if (F8 && t + 2 < w.c1) store((b + 2) & 3, st);
+    if (!STEADY && t + kAhead < w.c1) fetch(w, t + kAhead, to, st);
+    send(std::integral_constant<int, 0>{});
     read_values(b & 3, 0, vf[0]);
-    __builtin_amdgcn_sched_barrier(0);
-    scores(kf, next);
-    __builtin_amdgcn_sched_barrier(0);
+    apart();
+    scores(kf, s);
+    apart();
+    send(std::integral_constant<int, 1>{});
 #pragma unroll
     for (int n = 0; n < NB * 2; ++n) {
       if (n + 1 < NB * 2) read_values(b & 3, n + 1, vf[n + 1 & 1]);
-      __builtin_amdgcn_sched_barrier(0);
+      apart();
       add_values(vf[n & 1], wf[n]);
-      __builtin_amdgcn_sched_barrier(0);
+      apart();
+      if (n == 0) send(std::integral_constant<int, 2>{});
+      if (n == 1) send(std::integral_constant<int, 3>{});
     }
-    settle(w, t + 1, (b + 1) & 3, next);
+    if (t + kAhead + 1 < w.c1) look(w, t + kAhead + 1);
+    apart();
+    settle(STEADY || whole(w, t + 1), (b + 1) & 3, s);
+  }
+
+  // A wave's part in a stretch whose first tiles are on their way.
+  __device__ __forceinline__ void take(const WidePart& w, Staged (&st)[2]) {
+    place();
+    Scores s;
+    {
+      Frag kf[NB * KS];
+      read_keys(0, kf);
+      scores(kf, s);
+    }
+    settle(whole(w, w.c), 0, s);
+    int t = w.c;
+    const int steady = (holes ? 0 : min(w.c1, w.tokens / TT)) - kAhead;
+    if constexpr (F8) {  // the registers take turns
+      for (; t + 1 < steady; t += 2) {
+        step<true>(w, t, s, st[0]);
+        step<true>(w, t + 1, s, st[1]);
+      }
+      for (; t + 2 < w.c1; t += 2) {
+        step<false>(w, t, s, st[0]);
+        step<false>(w, t + 1, s, st[1]);
+      }
+      if (t + 1 < w.c1) step<false>(w, t, s, st[0]);
+    } else {
+      for (; t < steady; ++t) step<true>(w, t, s, st[0]);
+      for (; t + 1 < w.c1; ++t) step<false>(w, t, s, st[0]);
+    }
+    Frag wf[NB * 2];
+    weigh(s, wf);
+    values((w.c1 - 1 - w.c) & 3, wf);
+  }
+
+  __device__ __forceinline__ void run_stretch(const WidePart& w) {
+    const Params& a = p.a;
+    place();
+    __syncthreads();  // what was in LDS before has been read
+    page0 = w.c * TT >> a.page_shift;
+    bool hole = p.far;
+    const int n_pages = ((min(w.c1 * TT, w.tokens) - 1) >> a.page_shift) - page0 + 1;
+    for (int i = tid; i < n_pages; i += kThreads) {
+      const int32_t page = a.tables[(p.first + w.leader) * a.table_stride + page0 + i];
+      held[i] = page;
+      hole = hole || page < 0 || page >= a.pages;
+    }
+    if (!FULL && !F8) {
+#pragma unroll
+      for (int e = 0; e < ITER; ++e)
+        if (chunk_of(e, tid, true) * 8 >= a.dim)
+          for (int b = 0; b < kBuffers; ++b) *(uintx4*)(k_tile(b) + (e * kThreads + tid) * 16) = uintx4{0, 0, 0, 0};
+    }
+    holes = __builtin_amdgcn_readfirstlane(__syncthreads_or(hole));
+    look(w, w.c);
+    Staged st[2];
+    const int n = w.c1 - w.c;
+    if constexpr (F8) {
+      fetch(w, w.c, 0, st[0]);
+      if (n > 1) look(w, w.c + 1), fetch(w, w.c + 1, 1, st[1]);
+      store(0, st[0]);
+      if (n > 2) look(w, w.c + 2), fetch(w, w.c + 2, 2, st[0]);
+      if (n > 1) store(1, st[1]);
+      if (n > 3) look(w, w.c + 3), fetch(w, w.c + 3, 3, st[1]);
+      if (n > 4) look(w, w.c + 4);
+    } else {
+      for (int b = 0; b < min(n, 3); ++b) {
+        if (b) look(w, w.c + b);
+        fetch(w, w.c + b, b, st[0]);
+      }
+      if (n > 3) look(w, w.c + 3);
+      if (n > 2 && whole(w, w.c + 2)) loads_left<4 * ITER>();
+      else loads_left<0>();
+    }
+    __syncthreads();
+    take(w, st);
   }
 
   __device__ void run(const WidePart& w) {
     const Params& a = p.a;
+    place();
     const int row = rw * 32 + (lane & 31), at = w.row0 + row;
     const int member = w.leader + at / a.group, q_head = w.head * a.group + at % a.group;
     const char* const q_row = a.q + ((p.first + member) * a.q_stride + q_head * a.q_head) * 2;
@@ -475,95 +666,60 @@ struct Wide {
       for (int s = 0; s < KS; ++s) q[s] ^= 0x80008000u;
     }
     if (cs == 0.f) cs = 0x1p-126f;  // a masked score, -inf, times it stays that
-    look(w, w.c);
-    bool hole = p.far;
-    const int first = w.c * TT >> a.page_shift, last = (min(w.c1 * TT, w.tokens) - 1) >> a.page_shift;
-    for (int i = first + (int)threadIdx.x; i <= last; i += kThreads) {
-      const int32_t page = a.tables[(p.first + w.leader) * a.table_stride + i];
-      hole = hole || page < 0 || page >= a.pages;
-    }
-    holes = __syncthreads_or(hole);  // and what was in LDS before has been read
 #pragma unroll
     for (int e = 0; e < ITER; ++e) {
-      const int m = row_of(e), slot = slot_of(e);
-      const uint32_t r = (uint32_t)((token_of(m) & ((1 << a.page_shift) - 1)) * a.row_stride * ES);
-      k_off[e] = r + (slot ^ k_key(m)) * 16, v_off[e] = r + (slot ^ v_key(m)) * 16;
-      if (!FULL && !F8 && (slot ^ k_key(m)) * 8 >= a.dim)
-        for (int b = 0; b < kBuffers; ++b) *(uintx4*)(k_tile(b) + (e * kThreads + (int)threadIdx.x) * 16) = uintx4{0, 0, 0, 0};
+      const uint32_t r = (uint32_t)((token_of(row_of(e, tid)) & ((1 << a.page_shift) - 1)) * a.row_stride * ES);
+      k_off[e] = r + chunk_of(e, tid, true) * 16, v_off[e] = r + chunk_of(e, tid, false) * 16;
     }
-    Staged st[2];
-    Scores s[2];
-    const int n = w.c1 - w.c;
-    if constexpr (F8) {
-      fetch(w, w.c, 0, st[0]);
-      if (n > 1) look(w, w.c + 1), fetch(w, w.c + 1, 1, st[1]);
-      store(0, st[0]);
-      if (n > 2) look(w, w.c + 2), fetch(w, w.c + 2, 2, st[0]);
-      if (n > 1) store(1, st[1]);
-      if (n > 3) look(w, w.c + 3), fetch(w, w.c + 3, 3, st[1]);
-      if (n > 4) look(w, w.c + 4);
-    } else {
-      for (int b = 0; b < min(n, 3); ++b) {
-        if (b) look(w, w.c + b);
-        fetch(w, w.c + b, b, st[0]);
-      }
-      if (n > 3) look(w, w.c + 3);
-      if (n > 2 && whole(w, w.c + 2)) loads_left<4 * ITER>();
-      else loads_left<0>();
+    // as many tiles as there is room for pages of, and again
+    const int most = max(1, (kPages << a.page_shift) / TT);
+    WidePart stretch = w;
+    for (; stretch.c < w.c1; stretch.c = stretch.c1) {
+      stretch.c1 = min(w.c1, stretch.c + most);
+      run_stretch(stretch);
     }
-    __syncthreads();
-    Frag kf[NB * KS], wf[NB * 2];
-    read_keys(0, kf);
-    scores(kf, s[0]);
-    settle(w, w.c, 0, s[0]);
-    int t = w.c;
-    for (; t + 2 < w.c1; t += 2) {
-      step(w, t, s[0], s[1], st[0]);
-      step(w, t + 1, s[1], s[0], st[1]);
-    }
-    if (t + 1 < w.c1) {
-      step(w, t, s[0], s[1], st[0]);
-      weigh(s[1], wf);
-      ++t;
-    } else {
-      weigh(s[0], wf);
-    }
-    values((t - w.c) & 3, wf);
     sum += __shfl_xor(sum, 32, 64);
     if constexpr (TW > 1) {
+      // the waves of other tokens hand their sums over, 16 bytes of a lane at a time
       constexpr int kOne = (DB * 16 + 2) * 64;
       float* const all = (float*)lds;
       __syncthreads();
       if (tw) {
-        float* const mine = all + ((tw - 1) * 4 + rw) * kOne + lane;
+        float* const mine = all + ((tw - 1) * 4 + rw) * kOne;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) mine[(d * 16 + r) * 64] = o[d][r];
-        mine[DB * 16 * 64] = ref, mine[(DB * 16 + 1) * 64] = sum;
+          for (int r = 0; r < 16; r += 4)
+            *(floatx4*)(mine + ((d * 4 + r / 4) * 64 + lane) * 4) = floatx4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+        *(floatx2*)(mine + DB * 16 * 64 + 2 * lane) = floatx2{ref, sum};
       }
       __syncthreads();
       if (tw == 0) {
 #pragma unroll 1
         for (int other = 0; other < TW - 1; ++other) {
-          const float* const its = all + (other * 4 + rw) * kOne + lane;
-          const float its_ref = its[DB * 16 * 64], top = fmaxf(ref, its_ref);
+          const float* const its = all + (other * 4 + rw) * kOne;
+          const floatx2 its_stat = *(const floatx2*)(its + DB * 16 * 64 + 2 * lane);
+          const float its_ref = its_stat.x, top = fmaxf(ref, its_ref);
           // without scores so far the sums are zero (or NaN)
           const float mine = ref == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ref - top);
           const float theirs = its_ref == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(its_ref - top);
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * mine + its[(d * 16 + r) * 64] * theirs;
-          sum = sum * mine + its[(DB * 16 + 1) * 64] * theirs;
+            for (int r = 0; r < 16; r += 4) {
+              const floatx4 x = *(const floatx4*)(its + ((d * 4 + r / 4) * 64 + lane) * 4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][r + e] = o[d][r + e] * mine + x[e] * theirs;
+            }
+          sum = sum * mine + its_stat.y * theirs;
           ref = top;
         }
       }
     }
   }
 
-  // The sums to the workspace; range: the work-groups that have parts of the stream.
-  __device__ void write(const WidePart& w, int2 range, const Layout& l) {
+  // The sums to the workspace; parts: of the stream, every step-th work-group from this one on has one.
+  __device__ void write(const WidePart& w, int id, int parts, int step, const Layout& l) {
     if (tw) return;
     const Params& a = p.a;
     const int row = rw * 32 + (lane & 31), at = w.row0 + row;
@@ -571,7 +727,7 @@ struct Wide {
     const int member = w.leader + at / a.group;
     const int64_t out = (int64_t)member * a.q_heads + w.head * a.group + at % a.group;
     float* const part = w.c == 0 ? p.prefix_first + out * part_row(DT)
-                                 : p.wide_rest + ((int64_t)blockIdx.x * kRows + row) * part_row(DT);
+                                 : p.wide_rest + ((int64_t)id * kRows + row) * part_row(DT);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -579,7 +735,7 @@ struct Wide {
         *(floatx4*)(part + 32 * d + 2 * r + 4 * hi) = floatx4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
     if (hi == 0) {
       *(floatx2*)(part + DT) = floatx2{ref, sum};
-      if (w.c == 0 && l.from[member]) p.prefix_ends[out] = int4{range.x, range.y, row, 1};
+      if (w.c == 0 && l.from[member]) p.prefix_ends[out] = int4{id, parts, row, step};
     }
   }
 };
@@ -587,40 +743,47 @@ struct Wide {
 template <typename T, bool F8, int DT, bool FULL>
 __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_kernel(Shared p) {
   typedef Wide<T, F8, DT, FULL> W;
-  constexpr int NW = W::NW, kWideTile = wide_tile(DT);
+  constexpr int NW = W::NW;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ Layout l;
   __shared__ uint8_t ok[W::kBuffers][W::TT];
+  __shared__ int32_t held[kPages];
   const Params& a = p.a;
-  lay_out<NW, DT>(p, l);
-  const int wides = l.totals[0], thins = l.totals[1], total = wides + thins + l.totals[2];
+  const int team = lay_out<NW, DT>(p, l);
+  const int wides = __builtin_amdgcn_readfirstlane(l.totals[0]), thins = __builtin_amdgcn_readfirstlane(l.totals[1]);
+  const int total = wides + thins + __builtin_amdgcn_readfirstlane(l.totals[2]);
+  // Work-group i runs on XCD i % 8: teams go round the XCDs, a team's members
+  // follow each other on one.
+  const int rings = gridDim.x % 8 ? 1 : 8, place = blockIdx.x / rings, teams = gridDim.x / rings / team * rings;
+  const int me_team = place / team * rings + blockIdx.x % rings, member = place % team, id = me_team * team + member;
   Share share;
-  // a work-group has units for all of its waves, and at least a wide tile's: so
-  // that within a stream each has a part
-  share.waves = min(max(1, total / max(NW, kWideTile)), (int)gridDim.x);
+  // a team has units for all of its waves, and at least a wide tile's: so that
+  // within a stream each has a part
+  share.waves = min(max(1, total / (team * max(NW, kWideTile))), teams);
   share.each = total / share.waves;
   share.more = total % share.waves;
-  if ((int)blockIdx.x >= share.waves) return;
-  const int u0 = share.begin(blockIdx.x), u1 = share.begin(blockIdx.x + 1);
+  if (me_team >= share.waves) return;
+  const int u0 = share.begin(me_team), u1 = share.begin(me_team + 1);
 
+  const int tile_cost = kWideTile * team, start_cost = kWideStart * team;
   for (int u = u0; u < min(u1, wides);) {
     const int i = __builtin_amdgcn_readfirstlane(find(l.wide, p.count, u));
     WidePart w;
     w.leader = __builtin_amdgcn_readfirstlane(l.leader[i]);
     w.tokens = __builtin_amdgcn_readfirstlane(l.from[w.leader]);
-    const int m = (__builtin_amdgcn_readfirstlane(l.last[i]) - w.leader + 1) * a.group, row_tiles = ceil_div(m, kRows);
-    const int tiles = ceil_div(w.tokens, W::TT), cost = kWideStart + tiles * kWideTile;
-    const int x = (u - l.wide[i]) / cost, pos = (u - l.wide[i]) % cost, begin = u - pos;
-    w.head = __builtin_amdgcn_readfirstlane(x / row_tiles);
-    w.row0 = __builtin_amdgcn_readfirstlane(x % row_tiles * kRows);
+    const int m = (__builtin_amdgcn_readfirstlane(l.last[i]) - w.leader + 1) * a.group, blocks = blocks_of(m, team);
+    const int tiles = ceil_div(w.tokens, W::TT), cost = start_cost + tiles * tile_cost;
+    const int in = u - __builtin_amdgcn_readfirstlane(l.wide[i]), x = in / cost, pos = in - x * cost, begin = u - pos;
+    w.head = x / blocks;
+    w.row0 = (x % blocks * team + member) * kRows;
     w.rows = min(kRows, m - w.row0);
     const int end = min(cost, pos + (u1 - u));
-    w.c = __builtin_amdgcn_readfirstlane(ceil_div(max(0, pos - kWideStart), kWideTile));
-    w.c1 = __builtin_amdgcn_readfirstlane(ceil_div(max(0, end - kWideStart), kWideTile));
-    if (w.c < w.c1) {
-      W wide{p, lds, ok};
+    w.c = ceil_div(max(0, pos - start_cost), tile_cost);
+    w.c1 = ceil_div(max(0, end - start_cost), tile_cost);
+    if (w.c < w.c1 && w.rows > 0) {
+      W wide{p, lds, ok, held};
       wide.run(w);
-      wide.write(w, int2{(int)blockIdx.x, share.owner(begin + kWideStart + (tiles - 1) * kWideTile)}, l);
+      wide.write(w, id, share.owner(begin + start_cost + (tiles - 1) * tile_cost) - me_team + 1, team, l);
     }
     u += cost - pos;
   }
@@ -629,43 +792,43 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
   // the waves' shares of the rest
   constexpr int VD = DT / 16;
   const int lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = team * NW;
   const int x0 = max(u0, wides), span = u1 - x0;
   if (span <= 0) return;
-  // n units go to the last min(n, NW) waves of a work-group: only where the wide
-  // streams end there are fewer than NW, and the next one's first wave goes on
-  // with what the last of them began
-  const auto wave_begin = [&](int64_t n, int k) { return (int)(n * k / min(n, (int64_t)NW)); };
+  // n units go to the last min(n, waves) waves of a team: only where the wide
+  // streams end there are fewer, and the next one's first wave goes on with what
+  // the last of them began
+  const auto wave_begin = [&](int64_t n, int k) { return (int)(n * k / min(n, (int64_t)waves)); };
   const auto owner = [&](int u) {  // the wave that has unit u
-    const int group = share.owner(u), begin = max(share.begin(group), wides), n = share.begin(group + 1) - begin;
-    int k = (int)((int64_t)(u - begin) * min(n, NW) / n);
+    const int of = share.owner(u), begin = max(share.begin(of), wides), n = share.begin(of + 1) - begin;
+    int k = (int)((int64_t)(u - begin) * min(n, waves) / n);
     while (wave_begin(n, k + 1) <= u - begin) ++k;
-    return group * NW + NW - min(n, NW) + k;
+    return of * waves + waves - min(n, waves) + k;
   };
-  const int mine = wave - (NW - min(span, NW));
+  const int mine = member * NW + wave - (waves - min(span, waves));
   if (mine < 0) return;
-  const int me = blockIdx.x * NW + wave, a1 = x0 + wave_begin(span, mine + 1);
+  const int me = id * NW + wave, a1 = x0 + wave_begin(span, mine + 1);
   for (int u = x0 + wave_begin(span, mine); u < a1;) {
     Span sp{};
     Stream at;
     const char* q_row;
-    int pos, i;
+    int pos;
     const bool thin = u < wides + thins;
     if (thin) {
-      i = find(l.thin, p.count, u - wides);
+      const int i = __builtin_amdgcn_readfirstlane(find(l.thin, p.count, u - wides));
       const int leader = __builtin_amdgcn_readfirstlane(l.leader[i]);
       sp.end = __builtin_amdgcn_readfirstlane(l.from[leader]);
       sp.tiles = ceil_div(sp.end, kTile), sp.cost = kStart + sp.tiles;
       const int in = u - wides - __builtin_amdgcn_readfirstlane(l.thin[i]), head = in / sp.cost;
-      pos = in % sp.cost;
+      pos = in - head * sp.cost;
       at = Stream{p.first + leader, head, (__builtin_amdgcn_readfirstlane(l.last[i]) - leader + 1) * a.group, head * a.group, head};
       q_row = a.q + ((at.b + i16 / a.group) * a.q_stride + (at.q_head + i16 % a.group) * a.q_head) * 2;
     } else {
-      i = __builtin_amdgcn_readfirstlane(find(l.own, p.count, u - wides - thins));
-      sp.begin = __builtin_amdgcn_readfirstlane(l.from[i]), sp.base = sp.begin & ~7, sp.end = length_of(p, i);
+      const int i = __builtin_amdgcn_readfirstlane(find(l.own, p.count, u - wides - thins));
+      sp.begin = __builtin_amdgcn_readfirstlane(l.from[i]), sp.base = sp.begin & ~7, sp.end = __builtin_amdgcn_readfirstlane(l.len[i]);
       sp.tiles = max(1, ceil_div(sp.end - sp.base, kTile)), sp.cost = kStart + sp.tiles;
       const int in = u - wides - thins - __builtin_amdgcn_readfirstlane(l.own[i]), x = in / sp.cost;
-      pos = in % sp.cost;
+      pos = in - x * sp.cost;
       at = stream_of(a, p.first + i, x / a.head_tiles, x % a.head_tiles);
       q_row = query_of(a, at, i16);
     }
@@ -685,10 +848,10 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
         if (g == 0) {
           *(floatx2*)(part + DT) = floatx2{s.ref, s.sum};
           if (c == 0) {
-            const int last = owner(u - pos + sp.cost - 1);
-            if (!thin) p.own_ends[out] = int2{me, last};
-            if (thin && l.from[seq]) p.prefix_ends[out] = int4{me, last, i16, 0};
-            if (!thin && sp.begin == 0) p.prefix_ends[out] = int4{-1, -2, 0, 0};
+            const int parts = owner(u - pos + sp.cost - 1) - me + 1;
+            if (!thin) p.own_ends[out] = int2{me, parts};
+            if (thin && l.from[seq]) p.prefix_ends[out] = int4{me, parts, i16, 0};
+            if (!thin && sp.begin == 0) p.prefix_ends[out] = int4{0, 0, 0, 0};
           }
         }
       }
@@ -708,12 +871,12 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Shared p) {
   const int64_t out = blockIdx.x;
   const int4 prefix = p.prefix_ends[out];
   const int2 own = p.own_ends[out];
-  const int n_prefix = prefix.y - prefix.x + 1, parts = n_prefix + own.y - own.x + 1;
+  const int n_prefix = prefix.y, parts = n_prefix + own.y;
   const int head = (int)(out % a.q_heads);
   const auto part = [&](int i) -> const float* {
     if (i < n_prefix) {
       if (i == 0) return p.prefix_first + out * part_row(DT);
-      return prefix.w ? p.wide_rest + ((int64_t)(prefix.x + i) * kRows + prefix.z) * part_row(DT)
+      return prefix.w ? p.wide_rest + ((int64_t)(prefix.x + i * prefix.w) * kRows + prefix.z) * part_row(DT)
                       : p.wave_rest + ((int64_t)(prefix.x + i) * kHeads + prefix.z) * part_row(DT);
     }
     i -= n_prefix;
@@ -795,7 +958,7 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_l
   a.head_tiles = (a.group + kHeads - 1) / kHeads;
   const int64_t count = std::min<int64_t>(batch, kBatch);
   // units of a launch, at most
-  const int64_t tiles = max_len / kTile + 2 + kStart + 2 * kWideStart;
+  const int64_t tiles = max_len / kTile * kWideTile + 2 + kStart + kTeam * (kWideStart + kWideTile);
   const int64_t per_seq = pages.heads * (2 * (int64_t)a.head_tiles + a.group / 32 + 2);
   if (tiles > 0x7FFFFFFF / std::max<int64_t>(1, count * per_seq)) throw std::invalid_argument("batch x heads x tokens is too large");
   a.work_groups = std::min<int64_t>({kGroups, compute_units(), std::max<int64_t>(1, count * pages.heads * a.head_tiles * tiles)});
