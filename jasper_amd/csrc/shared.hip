@@ -30,7 +30,7 @@ namespace {
 using namespace attention;
 
 constexpr int kBatch = 512;      // sequences of a launch
-constexpr int kGroups = 256;     // work-groups at most
+constexpr int kGroups = 256;     // work-groups: one for each compute unit
 constexpr int kStage = 512;      // row offsets of a wave, in LDS
 constexpr int kJoin = 256;       // threads of a joining work-group
 constexpr int kPages = 1024;     // of a wide stream's table, in LDS
@@ -64,13 +64,28 @@ struct Layout {
   int leader[kBatch], last[kBatch];
   int wide[kBatch], thin[kBatch], own[kBatch];
   int len[kBatch];
+  // a group that began in an earlier launch: where, its prefix, and its first
+  // sequence that is long enough (none: kNone)
+  int cut_begin, cut_shared, cut;
   int totals[3];
   int part[3][8];
 };
 
+constexpr int kNone = 0x7FFFFFFF;
+
 __device__ __forceinline__ int length_of(const Shared& p, int i) { return min(max(p.a.lens[p.first + i], 0), p.a.limit); }
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Whether sequences read a prefix at place i: two or more, or what is left of a cut group.
+__device__ __forceinline__ bool shares(const Layout& l, int i) {
+  return l.leader[i] < l.last[i] || (i == 0 && l.cut != kNone && l.last[0] >= 0);
+}
+
+// The sequence in whose table it is.
+__device__ __forceinline__ int source_of(const Shared& p, const Layout& l, int i) {
+  return i == 0 && l.cut != kNone ? l.cut : p.first + l.leader[i];
+}
 
 // The sum of x over the lanes up to this one, without LDS.
 __device__ __forceinline__ int wave_scan(int x) {
@@ -117,7 +132,8 @@ template <int NW, int DT>
 __device__ int lay_out(const Shared& p, Layout& l) {
   constexpr int kThreads = NW * 64, kRun = kBatch / kThreads, TT = tokens_of(DT);
   const int t = threadIdx.x, gh = p.a.group;
-  for (int i = t; i < kBatch; i += kThreads) l.leader[i] = 0x7FFFFFFF, l.last[i] = -1, l.from[i] = 0, l.own[i] = 0;
+  for (int i = t; i < kBatch; i += kThreads) l.leader[i] = kNone, l.last[i] = -1, l.from[i] = 0, l.own[i] = 0;
+  if (t == 0) l.cut_begin = p.first, l.cut_shared = 0, l.cut = kNone;
   // the groups' first sequences and prefixes, where there is room for them
   const bool held = p.n_groups <= kBatch;
   if (held)
@@ -135,14 +151,20 @@ __device__ int lay_out(const Shared& p, Layout& l) {
     }
     const int g = lo - 1;
     if (g < 0 || b >= end) continue;
-    const int shared = held ? l.thin[g] : p.shared[g], slot = max((held ? l.wide[g] : p.groups[g]) - p.first, 0);
+    const int shared = held ? l.thin[g] : p.shared[g], begin = held ? l.wide[g] : p.groups[g], slot = max(begin - p.first, 0);
+    if (i == 0) l.cut_begin = max(begin, 0), l.cut_shared = shared;
     if (shared <= 0 || len < shared) continue;
     l.from[i] = shared, l.own[i] = slot;
     atomicMin(&l.leader[slot], i);
     atomicMax(&l.last[slot], i);
   }
   __syncthreads();
-  const auto rows_of = [&](int i) { return l.leader[i] < l.last[i] ? (l.last[i] - l.leader[i] + 1) * gh : 0; };
+  if (p.first) {
+    for (int b = l.cut_begin + t; b < p.first; b += kThreads)
+      if (l.cut_shared > 0 && length_of(p, b - p.first) >= l.cut_shared) atomicMin(&l.cut, b);
+    __syncthreads();
+  }
+  const auto rows_of = [&](int i) { return shares(l, i) ? (l.last[i] - l.leader[i] + 1) * gh : 0; };
   // the team that the largest group would have, and what all groups would make of it
   int most = 0, team = 1;
   for (int i = t; i < p.count; i += kThreads) most = max(most, ceil_div(rows_of(i), kRows));
@@ -180,14 +202,14 @@ __device__ int lay_out(const Shared& p, Layout& l) {
       if (rows > kHeads) units[0] += p.a.heads * blocks_of(rows, team) * (wide_start + ceil_div(shared, TT) * wide_tile);
       else units[1] += p.a.heads * (kStart + ceil_div(shared, kTile));
     }
-    const int slot = l.own[i], from = l.leader[slot] >= l.last[slot] ? 0 : l.from[i];
+    const int slot = l.own[i], from = shares(l, slot) ? l.from[i] : 0;
     units[2] += p.a.heads * p.a.head_tiles * (kStart + max(1, ceil_div(l.len[i] - (from & ~7), kTile)));
   }
   block_scan<NW>(units, before, total, l.part);
 #pragma unroll
   for (int k = 0; k < kRun; ++k) {
     const int i = t * kRun + k, slot = l.own[i];
-    if (l.leader[slot] >= l.last[slot]) l.from[i] = 0;  // alone with its prefix; nobody else reads this place
+    if (!shares(l, slot)) l.from[i] = 0;  // alone with its prefix; nobody else reads this place
     l.wide[i] = before[0] + each[0][k], l.thin[i] = before[1] + each[1][k], l.own[i] = before[2] + each[2][k];
   }
   if (t == 0) l.totals[0] = total[0], l.totals[1] = total[1], l.totals[2] = total[2];
@@ -226,7 +248,8 @@ __device__ __forceinline__ uintx2 read_column(const char* p) {
 
 // A stretch of a wide stream.
 struct WidePart {
-  int leader;  // the group's first sequence here
+  int leader;  // the group's first sequence here, counted from the launch's
+  int source;  // the sequence whose table has the prefix
   int head, row0, rows, tokens;
   int c, c1;  // its tiles
 };
@@ -607,7 +630,7 @@ struct Wide {
     bool hole = p.far;
     const int n_pages = ((min(w.c1 * TT, w.tokens) - 1) >> a.page_shift) - page0 + 1;
     for (int i = tid; i < n_pages; i += kThreads) {
-      const int32_t page = a.tables[(p.first + w.leader) * a.table_stride + page0 + i];
+      const int32_t page = a.tables[w.source * a.table_stride + page0 + i];
       held[i] = page;
       hole = hole || page < 0 || page >= a.pages;
     }
@@ -770,6 +793,7 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
     const int i = __builtin_amdgcn_readfirstlane(find(l.wide, p.count, u));
     WidePart w;
     w.leader = __builtin_amdgcn_readfirstlane(l.leader[i]);
+    w.source = __builtin_amdgcn_readfirstlane(source_of(p, l, i));
     w.tokens = __builtin_amdgcn_readfirstlane(l.from[w.leader]);
     const int m = (__builtin_amdgcn_readfirstlane(l.last[i]) - w.leader + 1) * a.group, blocks = blocks_of(m, team);
     const int tiles = ceil_div(w.tokens, W::TT), cost = start_cost + tiles * tile_cost;
@@ -812,7 +836,7 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
     Span sp{};
     Stream at;
     const char* q_row;
-    int pos;
+    int pos, first_seq;
     const bool thin = u < wides + thins;
     if (thin) {
       const int i = __builtin_amdgcn_readfirstlane(find(l.thin, p.count, u - wides));
@@ -821,14 +845,16 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
       sp.tiles = ceil_div(sp.end, kTile), sp.cost = kStart + sp.tiles;
       const int in = u - wides - __builtin_amdgcn_readfirstlane(l.thin[i]), head = in / sp.cost;
       pos = in - head * sp.cost;
-      at = Stream{p.first + leader, head, (__builtin_amdgcn_readfirstlane(l.last[i]) - leader + 1) * a.group, head * a.group, head};
-      q_row = a.q + ((at.b + i16 / a.group) * a.q_stride + (at.q_head + i16 % a.group) * a.q_head) * 2;
+      first_seq = leader;
+      at = Stream{__builtin_amdgcn_readfirstlane(source_of(p, l, i)), head, (__builtin_amdgcn_readfirstlane(l.last[i]) - leader + 1) * a.group, head * a.group, head};
+      q_row = a.q + ((p.first + leader + i16 / a.group) * a.q_stride + (at.q_head + i16 % a.group) * a.q_head) * 2;
     } else {
       const int i = __builtin_amdgcn_readfirstlane(find(l.own, p.count, u - wides - thins));
       sp.begin = __builtin_amdgcn_readfirstlane(l.from[i]), sp.base = sp.begin & ~7, sp.end = __builtin_amdgcn_readfirstlane(l.len[i]);
       sp.tiles = max(1, ceil_div(sp.end - sp.base, kTile)), sp.cost = kStart + sp.tiles;
       const int in = u - wides - thins - __builtin_amdgcn_readfirstlane(l.own[i]), x = in / sp.cost;
       pos = in - x * sp.cost;
+      first_seq = i;
       at = stream_of(a, p.first + i, x / a.head_tiles, x % a.head_tiles);
       q_row = query_of(a, at, i16);
     }
@@ -836,7 +862,7 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
     if (c < c1) {
       const Sums<DT> s = attend_tiles<T, F8, DT, false, FULL, kStage>(p.a, sp, at, q_row, c, c1, (int64_t*)lds + wave * kStage);
       if (i16 < at.heads) {
-        const int seq = at.b - p.first + (thin ? i16 / a.group : 0);
+        const int seq = first_seq + (thin ? i16 / a.group : 0);
         const int64_t out = (int64_t)seq * a.q_heads + at.q_head + (thin ? i16 % a.group : i16);
         float* const part = c ? p.wave_rest + ((int64_t)me * kHeads + i16) * part_row(DT)
                               : (thin ? p.prefix_first : p.own_first) + out * part_row(DT);
@@ -934,16 +960,6 @@ __global__ __launch_bounds__(kJoin) void join_kernel(Shared p) {
   if (d == 0 && a.lse) a.lse[at] = tot == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(tot)) * kLn2;
 }
 
-int compute_units() {
-  static const int n = [] {
-    int device = 0, v = 0;
-    hip_check(hipGetDevice(&device), "get device");
-    hip_check(hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, device), "device attribute");
-    return v > 0 ? v : 256;
-  }();
-  return n;
-}
-
 // How a call's work is laid out, from its sizes alone.
 struct Plan {
   int dt, group, head_tiles;
@@ -961,7 +977,7 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_l
   const int64_t tiles = max_len / kTile * kWideTile + 2 + kStart + kTeam * (kWideStart + kWideTile);
   const int64_t per_seq = pages.heads * (2 * (int64_t)a.head_tiles + a.group / 32 + 2);
   if (tiles > 0x7FFFFFFF / std::max<int64_t>(1, count * per_seq)) throw std::invalid_argument("batch x heads x tokens is too large");
-  a.work_groups = std::min<int64_t>({kGroups, compute_units(), std::max<int64_t>(1, count * pages.heads * a.head_tiles * tiles)});
+  a.work_groups = kGroups;  // those without units end at once
   const int64_t rows = count * q_heads, row = part_row(a.dt) * 4;
   a.ends = rows * 24, a.firsts = rows * row;
   a.wide_rest = a.work_groups * kRows * row;
