@@ -18,6 +18,7 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the planning work-group
 constexpr int kRowThreads = 256;
 constexpr int kGrowers = 4096;         // last pages held in LDS at once
+constexpr int kBases = 8192;           // words of the bitmap whose pages waves give out
 constexpr int kSequences = 1 << 18;    // at most: a bit for each in LDS
 
 // What the plan says of a request. fresh: the places of the table from which on
@@ -25,6 +26,7 @@ constexpr int kSequences = 1 << 18;    // at most: a bit for each in LDS
 struct Request {
   int32_t seq, from, to, fresh, last;
   int32_t offset, start, count;
+  int32_t owners;  // of the page that it grows in
 };
 
 struct Extend {
@@ -39,49 +41,96 @@ struct Extend {
   int32_t* growers;  // the last pages of requests that share theirs
 };
 
+// x of the lane that DPP control `ctrl` names, 0 where there is none.
+template <int ctrl, int rows>
+__device__ __forceinline__ int64_t moved(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), ctrl, rows, 0xF, false);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// The sum of x over the lanes up to this one, without LDS: rows of 16 lanes
+// shifted by 1, 2, 4 and 8, then a row's last lane to the next one and lane 31
+// to the last two.
 __device__ __forceinline__ int64_t wave_scan(int64_t x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(x, d, 64);
-    if (lane >= d) x += o;
-  }
+  x += moved<0x111, 0xF>(x);
+  x += moved<0x112, 0xF>(x);
+  x += moved<0x114, 0xF>(x);
+  x += moved<0x118, 0xF>(x);
+  x += moved<0x142, 0xA>(x);
+  x += moved<0x143, 0xC>(x);
   return x;
 }
 
-// The sum of x over the threads before this one; total: over all. `part` has
-// room for kWaves numbers and is free again after the next barrier.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t& total, int64_t* part) {
+// For N numbers at once: their sums over the threads before this one, and over
+// all. `part` has room for N * kWaves numbers and is free again after the next
+// barrier.
+template <int N>
+__device__ __forceinline__ void block_scan(const int64_t (&x)[N], int64_t (&before)[N], int64_t (&total)[N], int64_t* part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t incl = wave_scan(x);
-  if (lane == 63) part[wave] = incl;
-  __syncthreads();
-  int64_t before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w == wave) before = all;
-    all += part[w];
+  for (int k = 0; k < N; ++k) {
+    before[k] = wave_scan(x[k]);
+    if (lane == 63) part[k * kWaves + wave] = before[k];
+    before[k] -= x[k];
   }
   __syncthreads();
-  total = all;
-  return before + incl - x;
+  const int w = __builtin_amdgcn_readfirstlane(wave);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    // the waves' sums, summed up by the lanes of a row
+    int64_t x = part[k * kWaves + (lane & (kWaves - 1))];
+    x += moved<0x111, 0xF>(x);
+    x += moved<0x112, 0xF>(x);
+    x += moved<0x114, 0xF>(x);
+    x += moved<0x118, 0xF>(x);
+    const auto of = [&](int l) {
+      return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, l));
+    };
+    total[k] = of(kWaves - 1);
+    if (w) before[k] += of(w - 1);
+  }
 }
 
 __device__ __forceinline__ int pages_of(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
 
+struct PlanLds {
+  int32_t held[kGrowers];
+  int32_t bases[kBases];  // free pages before each word of the bitmap
+  int64_t part[5 * kWaves];
+};
+
 // One work-group decides: how many pages each request takes, which are free,
-// whether there are enough. A thread has a run of requests and a run of the
-// bitmap's words, so that ranks in order are ranks of threads. Bound by its
-// chain: two sums over the work-group's threads, the loads before them.
-__device__ void plan(const Extend& a, uint32_t* seen, int32_t* held, int64_t* part) {
+// whether there are enough. A thread has a run of requests (one of them, in
+// registers, where ONE) and a run of the bitmap's words, so that ranks in order
+// are ranks of threads. Bound by its chain of dependent loads (sequence, length,
+// last page, its owners) and two sums over the work-group.
+template <bool ONE>
+__device__ void plan(const Extend& a, uint32_t* seen, PlanLds& l) {
   const PageState& st = a.state;
   const int t = threadIdx.x, page = 1 << st.page_shift;
-  const int words_seen = (st.sequences + 31) / 32;
-  for (int i = t; i < words_seen; i += kThreads) seen[i] = 0;
-  __syncthreads();
+  const int run = ONE ? 1 : (a.n + kThreads - 1) / kThreads, r0 = min(t * run, a.n), r1 = min(r0 + run, a.n);
+  Request one{};
+  const auto get = [&](int i) -> Request { return ONE ? one : a.requests[i]; };
+  const auto put = [&](int i, const Request& q) {
+    if (ONE) one = q;
+    else a.requests[i] = q;
+  };
+  // the bitmap's words, on their way while the requests are looked at
+  const int words = (st.pages + 31) / 32, wrun = (words + kThreads - 1) / kThreads;
+  const int w0 = min(t * wrun, words), w1 = min(w0 + wrun, words);
+  const auto word = [&](int w) {
+    const uint32_t x = st.free[w];
+    return w == words - 1 && (st.pages & 31) ? x & ((1u << (st.pages & 31)) - 1) : x;
+  };
+  constexpr int kFirst = 4;
+  uint32_t early[kFirst];
+#pragma unroll
+  for (int k = 0; k < kFirst; ++k) early[k] = w0 + k < w1 ? word(w0 + k) : 0;
 
-  const int run = (a.n + kThreads - 1) / kThreads, r0 = min(t * run, a.n), r1 = min(r0 + run, a.n);
-  int64_t growing = 0;
+  for (int i = t; i < (st.sequences + 31) / 32; i += kThreads) seen[i] = 0;
+  __syncthreads();
+  int64_t growing[1] = {0}, at[1], n_growing[1];
   bool bad = false;
   for (int i = r0; i < r1; ++i) {
     Request q{};
@@ -101,64 +150,71 @@ __device__ void plan(const Extend& a, uint32_t* seen, int32_t* held, int64_t* pa
       q.fresh = pages_of(q.from, st.page_shift);
       if (q.count && (q.from & (page - 1))) {
         const int32_t last = st.tables[(int64_t)q.seq * st.width + q.fresh - 1];
-        if (last >= 0 && last < st.pages && st.refs[last] > 1) q.last = last, ++growing;
+        if (last >= 0 && last < st.pages) {
+          q.owners = st.refs[last];
+          if (q.owners > 1) q.last = last, ++growing[0];
+        }
       }
     }
-    a.requests[i] = q;
+    put(i, q);
   }
   // requests that share the page they grow in: each copies it, but for the last owner
-  int64_t n_growing;
-  int64_t at = block_scan(growing, n_growing, part);
-  if (n_growing) {
-    int64_t mine = at;
-    for (int i = r0; i < r1; ++i)
-      if (a.requests[i].last >= 0) a.growers[mine++] = a.requests[i].last;
+  block_scan<1>(growing, at, n_growing, l.part);
+  if (n_growing[0]) {
+    int64_t mine = at[0];
+    for (int i = r0; i < r1; ++i) {
+      const int32_t last = get(i).last;
+      if (last >= 0) a.growers[mine++] = last;
+    }
     __syncthreads();
-    for (int64_t c = 0; c < n_growing; c += kGrowers) {
-      const int m = (int)min((int64_t)kGrowers, n_growing - c);
-      for (int i = t; i < m; i += kThreads) held[i] = a.growers[c + i];
+    for (int64_t c = 0; c < n_growing[0]; c += kGrowers) {
+      const int m = (int)min((int64_t)kGrowers, n_growing[0] - c);
+      for (int i = t; i < (m + 3) / 4 * 4; i += kThreads) l.held[i] = i < m ? a.growers[c + i] : -1;
       __syncthreads();
-      mine = at;
+      mine = at[0];
       for (int i = r0; i < r1; ++i) {
-        const int32_t last = a.requests[i].last;
-        if (last < 0) continue;
+        Request q = get(i);
+        if (q.last < 0) continue;
+        // those before it that have the same page, four at a time
         const int end = (int)max((int64_t)0, min((int64_t)m, mine - c));
         int before = 0;
-        for (int j = 0; j < end; ++j) before += held[j] == last;
-        a.requests[i].offset += before;
+        typedef int32_t intx4 __attribute__((ext_vector_type(4)));
+#pragma unroll 8
+        for (int j = 0; j < end; j += 4) {
+          const intx4 h = *(const intx4*)(l.held + j);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) before += h[k] == q.last && j + k < end;
+        }
+        q.offset += before;
+        put(i, q);
         ++mine;
       }
       __syncthreads();
     }
   }
-  int64_t take = 0, tokens = 0;
+  int64_t sums[4] = {0, 0, 0, bad}, before[4], total[4];  // pages taken, tokens, free pages, what cannot be
   for (int i = r0; i < r1; ++i) {
-    Request& q = a.requests[i];
+    Request q = get(i);
     if (q.last >= 0) {
-      if (st.refs[q.last] - q.offset > 1) --q.fresh;
+      if (q.owners - q.offset > 1) --q.fresh;
       else q.last = -1;
+      put(i, q);
     }
-    take += pages_of(q.to, st.page_shift) - q.fresh;
-    tokens += q.count;
+    sums[0] += pages_of(q.to, st.page_shift) - q.fresh;
+    sums[1] += q.count;
   }
-  int64_t n_take, n_tokens, n_free;
-  int64_t offset = block_scan(take, n_take, part), start = block_scan(tokens, n_tokens, part);
-  const int words = (st.pages + 31) / 32, wrun = (words + kThreads - 1) / kThreads;
-  const int w0 = min(t * wrun, words), w1 = min(w0 + wrun, words);
-  const auto word = [&](int w) {
-    const uint32_t x = st.free[w];
-    return w == words - 1 && (st.pages & 31) ? x & ((1u << (st.pages & 31)) - 1) : x;
-  };
-  int64_t bits = 0;
-  for (int w = w0; w < w1; ++w) bits += __popc(word(w));
-  int64_t rank = block_scan(bits, n_free, part);
-  bad = __syncthreads_or(bad || n_tokens > a.n_tokens);
-  const bool done = !bad && n_take <= n_free;
+#pragma unroll
+  for (int k = 0; k < kFirst; ++k) sums[2] += __popc(early[k]);
+  for (int w = w0 + kFirst; w < w1; ++w) sums[2] += __popc(word(w));
+  block_scan<4>(sums, before, total, l.part + kWaves);
+  int64_t offset = before[0], start = before[1];
+  const int64_t n_take = total[0];
+  const bool possible = total[3] == 0 && total[1] <= a.n_tokens, done = possible && n_take <= total[2];
   if (t == 0 && a.n == 0) a.starts[0] = 0;
-  if (t == 0) *a.missing = bad ? -1 : (int32_t)max((int64_t)0, n_take - n_free);
+  if (t == 0) *a.missing = possible ? (int32_t)max((int64_t)0, n_take - total[2]) : -1;
 
   for (int i = r0; i < r1; ++i) {
-    Request& q = a.requests[i];
+    Request q = get(i);
     if (!done) {
       q.to = q.from, q.count = 0, q.last = -1, q.fresh = pages_of(q.from, st.page_shift);
       offset = start = 0;
@@ -166,13 +222,38 @@ __device__ void plan(const Extend& a, uint32_t* seen, int32_t* held, int64_t* pa
     q.offset = (int32_t)offset, q.start = (int32_t)start;
     offset += pages_of(q.to, st.page_shift) - q.fresh;
     start += q.count;
+    a.requests[i] = q;
     a.starts[i] = q.start;
     if (i == a.n - 1) a.starts[a.n] = (int32_t)start;
     a.step_lens[i] = q.to;
     if (q.seq >= 0 && q.count) st.lens[q.seq] = q.to;
     if (q.last >= 0) atomicSub(&st.refs[q.last], 1);
   }
-  if (!done) return;
+  if (!done || n_take == 0) return;
+  if (words <= kBases) {
+    // a wave takes two words at a time, a lane a page
+    int64_t rank = before[2];
+#pragma unroll
+    for (int k = 0; k < kFirst; ++k) {
+      if (w0 + k < w1) l.bases[w0 + k] = (int32_t)rank;
+      rank += __popc(early[k]);
+    }
+    for (int w = w0 + kFirst; w < w1; ++w) l.bases[w] = (int32_t)rank, rank += __popc(word(w));
+    __syncthreads();
+    const int lane = t & 63, b = lane & 31;
+    for (int w2 = t >> 6 << 1; w2 < words && l.bases[w2] < n_take; w2 += 2 * kWaves) {
+      const int w = w2 + (lane >> 5);
+      const uint32_t x = w < words ? word(w) : 0;
+      const int r = l.bases[min(w, words - 1)] + __popc(x & ((1u << b) - 1));
+      const bool taken = (x >> b & 1) && r < n_take;
+      if (taken) a.list[r] = 32 * w + b, st.refs[32 * w + b] = 1;
+      const uint64_t both = __ballot(taken);
+      const uint32_t gone = lane < 32 ? (uint32_t)both : (uint32_t)(both >> 32);
+      if (b == 0 && gone) st.free[w] &= ~gone;
+    }
+    return;
+  }
+  int64_t rank = before[2];
   for (int w = w0; w < w1 && rank < n_take; ++w) {
     const uint32_t x = word(w);
     uint32_t left = x;
@@ -194,13 +275,22 @@ __device__ void emit(const Extend& a, int i, int t, int threads) {
   const Request q = a.requests[i];
   const int have = q.fresh, need = pages_of(q.to, st.page_shift);
   int32_t* const row = st.tables + (int64_t)max(q.seq, 0) * st.width;
-  for (int j = t; j < a.width; j += threads) {
-    int32_t p = -1;
-    if (j < need) {
-      if (j < have) p = row[j];
-      else p = row[j] = a.list[q.offset + j - have];
+  constexpr int kLoads = 8;  // on their way at once
+  for (int j0 = t; j0 < a.width; j0 += threads * kLoads) {
+    int32_t p[kLoads];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const int j = j0 + k * threads;
+      p[k] = -1;
+      if (j < min(need, a.width)) p[k] = j < have ? row[j] : a.list[q.offset + j - have];
     }
-    a.step_tables[(int64_t)i * a.width + j] = p;
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const int j = j0 + k * threads;
+      if (j >= a.width) break;
+      if (j >= have && j < need) row[j] = p[k];
+      a.step_tables[(int64_t)i * a.width + j] = p[k];
+    }
   }
   if (t == 0) a.src[i] = q.last, a.dst[i] = q.last >= 0 ? a.list[q.offset] : -1;
   for (int j = t; j < q.count; j += threads) {
@@ -216,12 +306,11 @@ __device__ void pad(const Extend& a, int t, int threads) {
   for (int64_t j = a.starts[a.n] + t; j < a.n_tokens; j += threads) a.positions[j] = 0, a.slots[j] = -1;
 }
 
-template <bool ALL>
+template <bool ALL, bool ONE>
 __global__ __launch_bounds__(kThreads) void plan_kernel(Extend a) {
   extern __shared__ uint32_t seen[];
-  __shared__ int32_t held[kGrowers];
-  __shared__ int64_t part[kWaves];
-  plan(a, seen, held, part);
+  __shared__ PlanLds l;
+  plan<ONE>(a, seen, l);
   if (!ALL) return;
   __syncthreads();
   for (int i = threadIdx.x >> 6; i < a.n; i += kWaves) emit(a, i, threadIdx.x & 63, 64);
@@ -245,10 +334,26 @@ __global__ __launch_bounds__(kRowThreads) void truncate_kernel(PageState st, con
   if (__syncthreads_or(twice) || keep < 0 || keep >= from) return;
   const int p0 = pages_of(keep, st.page_shift), p1 = pages_of(from, st.page_shift);
   int32_t* const row = st.tables + (int64_t)seq * st.width;
-  for (int j = p0 + threadIdx.x; j < p1; j += kRowThreads) {
-    const int32_t p = row[j];
-    row[j] = -1;
-    if (p >= 0 && p < st.pages && atomicSub(&st.refs[p], 1) == 1) atomicOr(&st.free[p >> 5], 1u << (p & 31));
+  for (int j0 = p0; j0 < p1; j0 += kRowThreads) {
+    const int j = j0 + threadIdx.x;
+    int32_t p = -1;
+    if (j < p1) p = row[j], row[j] = -1;
+    bool freed = false;
+    if (p >= 0 && p < st.pages) {
+      // a page of one owner is nobody else's to count
+      if (st.refs[p] == 1) st.refs[p] = 0, freed = true;
+      else freed = atomicSub(&st.refs[p], 1) == 1;
+    }
+    // its bit, with those of the wave's other pages in the same word
+    for (uint64_t left = __ballot(freed); left;) {
+      const int w = __builtin_amdgcn_readlane(p, __builtin_ctzll(left)) >> 5;
+      const bool here = freed && p >> 5 == w;
+      uint32_t bits = here ? 1u << (p & 31) : 0;
+#pragma unroll
+      for (int d = 32; d; d >>= 1) bits |= __shfl_xor(bits, d, 64);
+      if (threadIdx.x % 64 == 0) atomicOr(&st.free[w], bits);
+      left &= ~__ballot(here);
+    }
   }
   if (threadIdx.x == 0) st.lens[seq] = keep;
 }
@@ -318,12 +423,14 @@ __device__ __forceinline__ void find_run(const Prefixes& a, int b) {
 
 __device__ void group_runs(const Prefixes& a, int64_t* part) {
   const int t = threadIdx.x, lane = t & 63, run = (a.n + kThreads - 1) / kThreads, b0 = min(t * run, a.n), b1 = min(b0 + run, a.n);
-  int64_t begun = 0, total;
-  for (int b = b0; b < b1; ++b) begun += a.runs[b] == 0;
-  int g = (int)block_scan(begun, total, part);
+  int64_t begun[1] = {0}, first[1], all[1];
+  for (int b = b0; b < b1; ++b) begun[0] += a.runs[b] == 0;
+  block_scan<1>(begun, first, all, part);
+  int g = (int)first[0];
+  const int total = (int)all[0];
   for (int b = b0; b < b1; ++b)
     if (a.runs[b] == 0) a.groups[g++] = b;
-  for (int i = (int)total + t; i <= a.n; i += kThreads) a.groups[i] = a.n;
+  for (int i = total + t; i <= a.n; i += kThreads) a.groups[i] = a.n;
   __syncthreads();
   // the least of a group's runs: a lane has a group, those of many sequences are gone through by all lanes
   constexpr int kFew = 8;
@@ -387,14 +494,18 @@ void extend_tables(const PageState& state, const ExtendArgs& a, hipStream_t s) {
   p.list = (int32_t*)(w + round16(a.n * (int64_t)sizeof(Request)));
   p.growers = (int32_t*)((char*)p.list + round16(4 * (int64_t)state.pages));
   const size_t lds = ((size_t)state.sequences + 31) / 32 * 4;
-  const bool all = a.n * a.width + a.n_tokens <= 32768;
-  if (all) {
-    plan_kernel<true><<<1, kThreads, lds, s>>>(p);
-    hip_check(hipGetLastError(), "extend tables");
-    return;
-  }
-  plan_kernel<false><<<1, kThreads, lds, s>>>(p);
+  // What little there is to write is written by the planning work-group: a second
+  // kernel is a launch. 48 requests with tables of 600 are worth one (16.3 us a step
+  // with its truncation, 17.0 otherwise).
+  const bool all = a.n * a.width + a.n_tokens <= 8192;
+  const bool one = a.n <= kThreads;
+  auto kernel = all ? (one ? plan_kernel<true, true> : plan_kernel<true, false>)
+                    : (one ? plan_kernel<false, true> : plan_kernel<false, false>);
+  if (lds > 8192)  // with what the kernel has anyway more than 64 KB
+    hip_check(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "extend tables");
+  kernel<<<1, kThreads, lds, s>>>(p);
   hip_check(hipGetLastError(), "extend tables");
+  if (all) return;
   const int64_t each = std::max<int64_t>((a.n_tokens + a.n) / (a.n + 1), a.width);
   const dim3 grid((unsigned)a.n + 1, (unsigned)std::clamp<int64_t>(each / (8 * kRowThreads), 1, 64));
   emit_kernel<<<grid, kRowThreads, 0, s>>>(p);

@@ -191,6 +191,19 @@ def test_many_forks_of_one_page(jasper, forks):
     assert m.refs.max() == forks + 1  # the first page is everyone's
 
 
+def test_very_many_sequences_and_pages(jasper):
+    """As many sequences as a call takes, and more pages than the bitmap's words that waves give out by themselves."""
+    m = Model(2 ** 18, 3, 300_000, 8)
+    seqs = [2 ** 18 - 1, 0, 131_071, 77]
+    assert extend(jasper, m, seqs, [20, 1, 24, 9], 60) == 0
+    assert extend(jasper, m, seqs[::-1], [1, 0, 7, 4], 12) == 0
+    wide = Model(10, 20_000, 290_000, 8)
+    assert extend(jasper, wide, [3, 9, 1], [150_000, 1, 77_777], 230_000) == 0
+    jasper.truncate_tables(*wide.gpu, ints([3]), ints([9]), 8)
+    wide.truncate([3], [9])
+    assert extend(jasper, wide, [2, 3], [160_000, 100_001], 260_001) == 0
+
+
 def ref_prefixes(tables, lens, page, least):
     groups, shared = [], []
     for b in range(len(lens)):
