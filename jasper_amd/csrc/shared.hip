@@ -35,8 +35,11 @@ constexpr int kStage = 512;      // row offsets of a wave, in LDS
 constexpr int kJoin = 256;       // threads of a joining work-group
 constexpr int kPages = 1024;     // of a wide stream's table, in LDS
 constexpr int kTeam = 8;         // work-groups of a team at most
-constexpr int kWideStart = 8;    // what beginning a wide stream and a tile of it
-constexpr int kWideTile = 3;     // cost, in tiles of 32 tokens of a wave
+// What beginning a wide stream and a tile of it cost a work-group, in tiles of 32
+// tokens of a wave: it waits for pages, queries and tiles, and its waves join.
+// 64 sequences over 16,384 tokens, 64 in four groups over 8,000: 57.3 and 46.1
+// us; with 8 and 2 62.2 and 48.8, with 20 and 3 59.3 and 48.3.
+constexpr int kWideStart = 14, kWideTile = 2;
 
 constexpr int waves_of(int dt) { return dt == 256 ? 4 : 8; }    // of a work-group
 constexpr int tokens_of(int dt) { return 8192 / dt; }             // of a wide tile: 16 KB of K
@@ -67,6 +70,7 @@ struct Layout {
   // a group that began in an earlier launch: where, its prefix, and its first
   // sequence that is long enough (none: kNone)
   int cut_begin, cut_shared, cut;
+  int wider;  // whether a group has more rows than a work-group
   int totals[3];
   int part[3][8];
 };
@@ -133,7 +137,7 @@ __device__ int lay_out(const Shared& p, Layout& l) {
   constexpr int kThreads = NW * 64, kRun = kBatch / kThreads, TT = tokens_of(DT);
   const int t = threadIdx.x, gh = p.a.group;
   for (int i = t; i < kBatch; i += kThreads) l.leader[i] = kNone, l.last[i] = -1, l.from[i] = 0, l.own[i] = 0;
-  if (t == 0) l.cut_begin = p.first, l.cut_shared = 0, l.cut = kNone;
+  if (t == 0) l.cut_begin = p.first, l.cut_shared = 0, l.cut = kNone, l.wider = 0;
   // the groups' first sequences and prefixes, where there is room for them
   const bool held = p.n_groups <= kBatch;
   if (held)
@@ -168,7 +172,9 @@ __device__ int lay_out(const Shared& p, Layout& l) {
   // the team that the largest group would have, and what all groups would make of it
   int most = 0, team = 1;
   for (int i = t; i < p.count; i += kThreads) most = max(most, ceil_div(rows_of(i), kRows));
-  if (__syncthreads_or(most > 1)) {
+  if (most > 1) l.wider = 1;
+  __syncthreads();
+  if (l.wider) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) most = max(most, __shfl_xor(most, d, 64));
     if ((t & 63) == 0) l.part[0][t >> 6] = most;
@@ -310,7 +316,7 @@ struct Wide {
   const Shared& p;
   char* const lds;
   uint8_t (*const ok)[TT];
-  int32_t* const held;  // kPages pages of the table, from page0 on
+  int32_t* const held;  // kPages pages of the table, from page0 on, and whether one of them is none
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = wave / TW, tw = wave % TW;
 
@@ -626,8 +632,9 @@ struct Wide {
     const Params& a = p.a;
     place();
     __syncthreads();  // what was in LDS before has been read
+    if (tid == 0) held[kPages] = p.far;
     page0 = w.c * TT >> a.page_shift;
-    bool hole = p.far;
+    bool hole = false;
     const int n_pages = ((min(w.c1 * TT, w.tokens) - 1) >> a.page_shift) - page0 + 1;
     for (int i = tid; i < n_pages; i += kThreads) {
       const int32_t page = a.tables[w.source * a.table_stride + page0 + i];
@@ -640,8 +647,11 @@ struct Wide {
         if (chunk_of(e, tid, true) * 8 >= a.dim)
           for (int b = 0; b < kBuffers; ++b) *(uintx4*)(k_tile(b) + (e * kThreads + tid) * 16) = uintx4{0, 0, 0, 0};
     }
-    holes = __builtin_amdgcn_readfirstlane(__syncthreads_or(hole));
+    __syncthreads();
+    if (hole) held[kPages] = 1;
     look(w, w.c);
+    __syncthreads();
+    holes = __builtin_amdgcn_readfirstlane(held[kPages]);
     Staged st[2];
     const int n = w.c1 - w.c;
     if constexpr (F8) {
@@ -770,7 +780,7 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ Layout l;
   __shared__ uint8_t ok[W::kBuffers][W::TT];
-  __shared__ int32_t held[kPages];
+  __shared__ int32_t held[kPages + 1];
   const Params& a = p.a;
   const int team = lay_out<NW, DT>(p, l);
   const int wides = __builtin_amdgcn_readfirstlane(l.totals[0]), thins = __builtin_amdgcn_readfirstlane(l.totals[1]);
