@@ -23,10 +23,10 @@ where said) in float16, bfloat16 or float8_e4m3fn, any strides that keep a
 row's dim values together and rows on 16 bytes. Calls run on the current
 stream of the tensors' device, synchronize nothing and may be captured in a
 graph (PagedCache's bookkeeping is on the host and is not captured,
-GpuPagedCache's is). They take
-tensors with memory, and are not operators registered with torch:
-torch.compile runs them as they are, between the graphs before and after, and
-vmap, torch.func's grad and jvp, export and fake tensors end in an error.
+GpuPagedCache's is). They take tensors with memory, and are not operators
+registered with torch: torch.compile runs them as they are, between the graphs
+before and after, and vmap, torch.func's grad and jvp, export and fake tensors
+end in an error.
 """
 
 from __future__ import annotations
