@@ -155,7 +155,7 @@ __device__ int lay_out(const Shared& p, Layout& l) {
     }
     const int g = lo - 1;
     if (g < 0 || b >= end) continue;
-    const int shared = held ? l.thin[g] : p.shared[g], begin = held ? l.wide[g] : p.groups[g], slot = max(begin - p.first, 0);
+    const int shared = held ? l.thin[g] : p.shared[g], begin = held ? l.wide[g] : p.groups[g], slot = max(begin, p.first) - p.first;
     if (i == 0) l.cut_begin = max(begin, 0), l.cut_shared = shared;
     if (shared <= 0 || len < shared) continue;
     l.from[i] = shared, l.own[i] = slot;

@@ -100,6 +100,18 @@ def test_many_rows(jasper, sizes, hq, heads):
           ref_shared(q, keys, values, dim ** -0.5, F16, F16))
 
 
+def test_a_group_that_begins_before_the_batch(jasper):
+    """It begins with the batch, however far before it is said to, in every launch."""
+    groups = [(40, [40 + i % 3 for i in range(600)])]
+    kp, vp, tables, lens, starts, both, keys, values = build_shared(groups, 1, 8, 16, F16, 32)
+    q = randn((600, 2, 16), F16, 33, 2.0)
+    want = jasper.shared_attention(q, kp, vp, tables, lens, starts, both, return_lse=True)
+    for first in (-1, -(2 ** 31)):
+        starts[0] = first
+        got = jasper.shared_attention(q, kp, vp, tables, lens, starts, both, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def alike(got, want, dtype):
     """Two attentions of the same inputs, each within its bound of the same values."""
     a, b = got[0].double(), want[0].double()
