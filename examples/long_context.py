@@ -7,7 +7,8 @@ built over the keys of every key head, and then, for every new token,
   1. the token's queries are turned and its key and value appended,
   2. its query heads search the index of their key head by inner product,
   3. retrieved_attention reads the first tokens, the latest ones and those
-     found, decode_attention all of them.
+     found, decode_attention all of them, shared_attention all of them with the
+     document read once for both continuations.
 
 The index holds the document; the tokens that came after it are all read, as the
 window grows with them (a much longer answer would append them to an index of its
@@ -111,12 +112,14 @@ def main(argv=None):
         full, full_lse = cache.decode(0, step, q, return_lse=True)
         weights.append(torch.exp(lse - full_lse).mean().item())
         errors.append(((out.float() - full.float()).norm() / full.float().norm()).item())
+    prefixes = cache.prefixes(step)
     us = [timed(lambda: cache.retrieved(0, step, q, ids, first=a.first, last=last)), timed(lambda: cache.decode(0, step, q)),
-          timed(lambda: retrieve(searches, q, a.k))]
+          timed(lambda: retrieve(searches, q, a.k)), timed(lambda: cache.shared(0, step, q, prefixes))]
     if not a.quiet:
         print(f"{a.tokens} tokens, {a.first} + {a.k} + {last} read per query head: "
               f"{100 * sum(weights) / a.steps:.1f}% of the weight, output off by {100 * sum(errors) / a.steps:.2f}%; "
-              f"attention {us[0]:.1f} us of the retrieved, after {us[2]:.1f} us of searches; {us[1]:.1f} us of all")
+              f"attention {us[0]:.1f} us of the retrieved, after {us[2]:.1f} us of searches; {us[1]:.1f} us of all, "
+              f"{us[3]:.1f} us of all with the document read once")
     cache.free(answers)
     return sum(weights) / a.steps, sum(errors) / a.steps
 

@@ -74,7 +74,8 @@ __device__ __forceinline__ int axis_of(const RotaryAxes& a, int i) {
 // 4.7), 6007 of 32 + 2 x 8 into e4m3 pages 32 us (4.3); one token 3.6 us.
 //
 // AXES: a pair's position is its axis's. Chunks of one axis load their angles
-// as before, those that several axes have a part of pair by pair.
+// as before, those that several axes have a part of pair by pair. The same three
+// calls with three axes: 37.9, 30.6 and 5.9 us.
 template <typename T, typename CT, int P, bool APPEND, bool AXES>
 __global__ void token_kernel(TokenParams a) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;

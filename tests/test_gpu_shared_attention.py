@@ -8,10 +8,7 @@ once, u_w sum p|v| more, with u_w half the distance of neighbours of that type
 of the largest, so that their smallest step adds 2^-37 max|v| a token at most.
 """
 
-import importlib.util
-import itertools
 import math
-from pathlib import Path
 
 import pytest
 import torch

@@ -127,6 +127,14 @@ def test_shared_workspace_refuses(lib, batch, q_heads, max_len, groups):
     refused(lib, lib.jasperx_shared_workspace(batch, q_heads, ctypes.byref(pages()), max_len, groups), "too large")
 
 
+def test_shared_workspace_refuses_more_rows_than_a_launch_joins(lib):
+    p = pages()
+    p.heads = 1
+    most = (2 ** 32 - 1) // (512 * 256)  # rows of a launch have 256 threads each
+    assert lib.jasperx_shared_workspace(512, most, ctypes.byref(p), 100, 1) > 0
+    refused(lib, lib.jasperx_shared_workspace(512, most + 1, ctypes.byref(p), 100, 1), "too large")
+
+
 def test_workspaces_that_are_given(lib):
     assert lib.jasperx_shared_workspace(0, 32, ctypes.byref(pages()), 100, 0) == 0
     assert lib.jasperx_shared_workspace(64, 32, ctypes.byref(pages()), 2 ** 20, 1) > 0
