@@ -40,6 +40,7 @@ constexpr int kTeam = 8;         // work-groups of a team at most
 // 64 sequences over 16,384 tokens, 64 in four groups over 8,000: 57.3 and 46.1
 // us; with 8 and 2 62.2 and 48.8, with 20 and 3 59.3 and 48.3.
 constexpr int kWideStart = 14, kWideTile = 2;
+constexpr int kLeast = 2;      // tiles of a wave
 
 constexpr int waves_of(int dt) { return dt == 256 ? 4 : 8; }    // of a work-group
 constexpr int tokens_of(int dt) { return 8192 / dt; }             // of a wide tile: 16 KB of K
@@ -70,6 +71,7 @@ struct Layout {
   // a group that began in an earlier launch: where, its prefix, and its first
   // sequence that is long enough (none: kNone)
   int cut_begin, cut_shared, cut;
+  int longest[8];  // tiles of the longest stream that is not wide, by waves
   int wider;  // whether a group has more rows than a work-group
   int totals[3];
   int part[3][8];
@@ -99,6 +101,17 @@ __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
   x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // lane 15 of a row to the next one
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // lane 31 to the last two
+  return x;
+}
+
+// In lane 63: the largest x of a wave, none below 0.
+__device__ __forceinline__ int wave_max(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false));
   return x;
 }
 
@@ -196,7 +209,7 @@ __device__ int lay_out(const Shared& p, Layout& l) {
   }
   const int wide_tile = kWideTile * team, wide_start = kWideStart * team;
   int units[3] = {0, 0, 0}, before[3], total[3];
-  int each[3][kRun];
+  int each[3][kRun], longest = 0;
 #pragma unroll
   for (int k = 0; k < kRun; ++k) {
     const int i = t * kRun + k;
@@ -206,11 +219,14 @@ __device__ int lay_out(const Shared& p, Layout& l) {
     if (rows) {
       const int shared = l.from[l.leader[i]];
       if (rows > kHeads) units[0] += p.a.heads * blocks_of(rows, team) * (wide_start + ceil_div(shared, TT) * wide_tile);
-      else units[1] += p.a.heads * (kStart + ceil_div(shared, kTile));
+      else units[1] += p.a.heads * (kStart + ceil_div(shared, kTile)), longest = max(longest, ceil_div(shared, kTile));
     }
     const int slot = l.own[i], from = shares(l, slot) ? l.from[i] : 0;
-    units[2] += p.a.heads * p.a.head_tiles * (kStart + max(1, ceil_div(l.len[i] - (from & ~7), kTile)));
+    const int tiles = max(1, ceil_div(l.len[i] - (from & ~7), kTile));
+    units[2] += p.a.heads * p.a.head_tiles * (kStart + tiles), longest = max(longest, tiles);
   }
+  longest = wave_max(longest);
+  if ((t & 63) == 63) l.longest[t >> 6] = longest;
   block_scan<NW>(units, before, total, l.part);
 #pragma unroll
   for (int k = 0; k < kRun; ++k) {
@@ -795,9 +811,17 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
   const int rings = gridDim.x % 8 ? 1 : 8, place = blockIdx.x / rings, teams = gridDim.x / rings / team * rings;
   const int me_team = place / team * rings + blockIdx.x % rings, member = place % team, id = me_team * team + member;
   Share share;
-  // a team has units for all of its waves, and at least a wide tile's: so that
-  // within a stream each has a part
-  share.waves = min(max(1, total / (team * max(NW, kWideTile))), teams);
+  // A wave has at least two tiles, more of long streams: a stream of n tiles takes
+  // as long as the tiles of one wave and the join of as many parts as there are
+  // waves, least where a wave has about sqrt(n) / 4 (2 sequences over 32,768 tokens
+  // of 2 key heads: 48 us with a tile each, 22 with eight). A team has at least a
+  // wide tile's units, so that within a stream each has a part, and eight, as it is
+  // the whole work-group that begins it.
+  int longest = l.longest[0];
+#pragma unroll
+  for (int k = 1; k < NW; ++k) longest = max(longest, l.longest[k]);
+  const int least = max(kLeast, (int)(0.25f * __builtin_amdgcn_sqrtf((float)__builtin_amdgcn_readfirstlane(longest))));
+  share.waves = min(max(1, total / (team * max(least, wides ? max(NW, kWideTile) : 1))), teams);
   share.each = total / share.waves;
   share.more = total % share.waves;
   if (me_team >= share.waves) return;
@@ -831,7 +855,9 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
   // the waves' shares of the rest
   constexpr int VD = DT / 16;
   const int lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = team * NW;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // waves of a team that take part: as many in each, so that a stream's are numbered one after the other
+  const int waves = min(max(1, share.each / least), team * NW);
   const int x0 = max(u0, wides), span = u1 - x0;
   if (span <= 0) return;
   // n units go to the last min(n, waves) waves of a team: only where the wide
@@ -844,9 +870,9 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
     while (wave_begin(n, k + 1) <= u - begin) ++k;
     return of * waves + waves - min(n, waves) + k;
   };
-  const int mine = member * NW + wave - (waves - min(span, waves));
-  if (mine < 0) return;
-  const int me = id * NW + wave, a1 = x0 + wave_begin(span, mine + 1);
+  const int at_wave = wave * team + member, mine = at_wave - (waves - min(span, waves));
+  if (mine < 0 || at_wave >= waves) return;
+  const int me = me_team * waves + at_wave, a1 = x0 + wave_begin(span, mine + 1);
   for (int u = x0 + wave_begin(span, mine); u < a1;) {
     Span sp{};
     Stream at;

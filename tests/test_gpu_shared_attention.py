@@ -97,6 +97,17 @@ def test_many_rows(jasper, sizes, hq, heads):
           ref_shared(q, keys, values, dim ** -0.5, F16, F16))
 
 
+@pytest.mark.parametrize("shared", [1, 63, 64, 500, 2100, 9000, 40_000])
+@pytest.mark.parametrize("hq,heads,dim,dtype,cache", [(4, 2, 64, F16, F16), (8, 1, 128, BF16, F8), (2, 1, 256, BF16, BF16)])
+def test_few_rows(jasper, shared, hq, heads, dim, dtype, cache):
+    """Waves have more tiles of longer prefixes, work-groups fewer of them; a long stream beside short ones."""
+    groups = [(shared, [shared + 3, shared]), (0, [5]), (shared // 2, [shared // 2 + 1, shared // 2 + 40])]
+    kp, vp, tables, lens, starts, both, keys, values = build_shared(groups, heads, 16, dim, cache, 34)
+    q = randn((5, hq, dim), dtype, 35, 2.0)
+    got = jasper.shared_attention(q, kp, vp, tables, lens, starts, both, return_lse=True)
+    check(got, ref_shared(q, keys, values, dim ** -0.5, dtype, cache))
+
+
 def test_a_group_that_begins_before_the_batch(jasper):
     """It begins with the batch, however far before it is said to, in every launch."""
     groups = [(40, [40 + i % 3 for i in range(600)])]
