@@ -792,8 +792,8 @@ struct Wide {
 // 64 sequences over 16,384 tokens of 8 key heads of 128 bf16 values, under 256
 // rows: 49 us, of which the first 11 go by before a wide stream's first product;
 // the matrix cores are busy 21% of it. 16 over 131,000 in e4m3, under 128 rows of
-// 8 heads: 110 to 115 us, 32%. 41 in seven groups of 900 to 12,345, heads of 64:
-// 26.5 us, 4.2 TB/s, waiting for reads 52% of its waves' cycles.
+// 8 heads: 112 to 119 us, 32%. 41 in seven groups of 900 to 12,345, heads of 64:
+// 26.6 us, 4.2 TB/s, waiting for reads 51% of its waves' cycles.
 template <typename T, bool F8, int DT, bool FULL>
 __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_kernel(Shared p) {
   typedef Wide<T, F8, DT, FULL> W;
@@ -928,7 +928,7 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
 }
 
 // Joins the parts of a query row: a thread has four dims of every kAtOnce-th part.
-// Bound by its chain of three reads (ends, parts, output): 4.7 to 7.6 us.
+// Bound by its chain of three reads (ends, parts, output): 4.0 to 7.6 us.
 template <typename T, int DT>
 __global__ __launch_bounds__(kJoin) void join_kernel(Shared p) {
   constexpr int kLanes = DT / 4, kAtOnce = kJoin / kLanes, kLoads = 8;

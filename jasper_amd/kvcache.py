@@ -215,7 +215,8 @@ def shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     A sequence that is shorter than its group's prefix reads its own pages, and
     so does one that is in no group. Groups are best as large as they come:
     every group costs as much as a sequence, and 16 query heads of one key head
-    fill a matrix instruction.
+    fill a matrix instruction. Two sequences of few heads with less than about
+    32,000 tokens in common are as well served by decode_attention.
     """
     return _kv().shared_attention(q, k_pages, v_pages, tables, lens, groups, shared, scale, k_scale, v_scale, max_len,
                                   return_lse)
