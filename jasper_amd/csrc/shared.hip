@@ -521,10 +521,9 @@ struct Wide {
     }
   }
 
-  // The weights of scores, rounded to their type once: a second term of them is
-  // half again as many products, and takes bf16's error from 0.0019 to the
-  // output's own 0.0017.
-  __device__ __forceinline__ void weigh(const Scores& s, Frag (&w)[NB * 2]) {
+  // The weights of scores in two terms of their type, as decode_attention's, so
+  // that their rounding adds nothing to the output's own.
+  __device__ __forceinline__ void weigh(const Scores& s, Frag (&hi)[NB * 2], Frag (&lo)[NB * 2]) {
 #pragma unroll
     for (int n = 0; n < NB * 2; ++n)
 #pragma unroll
@@ -532,7 +531,9 @@ struct Wide {
         const float y0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 2][n % 2 * 8 + r], cs, -use));
         const float y1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 2][n % 2 * 8 + r + 1], cs, -use));
         sum += y0 + y1;
-        w[n][r / 2] = pack2<PT>(y0, y1);
+        hi[n][r / 2] = pack2<PT>(y0, y1);
+        const floatx2 back = unpack2<PT>(hi[n][r / 2]);
+        lo[n][r / 2] = pack2<PT>(y0 - back.x, y1 - back.y);
       }
   }
 
@@ -549,19 +550,21 @@ struct Wide {
     }
   }
 
-  __device__ __forceinline__ void add_values(const Frag (&f)[DB], Frag w) {
+  __device__ __forceinline__ void add_values(const Frag (&f)[DB], Frag hi, Frag lo) {
 #pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] = mfma32<PT>(f[d], w, o[d]);
+    for (int d = 0; d < DB; ++d) o[d] = mfma32<PT>(f[d], hi, o[d]);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = mfma32<PT>(f[d], lo, o[d]);
   }
 
-  __device__ __forceinline__ void values(int b, const Frag (&w)[NB * 2]) {
+  __device__ __forceinline__ void values(int b, const Frag (&w)[NB * 2], const Frag (&lo)[NB * 2]) {
     Frag f[2][DB];
     read_values(b, 0, f[0]);
 #pragma unroll
     for (int n = 0; n < NB * 2; ++n) {
       if (n + 1 < NB * 2) read_values(b, n + 1, f[n + 1 & 1]);
       __builtin_amdgcn_sched_barrier(0);
-      add_values(f[n & 1], w[n]);
+      add_values(f[n & 1], w[n], lo[n]);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -576,7 +579,7 @@ struct Wide {
   template <bool STEADY>
   __device__ __forceinline__ void step(const WidePart& w, int t, Scores& s, Staged& st) {
     const int b = t - w.c, to = (b + kAhead) & 3;
-    Frag kf[NB * KS], wf[NB * 2], vf[2][DB];
+    Frag kf[NB * KS], wf[NB * 2], lf[NB * 2], vf[2][DB];
     const auto apart = [] { __builtin_amdgcn_sched_barrier(0); };
     const auto send = [&](auto part) {
       if constexpr (STEADY) fetch_part<decltype(part)::value>(w, t + kAhead, to, st);
@@ -589,7 +592,7 @@ struct Wide {
     __syncthreads();
     read_keys((b + 1) & 3, kf);
     apart();
-    weigh(s, wf);
+    weigh(s, wf, lf);
     apart();
     if (F8 && t + 2 < w.c1) store((b + 2) & 3, st);
     if (!STEADY && t + kAhead < w.c1) fetch(w, t + kAhead, to, st);
@@ -603,7 +606,7 @@ struct Wide {
     for (int n = 0; n < NB * 2; ++n) {
       if (n + 1 < NB * 2) read_values(b & 3, n + 1, vf[n + 1 & 1]);
       apart();
-      add_values(vf[n & 1], wf[n]);
+      add_values(vf[n & 1], wf[n], lf[n]);
       apart();
       if (n == 0) send(std::integral_constant<int, 2>{});
       if (n == 1) send(std::integral_constant<int, 3>{});
@@ -639,9 +642,9 @@ struct Wide {
       for (; t < steady; ++t) step<true>(w, t, s, st[0]);
       for (; t + 1 < w.c1; ++t) step<false>(w, t, s, st[0]);
     }
-    Frag wf[NB * 2];
-    weigh(s, wf);
-    values((w.c1 - 1 - w.c) & 3, wf);
+    Frag wf[NB * 2], lf[NB * 2];
+    weigh(s, wf, lf);
+    values((w.c1 - 1 - w.c) & 3, wf, lf);
   }
 
   __device__ __forceinline__ void run_stretch(const WidePart& w) {
