@@ -276,6 +276,28 @@ struct WidePart {
   int c, c1;  // its tiles
 };
 
+// Where a stretch ends that begins with tile c of `tokens` tokens: before c1, and
+// with the last of kPages pages, of which the first may have begun before the tile.
+__host__ __device__ constexpr int stretch_end(int c, int c1, int tokens, int page_shift) {
+  const int64_t last = ((int64_t)c * tokens >> page_shift) + kPages;
+  const int64_t end = (last << page_shift) / tokens;
+  return end < c1 ? (int)end : c1;
+}
+
+constexpr bool stretches_fit() {
+  for (int tokens = tokens_of(256); tokens <= tokens_of(64); tokens *= 2)
+    for (int shift = 3; shift <= 8; ++shift)
+      for (int c = 0, far = (int)(0x7FFFFF00ll / tokens); c < 32; ++c)
+        for (const int from : {c, far - 40'000 + c, far - c - 1}) {
+          const int end = stretch_end(from, far, tokens, shift);
+          const int64_t first = (int64_t)from * tokens >> shift, last = ((int64_t)end * tokens - 1) >> shift;
+          if (end <= from || last - first >= kPages) return false;
+          if (end < far && (((int64_t)end + 1) * tokens - 1 >> shift) - first < kPages) return false;  // there was room
+        }
+  return true;
+}
+static_assert(stretches_fit(), "a stretch has at least a tile and at most kPages pages");
+
 // A wave's 64 times 16 bytes from memory to LDS at `to` on, in the lanes' order,
 // past the registers; lanes that do not take part leave theirs out. They arrive
 // in order and are waited for by loads_left. (The compiler does not see these
@@ -332,7 +354,8 @@ struct Wide {
   const Shared& p;
   char* const lds;
   uint8_t (*const ok)[TT];
-  int32_t* const held;  // kPages pages of the table, from page0 on, and whether one of them is none
+  int32_t* const held;     // kPages pages of the table, from page0 on
+  int32_t* const masked;  // whether one of them is none, or rows are far apart
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = wave / TW, tw = wave % TW;
 
@@ -651,7 +674,7 @@ struct Wide {
     const Params& a = p.a;
     place();
     __syncthreads();  // what was in LDS before has been read
-    if (tid == 0) held[kPages] = p.far;
+    if (tid == 0) *masked = p.far;
     page0 = w.c * TT >> a.page_shift;
     bool hole = false;
     const int n_pages = ((min(w.c1 * TT, w.tokens) - 1) >> a.page_shift) - page0 + 1;
@@ -667,10 +690,10 @@ struct Wide {
           for (int b = 0; b < kBuffers; ++b) *(uintx4*)(k_tile(b) + (e * kThreads + tid) * 16) = uintx4{0, 0, 0, 0};
     }
     __syncthreads();
-    if (hole) held[kPages] = 1;
+    if (hole) *masked = 1;
     look(w, w.c);
     __syncthreads();
-    holes = __builtin_amdgcn_readfirstlane(held[kPages]);
+    holes = __builtin_amdgcn_readfirstlane(*masked);
     Staged st[2];
     const int n = w.c1 - w.c;
     if constexpr (F8) {
@@ -724,10 +747,9 @@ struct Wide {
       k_off[e] = r + chunk_of(e, tid, true) * 16, v_off[e] = r + chunk_of(e, tid, false) * 16;
     }
     // as many tiles as there is room for pages of, and again
-    const int most = max(1, (kPages << a.page_shift) / TT);
     WidePart stretch = w;
     for (; stretch.c < w.c1; stretch.c = stretch.c1) {
-      stretch.c1 = min(w.c1, stretch.c + most);
+      stretch.c1 = stretch_end(stretch.c, w.c1, TT, a.page_shift);
       run_stretch(stretch);
     }
     sum += __shfl_xor(sum, 32, 64);
@@ -804,7 +826,7 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ Layout l;
   __shared__ uint8_t ok[W::kBuffers][W::TT];
-  __shared__ int32_t held[kPages + 1];
+  __shared__ int32_t held[kPages], masked;
   const Params& a = p.a;
   const int team = lay_out<NW, DT>(p, l);
   const int wides = __builtin_amdgcn_readfirstlane(l.totals[0]), thins = __builtin_amdgcn_readfirstlane(l.totals[1]);
@@ -847,7 +869,7 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
     w.c = ceil_div(max(0, pos - start_cost), tile_cost);
     w.c1 = ceil_div(max(0, end - start_cost), tile_cost);
     if (w.c < w.c1 && w.rows > 0) {
-      W wide{p, lds, ok, held};
+      W wide{p, lds, ok, held, &masked};
       wide.run(w);
       wide.write(w, id, share.owner(begin + start_cost + (tiles - 1) * tile_cost) - me_team + 1, team, l);
     }
