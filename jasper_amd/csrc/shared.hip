@@ -302,15 +302,18 @@ static_assert(stretches_fit(), "a stretch has at least a tile and at most kPages
 // past the registers; lanes that do not take part leave theirs out. They arrive
 // in order and are waited for by loads_left. (The compiler does not see these
 // writes to LDS coming: they go to tiles that nobody reads before a barrier.)
+// Nor does it see the instruction's own hazards: one wait state after m0 is
+// written, five from a vector instruction that writes the scalar base
+// (readfirstlane) on, of which the write of m0 is one.
 __device__ __forceinline__ void load_lds(const void* from, uint32_t to) {
   to = __builtin_amdgcn_readfirstlane(to);
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "memory", "m0");
 }
 __device__ __forceinline__ void load_lds(const char* base, uint32_t offset, uint32_t to) {
   const uint64_t at = (uint64_t)base;
   base = (const char*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at));
   to = __builtin_amdgcn_readfirstlane(to);
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(to) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void loads_left() {
