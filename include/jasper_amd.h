@@ -449,8 +449,10 @@ int64_t jasperx_extend_workspace(int64_t n, int64_t pages);
 int64_t jasperx_truncate_tables(const jasperx_page_table* table, const int32_t* seqs, const int32_t* to, int64_t n,
                                 void* stream);
 /* Sequences into[i], empty until now, get the tokens of seqs[i], on the same
- * pages. Pairs with an id outside, with an into that is not empty, that is
- * listed before or that stands in the other list too are left out. */
+ * pages. Left out are pairs with an id outside, with an into that is not empty,
+ * that is listed before or that stands in seqs too, and with a sequence that
+ * stands in into too (of a pair with both ids inside), though that pair is left
+ * out as well: forks of forks take a call each. */
 int64_t jasperx_fork_tables(const jasperx_page_table* table, const int32_t* seqs, const int32_t* into, int64_t n,
                             void* stream);
 /* Neighbours in a batch that begin with the same pages, as

@@ -368,7 +368,7 @@ __global__ __launch_bounds__(kRowThreads) void fork_kernel(PageState st, const i
   const int i = blockIdx.x;
   const int32_t from = seqs[i], to = into[i];
   if (from < 0 || from >= st.sequences || to < 0 || to >= st.sequences) return;
-  bool clash = false;  // what another pair writes is neither read nor written
+  bool clash = false;  // what another pair names to be written is neither read nor written
   for (int j = threadIdx.x; j < n; j += kRowThreads) {
     const bool other = into[j] >= 0 && into[j] < st.sequences && seqs[j] >= 0 && seqs[j] < st.sequences;
     clash |= seqs[j] == to || (other && (into[j] == from || (j < i && into[j] == to)));

@@ -262,8 +262,10 @@ def fork_tables(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, fr
     """Gives the sequences into[i], empty until now, the tokens of seqs[i]
     (int32 [n]), on the same pages. State as in `extend_tables`. A sequence may
     be forked several times. Pairs are left out whose ids are outside the
-    tables, and whose into is not empty, is listed before, or stands in seqs
-    too."""
+    tables, whose into is not empty, is listed before or stands in seqs too,
+    and whose sequence stands in into too (of a pair with both ids inside):
+    with seqs 0 1 and into 1 2 neither is made. Forks of forks take a call
+    each."""
     _kv().fork_tables(tables, lens, refs, free, seqs, into, page_size)
 
 
