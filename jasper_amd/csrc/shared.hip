@@ -1043,10 +1043,13 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_l
   a.group = (int)(q_heads / pages.heads);
   a.head_tiles = (a.group + kHeads - 1) / kHeads;
   const int64_t count = std::min<int64_t>(batch, kBatch);
-  // units of a launch, at most
-  const int64_t tiles = max_len / kTile * kWideTile + 2 + kStart + kTeam * (kWideStart + kWideTile);
-  const int64_t per_seq = pages.heads * (2 * (int64_t)a.head_tiles + a.group / 32 + 2);
-  if (tiles > 0x7FFFFFFF / std::max<int64_t>(1, count * per_seq)) throw std::invalid_argument("batch x heads x tokens is too large");
+  // Units of a launch, at most: what a prefix of n tiles under more than 16 rows
+  // costs, a quarter more with teams, is no more than its members would cost for
+  // themselves, n for each 16 of their rows, but for its start and its last tile.
+  const int64_t tiles = max_len / kTile + 2 + kStart;
+  const int64_t start = (kTeam + a.group / kRows + 2) * (kWideStart + kWideTile);
+  const int64_t most = 0x7FFFFFFF / std::max<int64_t>(1, count * pages.heads);  // of a sequence's streams to a key head
+  if (tiles > most || tiles * a.head_tiles > most - start) throw std::invalid_argument("batch x heads x tokens is too large");
   if (count * q_heads * kJoin > 0xFFFFFFFFll) throw std::invalid_argument("batch x heads is too large");  // threads of the joining launch
   a.work_groups = kGroups;  // those without units end at once
   const int64_t rows = count * q_heads, row = part_row(a.dt) * 4;

@@ -568,6 +568,11 @@ class GpuPagedCache(PagedCache):
     nothing is stored, and step.missing says so (extend_tables), to be read
     when it suits.
 
+    max_pages (default: all n_pages), or max_len in `extend`, is the width of
+    the tables that every step writes, and the lengths that `decode` and
+    `shared` lay their workspaces out for and refuse when they are too large:
+    give the longest that a sequence may become.
+
         step = cache.extend(seqs, counts, n_tokens)       # int32 tensors
         prefixes = cache.prefixes(step)
         for layer in range(n_layers):

@@ -40,3 +40,19 @@ def test_stretches_that_begin_inside_a_page(jasper, dim, page, cache, prefix, ou
     both = torch.tensor([prefix], dtype=torch.int32, device="cuda")
     got = jasper.shared_attention(q, kp, vp, tables, lens, groups, both, k_scale=ks, v_scale=vs, return_lse=True)
     alike(got, jasper.decode_attention(q, kp, vp, tables, lens, k_scale=ks, v_scale=vs, return_lse=True), F16)
+
+
+def test_tables_of_a_whole_cache_under_a_large_batch(jasper):
+    """256 sequences of 32 heads whose tables have room for 2^20 tokens (refused before) are attended to as by decode."""
+    batch, heads, page, dim = 256, 32, 16, 64
+    kp, vp = make_pages(300, heads, page, dim, F16, seed=70)
+    tables = torch.full((batch, 2 ** 20 // page), -1, dtype=torch.int32, device="cuda")
+    own = torch.arange(batch, dtype=torch.int32, device="cuda")
+    tables[:, :30] = torch.arange(260, 290, dtype=torch.int32, device="cuda")
+    tables[:, 30] = own
+    lens = 480 + own % 16
+    q = randn((batch, heads, dim), F16, 71, 2.0)
+    groups = torch.tensor([0, 10, 130, batch], dtype=torch.int32, device="cuda")
+    both = torch.tensor([480, 33, 480], dtype=torch.int32, device="cuda")
+    got = jasper.shared_attention(q, kp, vp, tables, lens, groups, both, return_lse=True)
+    alike(got, jasper.decode_attention(q, kp, vp, tables, lens, return_lse=True), F16)
