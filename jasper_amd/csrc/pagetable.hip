@@ -95,10 +95,11 @@ __device__ __forceinline__ void block_scan(const int64_t (&x)[N], int64_t (&befo
 __device__ __forceinline__ int pages_of(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
 
 struct PlanLds {
-  int32_t held[kGrowers];
+  alignas(16) int32_t held[kGrowers];  // read four at a time
   int32_t bases[kBases];  // free pages before each word of the bitmap
   int64_t part[5 * kWaves];
 };
+static_assert(alignof(PlanLds) == 16, "dynamic LDS beside it gives no alignment");
 
 // One work-group decides: how many pages each request takes, which are free,
 // whether there are enough. A thread has a run of requests (one of them, in
