@@ -1128,7 +1128,7 @@ extern "C" int64_t jasperx_shared_workspace(int64_t batch, int64_t q_heads, cons
     if (batch < 0 || batch > 65535 || q_heads < 1 || q_heads > 65535 || q_heads % p.heads || max_len < 0 ||
         max_len > 0x7FFFFFFF || n_groups < 0 || n_groups > batch)
       throw std::invalid_argument("bad sizes (too large, or below 0)");
-    return shared_workspace(batch, q_heads, p, max_len, n_groups);
+    return shared_workspace(batch, q_heads, p, max_len);
   });
 }
 

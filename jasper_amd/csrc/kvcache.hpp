@@ -105,7 +105,7 @@ void attend(const AttendArgs& a, const KvPages& pages, hipStream_t s);
 // Attention of one new token per sequence, where sequences groups[g] to
 // groups[g + 1] - 1 have their first shared[g] tokens in common. max_len is
 // what the workspace was sized for.
-int64_t shared_workspace(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_len, int64_t n_groups);
+int64_t shared_workspace(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_len);
 void shared_attend(const AttendArgs& a, const int32_t* groups, const int32_t* shared, int64_t n_groups, const KvPages& pages,
                    hipStream_t s);
 

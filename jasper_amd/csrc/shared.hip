@@ -1037,7 +1037,7 @@ struct Plan {
   int64_t ends, firsts, wide_rest, wave_rest, bytes;  // of the workspace: bytes of each
 };
 
-Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_len, int64_t n_groups) {
+Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_len) {
   Plan a;
   a.dt = pages.dim <= 64 ? 64 : pages.dim <= 128 ? 128 : 256;
   a.group = (int)(q_heads / pages.heads);
@@ -1080,8 +1080,8 @@ void launch_dim(const Shared& p, const Plan& plan, hipStream_t s) {
 
 }  // namespace
 
-int64_t shared_workspace(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_len, int64_t n_groups) {
-  return batch ? plan_of(batch, q_heads, pages, max_len, n_groups).bytes : 0;
+int64_t shared_workspace(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_len) {
+  return batch ? plan_of(batch, q_heads, pages, max_len).bytes : 0;
 }
 
 void shared_attend(const AttendArgs& a, const int32_t* groups, const int32_t* shared, int64_t n_groups, const KvPages& pages,
@@ -1091,7 +1091,7 @@ void shared_attend(const AttendArgs& a, const int32_t* groups, const int32_t* sh
   Shared p{};
   Params& r = p.a;
   r.limit = pages.pages ? (int)std::min<int64_t>({a.max_len, width, 0x7FFFFF00}) : 0;
-  const Plan plan = plan_of(a.batch, a.q.heads, pages, a.max_len, n_groups);
+  const Plan plan = plan_of(a.batch, a.q.heads, pages, a.max_len);
   if (a.workspace_bytes < plan.bytes || !a.workspace || ((uintptr_t)a.workspace & 15u))
     throw std::invalid_argument("workspace must be 16-byte aligned and hold " + std::to_string(plan.bytes) + " bytes");
   r.q = (const char*)a.q.p, r.q_stride = a.q.stride, r.q_head = a.q.head_stride;
