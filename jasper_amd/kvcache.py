@@ -615,14 +615,15 @@ class GpuPagedCache(PagedCache):
 
     def extend(self, seqs: torch.Tensor, counts: torch.Tensor, n_tokens: int, max_len: int | None = None) -> Step:
         """extend_tables, and the copies of pages that are shared no longer, in all layers. n_tokens: the counts' sum,
-        or more (the rest are tokens without a slot). max_len: no sequence is longer than that now."""
+        or more (the rest are tokens without a slot). max_len: no sequence is longer than that now, in whole pages;
+        where one would be, nothing is stored (missing -1)."""
         width = self.tables.size(1)
         longest = width * self.page_size
         if max_len is not None:
             if max_len < 0:
                 raise ValueError("max_len must be at least 0")
-            longest = min(longest, max_len)
-            width = -(-longest // self.page_size)
+            width = min(width, -(-max_len // self.page_size))
+            longest = width * self.page_size  # what extend_tables lets a sequence have is attended to
         positions, slots, starts, tables, lens, src, dst, missing = extend_tables(
             *self._state(), seqs, counts, self.page_size, n_tokens, width)
         copy_pages(self.k_pages, self.v_pages, src, dst)
