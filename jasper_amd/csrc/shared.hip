@@ -292,7 +292,7 @@ constexpr bool stretches_fit() {
           const int end = stretch_end(from, far, tokens, shift);
           const int64_t first = (int64_t)from * tokens >> shift, last = ((int64_t)end * tokens - 1) >> shift;
           if (end <= from || last - first >= kPages) return false;
-          if (end < far && (((int64_t)end + 1) * tokens - 1 >> shift) - first < kPages) return false;  // there was room
+          if (end < far && ((((int64_t)end + 1) * tokens - 1) >> shift) - first < kPages) return false;  // there was room
         }
   return true;
 }
@@ -304,7 +304,10 @@ static_assert(stretches_fit(), "a stretch has at least a tile and at most kPages
 // writes to LDS coming: they go to tiles that nobody reads before a barrier.)
 // Nor does it see the instruction's own hazards: one wait state after m0 is
 // written, five from a vector instruction that writes the scalar base
-// (readfirstlane) on, of which the write of m0 is one.
+// (readfirstlane) on, of which the write of m0 is one. It is told of m0, which it
+// reserves and warns of: nothing is kept there.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_lds(const void* from, uint32_t to) {
   to = __builtin_amdgcn_readfirstlane(to);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "memory", "m0");
@@ -315,6 +318,7 @@ __device__ __forceinline__ void load_lds(const char* base, uint32_t offset, uint
   to = __builtin_amdgcn_readfirstlane(to);
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(to) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void loads_left() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
