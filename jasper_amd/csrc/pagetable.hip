@@ -18,7 +18,10 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the planning work-group
 constexpr int kRowThreads = 256;
 constexpr int kGrowers = 4096;         // last pages held in LDS at once
-constexpr int kBases = 8192;           // words of the bitmap whose pages waves give out
+// Words of the bitmap whose pages waves give out, what LDS holds numbers of; those
+// of more are gone through by a thread each: 20,000 pages and their truncation 33.6 us
+// in a cache of 262,144, 44.9 in one of 262,176, 162 in one of 2,000,000.
+constexpr int kBases = 8192;
 constexpr int kSequences = 1 << 18;    // at most: a bit for each in LDS
 
 // What the plan says of a request. fresh: the places of the table from which on
@@ -501,13 +504,15 @@ void extend_tables(const PageState& state, const ExtendArgs& a, hipStream_t s) {
   p.list = (int32_t*)(w + round16(a.n * (int64_t)sizeof(Request)));
   p.growers = (int32_t*)((char*)p.list + round16(4 * (int64_t)state.pages));
   const size_t lds = ((size_t)state.sequences + 31) / 32 * 4;
-  // What little there is to write is written by the planning work-group: a second
-  // kernel is a launch. 48 requests with tables of 600 are worth one (16.3 us a step
-  // with its truncation, 17.0 otherwise).
-  const bool all = a.n * a.width + a.n_tokens <= 8192;
+  // What little there is to write is written by the planning work-group's 16 waves,
+  // a request each: a second kernel is a launch. Next tokens with the truncation back,
+  // in a graph (and launched one by one), one kernel / two: 16 requests with tables of
+  // 40 10.9 / 11.5 us (12.5 / 14.9), of 256 11.2 / 11.4 (13.3 / 15.3); 32 with tables
+  // of 40 12.4 / 11.5 (12.4 / 15.0); 64 of 8 15.3 / 12.2 (15.9 / 14.9), 48 of 600
+  // 16.6 / 11.9; 4 with tables of 250 and 1,000 tokens each 14.1 / 12.8.
+  const bool all = a.n <= 2 * kWaves && a.n * a.width + a.n_tokens <= 512 * std::max<int64_t>(1, a.n);
   const bool one = a.n <= kThreads;
-  auto kernel = all ? (one ? plan_kernel<true, true> : plan_kernel<true, false>)
-                    : (one ? plan_kernel<false, true> : plan_kernel<false, false>);
+  auto kernel = all ? plan_kernel<true, true> : one ? plan_kernel<false, true> : plan_kernel<false, false>;
   if (lds > 8192)  // with what the kernel has anyway more than 64 KB
     hip_check(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "extend tables");
   kernel<<<1, kThreads, lds, s>>>(p);
@@ -542,7 +547,10 @@ void shared_prefixes(const int32_t* tables, int64_t stride, int64_t width, const
   if (workspace_bytes < prefixes_workspace(batch) || (batch && !workspace))
     throw std::invalid_argument("workspace must hold " + std::to_string(prefixes_workspace(batch)) + " bytes");
   Prefixes p{tables, stride, (int)width, lens, (int)batch, page_shift, least, groups, shared, (int32_t*)workspace};
-  if (batch * width <= 65536) {
+  // Few sequences' prefixes are found by the grouping work-group's waves: 16 with
+  // tables of 64 4.1 us, 5.0 with a kernel before it, of 4,096 14.2 and 14.6; 32 of
+  // 64 4.9 and 5.4, of 512 6.3 and 5.8; 48 of 64 5.9 and 5.3, 1,000 of 64 65 and 6.7.
+  if (batch <= kWaves || (batch <= 2 * kWaves && batch * width <= 8192)) {
     group_kernel<true><<<1, kThreads, 0, s>>>(p);
   } else {
     run_kernel<<<(unsigned)batch, 64, 0, s>>>(p);

@@ -143,7 +143,10 @@ __device__ __forceinline__ int blocks_of(int rows, int team) { return ceil_div(c
 // Work-groups form teams: those of one take the same tokens under different
 // rows, on one XCD, so that its L2 reads them from memory once (512 rows over
 // 65,536 tokens of 8 heads: 252 us without, and 185 with no loads at all). Groups
-// of unlike size might leave members without rows; then there are no teams.
+// of unlike size might leave members without rows; where that would be more than a
+// quarter more tiles there are no teams (512 rows over 131,072 tokens beside 128 over
+// 32,768, 1.18 times the tiles: 480 us with teams, 498 without; over 65,536, 1.33
+// times: 540 and 509; 512 and 384 over 16,384, 1.14 times: 127 and 125).
 // Returns the work-groups of a team.
 template <int NW, int DT>
 __device__ int lay_out(const Shared& p, Layout& l) {
