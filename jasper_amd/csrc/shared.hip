@@ -37,9 +37,11 @@ constexpr int kPages = 1024;     // of a wide stream's table, in LDS
 constexpr int kTeam = 8;         // work-groups of a team at most
 // What beginning a wide stream and a tile of it cost a work-group, in tiles of 32
 // tokens of a wave: it waits for pages, queries and tiles, and its waves join.
-// 64 sequences over 16,384 tokens, 64 in four groups over 8,000: 57.3 and 46.1
-// us; with 8 and 2 62.2 and 48.8, with 20 and 3 59.3 and 48.3.
-constexpr int kWideStart = 14, kWideTile = 2;
+// 64 sequences over 16,384 tokens, 64 in four groups over 8,000: 66.4 and 53.4
+// us; with tiles of 2 71.6 and 54.9, of 1 and a start of 6 81.4 and 59.6. Tiles of
+// heads of 256 values have half the tokens: 32 over 32,768 97.1, with 3 99.0.
+constexpr int kWideStart = 14;
+constexpr int wide_tile(int dt) { return dt == 256 ? 2 : 3; }
 constexpr int kLeast = 2;      // tiles of a wave
 
 constexpr int waves_of(int dt) { return dt == 256 ? 4 : 8; }    // of a work-group
@@ -210,7 +212,7 @@ __device__ int lay_out(const Shared& p, Layout& l) {
     if (all[1] > all[0] + all[0] / 4) team = 1;
     __syncthreads();
   }
-  const int wide_tile = kWideTile * team, wide_start = kWideStart * team;
+  const int tile_cost = wide_tile(DT) * team, start_cost = kWideStart * team;
   int units[3] = {0, 0, 0}, before[3], total[3];
   int each[3][kRun], longest = 0;
 #pragma unroll
@@ -221,7 +223,7 @@ __device__ int lay_out(const Shared& p, Layout& l) {
     const int rows = rows_of(i);
     if (rows) {
       const int shared = l.from[l.leader[i]];
-      if (rows > kHeads) units[0] += p.a.heads * blocks_of(rows, team) * (wide_start + ceil_div(shared, TT) * wide_tile);
+      if (rows > kHeads) units[0] += p.a.heads * blocks_of(rows, team) * (start_cost + ceil_div(shared, TT) * tile_cost);
       else units[1] += p.a.heads * (kStart + ceil_div(shared, kTile)), longest = max(longest, ceil_div(shared, kTile));
     }
     const int slot = l.own[i], from = shares(l, slot) ? l.from[i] : 0;
@@ -856,13 +858,13 @@ __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_ke
 #pragma unroll
   for (int k = 1; k < NW; ++k) longest = max(longest, l.longest[k]);
   const int least = max(kLeast, (int)(0.25f * __builtin_amdgcn_sqrtf((float)__builtin_amdgcn_readfirstlane(longest))));
-  share.waves = min(max(1, total / (team * max(least, wides ? max(NW, kWideTile) : 1))), teams);
+  share.waves = min(max(1, total / (team * max(least, wides ? max(NW, wide_tile(DT)) : 1))), teams);
   share.each = total / share.waves;
   share.more = total % share.waves;
   if (me_team >= share.waves) return;
   const int u0 = share.begin(me_team), u1 = share.begin(me_team + 1);
 
-  const int tile_cost = kWideTile * team, start_cost = kWideStart * team;
+  const int tile_cost = wide_tile(DT) * team, start_cost = kWideStart * team;
   for (int u = u0; u < min(u1, wides);) {
     const int i = __builtin_amdgcn_readfirstlane(find(l.wide, p.count, u));
     WidePart w;
@@ -1054,7 +1056,7 @@ Plan plan_of(int64_t batch, int64_t q_heads, const KvPages& pages, int64_t max_l
   // costs, a quarter more with teams, is no more than its members would cost for
   // themselves, n for each 16 of their rows, but for its start and its last tile.
   const int64_t tiles = max_len / kTile + 2 + kStart;
-  const int64_t start = (kTeam + a.group / kRows + 2) * (kWideStart + kWideTile);
+  const int64_t start = (kTeam + a.group / kRows + 2) * (kWideStart + wide_tile(a.dt));
   const int64_t most = 0x7FFFFFFF / std::max<int64_t>(1, count * pages.heads);  // of a sequence's streams to a key head
   if (tiles > most || tiles * a.head_tiles > most - start) throw std::invalid_argument("batch x heads x tokens is too large");
   if (count * q_heads * kJoin > 0xFFFFFFFFll) throw std::invalid_argument("batch x heads is too large");  // threads of the joining launch

@@ -31,8 +31,8 @@ def test_it_takes_what_decode_takes(lib, dim, heads, gh, batch):
     p = pages(heads=heads, dim=dim)
     # the longest that decode_attention takes: a stream's tiles of 32 tokens and 2 for its start, below 2^31 in all
     longest = min(2 ** 31 - 1, 32 * ((2 ** 31 - 1) // (batch * heads * -(-gh // 16)) - 2))
-    # a start: up to 8 + gh / 128 + 2 row tiles of 16 units, and 6 units more, of 32 tokens each
-    start = 32 * ((10 + gh // 128) * 16 + 6)
+    # a start: up to 8 + gh / 128 + 2 row tiles of 17 units, and 6 units more, of 32 tokens each
+    start = 32 * ((10 + gh // 128) * 17 + 6)
     assert longest > start
     assert lib.jasperx_shared_workspace(batch, heads * gh, ctypes.byref(p), longest - start, 1) > 0
     if longest + 32 < 2 ** 31:
