@@ -436,7 +436,8 @@ typedef struct jasperx_page_table {
  * pages that were missing, or -1 where a request cannot be: a sequence listed
  * twice, a count below 0, a sequence past width entries, more than n_tokens
  * tokens. Then nothing has changed, and the outputs are those of no new tokens.
- * Ids outside [0, sequences) are left out (padding: -1). */
+ * Ids outside [0, sequences) are left out (padding: -1). n up to 65535,
+ * sequences up to 2^18. */
 int64_t jasperx_extend_tables(const jasperx_page_table* table, const int32_t* seqs, const int32_t* counts, int64_t n,
                               int64_t n_tokens, int64_t width, int64_t* positions, int64_t* slots, int32_t* starts,
                               int32_t* step_tables, int32_t* step_lens, int32_t* src, int32_t* dst, int32_t* missing,

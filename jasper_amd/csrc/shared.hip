@@ -144,7 +144,7 @@ __device__ __forceinline__ int blocks_of(int rows, int team) { return ceil_div(c
 
 // Work-groups form teams: those of one take the same tokens under different
 // rows, on one XCD, so that its L2 reads them from memory once (512 rows over
-// 65,536 tokens of 8 heads: 252 us without, and 185 with no loads at all). Groups
+// 131,072 tokens of 8 heads: 426 us, 446 without). Groups
 // of unlike size might leave members without rows; where that would be more than a
 // quarter more tiles there are no teams (512 rows over 131,072 tokens beside 128 over
 // 32,768, 1.18 times the tiles: 480 us with teams, 498 without; over 65,536, 1.33
@@ -827,10 +827,12 @@ struct Wide {
 };
 
 // 64 sequences over 16,384 tokens of 8 key heads of 128 bf16 values, under 256
-// rows: 49 us, of which the first 11 go by before a wide stream's first product;
-// the matrix cores are busy 21% of it. 16 over 131,000 in e4m3, under 128 rows of
-// 8 heads: 112 to 119 us, 32%. 41 in seven groups of 900 to 12,345, heads of 64:
-// 26.6 us, 4.2 TB/s, waiting for reads 51% of its waves' cycles.
+// rows: 57 us, of which the first 11 go by before a wide stream's first product;
+// the matrix cores are busy 26% of it. 16 over 131,000 in e4m3, under 128 rows of
+// 8 heads: 139 to 156 us, 39%. (With weights of one term, and an error of 0.0019 in
+// place of 0.0017 of the bf16 output's norm: 49 and 112.) 41 in seven groups of 900
+// to 12,345, heads of 64: 26.7 us, 4.2 TB/s, waiting for reads 52% of its waves'
+// cycles.
 template <typename T, bool F8, int DT, bool FULL>
 __global__ __launch_bounds__(64 * waves_of(DT), waves_of(DT) / 4) void shared_kernel(Shared p) {
   typedef Wide<T, F8, DT, FULL> W;

@@ -215,8 +215,10 @@ def shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     A sequence that is shorter than its group's prefix reads its own pages, and
     so does one that is in no group. Groups are best as large as they come:
     every group costs as much as a sequence, and 16 query heads of one key head
-    fill a matrix instruction. Two sequences of few heads with less than about
-    32,000 tokens in common are as well served by decode_attention.
+    fill a matrix instruction. Where decode_attention would read less than 20 to
+    60 MB of pages again it is as fast or faster: with 8 key heads of 128 values
+    in 16 bits up to about 5,000 tokens in common of two sequences, 2,000 of
+    four, 1,000 of 16. Sums, weights and rounding are decode_attention's.
     """
     return _kv().shared_attention(q, k_pages, v_pages, tables, lens, groups, shared, scale, k_scale, v_scale, max_len,
                                   return_lse)
@@ -243,7 +245,8 @@ def extend_tables(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, 
     that are not there, or -1 where a request cannot be: a sequence listed
     twice, a count below 0, a sequence past width or max_pages, more than
     n_tokens tokens. Nothing has changed then, and the outputs are those of no
-    new tokens. Ids outside the tables, such as -1, are left out.
+    new tokens. Ids outside the tables, such as -1, are left out. At most 65,535
+    requests, and 2^18 sequences.
     """
     return _kv().extend_tables(tables, lens, refs, free, seqs, counts, page_size, n_tokens, width)
 
@@ -275,7 +278,11 @@ def shared_prefixes(tables: torch.Tensor, lens: torch.Tensor, page_size: int, le
     sequence is of its predecessor's group where both have at least `least`
     tokens in the same whole pages, and a group shares the whole pages that all
     of it have. Sequences with a prefix in common should be neighbours. Behind
-    the last group, groups is batch and shared 0."""
+    the last group, groups is batch and shared 0.
+
+    Groups are of one level: where all sequences begin alike and some go on
+    alike, one group shares what all have. With `least` past that there are
+    smaller groups that share more, and each reads the common part for itself."""
     return _kv().shared_prefixes(tables, lens, page_size, least)
 
 
